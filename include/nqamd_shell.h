@@ -164,6 +164,101 @@ int nq_greedy_select(const void* workspace, int64_t vocab, int64_t hidden, int64
                      int64_t* history, int64_t history_capacity, int32_t* step,
                      int32_t* position, void* stream);
 
+/* ---- Serving: ragged batches over an 8-bit paged KV cache ------------------ */
+
+/* An 8-bit paged KV cache and the batch that a call runs on it.
+ *
+ * A page holds page_size (16, 32, 64 or 128) consecutive cache rows of one
+ * sequence: for each kv head K as [page_size][head_dim] and V transposed, as
+ * [head_dim][page_size], OCP e4m3 bytes that stand for byte * scale, with one
+ * fp32 scale for each page, kv head and K or V ([num_pages][kv_heads]). head_dim
+ * is 64, 128 or 256; k_pages and v_pages are 16-byte aligned.
+ *
+ * The call's tokens lie one sequence after the other: sequence b has tokens
+ * [query_starts[b], query_starts[b + 1]) (int32, not decreasing; tokens before
+ * the first or behind the last start are nobody's, and their rows of every
+ * output stay as they were), at cache rows context_lens[b], context_lens[b] + 1,
+ * ... Row r of sequence b lies in page page_table[b][r / page_size] at row
+ * r % page_size. Entries of the table behind a sequence's last row are not
+ * read. All three arrays are device memory, so that a captured call replays
+ * with other lengths. */
+typedef struct nq_paged_kv {
+    void* k_pages;
+    void* v_pages;
+    float* k_scales;
+    float* v_scales;
+    int64_t num_pages;
+    int32_t kv_heads;
+    int32_t head_dim;
+    int32_t page_size;
+    int32_t reserved;              /* 0 */
+    const int32_t* page_table;     /* [batch][table_pages] */
+    int64_t table_pages;
+    const int32_t* query_starts;   /* [batch + 1] */
+    const int32_t* context_lens;   /* [batch] */
+    int64_t batch;
+} nq_paged_kv;
+
+/* Per-head RMSNorm of q and k (skipped when both weights are NULL), rotate-half
+ * RoPE at each token's cache row, and the append to the paged cache:
+ *   q_out[t, h, :] = rope(norm(q[t, h, :]))                     (q_out_dtype)
+ *   K row of token t = rope(norm(k[t, g, :])), V row = v[t, g, :], as e4m3(x / scale)
+ * A page's scale is the least power of two (from 2^-126 on) that brings all its
+ * rows within 448: the larger of the one it has and of what the new rows need;
+ * a page whose row 0 is written starts anew. When it grows, the rows before the
+ * new ones are rounded to the new scale. Rows behind the new ones stay as they
+ * are. Infinities and NaN are stored as NaN and do not count for the scale.
+ * q, k, v F32/F16/BF16 of one type, [tokens, heads * head_dim]; tables
+ * [rope_positions, head_dim / 2]. A token whose row lies outside the page table
+ * or the RoPE tables writes nothing; one whose table entry names no page writes
+ * q_out alone. A page that the call writes to belongs to one sequence.
+ * K is normed and rotated in fp64, so a stored byte is the rounding of the exact
+ * value. Replaces launch_decode_rope and launch_cache_prefix_update
+ * (src/nanoquant/runtime/cuda_kernels.py:401-447,546-587,715-815) for many
+ * sequences and pages. */
+int nq_paged_append(const void* q, const void* k, const void* v, int32_t dtype, int64_t tokens,
+                    int32_t q_heads, const void* q_norm, const void* k_norm, int32_t norm_dtype, float eps,
+                    const float* cos_table, const float* sin_table, int64_t rope_positions,
+                    const nq_paged_kv* kv, void* q_out, int32_t q_out_dtype, void* stream);
+
+/* Workspace bytes of nq_paged_attention (0: none needed). */
+int64_t nq_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int32_t q_heads, int32_t kv_heads,
+                                           int32_t head_dim, int32_t page_size, int64_t table_pages);
+
+/* Causal grouped-query attention of the call's tokens (after nq_paged_append
+ * with the same arrays): the token at cache row r attends rows [0, r] of its
+ * sequence, kv head h / (q_heads / kv_heads):
+ *   out[t, h, :] = softmax(scaling * q[t, h, :] . K) . V
+ * q F32/F16/BF16 [tokens, q_heads, head_dim], read exactly; out F32/F16/BF16
+ * [tokens, q_heads * head_dim]; both 16-byte aligned, q_heads a multiple of
+ * kv_heads. Scores and softmax in fp32, results joined in a fixed order
+ * (deterministic). A token whose row lies outside the page table gives zeros.
+ * A table entry in use that names no page counts as NaN rows. NaN in the cache,
+ * infinities and NaN in q do what fp32 arithmetic does with them, for the tokens
+ * that see them alone; rows that nobody sees may hold anything. Replaces
+ * launch_decode_attention (src/nanoquant/runtime/cuda_kernels.py:448-544) for
+ * many sequences and pages. */
+int nq_paged_attention(const void* q, int32_t q_dtype, int64_t tokens, int32_t q_heads, const nq_paged_kv* kv,
+                       float scaling, void* out, int32_t out_dtype, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+
+/* Workspace bytes of nq_token_logprobs. */
+int64_t nq_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top);
+
+/* For each row of logits (F32/F16/BF16, row_stride >= vocab elements apart):
+ *   logprobs[r] = log softmax(logits[r])[tokens[r]]   (NaN for a token outside [0, vocab))
+ *   entropy[r]  = -sum p log p over the row, 0 log 0 = 0
+ *   top_ids[r, :], top_logprobs[r, :] = the `top` likeliest tokens, likeliest first,
+ *     the lowest index first among equals, NaN above all
+ * top 0 to 32 (top_ids and top_logprobs may be NULL for 0), vocab up to about a
+ * million. Logits of -inf have probability 0; a row that holds NaN or +inf, or
+ * -inf alone, has NaN for every log probability and for the entropy. Beside
+ * nq_greedy_select for callers that report how likely an answer is; the
+ * reference's engine returns tokens alone (src/nanoquant/runtime/generation.py:240-246). */
+int nq_token_logprobs(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                      const int64_t* tokens, int32_t top, float* logprobs, float* entropy, int64_t* top_ids,
+                      float* top_logprobs, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,71 @@
+// The 8-bit paged KV cache: what its append and its attention share.
+#pragma once
+
+#include <math.h>
+
+#include "nq_common.h"
+#include "../../include/nqamd_shell.h"
+
+namespace nq {
+namespace paged {
+
+constexpr int kWave = 64;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// A checked nq_paged_kv as the kernels take it: rows of the cache and token
+// counts fit 32 bits, page offsets are formed in 64.
+struct Pages {
+    uint8_t* k;               // [pages][kv_heads][page][head_dim]
+    uint8_t* v;               // [pages][kv_heads][head_dim][page]
+    float* k_scales;          // [pages][kv_heads]
+    float* v_scales;
+    const int32_t* table;     // [batch][table_pages]
+    const int32_t* starts;    // [batch + 1]
+    const int32_t* contexts;  // [batch]
+    int64_t pages;
+    int32_t kv_heads, page_shift, table_pages, batch, tokens;
+};
+
+int check_pages(const nq_paged_kv* kv, int64_t tokens, Pages& out);
+
+// Tokens [begin, end) of sequence b, forced into [0, tokens] and into order:
+// whatever the caller's array holds, no token outside the buffers is named.
+struct Span {
+    int begin, end;
+};
+
+__device__ __forceinline__ Span span_of(const Pages& p, int b) {
+    const int begin = min(max(p.starts[b], 0), p.tokens);
+    return {begin, min(max(p.starts[b + 1], begin), p.tokens)};
+}
+
+// The last sequence b with first(b) <= slot, for a non-decreasing `first`
+// (sequence 0 when there is none). All lanes of a wave search together, 64
+// ways a round: one round of loads for up to 64 sequences, two for 4096. With
+// starts that are not in order some sequence comes out; its span decides
+// whether the slot names anything.
+template <class First>
+__device__ __forceinline__ int sequence_at(int batch, int64_t slot, const First& first) {
+    const int lane = threadIdx.x & (kWave - 1);
+    int low = 0, count = batch;
+    while (count > 1) {
+        const int step = (count + kWave - 1) / kWave;
+        const int at = lane * step;
+        const uint64_t below = __ballot(at < count && first(low + (at < count ? at : 0)) <= slot);
+        const int hit = below ? 63 - __builtin_clzll(below) : 0;
+        low += hit * step;
+        count = min(step, count - hit * step);
+    }
+    return __builtin_amdgcn_readfirstlane(low);
+}
+
+// A token's cache row: its sequence's context plus its place, or -1 outside
+// the rows [0, rows) that the page table holds.
+__device__ __forceinline__ int row_of(int context, int place, int rows) {
+    const int64_t row = static_cast<int64_t>(context) + place;
+    return row >= 0 && row < rows ? static_cast<int>(row) : -1;
+}
+
+}  // namespace paged
+}  // namespace nq

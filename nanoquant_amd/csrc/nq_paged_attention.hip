@@ -1,0 +1,137 @@
+// Attention over the 8-bit paged cache: plan, merge of the splits, entry points.
+#include "nq_paged_attention.h"
+
+namespace nq {
+namespace paged {
+
+template <> int launch_paged_attention<64>(const AttnArgs&, const AttnPlan&, int, hipStream_t);
+template <> int launch_paged_attention<128>(const AttnArgs&, const AttnPlan&, int, hipStream_t);
+template <> int launch_paged_attention<256>(const AttnArgs&, const AttnPlan&, int, hipStream_t);
+
+}  // namespace paged
+}  // namespace nq
+
+namespace {
+
+using namespace nq::paged;
+
+// One wave per token and q head: the splits' results, in split order.
+template <int D>
+__global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows) {
+    constexpr int E = D / kWave;
+    const Pages& p = a.p;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int token = static_cast<int>(item / a.q_heads), head = static_cast<int>(item % a.q_heads);
+    if (token >= p.tokens) return;
+    const int b = sequence_at(p.batch, token, [&](int i) { return static_cast<int64_t>(span_of(p, i).begin); });
+    const Span span = span_of(p, b);
+    if (token < span.begin || token >= span.end) return;
+    const int g = head / a.group;
+    const int r = (token - span.begin) * a.group + head - g * a.group;
+    const int64_t slot = first_slot_of(p, b, a.group, rows) + r / rows;
+    const SlotSpan s = slot_span(p, b, slot, a.group, rows);
+    const SplitPlan plan = split_plan(s.visible, a.splits, a.least);
+    if (plan.active <= 1) return;  // the attention wrote the output itself
+    const int64_t first = (slot * a.splits * p.kv_heads + g) * rows + r % rows;
+    const int64_t next = static_cast<int64_t>(p.kv_heads) * rows;  // from one split's row to the next split's
+    float m = -INFINITY;
+    for (int i = lane; i < plan.active; i += kWave) m = fmaxf(m, a.partial[2 * (first + i * next)]);
+#pragma unroll
+    for (int k = 1; k < kWave; k *= 2) m = fmaxf(m, __shfl_xor(m, k, kWave));
+    const float m_use = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f, o[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) o[j] = 0.0f;
+    for (int i = 0; i < plan.active; ++i) {
+        const int64_t at = first + i * next;
+        const float w = exp2_hw(a.partial[2 * at] - m_use);
+        sum += w * a.partial[2 * at + 1];
+#pragma unroll
+        for (int j = 0; j < E; ++j) o[j] += w * a.partial_o[at * D + lane + kWave * j];
+    }
+    const bool off = row_of(s.context, token - span.begin, p.table_pages << p.page_shift) < 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+        nq::store_f32_as(a.out, a.out_dtype, item * D + lane + kWave * j, off ? 0.0f : o[j] / sum);
+}
+
+// Few query rows to a sequence: a slot of 16 rows whose waves share them, and
+// the cache split until the chip has about two workgroups to a CU; more: slots
+// of 64 rows, 16 to a wave.
+AttnPlan plan_attention(int64_t tokens, int64_t batch, int q_heads, int kv_heads, int64_t cache_rows) {
+    constexpr int64_t kWorkgroups = 512;
+    AttnPlan plan;
+    const int64_t rows = tokens * (q_heads / kv_heads);
+    plan.shared = rows <= 16 * batch;
+    plan.rows = plan.shared ? 16 : 64;
+    plan.slots = static_cast<int>(rows / plan.rows + batch);
+    plan.least = plan.shared ? 4 : 8;
+    const int64_t tiles = (cache_rows + kTile - 1) / kTile;
+    int64_t splits = kWorkgroups / (static_cast<int64_t>(plan.slots) * kv_heads);
+    const int64_t most = (tiles + plan.least - 1) / plan.least;
+    splits = splits < most ? splits : most;
+    plan.splits = static_cast<int>(splits < 1 ? 1 : (splits > 128 ? 128 : splits));
+    return plan;
+}
+
+int64_t partial_rows(const AttnPlan& plan, int kv_heads) {
+    return plan.splits <= 1 ? 0 : static_cast<int64_t>(plan.slots) * plan.splits * kv_heads * plan.rows;
+}
+
+}  // namespace
+
+extern "C" int64_t nq_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int32_t q_heads, int32_t kv_heads,
+                                                      int32_t head_dim, int32_t page_size, int64_t table_pages) {
+    if (tokens <= 0 || tokens > 0xffffff || batch <= 0 || batch > 0xffffff || kv_heads <= 0 || q_heads <= 0 ||
+        q_heads > 65535 || q_heads % kv_heads || page_size <= 0 || page_size > 128 || table_pages <= 0 ||
+        table_pages > 0x7fffffff / page_size || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+        return -1;
+    if (tokens * (q_heads / kv_heads) > 0x3fffffff) return -1;
+    const AttnPlan plan = plan_attention(tokens, batch, q_heads, kv_heads, table_pages * page_size);
+    return partial_rows(plan, kv_heads) * (2 + head_dim) * static_cast<int64_t>(sizeof(float));
+}
+
+extern "C" int nq_paged_attention(const void* q, int32_t q_dtype, int64_t tokens, int32_t q_heads,
+                                  const nq_paged_kv* kv, float scaling, void* out, int32_t out_dtype, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+    if (!q || !out) return NQ_ERR_ARGUMENT;
+    if (!nq::is_float_dtype(q_dtype) || !nq::is_float_dtype(out_dtype)) return NQ_ERR_DTYPE;
+    AttnArgs a{};
+    if (const int st = check_pages(kv, tokens, a.p); st != NQ_OK) return st;
+    const int64_t need = nq_paged_attention_workspace_bytes(tokens, kv->batch, q_heads, kv->kv_heads, kv->head_dim,
+                                                            kv->page_size, kv->table_pages);
+    if (need < 0) return NQ_ERR_SHAPE;
+    if (!(scaling > 0.0f) || !(scaling < INFINITY)) return NQ_ERR_ARGUMENT;
+    if (need > 0 && !workspace) return NQ_ERR_ARGUMENT;
+    if (workspace_bytes < need) return NQ_ERR_WORKSPACE;
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
+        return NQ_ERR_ALIGNMENT;
+    const AttnPlan plan = plan_attention(tokens, kv->batch, q_heads, kv->kv_heads, kv->table_pages * kv->page_size);
+    a.q = q;
+    a.out = out;
+    a.partial_o = static_cast<float*>(workspace);
+    a.partial = a.partial_o ? a.partial_o + partial_rows(plan, kv->kv_heads) * kv->head_dim : nullptr;
+    a.scale = scaling * 1.4426950408889634f;
+    a.out_dtype = out_dtype;
+    a.q_heads = q_heads;
+    a.group = q_heads / kv->kv_heads;
+    a.slots = plan.slots;
+    a.splits = plan.splits;
+    a.least = plan.least;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    int status;
+    switch (kv->head_dim) {
+        case 64: status = launch_paged_attention<64>(a, plan, q_dtype, st); break;
+        case 128: status = launch_paged_attention<128>(a, plan, q_dtype, st); break;
+        default: status = launch_paged_attention<256>(a, plan, q_dtype, st); break;
+    }
+    if (status != NQ_OK || plan.splits <= 1) return status;
+    const dim3 grid(static_cast<unsigned>((tokens * q_heads + 3) / 4));
+    switch (kv->head_dim) {
+        case 64: hipLaunchKernelGGL(k_paged_merge<64>, grid, dim3(256), 0, st, a, plan.rows); break;
+        case 128: hipLaunchKernelGGL(k_paged_merge<128>, grid, dim3(256), 0, st, a, plan.rows); break;
+        default: hipLaunchKernelGGL(k_paged_merge<256>, grid, dim3(256), 0, st, a, plan.rows); break;
+    }
+    return nq::launch_status();
+}

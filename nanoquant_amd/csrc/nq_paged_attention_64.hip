@@ -1,0 +1,13 @@
+// Attention over the 8-bit paged cache, heads of 64.
+#include "nq_paged_attention.h"
+
+namespace nq {
+namespace paged {
+
+template <>
+int launch_paged_attention<64>(const AttnArgs& a, const AttnPlan& plan, int q_dtype, hipStream_t stream) {
+    return launch_attention_for<64>(a, plan, q_dtype, stream);
+}
+
+}  // namespace paged
+}  // namespace nq

@@ -73,6 +73,11 @@ EXPORTED_SYMBOLS = (
     "nq_output_projection_workspace_bytes",
     "nq_output_projection",
     "nq_greedy_select",
+    "nq_paged_append",
+    "nq_paged_attention_workspace_bytes",
+    "nq_paged_attention",
+    "nq_token_logprobs_workspace_bytes",
+    "nq_token_logprobs",
 )
 
 
@@ -161,6 +166,27 @@ class DecodeFusion(ctypes.Structure):
     ]
 
 
+class PagedKv(ctypes.Structure):
+    """nq_paged_kv (include/nqamd_shell.h)."""
+
+    _fields_ = [
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("page_table", ctypes.c_void_p),
+        ("table_pages", ctypes.c_int64),
+        ("query_starts", ctypes.c_void_p),
+        ("context_lens", ctypes.c_void_p),
+        ("batch", ctypes.c_int64),
+    ]
+
+
 _LIB: ctypes.CDLL | None = None
 
 
@@ -227,6 +253,16 @@ def _declare(lib: ctypes.CDLL) -> None:
         "nq_output_projection_workspace_bytes": (c_i64, [c_i64, c_i64]),
         "nq_output_projection": (c_int, [vp, i32, vp, c_i64, c_i64, vp, vp, c_i64, vp]),
         "nq_greedy_select": (c_int, [vp, c_i64, c_i64, vp, vp, c_i64, vp, vp, vp]),
+        "nq_paged_append": (
+            c_int,
+            [vp, vp, vp, i32, c_i64, i32, vp, vp, i32, f32, vp, vp, c_i64, ctypes.POINTER(PagedKv), vp, i32, vp],
+        ),
+        "nq_paged_attention_workspace_bytes": (c_i64, [c_i64, c_i64, i32, i32, i32, i32, c_i64]),
+        "nq_paged_attention": (
+            c_int, [vp, i32, c_i64, i32, ctypes.POINTER(PagedKv), f32, vp, i32, vp, c_i64, vp],
+        ),
+        "nq_token_logprobs_workspace_bytes": (c_i64, [c_i64, c_i64, i32]),
+        "nq_token_logprobs": (c_int, [vp, i32, c_i64, c_i64, c_i64, vp, i32, vp, vp, vp, vp, vp, c_i64, vp]),
     }
     for name, (restype, argtypes) in table.items():
         fn = getattr(lib, name)

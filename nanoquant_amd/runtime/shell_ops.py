@@ -11,6 +11,9 @@ first token) so a captured step replays at every position.
 
 from __future__ import annotations
 
+import ctypes
+from typing import NamedTuple
+
 import torch
 
 from nanoquant_amd.runtime import _native
@@ -438,3 +441,267 @@ def launch_greedy_select(
     )
     _native.check("nq_greedy_select", status)
     return token_out
+
+
+# -- serving: ragged batches over an 8-bit paged cache ---------------------------
+
+
+class PagedCache(NamedTuple):
+    """An 8-bit paged KV cache (``nq_paged_kv`` in ``include/nqamd_shell.h``): K
+    ``[pages, kv_heads, page_size, head_dim]`` and V, transposed,
+    ``[pages, kv_heads, head_dim, page_size]``, float8_e4m3fn values that stand
+    for value * scale, with one fp32 scale ``[pages, kv_heads]`` each."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scales: torch.Tensor
+    v_scales: torch.Tensor
+
+
+def paged_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, device: torch.device | str) -> PagedCache:
+    """An empty paged cache. ``page_size`` is 16, 32, 64 or 128, ``head_dim`` 64, 128 or 256."""
+
+    if pages < 1 or kv_heads < 1 or page_size not in _PAGE_SIZES or head_dim not in (64, 128, 256):
+        raise ValueError("paged cache geometry is unsupported")
+
+    def zeros(*shape: int) -> torch.Tensor:
+        return torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+
+    scales = torch.zeros((2, pages, kv_heads), dtype=torch.float32, device=device)
+    return PagedCache(zeros(pages, kv_heads, page_size, head_dim), zeros(pages, kv_heads, head_dim, page_size),
+                      scales[0], scales[1])
+
+
+_PAGE_SIZES = (16, 32, 64, 128)
+
+
+def _paged_kv(name: str, device: torch.device, cache: PagedCache, page_table: torch.Tensor,
+              query_starts: torch.Tensor, context_lens: torch.Tensor) -> _native.PagedKv:
+    """Checks of the cache and the batch; the C descriptor of both."""
+
+    k, v, k_scales, v_scales = cache
+    _check_device(name, device, k, v, k_scales, v_scales, page_table, query_starts, context_lens)
+    if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or k.ndim != 4:
+        raise ValueError(f"{name} cache pages must be 4-D float8_e4m3fn")
+    pages, kv_heads, page_size, head_dim = k.shape
+    if v.shape != (pages, kv_heads, head_dim, page_size):
+        raise ValueError(f"{name} cache must be K [pages, kv_heads, page_size, head_dim], V [pages, kv_heads, head_dim, page_size]")
+    if page_size not in _PAGE_SIZES or head_dim not in (64, 128, 256) or not pages or not kv_heads:
+        raise ValueError(f"{name} page size must be 16, 32, 64 or 128 and head_dim 64, 128 or 256")
+    if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32 or k_scales.shape != (pages, kv_heads) \
+            or v_scales.shape != (pages, kv_heads):
+        raise ValueError(f"{name} cache scales must be fp32 [pages, kv_heads]")
+    if page_table.dtype != torch.int32 or query_starts.dtype != torch.int32 or context_lens.dtype != torch.int32:
+        raise ValueError(f"{name} page_table, query_starts and context_lens must be int32")
+    if page_table.ndim != 2 or context_lens.ndim != 1 or query_starts.ndim != 1:
+        raise ValueError(f"{name} takes page_table [batch, pages], query_starts [batch + 1] and context_lens [batch]")
+    batch, table_pages = page_table.shape
+    if not batch or not table_pages or context_lens.shape[0] != batch or query_starts.shape[0] != batch + 1:
+        raise ValueError(f"{name} takes page_table [batch, pages], query_starts [batch + 1] and context_lens [batch]")
+    return _native.PagedKv(k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), pages, kv_heads,
+                           head_dim, page_size, 0, page_table.data_ptr(), table_pages, query_starts.data_ptr(),
+                           context_lens.data_ptr(), batch)
+
+
+def _on_device(device: torch.device, function, *args) -> int:
+    """``function(*args)`` with `device` current: a default stream's handle is
+    the same on every device, the launch goes to the current one's."""
+
+    if torch.cuda.current_device() == device.index:
+        return function(*args)
+    with torch.cuda.device(device):
+        return function(*args)
+
+
+def launch_paged_append(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cache: PagedCache,
+    *,
+    q_heads: int,
+    q_norm: torch.Tensor | None,
+    k_norm: torch.Tensor | None,
+    eps: float,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    page_table: torch.Tensor,
+    query_starts: torch.Tensor,
+    context_lens: torch.Tensor,
+    q_out: torch.Tensor | None = None,
+    q_dtype: torch.dtype = torch.float32,
+) -> torch.Tensor:
+    """Per-head RMSNorm + RoPE of a ragged batch's q and k and the append of k and
+    v to an 8-bit paged cache; returns the rotated q ``[tokens, q_heads,
+    head_dim]``. Tokens ``query_starts[b] .. query_starts[b + 1]`` are sequence
+    b's, at cache rows ``context_lens[b] ..``, in the pages ``page_table[b]``
+    (nq_paged_append). Mirrors ``launch_decode_rope`` and
+    ``launch_cache_prefix_update`` (src/nanoquant/runtime/cuda_kernels.py:715-815)
+    for many sequences."""
+
+    device = q.device
+    _check_device("paged append", device, q, k, v, q_norm, k_norm, cos, sin, q_out)
+    kv = _paged_kv("paged append", device, cache, page_table, query_starts, context_lens)
+    kv_heads, head_dim = kv.kv_heads, kv.head_dim
+    if q_heads < 1 or q_heads % kv_heads:
+        raise ValueError("paged append q heads must be a multiple of the cache's kv heads")
+    tokens = q.numel() // (q_heads * head_dim)
+    if tokens < 1 or q.numel() != tokens * q_heads * head_dim or k.numel() != tokens * kv_heads * head_dim \
+            or v.numel() != k.numel():
+        raise ValueError("paged append takes q [tokens, q_heads * head_dim], k and v [tokens, kv_heads * head_dim]")
+    if q.dtype not in _FLOAT or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("paged append q, k and v must share one of F32/F16/BF16")
+    if (q_norm is None) != (k_norm is None):
+        raise ValueError("q_norm and k_norm must be given together")
+    norm_code = 0
+    if q_norm is not None:
+        if q_norm.numel() != head_dim or k_norm.numel() != head_dim or q_norm.dtype != k_norm.dtype \
+                or q_norm.dtype not in _FLOAT:
+            raise ValueError("q/k norm weights must be [head_dim] of one of F32/F16/BF16")
+        norm_code = _native.DTYPE_CODES[q_norm.dtype]
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.ndim != 2 or cos.shape[1] != head_dim // 2 \
+            or cos.shape[0] < 1 or sin.shape != cos.shape:
+        raise ValueError("RoPE tables must be fp32 [positions, head_dim / 2]")
+    if q_out is None:
+        q_out = torch.empty((tokens, q_heads, head_dim), dtype=q_dtype, device=device)
+    elif q_out.numel() != tokens * q_heads * head_dim:
+        raise ValueError("q_out must be [tokens, q_heads, head_dim]")
+    if q_out.dtype not in _FLOAT:
+        raise ValueError("q_out must be F32/F16/BF16")
+    status = _on_device(
+        device, _native.load().nq_paged_append, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        _native.DTYPE_CODES[q.dtype], tokens, q_heads, _ptr(q_norm), _ptr(k_norm), norm_code, float(eps),
+        cos.data_ptr(), sin.data_ptr(), cos.shape[0], ctypes.byref(kv), q_out.data_ptr(),
+        _native.DTYPE_CODES[q_out.dtype], _stream(device),
+    )
+    _native.check("nq_paged_append", status)
+    return q_out
+
+
+def paged_attention_workspace_bytes(tokens: int, batch: int, q_heads: int, cache: PagedCache, table_pages: int) -> int:
+    _pages, kv_heads, page_size, head_dim = cache.k.shape
+    return int(_native.load().nq_paged_attention_workspace_bytes(tokens, batch, q_heads, kv_heads, head_dim, page_size,
+                                                                 table_pages))
+
+
+def launch_paged_attention(
+    q: torch.Tensor,
+    cache: PagedCache,
+    *,
+    page_table: torch.Tensor,
+    query_starts: torch.Tensor,
+    context_lens: torch.Tensor,
+    scaling: float,
+    out: torch.Tensor | None = None,
+    out_dtype: torch.dtype = torch.bfloat16,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Causal grouped-query attention of a ragged batch's ``q`` (F32/F16/BF16
+    ``[tokens, q_heads, head_dim]``) over an 8-bit paged cache that holds the
+    tokens' own rows too (``launch_paged_append`` with the same batch): the
+    token at cache row r attends rows ``[0, r]`` of its sequence
+    (nq_paged_attention). One token a sequence or a whole prompt each. Mirrors
+    ``launch_decode_attention`` (src/nanoquant/runtime/cuda_kernels.py:493-544)
+    for many sequences."""
+
+    device = q.device
+    if q.ndim != 3 or q.dtype not in _FLOAT:
+        raise ValueError("paged attention query must be F32/F16/BF16 [tokens, q_heads, head_dim]")
+    _check_device("paged attention", device, q, out, workspace)
+    kv = _paged_kv("paged attention", device, cache, page_table, query_starts, context_lens)
+    tokens, q_heads, head_dim = q.shape
+    if head_dim != kv.head_dim or not tokens or not q_heads or q_heads % kv.kv_heads:
+        raise ValueError("paged attention query geometry does not match the cache")
+    if not 0.0 < scaling < float("inf"):
+        raise ValueError("paged attention scaling must be positive and finite")
+    if out is None:
+        out = torch.empty((tokens, q_heads * head_dim), dtype=out_dtype, device=device)
+    elif out.numel() != q.numel():
+        raise ValueError("paged attention output geometry is incompatible")
+    if out.dtype not in _FLOAT:
+        raise ValueError("paged attention output must be F32/F16/BF16")
+    lib = _native.load()
+    need = lib.nq_paged_attention_workspace_bytes(tokens, kv.batch, q_heads, kv.kv_heads, head_dim, kv.page_size,
+                                                  kv.table_pages)
+    if need < 0:
+        raise ValueError("paged attention geometry was rejected")
+    if workspace is None and need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    status = _on_device(
+        device, lib.nq_paged_attention, q.data_ptr(), _native.DTYPE_CODES[q.dtype], tokens, q_heads, ctypes.byref(kv),
+        float(scaling), out.data_ptr(), _native.DTYPE_CODES[out.dtype], _ptr(workspace),
+        0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(device),
+    )
+    _native.check("nq_paged_attention", status)
+    return out
+
+
+# -- how likely the answers are ---------------------------------------------------
+
+
+class TokenLogprobs(NamedTuple):
+    """``launch_token_logprobs``' result: fp32 ``[rows]`` log probability of each
+    row's token and entropy of its distribution, int64 and fp32 ``[rows, top]``
+    likeliest tokens and their log probabilities, likeliest first."""
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+def token_logprobs_workspace_bytes(rows: int, vocab: int, top: int) -> int:
+    return int(_native.load().nq_token_logprobs_workspace_bytes(rows, vocab, top))
+
+
+def launch_token_logprobs(
+    logits: torch.Tensor,
+    tokens: torch.Tensor,
+    *,
+    top: int = 0,
+    out: TokenLogprobs | None = None,
+    workspace: torch.Tensor | None = None,
+) -> TokenLogprobs:
+    """Log probability of ``tokens[r]`` under ``softmax(logits[r])``, the entropy of
+    that distribution and its ``top`` (0 to 32) likeliest tokens, the lowest id
+    first among equals (nq_token_logprobs). ``logits`` is F32/F16/BF16 ``[rows,
+    vocab]``; its rows may lie further apart than vocab."""
+
+    device = logits.device
+    if logits.ndim != 2 or logits.dtype not in _FLOAT:
+        raise ValueError("token logprobs take F32/F16/BF16 logits [rows, vocab]")
+    rows, vocab = logits.shape
+    if not rows or not vocab:
+        raise ValueError("token logprobs need at least one row and one token")
+    stride = logits.stride(0) if rows > 1 else vocab
+    if (vocab > 1 and logits.stride(1) != 1) or stride < vocab:
+        raise ValueError("token logprobs need rows of adjacent logits that do not overlap")
+    if tokens.dtype != torch.int64 or tokens.shape != (rows,):
+        raise ValueError("token logprobs take int64 tokens [rows]")
+    if not 0 <= top <= 32 or top > vocab:
+        raise ValueError("token logprobs give 0 to 32 alternatives, at most the vocabulary")
+    if device.type != "cuda" or tokens.device != device:
+        raise ValueError("token logprobs require CUDA/HIP tensors on one device")
+    if out is None:
+        sums = torch.empty((2, rows), dtype=torch.float32, device=device)
+        out = TokenLogprobs(sums[0], sums[1], torch.empty((rows, top), dtype=torch.int64, device=device),
+                            torch.empty((rows, top), dtype=torch.float32, device=device))
+    _check_device("token logprobs", device, tokens, *out, workspace)
+    if out.logprobs.dtype != torch.float32 or out.entropy.dtype != torch.float32 or out.top_ids.dtype != torch.int64 \
+            or out.top_logprobs.dtype != torch.float32 or out.logprobs.shape != (rows,) or out.entropy.shape != (rows,) \
+            or out.top_ids.shape != (rows, top) or out.top_logprobs.shape != (rows, top):
+        raise ValueError("token logprobs outputs must be fp32 [rows] twice, int64 and fp32 [rows, top]")
+    lib = _native.load()
+    need = lib.nq_token_logprobs_workspace_bytes(rows, vocab, top)
+    if need < 0:
+        raise ValueError("token logprobs geometry was rejected")
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    status = _on_device(
+        device, lib.nq_token_logprobs, logits.data_ptr(), _native.DTYPE_CODES[logits.dtype], rows, vocab, stride,
+        tokens.data_ptr(), top, out.logprobs.data_ptr(), out.entropy.data_ptr(), _ptr(out.top_ids if top else None),
+        _ptr(out.top_logprobs if top else None), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+        _stream(device),
+    )
+    _native.check("nq_token_logprobs", status)
+    return out
