@@ -22,12 +22,19 @@ shell built from this library's kernels instead:
   the embedding writes the row statistics the first layer's folded norm reads,
   so a step is the layers, the embedding, the final norm, the output
   projection and the greedy selection;
-* the KV cache is one device tensor per layer ``[kv_heads, max_positions,
+* the KV cache is one device tensor per layer (another form below) ``[kv_heads, max_positions,
   head_dim]``, and the token position lives in device memory, so one HIP graph
   of the whole one-token step replays for every position with no host
   synchronisation; ``generate_greedy`` replays a graph of STEPS_PER_GRAPH
   consecutive steps (the one-step graph for the remainder), keeps the chosen
   tokens on the device and synchronises once at the end.
+
+With ``cache_dtype=torch.float8_e4m3fn`` the KV cache is the 8-bit paged one
+(``shell_ops.PagedCache``, a quarter of the fp32 cache's bytes, one scale for
+each PAGE_ROWS rows and head): every pass then appends with
+``launch_paged_append`` and attends with ``launch_paged_attention``.
+``generate_greedy_scored`` and ``score`` report how likely an answer or a given
+text is (``launch_token_logprobs``).
 
 ``forward_step`` implements the reference's ``GenerationModel`` protocol for
 batch 1 (a prompt without padding), returning ``[1, 1, vocab]`` fp32 logits
@@ -61,6 +68,13 @@ FOLD_MAX_BLOCKS = 16
 # kernel; measured on the same model and cache, tok/s with 1 / 2 / 4 / 8 / 16
 # steps per graph: 570.6 / 572.2 / 572.1 / 573.0 / 572.9.
 STEPS_PER_GRAPH = 8
+
+# Rows of a page of the 8-bit cache: one attention tile, so a tile's table entry
+# and scale are one.
+PAGE_ROWS = 64
+
+# Rows of logits that score() holds at once (156 MB at 151936 fp32 logits).
+SCORE_ROWS = 256
 
 
 class DecodeStep(NamedTuple):
@@ -225,6 +239,7 @@ class _Buffers:
     attn_ws: torch.Tensor
     o_slots: torch.Tensor      # fused decode: sums of residual^2 per 16 rows after the o-projection
     down_slots: torch.Tensor   # ... and after the down-projection
+    starts: torch.Tensor       # 8-bit cache: the one sequence's first token and end
 
 
 class PackedDecoder:
@@ -254,6 +269,8 @@ class PackedDecoder:
             raise DecoderShellError("unsupported attention geometry")
         if activation_dtype not in (torch.bfloat16, torch.float16, torch.float32):
             raise DecoderShellError("activation dtype must be BF16, F16 or F32")
+        if cache_dtype not in (torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn):
+            raise DecoderShellError("cache dtype must be BF16, F16, F32 or F8 E4M3")
         self.max_positions = int(max_positions)
         self.activation_dtype = activation_dtype
         self.cache_dtype = cache_dtype
@@ -300,12 +317,18 @@ class PackedDecoder:
         fold = (blocks <= FOLD_MAX_BLOCKS and cache_dtype != torch.float32 if fold_attention_merge is None
                 else bool(fold_attention_merge))
         self.fold_attention_merge = (
-            fold and self.fuse_decode
+            fold and self.fuse_decode and cache_dtype != torch.float8_e4m3fn
             and ops.decode_attention_partials_supported(c.q_heads, c.kv_heads, c.head_dim, cache_dtype)
             and c.q_heads * c.head_dim <= 4096 and blocks <= 16 and (c.q_heads * blocks) % 2 == 0)
-        cache_shape = (c.layers, c.kv_heads, self.max_positions, c.head_dim)
-        self.k_cache = torch.zeros(cache_shape, dtype=cache_dtype, device=dev)
-        self.v_cache = torch.zeros(cache_shape, dtype=cache_dtype, device=dev)
+        self.paged: list[ops.PagedCache] | None = None
+        if cache_dtype == torch.float8_e4m3fn:
+            pages = -(-self.max_positions // PAGE_ROWS)
+            self.paged = [ops.paged_cache(pages, c.kv_heads, PAGE_ROWS, c.head_dim, dev) for _ in range(c.layers)]
+            self.page_table = torch.arange(pages, dtype=torch.int32, device=dev)[None]
+        else:
+            cache_shape = (c.layers, c.kv_heads, self.max_positions, c.head_dim)
+            self.k_cache = torch.zeros(cache_shape, dtype=cache_dtype, device=dev)
+            self.v_cache = torch.zeros(cache_shape, dtype=cache_dtype, device=dev)
         cos, sin = rope_tables(c.head_dim, c.rope_theta, self.max_positions)
         self.cos, self.sin = cos.to(dev), sin.to(dev)
         self.scaling = c.head_dim**-0.5
@@ -344,17 +367,21 @@ class PackedDecoder:
         def a(*shape):
             return torch.empty(shape, dtype=act, device=dev)
 
+        if self.paged is not None:
+            workspace = ops.paged_attention_workspace_bytes(tokens, 1, c.q_heads, self.paged[0], self.page_table.shape[1])
+        elif tokens == 1:
+            workspace = ops.decode_attention_workspace_bytes(c.q_heads, c.kv_heads, c.head_dim, self.cache_dtype,
+                                                             self.max_positions)
+        else:
+            workspace = ops.attention_workspace_bytes(tokens, c.q_heads, c.head_dim, self.max_positions)
         return _Buffers(
             tokens, f32(tokens, c.hidden), a(tokens, c.hidden), f32(tokens, q_width), f32(tokens, kv_width),
             f32(tokens, kv_width), f32(tokens, c.q_heads, c.head_dim), a(tokens, q_width), f32(tokens, c.hidden),
             f32(tokens, c.intermediate), f32(tokens, c.intermediate), a(tokens, c.intermediate),
             f32(tokens, c.hidden), f32(tokens, c.hidden),
-            torch.empty(
-                ops.decode_attention_workspace_bytes(c.q_heads, c.kv_heads, c.head_dim, self.cache_dtype,
-                                                     self.max_positions)
-                if tokens == 1 else ops.attention_workspace_bytes(tokens, c.q_heads, c.head_dim, self.max_positions),
-                dtype=torch.uint8, device=dev),
+            torch.empty(workspace, dtype=torch.uint8, device=dev),
             f32(-(-c.hidden // 16)), f32(-(-c.hidden // 16)),
+            torch.tensor([0, tokens], dtype=torch.int32, device=dev),
         )
 
     # -- one forward -----------------------------------------------------------------
@@ -381,7 +408,13 @@ class PackedDecoder:
             else:
                 ops.launch_add_rmsnorm(b.residual, in_norm, c.eps, delta=b.down if i else None, out=b.xn)
                 self._linears([b.xn] * 3, qkv, [b.q, b.k, b.v], t)
-            if t == 1 and fused and self.fold_attention_merge:
+            if self.paged is not None:
+                batch = {"page_table": self.page_table, "query_starts": b.starts, "context_lens": self.position}
+                ops.launch_paged_append(b.q, b.k, b.v, self.paged[i], q_heads=c.q_heads, q_norm=qn, k_norm=kn,
+                                        eps=c.eps, cos=self.cos, sin=self.sin, q_out=b.q_rot, **batch)
+                ops.launch_paged_attention(b.q_rot, self.paged[i], scaling=self.scaling, out=b.attn,
+                                           workspace=b.attn_ws, **batch)
+            elif t == 1 and fused and self.fold_attention_merge:
                 ops.launch_decode_attention_partials(
                     b.q, b.k, b.v, q_heads=c.q_heads, kv_heads=c.kv_heads, head_dim=c.head_dim, q_norm=qn,
                     k_norm=kn, eps=c.eps, cos=self.cos, sin=self.sin, position=self.position,
@@ -480,15 +513,92 @@ class PackedDecoder:
         logits (fp32 [vocab], the decoder's own buffer) and leaves the greedy
         partials in the workspace."""
 
+        self._prefill(prompt, start)
+        return self.logits
+
+    def _prefill(self, prompt: torch.Tensor, start: int) -> tuple[torch.Tensor, _Buffers]:
+        """The prompt's ids on the device and the activations of its pass."""
+
         ids = prompt.reshape(-1).to(self.device, torch.int64).contiguous()
         t = ids.numel()
         if t < 1 or start + t > self.max_positions:
             raise DecoderShellError("prompt does not fit the KV cache")
         self.position.fill_(start)
-        self._forward(ids, self._buffers(t))
+        buffers = self._buffers(t)
+        self._forward(ids, buffers)
         self.position.fill_(start + t)
         self.host_position = start + t
-        return self.logits
+        return ids, buffers
+
+    def score(self, ids: torch.Tensor, *, top: int = 0) -> ops.TokenLogprobs:
+        """How likely a text is: for each of ``ids[1:]`` its log probability after
+        the ids before it, the entropy of that distribution and its `top`
+        likeliest tokens. One prompt pass, then the output projection row by row
+        (the logits that a decode step at that row would see) and one
+        ``launch_token_logprobs`` for SCORE_ROWS rows. Leaves the decoder as
+        ``prefill(ids)`` does."""
+
+        c = self.config
+        if ids.numel() < 2:
+            raise DecoderShellError("a text to score has at least two ids")
+        if not 0 <= top <= min(32, c.vocab):
+            raise DecoderShellError("top must be 0 to 32, at most the vocabulary")
+        self.reset()
+        ids, b = self._prefill(ids, 0)
+        rows = ids.numel() - 1
+        out = self._logprob_rows(rows, top)
+        logits = torch.empty((min(rows, SCORE_ROWS), c.vocab), dtype=torch.float32, device=self.device)
+        partials = torch.empty_like(self.proj_ws)  # proj_ws keeps the last row's
+        for first in range(0, rows, SCORE_ROWS):
+            n = min(SCORE_ROWS, rows - first)
+            for i in range(n):
+                ops.launch_output_projection(b.final[first + i], self.lm_head, logits=logits[i], workspace=partials)
+            ops.launch_token_logprobs(logits[:n], ids[first + 1:first + 1 + n], top=top,
+                                      out=ops.TokenLogprobs(*(x[first:first + n] for x in out)))
+        return out
+
+    def _logprob_rows(self, rows: int, top: int) -> ops.TokenLogprobs:
+        def empty(dtype, *shape):
+            return torch.empty(shape, dtype=dtype, device=self.device)
+
+        return ops.TokenLogprobs(empty(torch.float32, rows), empty(torch.float32, rows), empty(torch.int64, rows, top),
+                                 empty(torch.float32, rows, top))
+
+    def generate_greedy_scored(
+        self, prompt: torch.Tensor, max_new_tokens: int, *, top: int = 0, use_graph: bool = True
+    ) -> tuple[torch.Tensor, ops.TokenLogprobs]:
+        """``generate_greedy`` that also reports each chosen token's log
+        probability, the entropy of its step and the step's `top` likeliest
+        tokens (the chosen one first). Steps replay from the one-step graph: the
+        log probabilities read a step's logits before the next overwrites them."""
+
+        c = self.config
+        if not 0 <= top <= min(32, c.vocab):
+            raise DecoderShellError("top must be 0 to 32, at most the vocabulary")
+        self._check_generation(prompt, max_new_tokens)
+        graph = self._decode_graph() if use_graph else None
+        if not use_graph:
+            self._decode_bufs = self._decode_bufs or self._buffers(1)
+        out = self._logprob_rows(max_new_tokens, top)
+        workspace = torch.empty(ops.token_logprobs_workspace_bytes(1, c.vocab, top), dtype=torch.uint8, device=self.device)
+        self.reset()
+        self.prefill(prompt)
+        ops.launch_greedy_select(self.proj_ws, c.vocab, c.hidden, token_out=self.ids, history=self.history, step=self.step)
+        for i in range(max_new_tokens):
+            if i and graph is not None:
+                graph.replay()
+            elif i:
+                self._decode_body()
+            ops.launch_token_logprobs(self.logits.view(1, -1), self.ids, top=top, workspace=workspace,
+                                      out=ops.TokenLogprobs(*(x[i:i + 1] for x in out)))
+        self.host_position = int(prompt.numel()) + max_new_tokens - 1
+        return self.history[:max_new_tokens].clone(), out
+
+    def _check_generation(self, prompt: torch.Tensor, max_new_tokens: int) -> None:
+        if max_new_tokens < 1 or max_new_tokens > self.history.numel():
+            raise DecoderShellError("max_new_tokens outside the history capacity")
+        if int(prompt.numel()) + max_new_tokens - 1 > self.max_positions:
+            raise DecoderShellError("prompt plus generated tokens exceed the KV cache")
 
     def generate_greedy(
         self, prompt: torch.Tensor, max_new_tokens: int, *, use_graph: bool = True, timings: dict | None = None
@@ -502,11 +612,8 @@ class PackedDecoder:
         and their milliseconds are stored under "prefill_ms" / "decode_ms"
         (this synchronises once at the end)."""
 
-        if max_new_tokens < 1 or max_new_tokens > self.history.numel():
-            raise DecoderShellError("max_new_tokens outside the history capacity")
+        self._check_generation(prompt, max_new_tokens)
         t = int(prompt.numel())
-        if t + max_new_tokens - 1 > self.max_positions:
-            raise DecoderShellError("prompt plus generated tokens exceed the KV cache")
         steps = max_new_tokens - 1
         graph = self._decode_graph() if use_graph else None
         multi = self._decode_graph(STEPS_PER_GRAPH) if use_graph and steps >= STEPS_PER_GRAPH else None

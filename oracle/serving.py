@@ -17,6 +17,9 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.nn import functional as F
+
+from oracle import decoder_shell as ods
 
 MIN_EXPONENT = -126
 
@@ -152,3 +155,39 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int):
         ids.append(order[:top])
     ids = torch.tensor(ids, dtype=torch.int64).reshape(x.shape[0], top)
     return picked, entropy, ids, log_p.gather(1, ids)
+
+
+class PagedOracleDecoder(ods.OracleDecoder):
+    """``OracleDecoder`` whose KV cache is the 8-bit paged one: pages of `page`
+    rows in table order, appended call by call."""
+
+    def __init__(self, geometry, weights, *, max_positions: int, page: int) -> None:
+        self.page = page
+        super().__init__(geometry, weights, max_positions=max_positions)
+
+    def reset(self) -> None:
+        g, pages = self.g, -(-self.max_positions // self.page)
+        self.table = [list(range(pages))]
+        self.caches = [{"k": torch.zeros(pages, g.kv_heads, self.page, g.head_dim),
+                        "v": torch.zeros(pages, g.kv_heads, g.head_dim, self.page),
+                        "k_scales": torch.zeros(pages, g.kv_heads), "v_scales": torch.zeros(pages, g.kv_heads)}
+                       for _ in range(g.layers)]
+
+    def forward(self, ids: torch.Tensor, start: int) -> torch.Tensor:
+        g, w, t = self.g, self.w, ids.numel()
+        h = w.embed[ids.long()].float()
+        spans = [(0, t, start)]
+        for i, layer in enumerate(w.layers):
+            lin = self.linears[i]
+            x = ods.rms_norm(h, layer.input_norm, g.eps)
+            q, k, v = (lin[role](x).view(t, -1, g.head_dim) for role in ("q_proj", "k_proj", "v_proj"))
+            # q and k have norms of their own
+            kn = layer.k_norm
+            q = torch.stack([norm_rope(q[j], layer.q_norm, g.eps, self.cos[start + j], self.sin[start + j]) for j in range(t)])
+            _, self.caches[i] = append(k, k, v, self.caches[i], self.table, spans, page=self.page, q_norm=kn, k_norm=kn,
+                                       eps=g.eps, cos=self.cos, sin=self.sin)
+            attn, _, _ = attention(q, self.caches[i], self.table, spans, page=self.page, scaling=g.head_dim**-0.5)
+            h = h + lin["o_proj"](attn.reshape(t, -1).float())
+            x = ods.rms_norm(h, layer.post_norm, g.eps)
+            h = h + lin["down_proj"](F.silu(lin["gate_proj"](x)) * lin["up_proj"](x))
+        return ods.rms_norm(h, w.final_norm, g.eps) @ w.lm_head.float().T

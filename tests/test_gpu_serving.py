@@ -28,8 +28,12 @@ import pytest
 import torch
 
 from conftest import gpu_available
+from nanoquant_amd import synthetic as syn
 from nanoquant_amd.runtime import shell_ops as ops
+from nanoquant_amd.runtime.decoder_shell import PAGE_ROWS, DecoderShellConfig, DecoderShellError, PackedDecoder
+from oracle import decoder_shell as ods
 from oracle import serving as osv
+from oracle.nq_oracle import operands_from_state, relative_l2
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a HIP device")]
 
@@ -553,3 +557,77 @@ def test_work_on_another_stream():
     side.synchronize()
     assert torch.equal(here, there)
     assert torch.equal(lp.top_ids, ops.launch_token_logprobs(here.float(), torch.zeros(30, dtype=torch.int64, device=DEV), top=2).top_ids)
+
+
+# -- the decoder ---------------------------------------------------------------------
+
+SMALL = DecoderShellConfig(layers=3, hidden=256, intermediate=768, q_heads=4, kv_heads=2, head_dim=64, vocab=1000)
+
+
+def _decoder(act, **arguments):
+    weights = syn.synthetic_decoder(SMALL, seed=syn.BASE_SEED + 81, random_norms=True)
+    return weights, PackedDecoder(SMALL, weights, device=DEV, max_positions=150, activation_dtype=act,
+                                  cache_dtype=torch.float8_e4m3fn, **arguments)
+
+
+def test_decoder_with_the_8_bit_cache_matches_the_oracle():
+    """Logits against the oracle decoder with the same cache, teacher-forced. The
+    linears differ by 2e-5 relative, which moves about 16 * 2e-5 of the stored
+    values to the neighbouring e4m3 value, 1/8 away at most: sqrt(3.2e-4) / 8 =
+    2.2e-3 of K and of V, and over three layers sqrt(3) * 2 * 2.2e-3 = 8e-3."""
+
+    weights, decoder = _decoder(torch.float32)
+    prompt = torch.randint(0, SMALL.vocab, (70,), generator=_g(81))
+    tokens = decoder.generate_greedy(prompt.to(DEV), 8, use_graph=False).tolist()
+    geometry = ods.ShellGeometry(SMALL.layers, SMALL.hidden, SMALL.intermediate, SMALL.q_heads, SMALL.kv_heads,
+                                 SMALL.head_dim, SMALL.vocab, SMALL.eps, SMALL.rope_theta)
+    ow = ods.ShellWeights(weights.embed, weights.lm_head, weights.final_norm,
+                          [ods.LayerWeights(l.input_norm, l.post_norm, l.q_norm, l.k_norm,
+                                            {r: operands_from_state(st) for r, st in l.linears.items()})
+                           for l in weights.layers])
+    oracle = osv.PagedOracleDecoder(geometry, ow, max_positions=150, page=PAGE_ROWS)
+    expected = [oracle.forward(prompt, 0)[-1]]
+    for i, token in enumerate(tokens[:-1]):
+        expected.append(oracle.forward(torch.tensor([token]), 70 + i)[-1])
+    decoder.reset()
+    got = [decoder.prefill(prompt.to(DEV)).cpu().clone()]
+    for i, token in enumerate(tokens[:-1]):
+        got.append(decoder.prefill(torch.tensor([token]), start=70 + i).cpu().clone())
+    for step, (a, e) in enumerate(zip(got, expected)):
+        assert relative_l2(a, e) < 8e-3, step
+        assert int(a.argmax()) == tokens[step]
+
+
+@pytest.mark.parametrize("act", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fuse", [True, False])
+def test_decoder_with_the_8_bit_cache_graph_and_eager_agree(act, fuse):
+    _, decoder = _decoder(act, fuse_decode=fuse)
+    prompt = torch.randint(0, SMALL.vocab, (60,), generator=_g(82)).to(DEV)
+    eager = decoder.generate_greedy(prompt, 21, use_graph=False).tolist()
+    assert decoder.generate_greedy(prompt, 21).tolist() == eager
+    tokens, scores = decoder.generate_greedy_scored(prompt, 21, top=3)
+    assert tokens.tolist() == eager
+    eager_tokens, eager_scores = decoder.generate_greedy_scored(prompt, 21, top=3, use_graph=False)
+    assert eager_tokens.tolist() == eager
+    for a, b in zip(scores, eager_scores):
+        assert torch.equal(a, b)
+    assert torch.equal(scores.top_ids[:, 0], tokens)
+    assert torch.equal(scores.top_logprobs[:, 0], scores.logprobs)
+
+
+@pytest.mark.parametrize("cache", [torch.float8_e4m3fn, torch.float32])
+def test_decoder_scores_a_text_as_its_logits_do(cache):
+    weights = syn.synthetic_decoder(SMALL, seed=syn.BASE_SEED + 83, random_norms=True)
+    decoder = PackedDecoder(SMALL, weights, device=DEV, max_positions=300, activation_dtype=torch.float32, cache_dtype=cache)
+    ids = torch.randint(0, SMALL.vocab, (290,), generator=_g(83))
+    got = decoder.score(ids, top=5)
+    assert torch.equal(decoder.logits, decoder.prefill(ids))
+    logits = []
+    _, buffers = decoder._prefill(ids, 0)
+    for row in range(289):
+        logits.append(ops.launch_output_projection(buffers.final[row], decoder.lm_head)[0])
+    _check_logprobs(got, torch.stack(logits), ids[1:], 5)
+    with pytest.raises(DecoderShellError):
+        decoder.score(ids[:1])
+    with pytest.raises(DecoderShellError):
+        decoder.score(ids, top=33)
