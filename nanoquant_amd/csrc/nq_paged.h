@@ -35,29 +35,37 @@ struct Span {
     int begin, end;
 };
 
-__device__ __forceinline__ Span span_of(const Pages& p, int b) {
-    const int begin = min(max(p.starts[b], 0), p.tokens);
-    return {begin, min(max(p.starts[b + 1], begin), p.tokens)};
-}
+// A sequence with its span and the rows it had cached before the call.
+struct Found {
+    int b, context;
+    Span span;
+};
 
-// The last sequence b with first(b) <= slot, for a non-decreasing `first`
-// (sequence 0 when there is none). All lanes of a wave search together, 64
-// ways a round: one round of loads for up to 64 sequences, two for 4096. With
-// starts that are not in order some sequence comes out; its span decides
-// whether the slot names anything.
+// The last sequence b with first(b, its first token) <= slot, for a `first` that
+// does not decrease (sequence 0 when there is none). All lanes of a wave search
+// together, 64 ways a round; in the last round they load the sequences' ends
+// and contexts too, so up to 64 sequences take one round trip. With starts that
+// are not in order some sequence comes out; its span decides whether the slot
+// names anything.
 template <class First>
-__device__ __forceinline__ int sequence_at(int batch, int64_t slot, const First& first) {
+__device__ __forceinline__ Found sequence_at(const Pages& p, int64_t slot, const First& first) {
     const int lane = threadIdx.x & (kWave - 1);
-    int low = 0, count = batch;
-    while (count > 1) {
+    int low = 0, count = p.batch;
+    while (count > kWave) {
         const int step = (count + kWave - 1) / kWave;
-        const int at = lane * step;
-        const uint64_t below = __ballot(at < count && first(low + (at < count ? at : 0)) <= slot);
+        const int at = lane * step, b = low + (at < count ? at : 0);
+        const uint64_t below = __ballot(at < count && first(b, min(max(p.starts[b], 0), p.tokens)) <= slot);
         const int hit = below ? 63 - __builtin_clzll(below) : 0;
         low += hit * step;
         count = min(step, count - hit * step);
     }
-    return __builtin_amdgcn_readfirstlane(low);
+    const int b = low + (lane < count ? lane : 0);
+    const int start = p.starts[b], stop = p.starts[b + 1], context = p.contexts[b];
+    const int begin = min(max(start, 0), p.tokens), end = min(max(stop, begin), p.tokens);
+    const uint64_t below = __ballot(lane < count && first(b, begin) <= slot);
+    const int hit = below ? 63 - __builtin_clzll(below) : 0;
+    return {__builtin_amdgcn_readfirstlane(low + hit), __builtin_amdgcn_readlane(context, hit),
+            {__builtin_amdgcn_readlane(begin, hit), __builtin_amdgcn_readlane(end, hit)}};
 }
 
 // A token's cache row: its sequence's context plus its place, or -1 outside

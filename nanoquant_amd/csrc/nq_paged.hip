@@ -176,9 +176,9 @@ __global__ __launch_bounds__(WAVES* kWave) void k_paged_append(const AppendArgs 
         const int item = blockIdx.x - a.kv_blocks, token = item / a.q_groups;
         const int head = ((item - token * a.q_groups) * WAVES + wave) * 2;
         if (head >= a.q_heads) return;
-        const int b = sequence_at(p.batch, token, [&](int i) { return static_cast<int64_t>(span_of(p, i).begin); });
-        const Span s = span_of(p, b);
-        const int row = token >= s.begin && token < s.end ? row_of(p.contexts[b], token - s.begin, rows) : -1;
+        const Found f = sequence_at(p, token, [](int, int begin) { return static_cast<int64_t>(begin); });
+        const Span s = f.span;
+        const int row = token >= s.begin && token < s.end ? row_of(f.context, token - s.begin, rows) : -1;
         if (row < 0 || row >= a.rope_rows) return;
         load_weight<D>(a.q_norm, a.norm_dtype, lane, w);
         load_rope_row<D>(a, row, lane, cs, sn);
@@ -195,18 +195,19 @@ __global__ __launch_bounds__(WAVES* kWave) void k_paged_append(const AppendArgs 
     }
 
     const int slot = blockIdx.x / p.kv_heads, g = blockIdx.x - slot * p.kv_heads, page = 1 << p.page_shift;
-    const auto first_slot = [&](int i) {
-        return static_cast<int64_t>(span_of(p, i).begin >> p.page_shift) + 2 * static_cast<int64_t>(i);
+    const auto first_slot = [&](int i, int begin) {
+        return static_cast<int64_t>(begin >> p.page_shift) + 2 * static_cast<int64_t>(i);
     };
-    const int b = sequence_at(p.batch, slot, first_slot);
-    const Span s = span_of(p, b);
-    const int context = p.contexts[b];
+    const Found f = sequence_at(p, slot, first_slot);
+    const Span s = f.span;
+    const int b = f.b, context = f.context;
+    const int64_t slot0 = first_slot(b, s.begin);
     // New rows of the sequence that have a place: positions [low, high).
     const int64_t low = max(static_cast<int64_t>(context), int64_t{0});
     const int64_t high = min(static_cast<int64_t>(context) + (s.end - s.begin), static_cast<int64_t>(min(rows, a.rope_rows)));
-    const int64_t nth = (low >> p.page_shift) + (slot - first_slot(b));
+    const int64_t nth = (low >> p.page_shift) + (slot - slot0);
     const int64_t begin = max(low, nth << p.page_shift), end = min(high, (nth + 1) << p.page_shift);
-    if (slot < first_slot(b) || begin >= end) return;
+    if (slot < slot0 || begin >= end) return;
     const int32_t id = p.table[static_cast<int64_t>(b) * p.table_pages + nth];
     if (id < 0 || id >= p.pages) return;
     const int r0 = static_cast<int>(begin) & (page - 1), n = static_cast<int>(end - begin);

@@ -2,13 +2,13 @@
 //
 // A query row is one (token, q head) of a kv head's group: row r of a sequence
 // is token r / group, head r % group, so that the rows which share a kv head
-// fill the 16 columns of v_mfma_f32_16x16x32_bf16 whatever the group. Per 64
+// fill the 16 columns of v_mfma_f32_16x16x32_bf16 whatever the group. Per TILE
 // cache rows a wave forms S^T = K Q^T (A = 16 cache rows, B = 16 query rows),
 // a running softmax over its columns, and O^T += V^T P^T. S^T leaves a lane
-// with 16 cache rows of one query row; assigning cache row 16 g + 4 t + i to
-// row 4 g + i of the t-th score tile makes them 16 consecutive rows, which is
+// with TILE / 4 cache rows of one query row; assigning cache row TILE / 4 g + 4 t
+// + i to row 4 g + i of the t-th score tile makes them consecutive rows, which is
 // what the second product's B operand wants, so P never leaves its registers.
-// V lies transposed in the cache, so its A operand is 16 consecutive bytes.
+// V lies transposed in the cache, so its A operand is as many consecutive bytes.
 //
 // Precision: an e4m3 byte is exact in bf16. q enters as one bf16 part, two or
 // three (bf16 / fp16 / fp32: 8, 16, 24 bits: exact), so scores carry fp32
@@ -27,7 +27,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTile = 64;  // cache rows a wave takes at once
+constexpr int kTile = 64;  // cache rows that splits are counted in
 
 struct AttnArgs {
     Pages p;
@@ -46,18 +46,17 @@ struct SlotSpan {
     int visible;            // cache rows [0, visible) that some row of the slot sees
 };
 
-__device__ __forceinline__ int64_t first_slot_of(const Pages& p, int b, int group, int rows) {
-    return static_cast<int64_t>(span_of(p, b).begin) * group / rows + b;
+__device__ __forceinline__ int64_t first_slot_of(int b, int begin, int group, int rows) {
+    return static_cast<int64_t>(begin) * group / rows + b;
 }
 
-__device__ __forceinline__ SlotSpan slot_span(const Pages& p, int b, int64_t slot, int group, int rows) {
-    const Span s = span_of(p, b);
+__device__ __forceinline__ SlotSpan slot_span(const Pages& p, const Found& f, int64_t slot, int group, int rows) {
     SlotSpan o;
-    o.b = b;
-    o.begin = s.begin;
-    o.context = p.contexts[b];
-    const int64_t row0 = (slot - first_slot_of(p, b, group, rows)) * rows;
-    const int64_t all = static_cast<int64_t>(s.end - s.begin) * group;
+    o.b = f.b;
+    o.begin = f.span.begin;
+    o.context = f.context;
+    const int64_t row0 = (slot - first_slot_of(f.b, f.span.begin, group, rows)) * rows;
+    const int64_t all = static_cast<int64_t>(f.span.end - f.span.begin) * group;
     o.row0 = static_cast<int>(row0 < 0 || row0 >= all ? 0 : row0);
     o.rows = static_cast<int>(row0 < 0 || row0 >= all ? 0 : min(static_cast<int64_t>(rows), all - row0));
     const int64_t last = static_cast<int64_t>(o.context) + (o.row0 + o.rows - 1) / group;
@@ -194,31 +193,45 @@ __device__ __forceinline__ void store4(void* out, int dtype, int64_t at, const f
         *reinterpret_cast<f32x4*>(static_cast<float*>(out) + at) = f32x4{v[0], v[1], v[2], v[3]};
         return;
     }
-    uint16_t h[4];
+    uint32_t w[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        h[i] = dtype == NQ_DTYPE_BF16 ? nq::f32_to_bf16_bits(v[i])
-                                      : __builtin_bit_cast(uint16_t, static_cast<_Float16>(v[i]));
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) =
-        make_uint2(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16));
+    for (int i = 0; i < 2; ++i) {
+        if (dtype == NQ_DTYPE_BF16) {
+            const bf16x2 h = {static_cast<__bf16>(v[2 * i]), static_cast<__bf16>(v[2 * i + 1])};
+            w[i] = __builtin_bit_cast(uint32_t, h);
+        } else {
+            typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+            const f16x2 h = {static_cast<_Float16>(v[2 * i]), static_cast<_Float16>(v[2 * i + 1])};
+            w[i] = __builtin_bit_cast(uint32_t, h);
+        }
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = make_uint2(w[0], w[1]);
 }
+
+// Waves of a SIMD that the registers are held to.
+template <int D>
+constexpr int kWavesFor = D == 256 ? 1 : 2;
+template <int D>
+constexpr int kTileFor = D == 256 ? 32 : 64;
 
 // One workgroup of four waves: a slot of query rows of one kv head over one
 // split of the cache. SHARED: the waves hold the same 16 NT rows and take the
 // split's tiles in turn (few query rows: the cache's bytes are the work);
 // otherwise each wave holds 16 NT rows of its own and all take every tile.
-template <int D, int QP, int PP, int NT, bool SHARED>
-__global__ __launch_bounds__(256, 1) void k_paged_attention(const AttnArgs a) {
+template <int D, int QP, int PP, int NT, int TILE, bool SHARED>
+__global__ __launch_bounds__(256, kWavesFor<D>) void k_paged_attention(const AttnArgs a) {
     constexpr int kRows = (SHARED ? 1 : 4) * 16 * NT;
     constexpr int kChunks = D / 64, kDims = D / 16;
+    constexpr int kBlock = TILE / 4;   // consecutive cache rows of a lane: of V, and of the scores
+    constexpr int kScores = TILE / 16, kSteps = TILE / 32, kWords = kBlock / 4;
     const Pages& p = a.p;
     const int lane = threadIdx.x & (kWave - 1), n = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int g = blockIdx.x % p.kv_heads;
     const int rest = blockIdx.x / p.kv_heads;
     const int split = rest % a.splits, slot = rest / a.splits;
-    const int b = sequence_at(p.batch, slot, [&](int i) { return first_slot_of(p, i, a.group, kRows); });
-    const SlotSpan s = slot_span(p, b, slot, a.group, kRows);
+    const Found found = sequence_at(p, slot, [&](int i, int begin) { return first_slot_of(i, begin, a.group, kRows); });
+    const SlotSpan s = slot_span(p, found, slot, a.group, kRows);
     if (s.rows == 0) return;
     const int page = 1 << p.page_shift, cache_rows = p.table_pages << p.page_shift;
     const SplitPlan plan = split_plan(s.visible, a.splits, a.least);
@@ -261,38 +274,75 @@ __global__ __launch_bounds__(256, 1) void k_paged_attention(const AttnArgs a) {
         for (int d = 0; d < kDims; ++d) acc[d][t] = f32x4{0, 0, 0, 0};
     }
 
-    const int tile_end = min((split + 1) * plan.per, min(plan.tiles, (high_pos + kTile) / kTile));
+    const int tile_end = min((split + 1) * plan.per * (kTile / TILE), (min(high_pos + 1, s.visible) + TILE - 1) / TILE);
     const int step = SHARED ? 4 : 1;
-    for (int tile = split * plan.per + (SHARED ? wave : 0); tile < tile_end; tile += step) {
-        const int base = tile * kTile;
-        // Pages of this lane's blocks of 16 rows: block n / 4 for K, grp for
-        // the scores' scales and for V. Blocks that no query sees and entries
-        // that name no page read page 0; the latter with a scale of NaN.
-        const auto page_of = [&](int block, bool& bad) {
-            const int first = base + 16 * block;
-            int id = 0;
-            if (first < s.visible) id = p.table[static_cast<int64_t>(s.b) * p.table_pages + (first >> p.page_shift)];
-            bad = id < 0 || id >= p.pages;
-            return static_cast<int64_t>(bad ? 0 : id) * p.kv_heads + g;
-        };
-        bool bad_k, bad;
-        const int64_t k_page = page_of(n >> 2, bad_k), v_page = page_of(grp, bad);
-        const float ks = bad ? __builtin_nanf("") : p.k_scales[v_page] * a.scale;
-        const float vs = bad ? __builtin_nanf("") : p.v_scales[v_page];
-        const uint8_t* k_at = p.k + (k_page * page + ((base + 16 * (n >> 2)) & (page - 1)) + (n & 3)) * D + 16 * grp;
-        const uint8_t* v_at = p.v + (v_page * D + n) * page + ((base + 16 * grp) & (page - 1));
-        u32x4 kf[4][kChunks], vf[kDims];
+    const int tile_begin = split * plan.per * (kTile / TILE) + (SHARED ? wave : 0);
+    // Table entries of this lane's blocks of kBlock rows: block n / 4 for K, grp
+    // for the scores' scales and for V. What no query sees takes the last entry
+    // in use. All loads of the loop are unconditional and in one order (entries,
+    // scales, K, V), or a wait for the oldest becomes a wait for all: behind the
+    // last tile they read that tile again, from the L2.
+    const int32_t* table = p.table + static_cast<int64_t>(s.b) * p.table_pages;
+    const int last_row = max(s.visible - 1, 0);
+    const auto page_at = [&](int tile, int block) { return table[min(tile * TILE + kBlock * block, last_row) >> p.page_shift]; };
+    // An entry that names no page reads page 0 too, with a scale of NaN.
+    const auto base_of = [&](int id) {
+        return static_cast<int64_t>(static_cast<uint32_t>(id) < static_cast<uint32_t>(p.pages) ? id : 0) * p.kv_heads + g;
+    };
+    u32x4 kf[kScores][kChunks];
+    uint32_t vf[kDims][kWords];
+    float k_scale = 0.0f, v_scale = 0.0f;
+    const auto load_scales = [&](int id) {
+        const int64_t at = base_of(id);
+        k_scale = p.k_scales[at];
+        v_scale = p.v_scales[at];
+    };
+    const auto load_k = [&](int tile, int id) {
+        const uint8_t* at = p.k + (base_of(id) * page + ((tile * TILE + kBlock * (n >> 2)) & (page - 1)) + (n & 3)) * D + 16 * grp;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < kScores; ++t)
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c)
-                kf[t][c] = *reinterpret_cast<const u32x4*>(k_at + 4 * t * D + 64 * c);
+            for (int c = 0; c < kChunks; ++c) kf[t][c] = *reinterpret_cast<const u32x4*>(at + 4 * t * D + 64 * c);
+    };
+    const auto load_v = [&](int tile, int id) {
+        const uint8_t* at = p.v + (base_of(id) * D + n) * page + ((tile * TILE + kBlock * grp) & (page - 1));
 #pragma unroll
-        for (int d = 0; d < kDims; ++d) vf[d] = *reinterpret_cast<const u32x4*>(v_at + static_cast<int64_t>(16 * d) * page);
+        for (int d = 0; d < kDims; ++d) {
+            typedef uint32_t words __attribute__((ext_vector_type(kWords)));
+            const words w = *reinterpret_cast<const words*>(at + static_cast<int64_t>(16 * d) * page);
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) vf[d][i] = w[i];
+        }
+    };
+    // K and V of the next tile are on their way while this one is worked on,
+    // their table entries a tile ahead of that.
+    int id_k = page_at(tile_begin, n >> 2), id_v = page_at(tile_begin, grp);
+    int next_k = page_at(tile_begin + step, n >> 2), next_v = page_at(tile_begin + step, grp);
+    if (tile_begin < tile_end) {
+        load_scales(id_v);
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(tile_begin, id_k);
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(tile_begin, id_v);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    for (int tile = tile_begin; tile < tile_end; tile += step) {
+        const int base = tile * TILE;
+        const bool more = tile + step < tile_end;
+        const int then = more ? tile + step : tile;
+        const bool bad = static_cast<uint32_t>(id_v) >= static_cast<uint32_t>(p.pages);
+        const float ks = bad ? __builtin_nanf("") : k_scale * a.scale, vs = bad ? __builtin_nanf("") : v_scale;
+        if (more) {
+            id_k = next_k;
+            id_v = next_v;
+        }
+        next_k = page_at(tile + 2 * step, n >> 2);
+        next_v = page_at(tile + 2 * step, grp);
+        __builtin_amdgcn_sched_barrier(0);
 
-        f32x4 sc[4][NT];
+        f32x4 sc[kScores][NT];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < kScores; ++t) {
 #pragma unroll
             for (int u = 0; u < NT; ++u) sc[t][u] = f32x4{0, 0, 0, 0};
 #pragma unroll
@@ -308,37 +358,44 @@ __global__ __launch_bounds__(256, 1) void k_paged_attention(const AttnArgs a) {
             }
         }
 
-        const bool masked = base + kTile > low_pos + 1;  // uniform: some row of the wave does not see all 64
+        __builtin_amdgcn_sched_barrier(0);
+        load_scales(id_v);
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(then, id_k);
+        __builtin_amdgcn_sched_barrier(0);
+
+        const bool masked = base + TILE > low_pos + 1;  // uniform: some row of the wave does not see them all
         if (masked) {
             // Bytes of V rows that nobody sees may be anything. Among those
             // that only some see, a NaN must not meet a weight of zero: it is
             // taken out and given back to the queries that do see its row.
-            const int seen_rows = high_pos + 1 - (base + 16 * grp);
+            const int seen_rows = high_pos + 1 - (base + kBlock * grp);
             uint32_t any = 0;
 #pragma unroll
             for (int d = 0; d < kDims; ++d)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < kWords; ++i) {
                     vf[d][i] &= first_bytes(seen_rows, i);
                     any |= nan_bytes(vf[d][i]);
                 }
             if (__ballot(any != 0)) {
 #pragma unroll
                 for (int u = 0; u < NT; ++u) {
-                    bf16x8 see[2];
+                    bf16x8 see[kSteps];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < kSteps; ++h)
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
-                            see[h][j] = static_cast<__bf16>(base + 16 * grp + 8 * h + j <= pos[u] ? 1.0f : 0.0f);
+                            see[h][j] = static_cast<__bf16>(base + kBlock * grp + 8 * h + j <= pos[u] ? 1.0f : 0.0f);
 #pragma unroll
                     for (int d = 0; d < kDims; ++d) {
-                        uint32_t one[4];  // e4m3 1.0 where V holds NaN
+                        uint32_t one[kWords];  // e4m3 1.0 where V holds NaN
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) one[i] = (nan_bytes(vf[d][i]) >> 7) * 0x38u;
+                        for (int i = 0; i < kWords; ++i) one[i] = (nan_bytes(vf[d][i]) >> 7) * 0x38u;
                         f32x4 hits = {0, 0, 0, 0};
-                        hits = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(one[0], one[1]), see[0], hits, 0, 0, 0);
-                        hits = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(one[2], one[3]), see[1], hits, 0, 0, 0);
+#pragma unroll
+                        for (int h = 0; h < kSteps; ++h)
+                            hits = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(one[2 * h], one[2 * h + 1]), see[h], hits, 0, 0, 0);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             if (hits[i] > 0.0f) acc[d][u][i] = __builtin_nanf("");
@@ -347,17 +404,17 @@ __global__ __launch_bounds__(256, 1) void k_paged_attention(const AttnArgs a) {
 #pragma unroll
                 for (int d = 0; d < kDims; ++d)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) vf[d][i] &= ~((nan_bytes(vf[d][i]) >> 7) * 0xffu);
+                    for (int i = 0; i < kWords; ++i) vf[d][i] &= ~((nan_bytes(vf[d][i]) >> 7) * 0xffu);
             }
         }
 
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-            float x[16], top = -INFINITY;
+            float x[kBlock], top = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
+            for (int j = 0; j < kBlock; ++j) {
                 x[j] = sc[j >> 2][u][j & 3] * ks;
-                if (masked) x[j] = base + 16 * grp + j <= pos[u] ? x[j] : -INFINITY;
+                if (masked) x[j] = base + kBlock * grp + j <= pos[u] ? x[j] : -INFINITY;
                 top = fmaxf(top, x[j]);
             }
             const float m_new = fmaxf(m_run[u], rows_max(top));
@@ -372,16 +429,16 @@ __global__ __launch_bounds__(256, 1) void k_paged_attention(const AttnArgs a) {
             }
             float sum = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
+            for (int j = 0; j < kBlock; ++j) {
                 x[j] = exp2_hw(x[j] - m_use);
                 sum += x[j];
                 x[j] *= vs;
-                if (masked) x[j] = base + 16 * grp + j <= pos[u] ? x[j] : 0.0f;  // a scale that nobody sees may be anything
+                if (masked) x[j] = base + kBlock * grp + j <= pos[u] ? x[j] : 0.0f;  // a scale that nobody sees may be anything
             }
             l_run[u] += sum;
-            bf16x8 pf[2][PP];
+            bf16x8 pf[kSteps][PP];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < kSteps; ++h) {
                 float y[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) y[j] = x[8 * h + j];
@@ -389,14 +446,18 @@ __global__ __launch_bounds__(256, 1) void k_paged_attention(const AttnArgs a) {
             }
 #pragma unroll
             for (int d = 0; d < kDims; ++d) {
-                const bf16x8 v0 = widen(vf[d][0], vf[d][1]), v1 = widen(vf[d][2], vf[d][3]);
 #pragma unroll
-                for (int s2 = PP - 1; s2 >= 0; --s2) {
-                    acc[d][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pf[0][s2], acc[d][u], 0, 0, 0);
-                    acc[d][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pf[1][s2], acc[d][u], 0, 0, 0);
+                for (int h = 0; h < kSteps; ++h) {
+                    const bf16x8 v = widen(vf[d][2 * h], vf[d][2 * h + 1]);
+#pragma unroll
+                    for (int s2 = PP - 1; s2 >= 0; --s2)
+                        acc[d][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pf[h][s2], acc[d][u], 0, 0, 0);
                 }
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(then, id_v);
+        __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int u = 0; u < NT; ++u) l_run[u] = rows_sum(l_run[u]);
@@ -445,11 +506,12 @@ __global__ __launch_bounds__(256, 1) void k_paged_attention(const AttnArgs a) {
     for (int u = 0; u < NT; ++u) {
         if (row[u] >= s.rows) continue;
         if (plan.active <= 1) {
+            const float inv = 1.0f / l_run[u];
 #pragma unroll
             for (int d = 0; d < kDims; ++d) {
                 float v[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = pos[u] < 0 ? 0.0f : acc[d][u][i] / l_run[u];
+                for (int i = 0; i < 4; ++i) v[i] = pos[u] < 0 ? 0.0f : acc[d][u][i] * inv;
                 store4(a.out, a.out_dtype, out_at[u] + 16 * d + 4 * grp, v);
             }
         } else {
@@ -480,9 +542,9 @@ int launch_attention_as(const AttnArgs& a, const AttnPlan& plan, hipStream_t str
     if (blocks > 0x7fffffff) return NQ_ERR_SHAPE;
     const dim3 grid(static_cast<unsigned>(blocks));
     if (plan.shared) {
-        hipLaunchKernelGGL((k_paged_attention<D, QP, PP, 1, true>), grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_paged_attention<D, QP, PP, 1, kTileFor<D>, true>), grid, dim3(256), 0, stream, a);
     } else {
-        hipLaunchKernelGGL((k_paged_attention<D, QP, PP, 1, false>), grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_paged_attention<D, QP, PP, 1, kTileFor<D>, false>), grid, dim3(256), 0, stream, a);
     }
     return nq::launch_status();
 }

@@ -15,61 +15,81 @@ namespace {
 
 using namespace nq::paged;
 
-// One wave per token and q head: the splits' results, in split order.
+// One workgroup per token and q head: its waves take the splits in turn, eight
+// loads in flight, and meet in LDS.
 template <int D>
 __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows) {
-    constexpr int E = D / kWave;
+    constexpr int E = D / kWave, kWaves = 4, kMost = 2;  // kMost: 64 splits each
+    __shared__ float join[kWaves][D], weights[kMost * kWave];
     const Pages& p = a.p;
     const int lane = threadIdx.x & (kWave - 1);
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int token = static_cast<int>(item / a.q_heads), head = static_cast<int>(item % a.q_heads);
-    if (token >= p.tokens) return;
-    const int b = sequence_at(p.batch, token, [&](int i) { return static_cast<int64_t>(span_of(p, i).begin); });
-    const Span span = span_of(p, b);
-    if (token < span.begin || token >= span.end) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int token = blockIdx.x / a.q_heads, head = blockIdx.x - token * a.q_heads;
+    const Found f = sequence_at(p, token, [](int, int begin) { return static_cast<int64_t>(begin); });
+    if (token < f.span.begin || token >= f.span.end) return;
     const int g = head / a.group;
-    const int r = (token - span.begin) * a.group + head - g * a.group;
-    const int64_t slot = first_slot_of(p, b, a.group, rows) + r / rows;
-    const SlotSpan s = slot_span(p, b, slot, a.group, rows);
+    const int64_t r = static_cast<int64_t>(token - f.span.begin) * a.group + head - g * a.group;
+    const int64_t slot = first_slot_of(f.b, f.span.begin, a.group, rows) + r / rows;
+    const SlotSpan s = slot_span(p, f, slot, a.group, rows);
     const SplitPlan plan = split_plan(s.visible, a.splits, a.least);
     if (plan.active <= 1) return;  // the attention wrote the output itself
     const int64_t first = (slot * a.splits * p.kv_heads + g) * rows + r % rows;
     const int64_t next = static_cast<int64_t>(p.kv_heads) * rows;  // from one split's row to the next split's
-    float m = -INFINITY;
-    for (int i = lane; i < plan.active; i += kWave) m = fmaxf(m, a.partial[2 * (first + i * next)]);
+    float w[kMost], l[kMost], m = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kMost; ++c) {
+        const int i = lane + kWave * c;
+        const bool on = i < plan.active;
+        w[c] = on ? a.partial[2 * (first + i * next)] : -INFINITY;
+        l[c] = on ? a.partial[2 * (first + i * next) + 1] : 0.0f;
+        m = fmaxf(m, w[c]);
+    }
 #pragma unroll
     for (int k = 1; k < kWave; k *= 2) m = fmaxf(m, __shfl_xor(m, k, kWave));
     const float m_use = m == -INFINITY ? 0.0f : m;
     float sum = 0.0f, o[E];
 #pragma unroll
-    for (int j = 0; j < E; ++j) o[j] = 0.0f;
-    for (int i = 0; i < plan.active; ++i) {
-        const int64_t at = first + i * next;
-        const float w = exp2_hw(a.partial[2 * at] - m_use);
-        sum += w * a.partial[2 * at + 1];
-#pragma unroll
-        for (int j = 0; j < E; ++j) o[j] += w * a.partial_o[at * D + lane + kWave * j];
+    for (int c = 0; c < kMost; ++c) {
+        w[c] = exp2_hw(w[c] - m_use);
+        if (wave == 0) weights[lane + kWave * c] = w[c];
+        sum += w[c] * l[c];
     }
-    const bool off = row_of(s.context, token - span.begin, p.table_pages << p.page_shift) < 0;
 #pragma unroll
-    for (int j = 0; j < E; ++j)
-        nq::store_f32_as(a.out, a.out_dtype, item * D + lane + kWave * j, off ? 0.0f : o[j] / sum);
+    for (int k = 1; k < kWave; k *= 2) sum += __shfl_xor(sum, k, kWave);
+#pragma unroll
+    for (int j = 0; j < E; ++j) o[j] = 0.0f;
+    __syncthreads();
+#pragma unroll 8
+    for (int i = wave; i < plan.active; i += kWaves) {
+        const float weight = weights[i];
+        const float* at = a.partial_o + (first + i * next) * D + lane;
+#pragma unroll
+        for (int j = 0; j < E; ++j) o[j] += weight * at[kWave * j];
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) join[wave][lane + kWave * j] = o[j];
+    __syncthreads();
+    const bool off = row_of(s.context, token - s.begin, p.table_pages << p.page_shift) < 0;
+    for (int d = threadIdx.x; d < D; d += kWaves * kWave) {
+        const float all = (join[0][d] + join[1][d]) + (join[2][d] + join[3][d]);
+        nq::store_f32_as(a.out, a.out_dtype, static_cast<int64_t>(blockIdx.x) * D + d, off ? 0.0f : all / sum);
+    }
 }
 
 // Few query rows to a sequence: a slot of 16 rows whose waves share them, and
 // the cache split until the chip has about two workgroups to a CU; more: slots
 // of 64 rows, 16 to a wave.
 AttnPlan plan_attention(int64_t tokens, int64_t batch, int q_heads, int kv_heads, int64_t cache_rows) {
-    constexpr int64_t kWorkgroups = 512;
     AttnPlan plan;
     const int64_t rows = tokens * (q_heads / kv_heads);
     plan.shared = rows <= 16 * batch;
     plan.rows = plan.shared ? 16 : 64;
     plan.slots = static_cast<int>(rows / plan.rows + batch);
-    plan.least = plan.shared ? 4 : 8;
-    const int64_t tiles = (cache_rows + kTile - 1) / kTile;
-    int64_t splits = kWorkgroups / (static_cast<int64_t>(plan.slots) * kv_heads);
+    const int64_t tiles = (cache_rows + kTile - 1) / kTile, units = static_cast<int64_t>(plan.slots) * kv_heads;
+    const int64_t target = batch > 1 ? 1024 : 512;
+    plan.least = plan.shared && units * ((tiles + 7) / 8) < 512 ? 4 : 8;
     const int64_t most = (tiles + plan.least - 1) / plan.least;
+    int64_t splits = target / units;
     splits = splits < most ? splits : most;
     plan.splits = static_cast<int>(splits < 1 ? 1 : (splits > 128 ? 128 : splits));
     return plan;
@@ -87,7 +107,7 @@ extern "C" int64_t nq_paged_attention_workspace_bytes(int64_t tokens, int64_t ba
         q_heads > 65535 || q_heads % kv_heads || page_size <= 0 || page_size > 128 || table_pages <= 0 ||
         table_pages > 0x7fffffff / page_size || (head_dim != 64 && head_dim != 128 && head_dim != 256))
         return -1;
-    if (tokens * (q_heads / kv_heads) > 0x3fffffff) return -1;
+    if (tokens * q_heads > 0x3fffffff) return -1;
     const AttnPlan plan = plan_attention(tokens, batch, q_heads, kv_heads, table_pages * page_size);
     return partial_rows(plan, kv_heads) * (2 + head_dim) * static_cast<int64_t>(sizeof(float));
 }
@@ -127,7 +147,7 @@ extern "C" int nq_paged_attention(const void* q, int32_t q_dtype, int64_t tokens
         default: status = launch_paged_attention<256>(a, plan, q_dtype, st); break;
     }
     if (status != NQ_OK || plan.splits <= 1) return status;
-    const dim3 grid(static_cast<unsigned>((tokens * q_heads + 3) / 4));
+    const dim3 grid(static_cast<unsigned>(tokens * q_heads));
     switch (kv->head_dim) {
         case 64: hipLaunchKernelGGL(k_paged_merge<64>, grid, dim3(256), 0, st, a, plan.rows); break;
         case 128: hipLaunchKernelGGL(k_paged_merge<128>, grid, dim3(256), 0, st, a, plan.rows); break;
