@@ -242,7 +242,7 @@ int nq_paged_attention(const void* q, int32_t q_dtype, int64_t tokens, int32_t q
                        float scaling, void* out, int32_t out_dtype, void* workspace, int64_t workspace_bytes,
                        void* stream);
 
-/* Workspace bytes of nq_token_logprobs. */
+/* Workspace bytes of nq_token_logprobs (0: none needed). */
 int64_t nq_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top);
 
 /* For each row of logits (F32/F16/BF16, row_stride >= vocab elements apart):
@@ -250,8 +250,7 @@ int64_t nq_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t t
  *   entropy[r]  = -sum p log p over the row, 0 log 0 = 0
  *   top_ids[r, :], top_logprobs[r, :] = the `top` likeliest tokens, likeliest first,
  *     the lowest index first among equals, NaN above all
- * top 0 to 32 (top_ids and top_logprobs may be NULL for 0), vocab up to about a
- * million. Logits of -inf have probability 0; a row that holds NaN or +inf, or
+ * top 0 to 32 (top_ids and top_logprobs may be NULL for 0). Logits of -inf have probability 0; a row that holds NaN or +inf, or
  * -inf alone, has NaN for every log probability and for the entropy. Beside
  * nq_greedy_select for callers that report how likely an answer is; the
  * reference's engine returns tokens alone (src/nanoquant/runtime/generation.py:240-246). */

@@ -1,14 +1,14 @@
 // Log probability of given tokens, entropy of the distribution and its top
-// alternatives from rows of logits.
+// alternatives from rows of logits, in one read.
 //
-// One read of the logits. A workgroup takes a part of a row: each of its four
-// waves keeps 64 V values in registers, with m their maximum sums e^(x - m) and
-// e^(x - m) (x - m), and picks its top k from the registers; the four lists meet
-// in LDS. A second launch, one wave to a row, joins the parts: with M the
-// largest m,
-//   lse = M + log S, S = sum of S_p e^(m_p - M)
-//   log p(t) = x_t - lse, entropy = log S - T / S, T = sum of (T_p + S_p (m_p - M)) e^(m_p - M)
-// in fp64, rounded once.
+// A workgroup of four waves takes a part of a row, all of it where there are rows
+// enough. A lane keeps its own running maximum m and, relative to it, s = sum
+// e^(x - m) and t = sum e^(x - m) (x - m); the next 64 x 16 values of its wave
+// are on their way while these are worked on. With M the largest of the maxima,
+//   lse = M + log S, S = sum s e^(m - M)
+//   log p(x) = x - lse, entropy = log S - T / S, T = sum (t + s (m - M)) e^(m - M)
+// rounded once from fp64; a row's parts meet in a second launch. Each wave keeps its k largest values in LDS; a block of values costs one
+// comparison unless some value is above the smallest of them.
 #include <math.h>
 
 #include "nq_common.h"
@@ -19,16 +19,19 @@ namespace {
 constexpr int kWave = 64;
 constexpr int kWaves = 4;
 constexpr int kMostTop = 32;
-constexpr int kMostParts = 128;  // of a row: two to a lane of the joining wave
+constexpr int kRoom = kWave;  // values that a list takes in at once
+constexpr int kValues = 16;   // of a lane at once
+constexpr int kMostParts = 64;  // of a row: one to a lane of the joining wave
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
 
 struct Args {
     const void* logits;
     const int64_t* tokens;
     int64_t row_stride;
     int32_t vocab, top, parts;
-    float* sums;      // [rows][parts][4]: m, S, T
-    uint64_t* lists;  // [rows][parts][top]: keys, largest first, 0 where there is none
+    float* sums;       // [rows][parts][4]: M, S, T of a part (parts > 1)
+    uint64_t* lists;   // [rows][parts][top]: its keys, largest first, 0 where there is none
     float *logprobs, *entropy, *top_logprobs;
     int64_t* top_ids;
 };
@@ -50,16 +53,30 @@ __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t index) {
     return order ? (static_cast<uint64_t>(order) << 32) | (0xffffffffu - index) : 0;
 }
 
+// Wave reductions with DPP row operations and four lane reads, in a fixed order.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x, float identity) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(identity), __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+
+__device__ __forceinline__ float lane_of(float v, int lane) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int m = 1; m < kWave; m *= 2) v = fmaxf(v, __shfl_xor(v, m, kWave));
-    return v;
+    v = fmaxf(v, dpp<0xB1>(v, -INFINITY));   // quad_perm [1,0,3,2]
+    v = fmaxf(v, dpp<0x4E>(v, -INFINITY));   // quad_perm [2,3,0,1]
+    v = fmaxf(v, dpp<0x141>(v, -INFINITY));  // row_half_mirror
+    v = fmaxf(v, dpp<0x140>(v, -INFINITY));  // row_mirror
+    return fmaxf(fmaxf(lane_of(v, 0), lane_of(v, 16)), fmaxf(lane_of(v, 32), lane_of(v, 48)));
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int m = 1; m < kWave; m *= 2) v += __shfl_xor(v, m, kWave);
-    return v;
+    v += dpp<0xB1>(v, 0.0f);
+    v += dpp<0x4E>(v, 0.0f);
+    v += dpp<0x141>(v, 0.0f);
+    v += dpp<0x140>(v, 0.0f);
+    return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
@@ -81,307 +98,420 @@ __device__ __forceinline__ int lanes_before(uint64_t mask) {
 template <int DT>
 __device__ __forceinline__ float element(const void* p, int64_t i) { return nq::load_f32(p, DT, i); }
 
-// The wave's top k of its values key[V] (0: none) into list[0, k), largest
-// first. Element e of lane l has index first + (e / VEC) 64 VEC + l VEC + e % VEC.
-// The k-th largest of the lanes' maxima bounds the k-th largest value from
-// below: what reaches it is usually little more than k values. When it is more
-// than a wave can rank at once, the bound is made exact, and of the values
-// equal to it the lowest indexes are taken.
-template <int V, int VEC>
-__device__ __forceinline__ void wave_top(const uint32_t (&key)[V], int k, int64_t first, uint64_t* scratch,
-                                         uint64_t* list) {
-    const int lane = threadIdx.x & (kWave - 1);
-    uint32_t best = 0;
+// A wave's LDS operations stay in order; this keeps the compiler to it.
+__device__ __forceinline__ void wave_lds_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ __forceinline__ uint64_t lane_key(uint64_t key, int lane) {
+    return (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(key >> 32), lane))) << 32) |
+           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(key & 0xffffffffu), lane));
+}
+
+// How many of the k keys of a list, largest first, are above `key`.
+__device__ __forceinline__ int above_in(const uint64_t* list, int k, uint64_t key) {
+    int low = 0;
 #pragma unroll
-    for (int e = 0; e < V; ++e) best = max(best, key[e]);
-    uint32_t bound = 0;
-    for (int bit = 31; bit >= 8; --bit) {  // a bound from below need not be exact
-        const uint32_t next = bound | (1u << bit);
-        if (count(best >= next) >= k) bound = next;
-    }
-    if (bound == 0) bound = 1;
+    for (int step = kMostTop; step >= 1; step /= 2)
+        if (low + step <= k && list[low + step - 1] > key) low += step;
+    return low;
+}
+
+// The wave's list of its k largest keys so far, largest first (0 where there is
+// none), and the order of the smallest of them.
+struct Best {
+    uint64_t* list;  // LDS, [kMostTop + kRoom]: the list, then room for what comes in
+    uint32_t last;
+};
+
+// Takes a block of values into the list: key[e] is the order of the value with
+// index first + (e / VEC) 64 VEC + lane VEC + e % VEC, 0 for none. Blocks come in
+// index order, so a value equal to the last one stays out. When more than
+// kRoom values are above it, the k-th largest of the lanes' maxima bounds
+// from below what can get in; when that leaves too many, the block's own k-th
+// largest value is found bit by bit, and of those equal to it the lowest
+// indexes are taken.
+template <int VEC>
+__device__ __forceinline__ void take(Best& best, const uint32_t (&key)[kValues], int k, int64_t first) {
+    const int lane = threadIdx.x & (kWave - 1);
+    uint32_t bound = best.last + 1;
     int chosen = 0;
 #pragma unroll
-    for (int e = 0; e < V; ++e) chosen += count(key[e] >= bound);
-    int ties = 1 << 30;  // how many of the values equal to the bound are taken
-    if (chosen > kWave) {
+    for (int e = 0; e < kValues; ++e) chosen += count(key[e] >= bound);
+    if (chosen > kRoom) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int e = 0; e < kValues; ++e) most = max(most, key[e]);
+        uint32_t least = 0;
+        for (int bit = 31; bit >= 8; --bit) {  // a bound from below need not be exact
+            const uint32_t next = least | (1u << bit);
+            if (count(most >= next) >= k) least = next;
+        }
+        bound = max(bound, least);
+        chosen = 0;
+#pragma unroll
+        for (int e = 0; e < kValues; ++e) chosen += count(key[e] >= bound);
+    }
+    int at = 0;
+    const auto put = [&](int e, bool in) {
+        const uint64_t mask = __ballot(in);
+        if (!mask) return;
+        if (in)
+            best.list[kMostTop + at + lanes_before(mask)] =
+                key_of(key[e], static_cast<uint32_t>(first + (e / VEC) * (kWave * VEC) + lane * VEC + e % VEC));
+        at += __popcll(mask);
+    };
+    if (chosen <= kRoom) {
+#pragma unroll
+        for (int e = 0; e < kValues; ++e) put(e, key[e] >= bound);
+    } else {
+        // More than k values are at or above the last bound, so the k-th largest is no less.
         bound = 0;
         for (int bit = 31; bit >= 0; --bit) {
             const uint32_t next = bound | (1u << bit);
             int n = 0;
 #pragma unroll
-            for (int e = 0; e < V; ++e) n += count(key[e] >= next);
+            for (int e = 0; e < kValues; ++e) n += count(key[e] >= next);
             if (n >= k) bound = next;
         }
-        if (bound == 0) bound = 1;
-        int above = 0;
+        int ties = k, tied = 0;  // of the values equal to it: taken, seen so far
 #pragma unroll
-        for (int e = 0; e < V; ++e) above += count(key[e] > bound);
-        ties = k - above;
-    }
-    int at = 0, tied = 0;
+        for (int e = 0; e < kValues; ++e) ties -= count(key[e] > bound);
 #pragma unroll
-    for (int c = 0; c < V / VEC; ++c) {
-        // Places in index order: lanes before this one, then its own elements.
-        int tie_rank = tied;
+        for (int c = 0; c < kValues / VEC; ++c) {
+            // Places in index order: lanes before this one, then its own values.
+            int tie_rank = tied;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const uint64_t mask = __ballot(key[c * VEC + e] == bound);
-            tie_rank += lanes_before(mask);
-            tied += __popcll(mask);
-        }
+            for (int e = c * VEC; e < (c + 1) * VEC; ++e) {
+                const uint64_t mask = __ballot(key[e] == bound);
+                tie_rank += lanes_before(mask);
+                tied += __popcll(mask);
+            }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const uint32_t x = key[c * VEC + e];
-            const bool tie = x == bound;
-            const bool take = x > bound || (tie && tie_rank < ties);
-            tie_rank += tie;
-            const uint64_t mask = __ballot(take);
-            if (take)
-                scratch[at + lanes_before(mask)] =
-                    key_of(x, static_cast<uint32_t>(first + c * (kWave * VEC) + lane * VEC + e));
-            at += __popcll(mask);
+            for (int e = c * VEC; e < (c + 1) * VEC; ++e) {
+                const bool tie = key[e] == bound;
+                put(e, key[e] > bound || (tie && tie_rank < ties));
+                tie_rank += tie;
+            }
         }
     }
-    // A wave's LDS operations stay in order; the fence keeps the compiler to it.
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const uint64_t mine = lane < at ? scratch[lane] : 0;
-    int rank = 0;
-    for (int i = 0; i < at; ++i) rank += scratch[i] > mine;
-    if (lane < at && rank < k) list[rank] = mine;
-    if (lane >= at && lane < k) list[lane] = 0;
+    wave_lds_sync();
+    // Lane i holds the list's i-th key and the i-th that came in: their ranks.
+    const uint64_t had = lane < k ? best.list[lane] : 0, came = lane < at ? best.list[kMostTop + lane] : 0;
+    const int held = count(had != 0);
+    int had_rank = lane, came_rank = 0;
+    for (int i = 0; i < held; ++i) came_rank += lane_key(had, i) > came;
+    for (int i = 0; i < at; ++i) {
+        const uint64_t key = lane_key(came, i);
+        had_rank += key > had;
+        came_rank += key > came;
+    }
+    wave_lds_sync();
+    if (had && had_rank < k) best.list[had_rank] = had;
+    if (came && came_rank < k) best.list[came_rank] = came;
+    wave_lds_sync();
+    best.last = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(best.list[k - 1] >> 32));
 }
 
-template <int DT, int V>
-__global__ __launch_bounds__(kWaves* kWave) void k_logprob_parts(const Args a) {
-    constexpr int VEC = DT == NQ_DTYPE_F32 ? 4 : 8;
-    constexpr int kPart = kWaves * kWave * V;
-    __shared__ uint64_t scratch[kWaves][kWave];
-    __shared__ uint64_t lists[kWaves][kMostTop];
-    __shared__ float part_sums[kWaves][3];
+template <int DT>
+struct Block {
+    static constexpr int kVec = DT == NQ_DTYPE_F32 ? 4 : 8, kBytes = DT == NQ_DTYPE_F32 ? 4 : 2;
+    u32x4 w[kValues / kVec];
+};
+
+// One lane's values of a block, 16 bytes at a time (rows may begin anywhere: such
+// loads need no alignment); at a row's end, where 16 bytes would leave it, each
+// value by itself and -inf outside.
+template <int DT>
+__device__ __forceinline__ void load_block(Block<DT>& b, const char* row, int64_t first, int vocab) {
+    using B = Block<DT>;
+    const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+    for (int c = 0; c < kValues / B::kVec; ++c) {
+        const int64_t i = first + (c * kWave + lane) * B::kVec;
+        if (i + B::kVec <= vocab) {
+            b.w[c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_at2*>(row + i * B::kBytes));
+        } else {
+            u32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (DT == NQ_DTYPE_F32) {
+                    w[e] = i + e < vocab ? reinterpret_cast<const uint32_t*>(row)[i + e] : 0xff800000u;
+                } else {
+                    constexpr uint32_t low = DT == NQ_DTYPE_BF16 ? 0xff80u : 0xfc00u;
+                    const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
+                    const int64_t j = i + 2 * e;
+                    const uint32_t h0 = j < vocab ? h[j] : low, h1 = j + 1 < vocab ? h[j + 1] : low;
+                    w[e] = h0 | (h1 << 16);
+                }
+            }
+            b.w[c] = w;
+        }
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void unpack(const Block<DT>& b, float (&x)[kValues]) {
+    constexpr int VEC = Block<DT>::kVec;
+#pragma unroll
+    for (int e = 0; e < kValues; ++e) {
+        if constexpr (DT == NQ_DTYPE_F32) {
+            x[e] = __uint_as_float(b.w[e / VEC][e % VEC]);
+        } else {
+            const uint32_t w = b.w[e / VEC][(e % VEC) / 2];
+            if constexpr (DT == NQ_DTYPE_BF16) {
+                x[e] = __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+            } else {
+                x[e] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(e & 1 ? w >> 16 : w & 0xffffu)));
+            }
+        }
+    }
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Sums s and t relative to m, and to a larger maximum (0 -inf is not meant; an
+// infinite or NaN sum stays one).
+struct Sums {
+    float m, s, t;
+};
+
+__device__ __forceinline__ Sums moved(const Sums& a, float to) {
+    const float d = a.m == -INFINITY ? -INFINITY : a.m - to;
+    const float f = __builtin_amdgcn_exp2f(d * kLog2e);
+    return {to, a.s * f, (a.t + a.s * fmaxf(d, -1000.0f)) * f};
+}
+
+// A row's log of its sum and entropy; NaN where there is no distribution
+// (nothing above -inf, an infinity, a NaN).
+__device__ __forceinline__ double finish(const Args& a, int64_t row, float m, double s, double t, float x, bool writes) {
+    const double log_s = log(s);
+    const double lse = static_cast<double>(m) + log_s;
+    if (writes) {
+        a.logprobs[row] = static_cast<float>(static_cast<double>(x) - lse);
+        a.entropy[row] = static_cast<float>(log_s - t / s);
+    }
+    return lse;
+}
+
+__device__ __forceinline__ void put_top(const Args& a, int64_t row, uint64_t key, int rank, double lse) {
+    if (!key || rank >= a.top) return;
+    a.top_ids[row * a.top + rank] = 0xffffffffu - static_cast<uint32_t>(key & 0xffffffffu);
+    a.top_logprobs[row * a.top + rank] =
+        static_cast<float>(static_cast<double>(value_of(static_cast<uint32_t>(key >> 32))) - lse);
+}
+
+__device__ __forceinline__ float logit_of(const Args& a, int dtype, int64_t row) {
+    const int64_t token = a.tokens[row];
+    return token >= 0 && token < a.vocab ? nq::load_f32(a.logits, dtype, row * a.row_stride + token) : __builtin_nanf("");
+}
+
+template <int DT, bool TOP>
+__global__ __launch_bounds__(kWaves* kWave) void k_token_logprobs(const Args a) {
+    constexpr int VEC = Block<DT>::kVec, kBytes = Block<DT>::kBytes;
+    constexpr int kBlock = kWave * kValues;
+    __shared__ uint64_t lists[TOP ? kWaves : 1][kMostTop + kRoom];
+    __shared__ Sums sums[kWaves];
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int64_t row = blockIdx.x / a.parts;
     const int part = blockIdx.x - static_cast<int>(row) * a.parts;
-    constexpr int kBytes = DT == NQ_DTYPE_F32 ? 4 : 2;
     const char* base = static_cast<const char*>(a.logits) + row * a.row_stride * kBytes;
-    // Places count from the 16-byte boundary at or before the row's start.
-    const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(base) & 15) / kBytes;
-    const int64_t first = static_cast<int64_t>(part) * kPart + wave * (kWave * V) - lead;
+    const int blocks = (a.vocab + kBlock - 1) / kBlock, each = (blocks + a.parts - 1) / a.parts;
+    const int begin = part * each + wave, end = min(blocks, (part + 1) * each);
+    const auto first_of = [&](int block) { return static_cast<int64_t>(block) * kBlock; };
+    Best best{lists[TOP ? wave : 0], 0};
+    if (TOP) {
+        if (lane < kMostTop) best.list[lane] = 0;
+        wave_lds_sync();
+    }
 
-    float x[V];
-    float m = -INFINITY;
+    float m = -INFINITY, s = 0.0f, t = 0.0f;
+    Block<DT> next;
+    if (begin < end) load_block<DT>(next, base, first_of(begin), a.vocab);
+    for (int block = begin; block < end; block += kWaves) {
+        float x[kValues];
+        unpack<DT>(next, x);
+        if (block + kWaves < end) load_block<DT>(next, base, first_of(block + kWaves), a.vocab);
+        float high = x[0];
+        bool nan = x[0] != x[0];
 #pragma unroll
-    for (int c = 0; c < V / VEC; ++c) {
-        const int64_t i = first + c * (kWave * VEC) + lane * VEC;
-        if (i >= 0 && i + VEC <= a.vocab) {
-            const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(base + i * kBytes));
+        for (int e = 1; e < kValues; ++e) {
+            high = fmaxf(high, x[e]);
+            if (TOP) nan |= x[e] != x[e];
+        }
+        const float m_new = fmaxf(m, high);
+        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+        // What was summed so far moves to the new maximum.
+        const float keep = __builtin_amdgcn_exp2f((m - m_use) * kLog2e);
+        t = keep * fmaf(s, fmaxf(m - m_use, -1000.0f), t);
+        s *= keep;
+        float bs = 0.0f, bt = 0.0f;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                if constexpr (DT == NQ_DTYPE_F32) {
-                    x[c * VEC + e] = __uint_as_float(w[e]);
-                } else {
-                    const uint32_t h = e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
-                    x[c * VEC + e] = DT == NQ_DTYPE_BF16
-                                         ? __uint_as_float(h << 16)
-                                         : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
-                }
+        for (int e = 0; e < kValues; ++e) {
+            const float d = x[e] - m_use;
+            const float w = __builtin_amdgcn_exp2f(d * kLog2e);
+            bs += w;
+            bt = fmaf(w, fmaxf(d, -1000.0f), bt);  // w is 0 there: 0 * -inf is not meant
+        }
+        s += bs;
+        t += bt;
+        m = m_new;
+        if (TOP && __ballot(nan || ordered(high) > best.last)) {
+            const int64_t first = first_of(block);
+            uint32_t key[kValues];
+#pragma unroll
+            for (int e = 0; e < kValues; ++e) {
+                const int64_t i = first + (e / VEC) * (kWave * VEC) + lane * VEC + e % VEC;
+                key[e] = i < a.vocab ? ordered(x[e]) : 0;  // outside the row: -inf for the sums, nothing here
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                x[c * VEC + e] = i + e >= 0 && i + e < a.vocab ? element<DT>(base, i + e) : -INFINITY;
+            take<VEC>(best, key, a.top, first);
         }
     }
-#pragma unroll
-    for (int e = 0; e < V; ++e) m = fmaxf(m, x[e]);
-    m = wave_max(m);
-    const float m_use = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f, t = 0.0f;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const float d = x[e] - m_use;
-        const float w = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
-        s += w;
-        t = fmaf(w, fmaxf(d, -1000.0f), t);  // w is 0 there: 0 * -inf is not meant
-    }
-    s = wave_sum(s);
-    t = wave_sum(t);
-    if (lane == 0) {
-        part_sums[wave][0] = m;
-        part_sums[wave][1] = s;
-        part_sums[wave][2] = t;
-    }
-    if (a.top > 0) {
-        uint32_t key[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const int64_t i = first + (e / VEC) * (kWave * VEC) + lane * VEC + e % VEC;
-            key[e] = i >= 0 && i < a.vocab ? ordered(x[e]) : 0;
-        }
-        wave_top<V, VEC>(key, a.top, first, scratch[wave], lists[wave]);
-    }
+
+    const float wave_m = wave_max(m);
+    const Sums mine = moved({m, s, t}, wave_m);
+    const Sums joined{wave_m, wave_sum(mine.s), wave_sum(mine.t)};
+    if (lane == 0) sums[wave] = joined;
+    const float x = wave == 0 && a.parts == 1 ? logit_of(a, DT, row) : 0.0f;
     __syncthreads();
+    float high = sums[0].m;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) high = fmaxf(high, sums[w].m);
+    Sums all{high, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        const Sums b = moved(sums[w], high);
+        all.s += b.s;
+        all.t += b.t;
+    }
     const int64_t at = row * a.parts + part;
-    if (threadIdx.x == 0) {
-        float mm = part_sums[0][0];
-        for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, part_sums[w][0]);
-        const float mu = mm == -INFINITY ? 0.0f : mm;
-        float ss = 0.0f, tt = 0.0f;
-        for (int w = 0; w < kWaves; ++w) {
-            const float d = fmaxf(part_sums[w][0] - mu, -1000.0f);
-            const float f = __builtin_amdgcn_exp2f((part_sums[w][0] - mu) * 1.4426950408889634f);
-            ss += f * part_sums[w][1];
-            tt += f * (part_sums[w][2] + d * part_sums[w][1]);
-        }
-        a.sums[4 * at] = mm;
-        a.sums[4 * at + 1] = ss;
-        a.sums[4 * at + 2] = tt;
+    double lse = 0.0;
+    if (a.parts == 1) {
+        lse = finish(a, row, all.m, all.s, all.t, x, threadIdx.x == 0);
+    } else if (threadIdx.x == 0) {
+        a.sums[4 * at] = all.m;
+        a.sums[4 * at + 1] = all.s;
+        a.sums[4 * at + 2] = all.t;
     }
-    // The four lists' keys, ranked against each other.
-    const int n = kWaves * a.top;
-    for (int i = threadIdx.x; i < n; i += kWaves * kWave) {
-        const uint64_t mine = lists[i / a.top][i % a.top];
-        int rank = 0;
+    if (!TOP) return;
+    // The waves' lists as one: a key's rank is its place in its own and what the others have above it.
+    for (int i = threadIdx.x; i < kWaves * kMostTop; i += kWaves * kWave) {
+        const int w0 = i / kMostTop, j = i % kMostTop;
+        if (j >= a.top) continue;
+        const uint64_t key = lists[w0][j];
+        int rank = j;
+#pragma unroll
         for (int w = 0; w < kWaves; ++w)
-            for (int j = 0; j < a.top; ++j) {
-                const uint64_t other = lists[w][j];
-                rank += other > mine || (other == 0 && mine == 0 && w * a.top + j < i);
-            }
-        if (rank < a.top) a.lists[at * a.top + rank] = mine;
+            if (w != w0) rank += above_in(lists[w], a.top, key);
+        if (a.parts == 1) {
+            put_top(a, row, key, rank, lse);
+        } else if (key) {
+            if (rank < a.top) a.lists[at * a.top + rank] = key;
+        } else {
+            // Empty places follow all lists' keys (rank counts the others' and j its
+            // own): those of the lists before this one come first.
+            for (int w = 0; w < w0; ++w) rank += a.top - above_in(lists[w], a.top, 0);
+            if (rank < a.top) a.lists[at * a.top + rank] = 0;
+        }
     }
 }
 
-// One wave per row.
-__global__ __launch_bounds__(kWave) void k_logprob_join(const Args a, int dtype) {
-    // Keys that reach the k-th largest of the lanes' best: at most k lanes with
-    // two parts of k keys each.
-    __shared__ uint64_t keys[2 * kMostTop * kMostTop];
-    const int lane = threadIdx.x;
+// A row's parts: one to a lane for the sums; the lists in LDS.
+__global__ __launch_bounds__(kWaves* kWave) void k_token_logprobs_join(const Args a, int dtype) {
+    __shared__ uint64_t lists[kMostParts * kMostTop], reach[kMostParts * kMostTop];
+    __shared__ int reached;
+    const int lane = threadIdx.x & (kWave - 1);
     const int64_t row = blockIdx.x;
-    float m = -INFINITY;
-    for (int p = lane; p < a.parts; p += kWave) m = fmaxf(m, a.sums[4 * (row * a.parts + p)]);
-    m = wave_max(m);
-    double s = 0.0, t = 0.0;
-    for (int p = lane; p < a.parts; p += kWave) {
-        const float* sums = a.sums + 4 * (row * a.parts + p);
-        const double d = static_cast<double>(sums[0]) - (m == -INFINITY ? 0.0 : static_cast<double>(m));
-        const double f = exp(d);
-        s += f * static_cast<double>(sums[1]);
-        t += f * (static_cast<double>(sums[2]) + fmax(d, -1000.0) * static_cast<double>(sums[1]));
-    }
-    s = wave_sum(s);
-    t = wave_sum(t);
-    const double log_s = log(s);
-    const double lse = static_cast<double>(m) + log_s;
-    if (lane == 0) {
-        const int64_t token = a.tokens[row];
-        const bool ok = token >= 0 && token < a.vocab;
-        const float x = ok ? nq::load_f32(a.logits, dtype, row * a.row_stride + token) : __builtin_nanf("");
-        a.logprobs[row] = static_cast<float>(static_cast<double>(x) - lse);
-        // Nothing to weigh (m -inf), an infinity or a NaN: no distribution, NaN.
-        a.entropy[row] = static_cast<float>(log_s - t / s);
-    }
+    const int keys = a.parts * a.top;
+    for (int i = threadIdx.x; i < keys; i += kWaves * kWave) lists[i] = a.lists[row * keys + i];
+    if (threadIdx.x == 0) reached = 0;
+    const float* at = a.sums + 4 * (row * a.parts + (lane < a.parts ? lane : 0));
+    Sums mine{at[0], at[1], at[2]};
+    const float x = logit_of(a, dtype, row);
+    if (lane >= a.parts) mine = {-INFINITY, 0.0f, 0.0f};
+    const float high = wave_max(mine.m);
+    const double d = mine.m == -INFINITY ? -INFINITY : static_cast<double>(mine.m) - static_cast<double>(high);
+    const double f = exp(d);
+    const double s = wave_sum(mine.s * f), t = wave_sum((mine.t + mine.s * fmax(d, -1000.0)) * f);
+    const double lse = finish(a, row, high, s, t, x, threadIdx.x == 0);
     if (a.top == 0) return;
-    const uint64_t* lists = a.lists + row * a.parts * a.top;
-    uint64_t best = 0;
-    for (int p = lane; p < a.parts; p += kWave) {
-        const uint64_t head = lists[p * a.top];
-        best = head > best ? head : best;
+    __syncthreads();
+    // The r-th largest of the lists' j-th keys, with r lists of j keys each at
+    // least top together, bounds the top-th largest key from below.
+    const int j = (a.top + a.parts - 1) / a.parts, r = (a.top + j - 1) / j;
+    const uint32_t best = lane < a.parts ? static_cast<uint32_t>(lists[lane * a.top + j - 1] >> 32) : 0;
+    uint32_t bound = 0;
+    for (int bit = 31; bit >= 8; --bit) {
+        const uint32_t next = bound | (1u << bit);
+        if (count(best >= next) >= r) bound = next;
     }
-    uint64_t bound = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-        const uint64_t next = bound | (uint64_t{1} << bit);
-        if (count(best >= next) >= a.top) bound = next;
-    }
-    if (bound == 0) bound = 1;
-    int at = 0;
-    for (int p0 = 0; p0 < a.parts; p0 += kWave) {
-        for (int j = 0; j < a.top; ++j) {
-            const uint64_t key = p0 + lane < a.parts ? lists[(p0 + lane) * a.top + j] : 0;
-            const uint64_t mask = __ballot(key >= bound);
-            if (!mask) break;  // each list falls
-            if (key >= bound) keys[at + lanes_before(mask)] = key;
-            at += __popcll(mask);
-        }
+    // The keys that reach it, in any order: a rank is a count of larger keys.
+    for (int i = threadIdx.x; i < keys; i += kWaves * kWave) {
+        const uint64_t key = lists[i];
+        if (key && static_cast<uint32_t>(key >> 32) >= bound) reach[atomicAdd(&reached, 1)] = key;
     }
     __syncthreads();
-    for (int i = lane; i < at; i += kWave) {
-        const uint64_t mine = keys[i];
+    const int n = reached;
+    for (int i = threadIdx.x; i < n; i += kWaves * kWave) {
+        const uint64_t key = reach[i];
         int rank = 0;
-        for (int j = 0; j < at; ++j) rank += keys[j] > mine;
-        if (rank < a.top) {
-            a.top_ids[row * a.top + rank] = 0xffffffffu - static_cast<uint32_t>(mine & 0xffffffffu);
-            a.top_logprobs[row * a.top + rank] =
-                static_cast<float>(static_cast<double>(value_of(static_cast<uint32_t>(mine >> 32))) - lse);
-        }
+#pragma unroll 8
+        for (int c = 0; c < n; ++c) rank += reach[c] > key;
+        put_top(a, row, key, rank, lse);
     }
 }
 
-struct Plan {
-    int values, parts;  // values to a lane, parts of a row
-};
-
-// 8 values to a lane where 32 would leave CUs without work, unless a row then
-// has more parts than the joining wave holds.
-Plan plan_for(int64_t rows, int64_t vocab) {
-    const int64_t lead = 7;  // places before a row's start, at most
-    const auto parts = [&](int v) { return (vocab + lead + kWaves * kWave * v - 1) / (kWaves * kWave * v); };
-    const int v = rows * parts(32) < 1024 && parts(8) <= kMostParts ? 8 : 32;
-    return {v, static_cast<int>(parts(v) < (1 << 20) ? parts(v) : (1 << 20))};
+// Parts of a row: enough workgroups for the chip, but a block for each wave.
+int parts_for(int64_t rows, int64_t vocab) {
+    constexpr int64_t kWorkgroups = 1024;
+    const int64_t blocks = (vocab + kWave * kValues - 1) / (kWave * kValues);
+    int64_t parts = (kWorkgroups + rows - 1) / rows;
+    const int64_t most = (blocks + kWaves - 1) / kWaves;
+    parts = parts < most ? parts : most;
+    return static_cast<int>(parts < kMostParts ? parts : kMostParts);
 }
-
-int64_t bytes_for(int64_t rows, int64_t parts, int64_t top) { return rows * parts * (16 + 8 * top); }
 
 }  // namespace
 
 extern "C" int64_t nq_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top) {
-    if (rows <= 0 || rows > 0xffffff || vocab <= 0 || top < 0 || top > kMostTop || top > vocab) return -1;
-    const Plan plan = plan_for(rows, vocab);
-    if (plan.parts > kMostParts || rows * plan.parts > 0x7fffffff) return -1;
-    return bytes_for(rows, plan.parts, top);
+    if (rows <= 0 || rows > 0xffffff || vocab <= 0 || vocab > 0x7fffff00 || top < 0 || top > kMostTop || top > vocab)
+        return -1;
+    const int parts = parts_for(rows, vocab);
+    return parts == 1 ? 0 : rows * parts * (16 + 8 * static_cast<int64_t>(top));
 }
 
 extern "C" int nq_token_logprobs(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,
                                  const int64_t* tokens, int32_t top, float* logprobs, float* entropy,
                                  int64_t* top_ids, float* top_logprobs, void* workspace, int64_t workspace_bytes,
                                  void* stream) {
-    if (!logits || !tokens || !logprobs || !entropy || !workspace || (top > 0 && (!top_ids || !top_logprobs)))
+    if (!logits || !tokens || !logprobs || !entropy || (top > 0 && (!top_ids || !top_logprobs)))
         return NQ_ERR_ARGUMENT;
     if (!nq::is_float_dtype(dtype)) return NQ_ERR_DTYPE;
     const int64_t need = nq_token_logprobs_workspace_bytes(rows, vocab, top);
     if (need < 0 || row_stride < vocab || row_stride > (int64_t{1} << 40)) return NQ_ERR_SHAPE;
+    if (need > 0 && !workspace) return NQ_ERR_ARGUMENT;
     if (workspace_bytes < need) return NQ_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(logits) % nq::dtype_bytes(dtype) || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return NQ_ERR_ALIGNMENT;
-    const Plan plan = plan_for(rows, vocab);
-    Args a{};
-    a.logits = logits;
-    a.tokens = tokens;
-    a.row_stride = row_stride;
-    a.vocab = static_cast<int32_t>(vocab);
-    a.top = top;
-    a.parts = plan.parts;
-    a.sums = static_cast<float*>(workspace);
-    a.lists = reinterpret_cast<uint64_t*>(a.sums + 4 * rows * plan.parts);
-    a.logprobs = logprobs;
-    a.entropy = entropy;
-    a.top_ids = top_ids;
-    a.top_logprobs = top_logprobs;
+    const int parts = parts_for(rows, vocab);
+    float* sums = static_cast<float*>(workspace);
+    const Args a = {logits, tokens, row_stride, static_cast<int32_t>(vocab), top, parts, sums,
+                    reinterpret_cast<uint64_t*>(sums + 4 * rows * parts), logprobs, entropy, top_logprobs, top_ids};
+    const dim3 grid(static_cast<unsigned>(rows * parts)), block(kWaves * kWave);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid(static_cast<unsigned>(rows * plan.parts)), block(kWaves * kWave);
-#define NQ_PARTS(DT)                                                                        \
-    if (plan.values == 8) hipLaunchKernelGGL((k_logprob_parts<DT, 8>), grid, block, 0, st, a); \
-    else hipLaunchKernelGGL((k_logprob_parts<DT, 32>), grid, block, 0, st, a)
+#define NQ_LOGPROBS(DT)                                                                  \
+    if (top) hipLaunchKernelGGL((k_token_logprobs<DT, true>), grid, block, 0, st, a);    \
+    else hipLaunchKernelGGL((k_token_logprobs<DT, false>), grid, block, 0, st, a)
     switch (dtype) {
-        case NQ_DTYPE_F32: NQ_PARTS(NQ_DTYPE_F32); break;
-        case NQ_DTYPE_F16: NQ_PARTS(NQ_DTYPE_F16); break;
-        default: NQ_PARTS(NQ_DTYPE_BF16); break;
+        case NQ_DTYPE_F32: NQ_LOGPROBS(NQ_DTYPE_F32); break;
+        case NQ_DTYPE_F16: NQ_LOGPROBS(NQ_DTYPE_F16); break;
+        default: NQ_LOGPROBS(NQ_DTYPE_BF16); break;
     }
-#undef NQ_PARTS
-    if (const int status = nq::launch_status(); status != NQ_OK) return status;
-    hipLaunchKernelGGL(k_logprob_join, dim3(static_cast<unsigned>(rows)), dim3(kWave), 0, st, a, dtype);
+#undef NQ_LOGPROBS
+    if (const int status = nq::launch_status(); status != NQ_OK || parts == 1) return status;
+    hipLaunchKernelGGL(k_token_logprobs_join, dim3(static_cast<unsigned>(rows)), block, 0, st, a, dtype);
     return nq::launch_status();
 }

@@ -695,13 +695,13 @@ def launch_token_logprobs(
     need = lib.nq_token_logprobs_workspace_bytes(rows, vocab, top)
     if need < 0:
         raise ValueError("token logprobs geometry was rejected")
-    if workspace is None:
+    if workspace is None and need:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
     status = _on_device(
         device, lib.nq_token_logprobs, logits.data_ptr(), _native.DTYPE_CODES[logits.dtype], rows, vocab, stride,
         tokens.data_ptr(), top, out.logprobs.data_ptr(), out.entropy.data_ptr(), _ptr(out.top_ids if top else None),
-        _ptr(out.top_logprobs if top else None), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-        _stream(device),
+        _ptr(out.top_logprobs if top else None), _ptr(workspace),
+        0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(device),
     )
     _native.check("nq_token_logprobs", status)
     return out

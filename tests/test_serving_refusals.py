@@ -74,11 +74,11 @@ def test_attention_workspace():
 
 @pytest.mark.parametrize("arguments,status", [
     ({"logits": None}, -1), ({"top_ids": None}, -1), ({"workspace": None}, -1), ({"dtype": 3}, -2), ({"rows": 0}, -3),
-    ({"vocab": 0}, -3), ({"stride": 99}, -3), ({"top": 33}, -3), ({"top": -1}, -3), ({"vocab": 4, "stride": 4, "top": 5}, -3),
-    ({"vocab": 1 << 21, "stride": 1 << 21}, -3), ({"logits": A + 2}, -4), ({"size": 8}, -5),
+    ({"vocab": 0}, -3), ({"stride": 8999}, -3), ({"top": 33}, -3), ({"top": -1}, -3), ({"vocab": 4, "stride": 4, "top": 5}, -3),
+    ({"vocab": 1 << 31, "stride": 1 << 31}, -3), ({"logits": A + 2}, -4), ({"size": 8}, -5),
 ])
 def test_token_logprobs(arguments, status):
-    a = {"logits": A, "dtype": 0, "rows": 2, "vocab": 100, "stride": 100, "top": 5, "top_ids": A, "workspace": A, "size": 1 << 30}
+    a = {"logits": A, "dtype": 0, "rows": 2, "vocab": 9000, "stride": 9000, "top": 5, "top_ids": A, "workspace": A, "size": 1 << 30}
     a.update(arguments)
     assert _native.load().nq_token_logprobs(a["logits"], a["dtype"], a["rows"], a["vocab"], a["stride"], A, a["top"], A, A,
                                             a["top_ids"], A, a["workspace"], a["size"], None) == status
