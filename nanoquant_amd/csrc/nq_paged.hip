@@ -48,42 +48,63 @@ struct AppendArgs {
     const float *cos_table, *sin_table;
     void* q_out;
     float eps;
-    int32_t dtype, norm_dtype, q_dtype, q_heads, q_groups, rope_rows, kv_blocks;
+    int32_t norm_dtype, q_dtype, q_heads, q_groups, rope_rows, kv_blocks;
 };
 
 constexpr int kPageTokens = 8;  // new rows of a page that a wave holds in registers
-constexpr int kQHeads = 4;      // q heads of a token that a wave takes
+constexpr int kQHeads = 8;      // q heads of a token that a wave takes
+constexpr int E = 4;            // adjacent values of a head vector that a lane holds
 
-// Lane values permuted within rows of 16 (DPP), 0 where a source lane is off.
+// A head vector takes D / 4 lanes: a wave works on this many at once.
+template <int D>
+constexpr int kHeads = kWave * E / D;
+
+// Lane values permuted within rows of 16 (DPP).
 template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, 0xf, 0xf, false));
+}
+
+// The value of lane l ^ 8, l ^ 16 or l ^ 32: half a head vector away.
+template <int D>
+__device__ __forceinline__ uint32_t partner_of(uint32_t v) {
+    if constexpr (D == 64) return dpp<0x128>(v);  // row_ror:8
+    if constexpr (D == 128) {
+        const auto rows = __builtin_amdgcn_permlane16_swap(v, v, false, false);  // both rows' lower and upper values
+        return (threadIdx.x & 16) ? rows[0] : rows[1];
+    }
+    const auto halves = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return (threadIdx.x & 32) ? halves[0] : halves[1];
+}
+
+template <int D>
+__device__ __forceinline__ float partner_of(float v) { return __uint_as_float(partner_of<D>(__float_as_uint(v))); }
+
+template <int D>
+__device__ __forceinline__ double partner_of(double v) {
+    const uint2 w = __builtin_bit_cast(uint2, v);
+    return __builtin_bit_cast(double, make_uint2(partner_of<D>(w.x), partner_of<D>(w.y)));
 }
 
 template <int CTRL>
-__device__ __forceinline__ double dpp(double x) {
-    const int2 w = __builtin_bit_cast(int2, x);
-    return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_update_dpp(0, w.x, CTRL, 0xf, 0xf, false),
-                                                __builtin_amdgcn_update_dpp(0, w.y, CTRL, 0xf, 0xf, false)));
+__device__ __forceinline__ float dpp(float v) { return __uint_as_float(dpp<CTRL>(__float_as_uint(v))); }
+
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+    const uint2 w = __builtin_bit_cast(uint2, v);
+    return __builtin_bit_cast(double, make_uint2(dpp<CTRL>(w.x), dpp<CTRL>(w.y)));
 }
 
-__device__ __forceinline__ float lane_of(float v, int lane) {
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
-}
-
-__device__ __forceinline__ double lane_of(double v, int lane) {
-    const int2 w = __builtin_bit_cast(int2, v);
-    return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_readlane(w.x, lane), __builtin_amdgcn_readlane(w.y, lane)));
-}
-
-// Sum over the wave, in a fixed order.
-template <class T>
-__device__ __forceinline__ T wave_sum(T v) {
+// Sum over a head vector's lanes, in a fixed order.
+template <int D, class T>
+__device__ __forceinline__ T head_sum(T v) {
     v += dpp<0xB1>(v);   // quad_perm [1,0,3,2]
     v += dpp<0x4E>(v);   // quad_perm [2,3,0,1]
     v += dpp<0x141>(v);  // row_half_mirror
     v += dpp<0x140>(v);  // row_mirror
-    return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+    if constexpr (D >= 128) v += partner_of<128>(v);
+    if constexpr (D >= 256) v += partner_of<256>(v);
+    return v;
 }
 
 // Maximum of values >= 0 over the wave.
@@ -92,17 +113,12 @@ __device__ __forceinline__ float wave_max(float v) {
     v = fmaxf(v, dpp<0x4E>(v));
     v = fmaxf(v, dpp<0x141>(v));
     v = fmaxf(v, dpp<0x140>(v));
-    return fmaxf(fmaxf(lane_of(v, 0), lane_of(v, 16)), fmaxf(lane_of(v, 32), lane_of(v, 48)));
+    v = fmaxf(v, partner_of<128>(v));
+    return fmaxf(v, partner_of<256>(v));
 }
 
-__device__ __forceinline__ float partner_of(float v) { return __shfl_xor(v, 32, kWave); }
-
-__device__ __forceinline__ double partner_of(double v) {
-    const int2 w = __builtin_bit_cast(int2, v);
-    return __builtin_bit_cast(double, make_int2(__shfl_xor(w.x, 32, kWave), __shfl_xor(w.y, 32, kWave)));
-}
-
-__device__ __forceinline__ float inverse_root(float x) { return 1.0f / sqrtf(x); }
+// The hardware's estimate (1 ulp) does for q.
+__device__ __forceinline__ float inverse_root(float x) { return __builtin_amdgcn_rsqf(x); }
 
 // The hardware's estimate is good to 2^-24; each step y (3 - x y^2) / 2 squares
 // the error. 0 and infinity (of an infinite or a zero mean) are kept.
@@ -136,49 +152,77 @@ __device__ __forceinline__ float for_e4m3(double x) {
     return f;
 }
 
-// One wave's head vector, lane l holding d = l + 64 j: RMSNorm with weight w
-// (has_w), then rotate-half RoPE, in place. In T = double the result is correct
-// to far below an e4m3 rounding's border.
+// E adjacent values, at any address that fits the value's type.
+template <int DT>
+__device__ __forceinline__ void load_values(const void* p, int64_t i, float (&v)[E]) {
+    if constexpr (DT == NQ_DTYPE_F32) {
+        typedef float vec __attribute__((ext_vector_type(E), aligned(4)));
+        const vec x = *reinterpret_cast<const vec*>(static_cast<const float*>(p) + i);
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = x[j];
+    } else {
+        typedef uint16_t vec __attribute__((ext_vector_type(E), aligned(2)));
+        const vec x = *reinterpret_cast<const vec*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            if constexpr (DT == NQ_DTYPE_BF16) v[j] = __uint_as_float(static_cast<uint32_t>(x[j]) << 16);
+            else v[j] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(x[j])));
+        }
+    }
+}
+
+__device__ __forceinline__ void store_values(void* p, int dtype, int64_t i, const float (&v)[E]) {
+    if (dtype == NQ_DTYPE_F32) {
+        typedef float vec __attribute__((ext_vector_type(E), aligned(4)));
+        vec x;
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[j] = v[j];
+        *reinterpret_cast<vec*>(static_cast<float*>(p) + i) = x;
+        return;
+    }
+    typedef uint16_t vec __attribute__((ext_vector_type(E), aligned(2)));
+    vec x;
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+        x[j] = dtype == NQ_DTYPE_BF16 ? __builtin_bit_cast(uint16_t, static_cast<__bf16>(v[j]))
+                                      : __builtin_bit_cast(uint16_t, static_cast<_Float16>(v[j]));
+    *reinterpret_cast<vec*>(static_cast<uint16_t*>(p) + i) = x;
+}
+
+// Head vectors, lane l of one holding the values from d = 4 l on: RMSNorm with
+// weight w (has_w), then rotate-half RoPE, in place; sn is negative in the first
+// half. In T = double the result is correct to far below an e4m3 rounding's
+// border.
 template <int D, class T>
-__device__ __forceinline__ void norm_rope(T (&v)[D / kWave], const float (&w)[D / kWave], bool has_w, float eps,
-                                          const float (&cs)[D / kWave], const float (&sn)[D / kWave], int lane) {
-    constexpr int E = D / kWave;
+__device__ __forceinline__ void norm_rope(T (&v)[E], const float (&w)[E], bool has_w, float eps, const float (&cs)[E],
+                                          const float (&sn)[E]) {
     if (has_w) {
         T ss = 0;
 #pragma unroll
         for (int j = 0; j < E; ++j) ss += v[j] * v[j];
-        const T inv = inverse_root(wave_sum(ss) * static_cast<T>(1.0 / D) + static_cast<T>(eps));
+        const T inv = inverse_root(head_sum<D>(ss) * static_cast<T>(1.0 / D) + static_cast<T>(eps));
 #pragma unroll
         for (int j = 0; j < E; ++j) v[j] = static_cast<T>(w[j]) * (v[j] * inv);
     }
-    T y[E];
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-        const bool first = lane + kWave * j < D / 2;
-        T partner;
-        if constexpr (E == 1) partner = partner_of(v[0]);
-        else partner = first ? v[j + E / 2] : v[j - E / 2];
-        y[j] = v[j] * static_cast<T>(cs[j]) + (first ? -partner : partner) * static_cast<T>(sn[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < E; ++j) v[j] = y[j];
+    for (int j = 0; j < E; ++j) v[j] = v[j] * static_cast<T>(cs[j]) + partner_of<D>(v[j]) * static_cast<T>(sn[j]);
 }
 
 template <int D>
-__device__ __forceinline__ void load_rope_row(const AppendArgs& a, int row, int lane, float (&cs)[D / kWave],
-                                              float (&sn)[D / kWave]) {
+__device__ __forceinline__ void load_rope_row(const AppendArgs& a, int row, int place, float (&cs)[E], float (&sn)[E]) {
+    const int64_t i = static_cast<int64_t>(row) * (D / 2) + (place & (D / 2 - 1));
+    load_values<NQ_DTYPE_F32>(a.cos_table, i, cs);
+    load_values<NQ_DTYPE_F32>(a.sin_table, i, sn);
+    if (place < D / 2)
 #pragma unroll
-    for (int j = 0; j < D / kWave; ++j) {
-        const int64_t i = static_cast<int64_t>(row) * (D / 2) + ((lane + kWave * j) & (D / 2 - 1));
-        cs[j] = a.cos_table[i];
-        sn[j] = a.sin_table[i];
-    }
+        for (int j = 0; j < E; ++j) sn[j] = -sn[j];
 }
 
-template <int D>
-__device__ __forceinline__ void load_weight(const void* w, int dtype, int lane, float (&out)[D / kWave]) {
-#pragma unroll
-    for (int j = 0; j < D / kWave; ++j) out[j] = w ? nq::load_f32(w, dtype, lane + kWave * j) : 1.0f;
+__device__ __forceinline__ void load_weight(const void* w, int dtype, int place, float (&out)[E]) {
+    if (!w) return;
+    if (dtype == NQ_DTYPE_F32) load_values<NQ_DTYPE_F32>(w, place, out);
+    else if (dtype == NQ_DTYPE_F16) load_values<NQ_DTYPE_F16>(w, place, out);
+    else load_values<NQ_DTYPE_BF16>(w, place, out);
 }
 
 // The least power of two 2^e, e >= -126, with amax <= 448 * 2^e = 1.75 * 2^(8 + e).
@@ -190,10 +234,14 @@ __device__ __forceinline__ float scale_for(float amax) {
 
 __device__ __forceinline__ float finite_or_zero(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; }
 
-// e4m3 byte of x (|x| <= 448), NaN for what is not finite.
-__device__ __forceinline__ uint8_t e4m3(float x) {
-    const float y = fabsf(x) < INFINITY ? x : __builtin_nanf("");
-    return static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false) & 0xff);
+// e4m3 bytes of x inv (at most 448), NaN for what is not finite.
+__device__ __forceinline__ uint32_t e4m3x4(const float (&x)[E], float inv) {
+    float y[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) y[j] = fabsf(x[j]) < INFINITY ? x[j] * inv : __builtin_nanf("");
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], r, true);
+    return static_cast<uint32_t>(r);
 }
 
 __device__ __forceinline__ uint32_t moved4(uint32_t w, float ratio) {
@@ -205,43 +253,16 @@ __device__ __forceinline__ uint32_t moved4(uint32_t w, float ratio) {
     return static_cast<uint32_t>(r);
 }
 
-template <int D>
-__device__ __forceinline__ void load_head(const void* x, int dtype, int64_t at, int lane, float (&v)[D / kWave]) {
-#pragma unroll
-    for (int j = 0; j < D / kWave; ++j) v[j] = nq::load_f32(x, dtype, at + lane + kWave * j);
-}
-
-// A tile of bytes in LDS, [lines][width] with each line's bytes [first, first +
-// n) new, to memory: whole words where they are new, single bytes at the ends.
-__device__ __forceinline__ void store_lines(const uint8_t* tile, int stride, uint8_t* out, int lines, int width, int first, int n,
-                                            int threads) {
-    const int words = width / 4;
-    for (int i = threadIdx.x; i < lines * words; i += threads) {
-        const int line = i / words, c = (i - line * words) * 4;
-        if (c + 4 <= first || c >= first + n) continue;
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + line * stride + c);
-        uint8_t* at = out + line * width + c;
-        if (c >= first && c + 4 <= first + n) {
-            *reinterpret_cast<uint32_t*>(at) = w;
-        } else {
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-                if (c + b >= first && c + b < first + n) at[b] = static_cast<uint8_t>(w >> (8 * b));
-        }
-    }
-}
-
 // Workgroups [0, kv_blocks): the new rows of one page and kv head, kPageTokens
-// to a wave, which holds them in registers until the page's scale is known; the
-// bytes go out through LDS, V's transposed. Sequence b has at most (its tokens)
+// to a wave, which holds them in registers until the page's scale is known;
+// V's bytes are transposed in LDS. Sequence b has at most (its tokens)
 // / page + 2 pages with new rows, and its slots begin at starts[b] / page + 2 b:
 // the grid follows from the host's counts alone. The rest: q, one wave per token
 // and kQHeads of its heads.
-template <int D, int WAVES>
+template <int D, int DT, int WAVES>
 __global__ __launch_bounds__(WAVES* kWave) void k_paged_append(const AppendArgs a) {
-    constexpr int E = D / kWave, kPage = WAVES * kPageTokens, kThreads = WAVES * kWave;
-    // K: a row of D bytes after the other; V: a line of kPage bytes, padded by a
-    // word against bank conflicts, for each of D.
+    constexpr int kPage = WAVES * kPageTokens, kThreads = WAVES * kWave, H = kHeads<D>;
+    // V's bytes: a line of kPage for each of D, padded by a word against bank conflicts.
     constexpr int kLine = kPage + 4;
     __shared__ float red[2][WAVES];
     __shared__ uint32_t tile[D * kLine / 4];
@@ -249,7 +270,8 @@ __global__ __launch_bounds__(WAVES* kWave) void k_paged_append(const AppendArgs 
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int rows = p.table_pages << p.page_shift;
-    float w[E];
+    const int sub = lane / (kWave / H), place = (lane & (kWave / H - 1)) * E;  // head vector of the wave, place in it
+    float w[E] = {};
 
     if (static_cast<int>(blockIdx.x) >= a.kv_blocks) {
         const int64_t item = static_cast<int64_t>(blockIdx.x - a.kv_blocks) * WAVES + wave;
@@ -260,18 +282,17 @@ __global__ __launch_bounds__(WAVES* kWave) void k_paged_append(const AppendArgs 
         const Span s = f.span;
         const int row = token >= s.begin && token < s.end ? row_of(f.context, token - s.begin, rows) : -1;
         if (row < 0 || row >= a.rope_rows) return;
-        float cs[E], sn[E], x[kQHeads][E];
-        const int64_t at = (static_cast<int64_t>(token) * a.q_heads + head) * D;
+        float cs[E], sn[E], x[kQHeads / H][E];
+        const int64_t at = (static_cast<int64_t>(token) * a.q_heads + head) * D + place;
+        const int last = a.q_heads - 1 - head;
 #pragma unroll
-        for (int i = 0; i < kQHeads; ++i) load_head<D>(a.q, a.dtype, at + min(i, a.q_heads - 1 - head) * D, lane, x[i]);
-        load_weight<D>(a.q_norm, a.norm_dtype, lane, w);
-        load_rope_row<D>(a, row, lane, cs, sn);
+        for (int i = 0; i < kQHeads / H; ++i) load_values<DT>(a.q, at + min(i * H + sub, last) * D, x[i]);
+        load_weight(a.q_norm, a.norm_dtype, place, w);
+        load_rope_row<D>(a, row, place, cs, sn);
 #pragma unroll
-        for (int i = 0; i < kQHeads; ++i) {
-            norm_rope<D, float>(x[i], w, a.q_norm != nullptr, a.eps, cs, sn, lane);
-            if (head + i >= a.q_heads) continue;
-#pragma unroll
-            for (int j = 0; j < E; ++j) nq::store_f32_as(a.q_out, a.q_dtype, at + i * D + lane + kWave * j, x[i][j]);
+        for (int i = 0; i < kQHeads / H; ++i) {
+            norm_rope<D>(x[i], w, a.q_norm != nullptr, a.eps, cs, sn);
+            if (i * H + sub <= last) store_values(a.q_out, a.q_dtype, at + (i * H + sub) * D, x[i]);
         }
         return;
     }
@@ -294,37 +315,35 @@ __global__ __launch_bounds__(WAVES* kWave) void k_paged_append(const AppendArgs 
     const int r0 = static_cast<int>(begin) & (kPage - 1), n = static_cast<int>(end - begin);
     const int64_t token0 = s.begin + (begin - context);
 
-    // Loads first, of the wave's last row again where it has fewer.
-    float kf[kPageTokens][E], vf[kPageTokens][E];
-    const int mine = wave < n ? (n - wave + WAVES - 1) / WAVES : 0;  // rows wave, wave + WAVES, ...
-    load_weight<D>(a.k_norm, a.norm_dtype, lane, w);
+    // Row wave H + i WAVES H + sub of the new ones; the last one again behind it,
+    // which changes no maximum and is not stored.
+    float kf[kPageTokens / H][E], vf[kPageTokens / H][E];
+    const auto row_at = [&](int i) { return (wave + i * WAVES) * H + sub; };
+    const auto any_at = [&](int i) { return (wave + i * WAVES) * H < n; };  // the same for the wave
+    load_weight(a.k_norm, a.norm_dtype, place, w);
     float kmax = 0.0f, vmax = 0.0f;
-    const auto load_row = [&](int i) {
-        const int64_t at = ((token0 + wave + i * WAVES) * p.kv_heads + g) * D;
-        load_head<D>(a.k, a.dtype, at, lane, kf[i]);
-        load_head<D>(a.v, a.dtype, at, lane, vf[i]);
-    };
-    const auto turn_row = [&](int i, const float (&cs)[E], const float (&sn)[E]) {
+#pragma unroll
+    for (int i = 0; i < kPageTokens / H; ++i) {
+        if (!any_at(i)) break;
+        const int64_t at = ((token0 + min(row_at(i), n - 1)) * p.kv_heads + g) * D + place;
+        load_values<DT>(a.k, at, kf[i]);
+        load_values<DT>(a.v, at, vf[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kPageTokens / H; ++i) {
+        if (!any_at(i)) break;
+        float cs[E], sn[E];
+        load_rope_row<D>(a, static_cast<int>(begin) + min(row_at(i), n - 1), place, cs, sn);
         double y[E];
 #pragma unroll
         for (int j = 0; j < E; ++j) y[j] = static_cast<double>(kf[i][j]);
-        norm_rope<D, double>(y, w, a.k_norm != nullptr, a.eps, cs, sn, lane);
+        norm_rope<D>(y, w, a.k_norm != nullptr, a.eps, cs, sn);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
             kf[i][j] = for_e4m3(y[j]);
             kmax = fmaxf(kmax, finite_or_zero(kf[i][j]));
             vmax = fmaxf(vmax, finite_or_zero(vf[i][j]));
         }
-    };
-#pragma unroll
-    for (int i = 0; i < kPageTokens; ++i)
-        if (i < mine) load_row(i);
-#pragma unroll
-    for (int i = 0; i < kPageTokens; ++i) {
-        if (i >= mine) break;
-        float cs[E], sn[E];
-        load_rope_row<D>(a, static_cast<int>(begin) + wave + i * WAVES, lane, cs, sn);
-        turn_row(i, cs, sn);
     }
     if (id < 0 || id >= p.pages) return;  // the same for all waves
     const int64_t base = static_cast<int64_t>(id) * p.kv_heads + g;
@@ -371,36 +390,45 @@ __global__ __launch_bounds__(WAVES* kWave) void k_paged_append(const AppendArgs 
     // Exact for the powers of two that this kernel writes.
     const float ki = 1.0f / ks, vi = 1.0f / vs;
     if (n == 1) {  // one row: nothing to gain from LDS
-        if (wave == 0)
+        if (wave == 0 && sub == 0) {
+            *reinterpret_cast<uint32_t*>(kp + r0 * D + place) = e4m3x4(kf[0], ki);
+            const uint32_t w4 = e4m3x4(vf[0], vi);
 #pragma unroll
-            for (int j = 0; j < E; ++j) {
-                const int d = lane + kWave * j;
-                kp[r0 * D + d] = e4m3(kf[0][j] * ki);
-                vp[d * kPage + r0] = e4m3(vf[0][j] * vi);
-            }
+            for (int j = 0; j < E; ++j) vp[(place + j) * kPage + r0] = static_cast<uint8_t>(w4 >> (8 * j));
+        }
         return;
     }
+#pragma unroll
+    for (int i = 0; i < kPageTokens / H; ++i)
+        if (any_at(i) && row_at(i) < n)
+            *reinterpret_cast<uint32_t*>(kp + (r0 + row_at(i)) * D + place) = e4m3x4(kf[i], ki);
     uint8_t* bytes = reinterpret_cast<uint8_t*>(tile);
 #pragma unroll
-    for (int i = 0; i < kPageTokens; ++i) {
-        if (i >= mine) break;
+    for (int i = 0; i < kPageTokens / H; ++i)
+        if (any_at(i) && row_at(i) < n) {
+            const uint32_t w4 = e4m3x4(vf[i], vi);
 #pragma unroll
-        for (int j = 0; j < E; ++j) bytes[(wave + i * WAVES) * D + lane + kWave * j] = e4m3(kf[i][j] * ki);
+            for (int j = 0; j < E; ++j) bytes[(place + j) * kLine + r0 + row_at(i)] = static_cast<uint8_t>(w4 >> (8 * j));
+        }
+    __syncthreads();
+    // Whole words of V's lines where they are new, single bytes at the ends.
+    constexpr int kWords = kPage / 4;
+    for (int i = threadIdx.x; i < D * kWords; i += kThreads) {
+        const int line = i / kWords, c = (i - line * kWords) * 4;
+        if (c + 4 <= r0 || c >= r0 + n) continue;
+        const uint32_t w4 = tile[line * (kLine / 4) + c / 4];
+        uint8_t* at = vp + line * kPage + c;
+        if (c >= r0 && c + 4 <= r0 + n) {
+            *reinterpret_cast<uint32_t*>(at) = w4;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (c + k >= r0 && c + k < r0 + n) at[k] = static_cast<uint8_t>(w4 >> (8 * k));
+        }
     }
-    __syncthreads();
-    store_lines(bytes, D, kp + r0 * D, n, D, 0, D, kThreads);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kPageTokens; ++i) {
-        if (i >= mine) break;
-#pragma unroll
-        for (int j = 0; j < E; ++j) bytes[(lane + kWave * j) * kLine + r0 + wave + i * WAVES] = e4m3(vf[i][j] * vi);
-    }
-    __syncthreads();
-    store_lines(bytes, kLine, vp, D, kPage, r0, n, kThreads);
 }
 
-template <int D>
+template <int D, int DT>
 int launch_append(AppendArgs& a, int64_t tokens, int kv_heads, int64_t batch, hipStream_t stream) {
     const int waves = (1 << a.p.page_shift) / kPageTokens;
     const int64_t kv_blocks = ((tokens >> a.p.page_shift) + 2 * batch) * kv_heads;
@@ -409,12 +437,21 @@ int launch_append(AppendArgs& a, int64_t tokens, int kv_heads, int64_t batch, hi
     a.kv_blocks = static_cast<int32_t>(kv_blocks);
     const dim3 grid(static_cast<unsigned>(blocks)), block(static_cast<unsigned>(waves * kWave));
     switch (waves) {
-        case 2: hipLaunchKernelGGL((k_paged_append<D, 2>), grid, block, 0, stream, a); break;
-        case 4: hipLaunchKernelGGL((k_paged_append<D, 4>), grid, block, 0, stream, a); break;
-        case 8: hipLaunchKernelGGL((k_paged_append<D, 8>), grid, block, 0, stream, a); break;
-        default: hipLaunchKernelGGL((k_paged_append<D, 16>), grid, block, 0, stream, a); break;
+        case 2: hipLaunchKernelGGL((k_paged_append<D, DT, 2>), grid, block, 0, stream, a); break;
+        case 4: hipLaunchKernelGGL((k_paged_append<D, DT, 4>), grid, block, 0, stream, a); break;
+        case 8: hipLaunchKernelGGL((k_paged_append<D, DT, 8>), grid, block, 0, stream, a); break;
+        default: hipLaunchKernelGGL((k_paged_append<D, DT, 16>), grid, block, 0, stream, a); break;
     }
     return nq::launch_status();
+}
+
+template <int D>
+int launch_append(AppendArgs& a, int dtype, int64_t tokens, int kv_heads, int64_t batch, hipStream_t stream) {
+    switch (dtype) {
+        case NQ_DTYPE_F32: return launch_append<D, NQ_DTYPE_F32>(a, tokens, kv_heads, batch, stream);
+        case NQ_DTYPE_F16: return launch_append<D, NQ_DTYPE_F16>(a, tokens, kv_heads, batch, stream);
+        default: return launch_append<D, NQ_DTYPE_BF16>(a, tokens, kv_heads, batch, stream);
+    }
 }
 
 bool float_code(int d) { return nq::is_float_dtype(d); }
@@ -434,13 +471,13 @@ extern "C" int nq_paged_append(const void* q, const void* k, const void* v, int3
     if (!(eps >= 0.0f)) return NQ_ERR_ARGUMENT;
     a.q = q; a.k = k; a.v = v; a.q_norm = q_norm; a.k_norm = k_norm;
     a.cos_table = cos_table; a.sin_table = sin_table; a.q_out = q_out;
-    a.eps = eps; a.dtype = dtype; a.norm_dtype = norm_dtype; a.q_dtype = q_out_dtype; a.q_heads = q_heads;
+    a.eps = eps; a.norm_dtype = norm_dtype; a.q_dtype = q_out_dtype; a.q_heads = q_heads;
     a.rope_rows = static_cast<int32_t>(rope_positions < 0x7fffffff ? rope_positions : 0x7fffffff);
     a.q_groups = (q_heads + kQHeads - 1) / kQHeads;
     hipStream_t st = static_cast<hipStream_t>(stream);
     switch (kv->head_dim) {
-        case 64: return launch_append<64>(a, tokens, kv->kv_heads, kv->batch, st);
-        case 128: return launch_append<128>(a, tokens, kv->kv_heads, kv->batch, st);
-        default: return launch_append<256>(a, tokens, kv->kv_heads, kv->batch, st);
+        case 64: return launch_append<64>(a, dtype, tokens, kv->kv_heads, kv->batch, st);
+        case 128: return launch_append<128>(a, dtype, tokens, kv->kv_heads, kv->batch, st);
+        default: return launch_append<256>(a, dtype, tokens, kv->kv_heads, kv->batch, st);
     }
 }
