@@ -10,12 +10,14 @@
 // what the second product's B operand wants, so P never leaves its registers.
 // V lies transposed in the cache, so its A operand is as many consecutive bytes.
 //
-// Precision: an e4m3 byte is exact in bf16. q enters as one bf16 part, two or
-// three (bf16 / fp16 / fp32: 8, 16, 24 bits: exact), so scores carry fp32
-// rounding only. The weights enter the second product as two bf16 parts (16
-// bits, 2^-17 of a weight at most) for 16-bit outputs, whose own rounding is
-// 2^-9 or 2^-12, and as three for fp32 outputs. Scales: K's multiplies the
-// fp32 score, V's the fp32 weight before it is split.
+// Precision: an e4m3 byte is exact in bf16 and in fp16. bf16 and fp16 queries
+// enter as they are; an fp32 query row enters as two fp16 parts after a power of
+// two that brings its largest value to 2^14..2^15 (24 bits of every value down to
+// 2^-28 of that, 2^-25 * 2^-14 of it below): scores carry fp32 rounding only. The
+// weights enter the second product as two bf16 parts (16 bits, 2^-17 of a weight
+// at most) for 16-bit outputs, whose own rounding is 2^-9 or 2^-12, and as three
+// for fp32 outputs. Scales: K's multiplies the fp32 score; V's goes into the
+// widening of its bytes (a power of two; any other multiplies the fp32 weight).
 #pragma once
 
 #include "nq_paged.h"
@@ -25,6 +27,8 @@ namespace paged {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 64;  // cache rows that splits are counted in
@@ -97,12 +101,12 @@ __device__ __forceinline__ float rows_sum(float x) {
     return __uint_as_float(c[0]) + __uint_as_float(c[1]);
 }
 
-// Eight e4m3 bytes as bf16 (exact).
-__device__ __forceinline__ bf16x8 widen(uint32_t a, uint32_t b) {
-    const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false);
-    const bf16x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
-    const bf16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
-    const bf16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+// Eight e4m3 bytes times a power of two as bf16 (exact).
+__device__ __forceinline__ bf16x8 widen(uint32_t a, uint32_t b, float power) {
+    const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, power, false);
+    const bf16x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, power, true);
+    const bf16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, power, false);
+    const bf16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, power, true);
     return bf16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
 }
 
@@ -113,8 +117,7 @@ __device__ __forceinline__ uint32_t high_halves(float a, float b) {
 __device__ __forceinline__ float cut(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
 // PARTS bf16 parts of eight values: each but the last cuts 8 bits off what the
-// ones before left (exact), the last rounds (the third of three is exact). An
-// infinite or NaN value is its own first part and leaves nothing.
+// ones before left (exact), the last rounds (the third of three is exact).
 template <int PARTS>
 __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&part)[PARTS]) {
     float rest[8];
@@ -140,40 +143,76 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&part)[PARTS
     }
 }
 
-// q parts: 3 from fp32, 2 from fp16, 1 from bf16.
-template <int QP>
-__device__ __forceinline__ void load_q8(const void* q, int64_t at, bool on, bf16x8 (&part)[QP]) {
-    if constexpr (QP == 1) {
-        u32x4 v = {0, 0, 0, 0};
-        if (on) v = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(q) + at);
-        part[0] = __builtin_bit_cast(bf16x8, v);
+// The first product's operands: K's bytes widened to the query's 16-bit type.
+template <int QT>
+struct Query {
+    static constexpr bool kHalf = QT != NQ_DTYPE_BF16;  // fp16 operands
+    static constexpr int kParts = QT == NQ_DTYPE_F32 ? 2 : 1;
+};
+
+template <int QT>
+__device__ __forceinline__ u32x4 widen_k(uint32_t a, uint32_t b) {
+    if constexpr (Query<QT>::kHalf) {
+        const f16x2 x[4] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false),
+                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true),
+                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false),
+                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true)};
+        return u32x4{__builtin_bit_cast(uint32_t, x[0]), __builtin_bit_cast(uint32_t, x[1]),
+                     __builtin_bit_cast(uint32_t, x[2]), __builtin_bit_cast(uint32_t, x[3])};
     } else {
-        float x[8];
-        if constexpr (QP == 2) {
-            typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-            f16x8 v = {};
-            if (on) v = *reinterpret_cast<const f16x8*>(static_cast<const _Float16*>(q) + at);
+        return __builtin_bit_cast(u32x4, widen(a, b, 1.0f));
+    }
+}
+
+template <int QT>
+__device__ __forceinline__ f32x4 mfma_k(u32x4 k, u32x4 q, f32x4 c) {
+    if constexpr (Query<QT>::kHalf)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
+}
+
+// A lane's share of a query row, STEPS times eight values at `at` + 64 (c / 2) +
+// 8 (c & 1), as parts; returns the power of two that the parts have to be
+// multiplied by (1 but for fp32).
+template <int QT, int STEPS>
+__device__ __forceinline__ float load_query(const void* q, int64_t at, bool on, u32x4 (&part)[STEPS][Query<QT>::kParts]) {
+    if constexpr (QT != NQ_DTYPE_F32) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = static_cast<float>(v[j]);
-        } else {
-            f32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-            if (on) {
-                a = *reinterpret_cast<const f32x4*>(static_cast<const float*>(q) + at);
-                b = *reinterpret_cast<const f32x4*>(static_cast<const float*>(q) + at + 4);
-            }
+        for (int c = 0; c < STEPS; ++c)
+            part[c][0] = on ? *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(q) + at + 64 * (c / 2) + 8 * (c & 1))
+                            : u32x4{0, 0, 0, 0};
+        return 1.0f;
+    } else {
+        f32x4 x[STEPS][2];
+        float most = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[j] = a[j];
-                x[4 + j] = b[j];
+        for (int c = 0; c < STEPS; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                x[c][h] = on ? *reinterpret_cast<const f32x4*>(static_cast<const float*>(q) + at + 64 * (c / 2) + 8 * (c & 1) + 4 * h)
+                             : f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[c][h][j]));
             }
+        most = rows_max(most);
+        // 2^e <= the largest value < 2^(e + 1); from 2^-100 on, so that 2^(14 - e) is a number.
+        const int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100);
+        const float up = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c) {
+            f16x8 high, low;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float y = x[c][j >> 2][j & 3] * up;
+                high[j] = static_cast<_Float16>(y);
+                // What is not finite has no remainder.
+                low[j] = fabsf(y) < INFINITY ? static_cast<_Float16>(y - static_cast<float>(high[j])) : static_cast<_Float16>(0.0f);
+            }
+            part[c][0] = __builtin_bit_cast(u32x4, high);
+            part[c][1] = __builtin_bit_cast(u32x4, low);
         }
-        split8<QP>(x, part);
-        // What is not finite has no remainder.
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (!(fabsf(x[j]) < INFINITY))
-#pragma unroll
-                for (int s = 1; s < QP; ++s) part[s][j] = static_cast<__bf16>(0.0f);
+        return __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
     }
 }
 
@@ -200,7 +239,6 @@ __device__ __forceinline__ void store4(void* out, int dtype, int64_t at, const f
             const bf16x2 h = {static_cast<__bf16>(v[2 * i]), static_cast<__bf16>(v[2 * i + 1])};
             w[i] = __builtin_bit_cast(uint32_t, h);
         } else {
-            typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
             const f16x2 h = {static_cast<_Float16>(v[2 * i]), static_cast<_Float16>(v[2 * i + 1])};
             w[i] = __builtin_bit_cast(uint32_t, h);
         }
@@ -208,28 +246,26 @@ __device__ __forceinline__ void store4(void* out, int dtype, int64_t at, const f
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = make_uint2(w[0], w[1]);
 }
 
-// Waves of a SIMD that the registers are held to.
-template <int D>
-constexpr int kWavesFor = D == 256 ? 1 : 2;
-template <int D>
-constexpr int kTileFor = D == 256 ? 32 : 64;
-
 // One workgroup of four waves: a slot of query rows of one kv head over one
 // split of the cache. SHARED: the waves hold the same 16 NT rows and take the
 // split's tiles in turn (few query rows: the cache's bytes are the work);
-// otherwise each wave holds 16 NT rows of its own and all take every tile.
-template <int D, int QP, int PP, int NT, int TILE, bool SHARED>
-__global__ __launch_bounds__(256, kWavesFor<D>) void k_paged_attention(const AttnArgs a) {
+// otherwise each wave has 16 NT rows of its own, whose parts wait in LDS (in
+// registers they would leave room for one wave to a SIMD, and nothing would fill
+// the matrix unit during a softmax), and all take every tile.
+template <int D, int QT, int PP, int NT, int TILE, bool SHARED>
+__global__ __launch_bounds__(256, D == 256 ? 1 : SHARED ? 2 : 2) void k_paged_attention(const AttnArgs a) {
     constexpr int kRows = (SHARED ? 1 : 4) * 16 * NT;
     constexpr int kChunks = D / 64, kDims = D / 16;
     constexpr int kBlock = TILE / 4;   // consecutive cache rows of a lane: of V, and of the scores
     constexpr int kScores = TILE / 16, kSteps = TILE / 32, kWords = kBlock / 4;
+    constexpr bool kEarly = SHARED || D == 256;  // the next K before the softmax, with registers of its own
     const Pages& p = a.p;
     const int lane = threadIdx.x & (kWave - 1), n = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int g = blockIdx.x % p.kv_heads;
     const int rest = blockIdx.x / p.kv_heads;
-    const int split = rest % a.splits, slot = rest / a.splits;
+    // Of a prompt's rows the last see the most: their slots go first.
+    const int split = rest % a.splits, slot = SHARED ? rest / a.splits : a.slots - 1 - rest / a.splits;
     const Found found = sequence_at(p, slot, [&](int i, int begin) { return first_slot_of(i, begin, a.group, kRows); });
     const SlotSpan s = slot_span(p, found, slot, a.group, kRows);
     if (s.rows == 0) return;
@@ -238,10 +274,13 @@ __global__ __launch_bounds__(256, kWavesFor<D>) void k_paged_attention(const Att
     if (split > 0 && split >= plan.active) return;
 
     // This wave's query rows: row numbers, positions (-1: sees nothing), q.
+    constexpr int QP = Query<QT>::kParts, kQSteps = 2 * kChunks;
+    __shared__ u32x4 q_lds[SHARED ? 1 : 4][SHARED ? 1 : kQSteps * NT * QP][kWave];
+    u32x4 q_regs[SHARED ? NT : 1][kQSteps][QP];
     const int wave_row = SHARED ? 0 : wave * 16 * NT;
     int row[NT], pos[NT];
+    float q_scale[NT];
     int64_t out_at[NT];
-    bf16x8 qf[NT][2 * kChunks][QP];
     int low_pos = 0x7fffffff, high_pos = -1;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -251,9 +290,13 @@ __global__ __launch_bounds__(256, kWavesFor<D>) void k_paged_attention(const Att
         const int place = r / a.group, head = g * a.group + r - place * a.group;
         pos[t] = on ? row_of(s.context, place, cache_rows) : -1;
         out_at[t] = (static_cast<int64_t>(s.begin + place) * a.q_heads + head) * D;
+        q_scale[t] = a.scale * load_query<QT, kQSteps>(a.q, out_at[t] + 16 * grp, on, q_regs[SHARED ? t : 0]);
+        if constexpr (!SHARED) {
 #pragma unroll
-        for (int c = 0; c < 2 * kChunks; ++c)
-            load_q8<QP>(a.q, out_at[t] + 64 * (c / 2) + 16 * grp + 8 * (c & 1), on, qf[t][c]);
+            for (int c = 0; c < kQSteps; ++c)
+#pragma unroll
+                for (int x = 0; x < QP; ++x) q_lds[wave][(c * NT + t) * QP + x][lane] = q_regs[0][c][x];
+        }
         int lo = on ? pos[t] : 0x7fffffff, hi = pos[t];
 #pragma unroll
         for (int m = 1; m < 16; m *= 2) {
@@ -263,9 +306,11 @@ __global__ __launch_bounds__(256, kWavesFor<D>) void k_paged_attention(const Att
         low_pos = min(low_pos, __builtin_amdgcn_readfirstlane(lo));
         high_pos = max(high_pos, __builtin_amdgcn_readfirstlane(hi));
     }
+    // A lane reads back what it wrote itself: nothing to wait for but the LDS.
 
     f32x4 acc[kDims][NT];
     float m_run[NT], l_run[NT];
+    uint32_t nan_at[NT][(kDims + 7) / 8] = {};  // a bit for each output that a NaN of V reaches behind a mask
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         m_run[t] = -INFINITY;
@@ -331,7 +376,7 @@ __global__ __launch_bounds__(256, kWavesFor<D>) void k_paged_attention(const Att
         const bool more = tile + step < tile_end;
         const int then = more ? tile + step : tile;
         const bool bad = static_cast<uint32_t>(id_v) >= static_cast<uint32_t>(p.pages);
-        const float ks = bad ? __builtin_nanf("") : k_scale * a.scale, vs = bad ? __builtin_nanf("") : v_scale;
+        const float ks = bad ? __builtin_nanf("") : k_scale, vs = bad ? 1.0f : v_scale;
         if (more) {
             id_k = next_k;
             id_v = next_v;
@@ -342,29 +387,99 @@ __global__ __launch_bounds__(256, kWavesFor<D>) void k_paged_attention(const Att
 
         f32x4 sc[kScores][NT];
 #pragma unroll
-        for (int t = 0; t < kScores; ++t) {
+        for (int t = 0; t < kScores; ++t)
 #pragma unroll
             for (int u = 0; u < NT; ++u) sc[t][u] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-                const bf16x8 k0 = widen(kf[t][c][0], kf[t][c][1]), k1 = widen(kf[t][c][2], kf[t][c][3]);
+        for (int c = 0; c < kQSteps; ++c) {
+            u32x4 qf[NT][QP];
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int x = 0; x < QP; ++x)
+                    qf[u][x] = SHARED ? q_regs[SHARED ? u : 0][c][x] : q_lds[SHARED ? 0 : wave][SHARED ? 0 : (c * NT + u) * QP + x][lane];
+#pragma unroll
+            for (int t = 0; t < kScores; ++t) {
+                const u32x4 k = widen_k<QT>(kf[t][c / 2][2 * (c & 1)], kf[t][c / 2][2 * (c & 1) + 1]);
 #pragma unroll
                 for (int u = 0; u < NT; ++u)
 #pragma unroll
-                    for (int s2 = QP - 1; s2 >= 0; --s2) {
-                        sc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qf[u][2 * c][s2], sc[t][u], 0, 0, 0);
-                        sc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qf[u][2 * c + 1][s2], sc[t][u], 0, 0, 0);
-                    }
+                    for (int x = QP - 1; x >= 0; --x) sc[t][u] = mfma_k<QT>(k, qf[u][x], sc[t][u]);
             }
         }
 
-        __builtin_amdgcn_sched_barrier(0);
-        load_scales(id_v);
-        __builtin_amdgcn_sched_barrier(0);
-        load_k(then, id_k);
-        __builtin_amdgcn_sched_barrier(0);
+        // Many query rows (not early): K's registers serve the softmax meanwhile, and
+        // the SIMD's other wave fills the wait for the next ones.
+        const auto load_next_k = [&] {
+            __builtin_amdgcn_sched_barrier(0);
+            load_scales(id_v);
+            __builtin_amdgcn_sched_barrier(0);
+            load_k(then, id_k);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if constexpr (kEarly) load_next_k();
+
+        // What the scores and the weights are multiplied by. A power of two for V, as
+        // the append writes, goes into its widening instead.
+        const uint32_t v_bits = __float_as_uint(vs);
+        const bool v_power = (v_bits & 0x807fffffu) == 0 && v_bits - 1u < 0x7f7fffffu;
+        const float v_up = v_power ? vs : 1.0f;
+        float f[NT], weight_up[NT];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            f[u] = ks * q_scale[u];
+            weight_up[u] = v_power ? 1.0f : vs;
+        }
 
         const bool masked = base + TILE > low_pos + 1;  // uniform: some row of the wave does not see them all
+        if (masked) {
+            // A block that a row does not see may have any scale; one that it sees in
+            // part has a page.
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                const int seen = pos[u] + 1 - (base + kBlock * grp);
+                if (seen <= 0) f[u] = weight_up[u] = 1.0f;
+#pragma unroll
+                for (int j = 0; j < kBlock; ++j)
+                    if (j >= seen) sc[j >> 2][u][j & 3] = -INFINITY;
+            }
+        }
+
+        bf16x8 pf[NT][kSteps][PP];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            float x[kBlock], top = sc[0][u][0];
+#pragma unroll
+            for (int j = 1; j < kBlock; ++j) top = fmaxf(top, sc[j >> 2][u][j & 3]);
+            const float m_new = fmaxf(m_run[u], rows_max(top * f[u]));
+            // Nothing seen so far (or only -inf): subtract 0, the weights are 0.
+            const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+            if (__ballot(m_new != m_run[u])) {
+                const float keep = exp2_hw(m_run[u] - m_use);
+                l_run[u] *= keep;
+#pragma unroll
+                for (int d = 0; d < kDims; ++d) acc[d][u] *= keep;
+                m_run[u] = m_new;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kBlock; ++j) {
+                x[j] = exp2_hw(fmaf(sc[j >> 2][u][j & 3], f[u], -m_use));
+                sum += x[j];
+            }
+            if (__ballot(weight_up[u] != 1.0f)) {
+#pragma unroll
+                for (int j = 0; j < kBlock; ++j) x[j] *= weight_up[u];
+            }
+            l_run[u] += sum;
+#pragma unroll
+            for (int h = 0; h < kSteps; ++h) {
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = x[8 * h + j];
+                split8<PP>(y, pf[u][h]);
+            }
+        }
         if (masked) {
             // Bytes of V rows that nobody sees may be anything. Among those
             // that only some see, a NaN must not meet a weight of zero: it is
@@ -395,10 +510,10 @@ __global__ __launch_bounds__(256, kWavesFor<D>) void k_paged_attention(const Att
                         f32x4 hits = {0, 0, 0, 0};
 #pragma unroll
                         for (int h = 0; h < kSteps; ++h)
-                            hits = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(one[2 * h], one[2 * h + 1]), see[h], hits, 0, 0, 0);
+                            hits = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(one[2 * h], one[2 * h + 1], 1.0f), see[h], hits, 0, 0, 0);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (hits[i] > 0.0f) acc[d][u][i] = __builtin_nanf("");
+                            if (hits[i] > 0.0f) nan_at[u][d / 8] |= 1u << (4 * (d % 8) + i);
                     }
                 }
 #pragma unroll
@@ -407,60 +522,31 @@ __global__ __launch_bounds__(256, kWavesFor<D>) void k_paged_attention(const Att
                     for (int i = 0; i < kWords; ++i) vf[d][i] &= ~((nan_bytes(vf[d][i]) >> 7) * 0xffu);
             }
         }
-
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            float x[kBlock], top = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < kBlock; ++j) {
-                x[j] = sc[j >> 2][u][j & 3] * ks;
-                if (masked) x[j] = base + kBlock * grp + j <= pos[u] ? x[j] : -INFINITY;
-                top = fmaxf(top, x[j]);
-            }
-            const float m_new = fmaxf(m_run[u], rows_max(top));
-            // Nothing seen so far (or only -inf): subtract 0, the weights are 0.
-            const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-            if (__ballot(m_new != m_run[u])) {
-                const float keep = exp2_hw(m_run[u] - m_use);
-                l_run[u] *= keep;
-#pragma unroll
-                for (int d = 0; d < kDims; ++d) acc[d][u] *= keep;
-                m_run[u] = m_new;
-            }
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < kBlock; ++j) {
-                x[j] = exp2_hw(x[j] - m_use);
-                sum += x[j];
-                x[j] *= vs;
-                if (masked) x[j] = base + kBlock * grp + j <= pos[u] ? x[j] : 0.0f;  // a scale that nobody sees may be anything
-            }
-            l_run[u] += sum;
-            bf16x8 pf[kSteps][PP];
+        for (int d = 0; d < kDims; ++d)
 #pragma unroll
             for (int h = 0; h < kSteps; ++h) {
-                float y[8];
+                const bf16x8 v = widen(vf[d][2 * h], vf[d][2 * h + 1], v_up);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = x[8 * h + j];
-                split8<PP>(y, pf[h]);
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int x = PP - 1; x >= 0; --x)
+                        acc[d][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pf[u][h][x], acc[d][u], 0, 0, 0);
             }
-#pragma unroll
-            for (int d = 0; d < kDims; ++d) {
-#pragma unroll
-                for (int h = 0; h < kSteps; ++h) {
-                    const bf16x8 v = widen(vf[d][2 * h], vf[d][2 * h + 1]);
-#pragma unroll
-                    for (int s2 = PP - 1; s2 >= 0; --s2)
-                        acc[d][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pf[h][s2], acc[d][u], 0, 0, 0);
-                }
-            }
-        }
+        if constexpr (!kEarly) load_next_k();
         __builtin_amdgcn_sched_barrier(0);
         load_v(then, id_v);
         __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int u = 0; u < NT; ++u) l_run[u] = rows_sum(l_run[u]);
+    for (int u = 0; u < NT; ++u) {
+        l_run[u] = rows_sum(l_run[u]);
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (nan_at[u][d / 8] >> (4 * (d % 8) + i) & 1u) acc[d][u][i] = __builtin_nanf("");
+    }
 
     // The waves' shares of the same rows meet in LDS, in wave order.
     __shared__ float join_ml[SHARED ? 4 : 1][2][16 * NT];
@@ -533,32 +619,43 @@ struct AttnPlan {
     bool shared;
 };
 
+// Query rows of a wave where each has its own: 32, of 256-wide heads 16.
+template <int D>
+constexpr int kOwnTiles = D == 256 ? 1 : 2;
+// Cache rows that a wave takes at once.
+template <int D, bool SHARED>
+constexpr int kRowsAtOnce = D == 256 ? 32 : SHARED ? 64 : 64;
+
+constexpr int own_rows(int head_dim) { return 64 * (head_dim == 256 ? 1 : 2); }
+
 template <int D>
 int launch_paged_attention(const AttnArgs& a, const AttnPlan& plan, int q_dtype, hipStream_t stream);
 
-template <int D, int QP, int PP>
+template <int D, int QT, int PP>
 int launch_attention_as(const AttnArgs& a, const AttnPlan& plan, hipStream_t stream) {
     const int64_t blocks = static_cast<int64_t>(plan.slots) * plan.splits * a.p.kv_heads;
     if (blocks > 0x7fffffff) return NQ_ERR_SHAPE;
     const dim3 grid(static_cast<unsigned>(blocks));
     if (plan.shared) {
-        hipLaunchKernelGGL((k_paged_attention<D, QP, PP, 1, kTileFor<D>, true>), grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 1, kRowsAtOnce<D, true>, true>), grid, dim3(256), 0, stream, a);
     } else {
-        hipLaunchKernelGGL((k_paged_attention<D, QP, PP, 1, kTileFor<D>, false>), grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_paged_attention<D, QT, PP, kOwnTiles<D>, kRowsAtOnce<D, false>, false>), grid, dim3(256), 0, stream, a);
     }
     return nq::launch_status();
 }
 
+template <int D, int QT>
+int launch_attention_out(const AttnArgs& a, const AttnPlan& plan, hipStream_t stream) {
+    return a.out_dtype == NQ_DTYPE_F32 ? launch_attention_as<D, QT, 3>(a, plan, stream)
+                                       : launch_attention_as<D, QT, 2>(a, plan, stream);
+}
+
 template <int D>
 int launch_attention_for(const AttnArgs& a, const AttnPlan& plan, int q_dtype, hipStream_t stream) {
-    const bool wide = a.out_dtype == NQ_DTYPE_F32;
     switch (q_dtype) {
-        case NQ_DTYPE_F32:
-            return wide ? launch_attention_as<D, 3, 3>(a, plan, stream) : launch_attention_as<D, 3, 2>(a, plan, stream);
-        case NQ_DTYPE_F16:
-            return wide ? launch_attention_as<D, 2, 3>(a, plan, stream) : launch_attention_as<D, 2, 2>(a, plan, stream);
-        default:
-            return wide ? launch_attention_as<D, 1, 3>(a, plan, stream) : launch_attention_as<D, 1, 2>(a, plan, stream);
+        case NQ_DTYPE_F32: return launch_attention_out<D, NQ_DTYPE_F32>(a, plan, stream);
+        case NQ_DTYPE_F16: return launch_attention_out<D, NQ_DTYPE_F16>(a, plan, stream);
+        default: return launch_attention_out<D, NQ_DTYPE_BF16>(a, plan, stream);
     }
 }
 

@@ -78,15 +78,15 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows)
 
 // Few query rows to a sequence: a slot of 16 rows whose waves share them, and
 // the cache split until the chip has about two workgroups to a CU; more: slots
-// of 64 rows, 16 to a wave.
-AttnPlan plan_attention(int64_t tokens, int64_t batch, int q_heads, int kv_heads, int64_t cache_rows) {
+// of 128 rows (64 of 256-wide heads), a quarter to each wave.
+AttnPlan plan_attention(int64_t tokens, int64_t batch, int q_heads, int kv_heads, int head_dim, int64_t cache_rows) {
     AttnPlan plan;
     const int64_t rows = tokens * (q_heads / kv_heads);
     plan.shared = rows <= 16 * batch;
-    plan.rows = plan.shared ? 16 : 64;
+    plan.rows = plan.shared ? 16 : own_rows(head_dim);
     plan.slots = static_cast<int>(rows / plan.rows + batch);
     const int64_t tiles = (cache_rows + kTile - 1) / kTile, units = static_cast<int64_t>(plan.slots) * kv_heads;
-    const int64_t target = batch > 1 ? 1024 : 512;
+    const int64_t target = plan.shared ? (batch > 1 ? 1024 : 512) : 256;
     plan.least = plan.shared && units * ((tiles + 7) / 8) < 512 ? 4 : 8;
     const int64_t most = (tiles + plan.least - 1) / plan.least;
     int64_t splits = target / units;
@@ -108,7 +108,7 @@ extern "C" int64_t nq_paged_attention_workspace_bytes(int64_t tokens, int64_t ba
         table_pages > 0x7fffffff / page_size || (head_dim != 64 && head_dim != 128 && head_dim != 256))
         return -1;
     if (tokens * q_heads > 0x3fffffff) return -1;
-    const AttnPlan plan = plan_attention(tokens, batch, q_heads, kv_heads, table_pages * page_size);
+    const AttnPlan plan = plan_attention(tokens, batch, q_heads, kv_heads, head_dim, table_pages * page_size);
     return partial_rows(plan, kv_heads) * (2 + head_dim) * static_cast<int64_t>(sizeof(float));
 }
 
@@ -127,7 +127,7 @@ extern "C" int nq_paged_attention(const void* q, int32_t q_dtype, int64_t tokens
     if (workspace_bytes < need) return NQ_ERR_WORKSPACE;
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
         return NQ_ERR_ALIGNMENT;
-    const AttnPlan plan = plan_attention(tokens, kv->batch, q_heads, kv->kv_heads, kv->table_pages * kv->page_size);
+    const AttnPlan plan = plan_attention(tokens, kv->batch, q_heads, kv->kv_heads, kv->head_dim, kv->table_pages * kv->page_size);
     a.q = q;
     a.out = out;
     a.partial_o = static_cast<float*>(workspace);
