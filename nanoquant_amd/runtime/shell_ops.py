@@ -473,6 +473,7 @@ def paged_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, device
 
 
 _PAGE_SIZES = (16, 32, 64, 128)
+_HEAD_DIMS = (64, 128, 256)
 
 
 def _paged_kv(name: str, device: torch.device, cache: PagedCache, page_table: torch.Tensor,
@@ -481,36 +482,34 @@ def _paged_kv(name: str, device: torch.device, cache: PagedCache, page_table: to
 
     k, v, k_scales, v_scales = cache
     _check_device(name, device, k, v, k_scales, v_scales, page_table, query_starts, context_lens)
-    if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or k.ndim != 4:
+    if k.dtype is not torch.float8_e4m3fn or v.dtype is not torch.float8_e4m3fn or k.ndim != 4:
         raise ValueError(f"{name} cache pages must be 4-D float8_e4m3fn")
     pages, kv_heads, page_size, head_dim = k.shape
+    scales = (pages, kv_heads)
     if v.shape != (pages, kv_heads, head_dim, page_size):
         raise ValueError(f"{name} cache must be K [pages, kv_heads, page_size, head_dim], V [pages, kv_heads, head_dim, page_size]")
-    if page_size not in _PAGE_SIZES or head_dim not in (64, 128, 256) or not pages or not kv_heads:
+    if page_size not in _PAGE_SIZES or head_dim not in _HEAD_DIMS or not pages or not kv_heads:
         raise ValueError(f"{name} page size must be 16, 32, 64 or 128 and head_dim 64, 128 or 256")
-    if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32 or k_scales.shape != (pages, kv_heads) \
-            or v_scales.shape != (pages, kv_heads):
+    if k_scales.dtype is not torch.float32 or v_scales.dtype is not torch.float32 or k_scales.shape != scales \
+            or v_scales.shape != scales:
         raise ValueError(f"{name} cache scales must be fp32 [pages, kv_heads]")
-    if page_table.dtype != torch.int32 or query_starts.dtype != torch.int32 or context_lens.dtype != torch.int32:
+    if page_table.dtype is not torch.int32 or query_starts.dtype is not torch.int32 \
+            or context_lens.dtype is not torch.int32:
         raise ValueError(f"{name} page_table, query_starts and context_lens must be int32")
-    if page_table.ndim != 2 or context_lens.ndim != 1 or query_starts.ndim != 1:
-        raise ValueError(f"{name} takes page_table [batch, pages], query_starts [batch + 1] and context_lens [batch]")
-    batch, table_pages = page_table.shape
-    if not batch or not table_pages or context_lens.shape[0] != batch or query_starts.shape[0] != batch + 1:
+    shape = page_table.shape
+    if len(shape) != 2 or not shape[0] or not shape[1] or context_lens.shape != (shape[0],) \
+            or query_starts.shape != (shape[0] + 1,):
         raise ValueError(f"{name} takes page_table [batch, pages], query_starts [batch + 1] and context_lens [batch]")
     return _native.PagedKv(k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), pages, kv_heads,
-                           head_dim, page_size, 0, page_table.data_ptr(), table_pages, query_starts.data_ptr(),
-                           context_lens.data_ptr(), batch)
+                           head_dim, page_size, 0, page_table.data_ptr(), shape[1], query_starts.data_ptr(),
+                           context_lens.data_ptr(), shape[0])
 
 
-def _on_device(device: torch.device, function, *args) -> int:
-    """``function(*args)`` with `device` current: a default stream's handle is
-    the same on every device, the launch goes to the current one's."""
+def _elsewhere(device: torch.device) -> bool:
+    """Whether another device than `device` is current. A default stream's handle
+    is the same on every device and a launch goes to the current one's."""
 
-    if torch.cuda.current_device() == device.index:
-        return function(*args)
-    with torch.cuda.device(device):
-        return function(*args)
+    return device.type == "cuda" and torch._C._cuda_getDevice() != device.index
 
 
 def launch_paged_append(
@@ -540,16 +539,23 @@ def launch_paged_append(
     for many sequences."""
 
     device = q.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return launch_paged_append(
+                q, k, v, cache, q_heads=q_heads, q_norm=q_norm, k_norm=k_norm, eps=eps, cos=cos, sin=sin,
+                page_table=page_table, query_starts=query_starts, context_lens=context_lens, q_out=q_out, q_dtype=q_dtype)
     _check_device("paged append", device, q, k, v, q_norm, k_norm, cos, sin, q_out)
     kv = _paged_kv("paged append", device, cache, page_table, query_starts, context_lens)
     kv_heads, head_dim = kv.kv_heads, kv.head_dim
     if q_heads < 1 or q_heads % kv_heads:
         raise ValueError("paged append q heads must be a multiple of the cache's kv heads")
-    tokens = q.numel() // (q_heads * head_dim)
-    if tokens < 1 or q.numel() != tokens * q_heads * head_dim or k.numel() != tokens * kv_heads * head_dim \
-            or v.numel() != k.numel():
+    size = q.numel()
+    tokens = size // (q_heads * head_dim)
+    rows = tokens * kv_heads * head_dim
+    if tokens < 1 or size != tokens * q_heads * head_dim or k.numel() != rows or v.numel() != rows:
         raise ValueError("paged append takes q [tokens, q_heads * head_dim], k and v [tokens, kv_heads * head_dim]")
-    if q.dtype not in _FLOAT or k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    if dtype not in _FLOAT or k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError("paged append q, k and v must share one of F32/F16/BF16")
     if (q_norm is None) != (k_norm is None):
         raise ValueError("q_norm and k_norm must be given together")
@@ -559,8 +565,9 @@ def launch_paged_append(
                 or q_norm.dtype not in _FLOAT:
             raise ValueError("q/k norm weights must be [head_dim] of one of F32/F16/BF16")
         norm_code = _native.DTYPE_CODES[q_norm.dtype]
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.ndim != 2 or cos.shape[1] != head_dim // 2 \
-            or cos.shape[0] < 1 or sin.shape != cos.shape:
+    table = cos.shape
+    if cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or len(table) != 2 \
+            or table[1] * 2 != head_dim or not table[0] or sin.shape != table:
         raise ValueError("RoPE tables must be fp32 [positions, head_dim / 2]")
     if q_out is None:
         q_out = torch.empty((tokens, q_heads, head_dim), dtype=q_dtype, device=device)
@@ -568,10 +575,9 @@ def launch_paged_append(
         raise ValueError("q_out must be [tokens, q_heads, head_dim]")
     if q_out.dtype not in _FLOAT:
         raise ValueError("q_out must be F32/F16/BF16")
-    status = _on_device(
-        device, _native.load().nq_paged_append, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-        _native.DTYPE_CODES[q.dtype], tokens, q_heads, _ptr(q_norm), _ptr(k_norm), norm_code, float(eps),
-        cos.data_ptr(), sin.data_ptr(), cos.shape[0], ctypes.byref(kv), q_out.data_ptr(),
+    status = _native.load().nq_paged_append(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _native.DTYPE_CODES[dtype], tokens, q_heads, _ptr(q_norm),
+        _ptr(k_norm), norm_code, eps, cos.data_ptr(), sin.data_ptr(), table[0], ctypes.byref(kv), q_out.data_ptr(),
         _native.DTYPE_CODES[q_out.dtype], _stream(device),
     )
     _native.check("nq_paged_append", status)
@@ -605,6 +611,11 @@ def launch_paged_attention(
     for many sequences."""
 
     device = q.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return launch_paged_attention(
+                q, cache, page_table=page_table, query_starts=query_starts, context_lens=context_lens, scaling=scaling,
+                out=out, out_dtype=out_dtype, workspace=workspace)
     if q.ndim != 3 or q.dtype not in _FLOAT:
         raise ValueError("paged attention query must be F32/F16/BF16 [tokens, q_heads, head_dim]")
     _check_device("paged attention", device, q, out, workspace)
@@ -627,9 +638,8 @@ def launch_paged_attention(
         raise ValueError("paged attention geometry was rejected")
     if workspace is None and need:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    status = _on_device(
-        device, lib.nq_paged_attention, q.data_ptr(), _native.DTYPE_CODES[q.dtype], tokens, q_heads, ctypes.byref(kv),
-        float(scaling), out.data_ptr(), _native.DTYPE_CODES[out.dtype], _ptr(workspace),
+    status = lib.nq_paged_attention(
+        q.data_ptr(), _native.DTYPE_CODES[q.dtype], tokens, q_heads, ctypes.byref(kv), scaling, out.data_ptr(), _native.DTYPE_CODES[out.dtype], _ptr(workspace),
         0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(device),
     )
     _native.check("nq_paged_attention", status)
@@ -668,6 +678,9 @@ def launch_token_logprobs(
     vocab]``; its rows may lie further apart than vocab."""
 
     device = logits.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return launch_token_logprobs(logits, tokens, top=top, out=out, workspace=workspace)
     if logits.ndim != 2 or logits.dtype not in _FLOAT:
         raise ValueError("token logprobs take F32/F16/BF16 logits [rows, vocab]")
     rows, vocab = logits.shape
@@ -683,23 +696,26 @@ def launch_token_logprobs(
     if device.type != "cuda" or tokens.device != device:
         raise ValueError("token logprobs require CUDA/HIP tensors on one device")
     if out is None:
-        sums = torch.empty((2, rows), dtype=torch.float32, device=device)
-        out = TokenLogprobs(sums[0], sums[1], torch.empty((rows, top), dtype=torch.int64, device=device),
+        _check_device("token logprobs", device, tokens, workspace)
+        out = TokenLogprobs(torch.empty(rows, dtype=torch.float32, device=device),
+                            torch.empty(rows, dtype=torch.float32, device=device),
+                            torch.empty((rows, top), dtype=torch.int64, device=device),
                             torch.empty((rows, top), dtype=torch.float32, device=device))
-    _check_device("token logprobs", device, tokens, *out, workspace)
-    if out.logprobs.dtype != torch.float32 or out.entropy.dtype != torch.float32 or out.top_ids.dtype != torch.int64 \
-            or out.top_logprobs.dtype != torch.float32 or out.logprobs.shape != (rows,) or out.entropy.shape != (rows,) \
-            or out.top_ids.shape != (rows, top) or out.top_logprobs.shape != (rows, top):
-        raise ValueError("token logprobs outputs must be fp32 [rows] twice, int64 and fp32 [rows, top]")
+    else:
+        _check_device("token logprobs", device, tokens, *out, workspace)
+        if out.logprobs.dtype != torch.float32 or out.entropy.dtype != torch.float32 or out.top_ids.dtype != torch.int64 \
+                or out.top_logprobs.dtype != torch.float32 or out.logprobs.shape != (rows,) \
+                or out.entropy.shape != (rows,) or out.top_ids.shape != (rows, top) \
+                or out.top_logprobs.shape != (rows, top):
+            raise ValueError("token logprobs outputs must be fp32 [rows] twice, int64 and fp32 [rows, top]")
     lib = _native.load()
     need = lib.nq_token_logprobs_workspace_bytes(rows, vocab, top)
     if need < 0:
         raise ValueError("token logprobs geometry was rejected")
     if workspace is None and need:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    status = _on_device(
-        device, lib.nq_token_logprobs, logits.data_ptr(), _native.DTYPE_CODES[logits.dtype], rows, vocab, stride,
-        tokens.data_ptr(), top, out.logprobs.data_ptr(), out.entropy.data_ptr(), _ptr(out.top_ids if top else None),
+    status = lib.nq_token_logprobs(
+        logits.data_ptr(), _native.DTYPE_CODES[logits.dtype], rows, vocab, stride, tokens.data_ptr(), top, out.logprobs.data_ptr(), out.entropy.data_ptr(), _ptr(out.top_ids if top else None),
         _ptr(out.top_logprobs if top else None), _ptr(workspace),
         0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(device),
     )
