@@ -246,15 +246,15 @@ __device__ __forceinline__ void store4(void* out, int dtype, int64_t at, const f
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = make_uint2(w[0], w[1]);
 }
 
-// One workgroup of four waves: a slot of query rows of one kv head over one
+// One workgroup of WAVES waves: a slot of query rows of one kv head over one
 // split of the cache. SHARED: the waves hold the same 16 NT rows and take the
 // split's tiles in turn (few query rows: the cache's bytes are the work);
 // otherwise each wave has 16 NT rows of its own, whose parts wait in LDS (in
 // registers they would leave room for one wave to a SIMD, and nothing would fill
 // the matrix unit during a softmax), and all take every tile.
-template <int D, int QT, int PP, int NT, int TILE, bool SHARED>
-__global__ __launch_bounds__(256, D == 256 ? 1 : SHARED ? 2 : 2) void k_paged_attention(const AttnArgs a) {
-    constexpr int kRows = (SHARED ? 1 : 4) * 16 * NT;
+template <int D, int QT, int PP, int NT, int TILE, bool SHARED, int WAVES>
+__global__ __launch_bounds__(WAVES* kWave, D == 256 ? 1 : 2) void k_paged_attention(const AttnArgs a) {
+    constexpr int kRows = (SHARED ? 1 : WAVES) * 16 * NT;
     constexpr int kChunks = D / 64, kDims = D / 16;
     constexpr int kBlock = TILE / 4;   // consecutive cache rows of a lane: of V, and of the scores
     constexpr int kScores = TILE / 16, kSteps = TILE / 32, kWords = kBlock / 4;
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : SHARED ? 2 : 2) void k_paged_at
 
     // This wave's query rows: row numbers, positions (-1: sees nothing), q.
     constexpr int QP = Query<QT>::kParts, kQSteps = 2 * kChunks;
-    __shared__ u32x4 q_lds[SHARED ? 1 : 4][SHARED ? 1 : kQSteps * NT * QP][kWave];
+    __shared__ u32x4 q_lds[SHARED ? 1 : WAVES][SHARED ? 1 : kQSteps * NT * QP][kWave];
     u32x4 q_regs[SHARED ? NT : 1][kQSteps][QP];
     const int wave_row = SHARED ? 0 : wave * 16 * NT;
     int row[NT], pos[NT];
@@ -320,7 +320,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : SHARED ? 2 : 2) void k_paged_at
     }
 
     const int tile_end = min((split + 1) * plan.per * (kTile / TILE), (min(high_pos + 1, s.visible) + TILE - 1) / TILE);
-    const int step = SHARED ? 4 : 1;
+    const int step = SHARED ? WAVES : 1;
     const int tile_begin = split * plan.per * (kTile / TILE) + (SHARED ? wave : 0);
     // Table entries of this lane's blocks of kBlock rows: block n / 4 for K, grp
     // for the scores' scales and for V. What no query sees takes the last entry
@@ -548,10 +548,29 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : SHARED ? 2 : 2) void k_paged_at
                 if (nan_at[u][d / 8] >> (4 * (d % 8) + i) & 1u) acc[d][u][i] = __builtin_nanf("");
     }
 
-    // The waves' shares of the same rows meet in LDS, in wave order.
-    __shared__ float join_ml[SHARED ? 4 : 1][2][16 * NT];
-    __shared__ f32x4 join_o[SHARED ? 3 : 1][SHARED ? kDims * NT : 1][kWave];
+    // Output o of query row t, or its share for the merge.
+    const auto put = [&](int t, int d, const f32x4& o, float m, float l) {
+        if (row[t] >= s.rows) return;
+        if (plan.active <= 1) {
+            const float inv = pos[t] < 0 ? 0.0f : 1.0f / l;
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = pos[t] < 0 ? 0.0f : o[i] * inv;
+            store4(a.out, a.out_dtype, out_at[t] + 16 * d + 4 * grp, v);
+        } else {
+            const int64_t at = ((static_cast<int64_t>(slot) * a.splits + split) * p.kv_heads + g) * kRows + row[t];
+            if (d == 0 && grp == 0) {
+                a.partial[2 * at] = m;
+                a.partial[2 * at + 1] = l;
+            }
+            *reinterpret_cast<f32x4*>(a.partial_o + at * D + 16 * d + 4 * grp) = o;
+        }
+    };
     if constexpr (SHARED) {
+        // The waves' shares of the same rows meet in LDS; each wave joins some of the
+        // dimensions, the shares in wave order.
+        __shared__ float join_ml[WAVES][2][16 * NT];
+        __shared__ f32x4 join_o[WAVES][kDims * NT][kWave];
         if (grp == 0) {
 #pragma unroll
             for (int u = 0; u < NT; ++u) {
@@ -559,63 +578,42 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : SHARED ? 2 : 2) void k_paged_at
                 join_ml[wave][1][16 * u + n] = l_run[u];
             }
         }
-        if (wave > 0) {
 #pragma unroll
-            for (int d = 0; d < kDims; ++d)
+        for (int d = 0; d < kDims; ++d)
 #pragma unroll
-                for (int u = 0; u < NT; ++u) join_o[wave - 1][d * NT + u][lane] = acc[d][u];
-        }
+            for (int u = 0; u < NT; ++u) join_o[wave][d * NT + u][lane] = acc[d][u];
         __syncthreads();
-        if (wave > 0) return;
+        if (wave >= kDims) return;
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-            float m_all = m_run[u];
+            float weight[WAVES], m_all = -INFINITY, l_all = 0.0f;
 #pragma unroll
-            for (int w = 1; w < 4; ++w) m_all = fmaxf(m_all, join_ml[w][0][16 * u + n]);
+            for (int w = 0; w < WAVES; ++w) m_all = fmaxf(m_all, join_ml[w][0][16 * u + n]);
             const float m_use = m_all == -INFINITY ? 0.0f : m_all;
-            float keep = exp2_hw(m_run[u] - m_use);
-            l_run[u] *= keep;
 #pragma unroll
-            for (int d = 0; d < kDims; ++d) acc[d][u] *= keep;
-#pragma unroll
-            for (int w = 1; w < 4; ++w) {
-                keep = exp2_hw(join_ml[w][0][16 * u + n] - m_use);
-                l_run[u] += keep * join_ml[w][1][16 * u + n];
-#pragma unroll
-                for (int d = 0; d < kDims; ++d) acc[d][u] += keep * join_o[w - 1][d * NT + u][lane];
+            for (int w = 0; w < WAVES; ++w) {
+                weight[w] = exp2_hw(join_ml[w][0][16 * u + n] - m_use);
+                l_all += weight[w] * join_ml[w][1][16 * u + n];
             }
-            m_run[u] = m_all;
+#pragma unroll
+            for (int d = wave; d < kDims; d += WAVES) {
+                f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) o += weight[w] * join_o[w][d * NT + u][lane];
+                put(u, d, o, m_all, l_all);
+            }
         }
-    }
-
+    } else {
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-        if (row[u] >= s.rows) continue;
-        if (plan.active <= 1) {
-            const float inv = 1.0f / l_run[u];
+        for (int u = 0; u < NT; ++u)
 #pragma unroll
-            for (int d = 0; d < kDims; ++d) {
-                float v[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = pos[u] < 0 ? 0.0f : acc[d][u][i] * inv;
-                store4(a.out, a.out_dtype, out_at[u] + 16 * d + 4 * grp, v);
-            }
-        } else {
-            const int64_t at = ((static_cast<int64_t>(slot) * a.splits + split) * p.kv_heads + g) * kRows + row[u];
-            if (grp == 0) {
-                a.partial[2 * at] = m_run[u];
-                a.partial[2 * at + 1] = l_run[u];
-            }
-#pragma unroll
-            for (int d = 0; d < kDims; ++d)
-                *reinterpret_cast<f32x4*>(a.partial_o + at * D + 16 * d + 4 * grp) = acc[d][u];
-        }
+            for (int d = 0; d < kDims; ++d) put(u, d, acc[d][u], m_run[u], l_run[u]);
     }
 }
 
 // Host side: grid and rows of a slot for a call, and its launch.
 struct AttnPlan {
-    int rows, slots, splits, least;
+    int rows, slots, splits, least, waves;
     bool shared;
 };
 
@@ -623,8 +621,8 @@ struct AttnPlan {
 template <int D>
 constexpr int kOwnTiles = D == 256 ? 1 : 2;
 // Cache rows that a wave takes at once.
-template <int D, bool SHARED>
-constexpr int kRowsAtOnce = D == 256 ? 32 : SHARED ? 64 : 64;
+template <int D>
+constexpr int kRowsAtOnce = D == 256 ? 32 : 64;
 
 constexpr int own_rows(int head_dim) { return 64 * (head_dim == 256 ? 1 : 2); }
 
@@ -635,11 +633,15 @@ template <int D, int QT, int PP>
 int launch_attention_as(const AttnArgs& a, const AttnPlan& plan, hipStream_t stream) {
     const int64_t blocks = static_cast<int64_t>(plan.slots) * plan.splits * a.p.kv_heads;
     if (blocks > 0x7fffffff) return NQ_ERR_SHAPE;
-    const dim3 grid(static_cast<unsigned>(blocks));
-    if (plan.shared) {
-        hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 1, kRowsAtOnce<D, true>, true>), grid, dim3(256), 0, stream, a);
+    const dim3 grid(static_cast<unsigned>(blocks)), block(static_cast<unsigned>(plan.waves * kWave));
+    constexpr int kTileRows = kRowsAtOnce<D>;
+    if (plan.waves == 8) {
+        if constexpr (D < 256)
+            hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 1, kTileRows, true, 8>), grid, block, 0, stream, a);
+    } else if (plan.shared) {
+        hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 1, kTileRows, true, 4>), grid, block, 0, stream, a);
     } else {
-        hipLaunchKernelGGL((k_paged_attention<D, QT, PP, kOwnTiles<D>, kRowsAtOnce<D, false>, false>), grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_paged_attention<D, QT, PP, kOwnTiles<D>, kTileRows, false, 4>), grid, block, 0, stream, a);
     }
     return nq::launch_status();
 }

@@ -76,22 +76,47 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows)
     }
 }
 
-// Few query rows to a sequence: a slot of 16 rows whose waves share them, and
-// the cache split until the chip has about two workgroups to a CU; more: slots
-// of 128 rows (64 of 256-wide heads), a quarter to each wave.
+// How a call is laid out. All rules go by sizes that the host knows: the page
+// table's width stands for the cache's length.
+//
+// Few query rows to a sequence (at most 16): a slot of 16 rows whose waves share
+// them and take the cache's tiles in turn.
+//  - Short caches (up to 12 tiles of 64 rows) are not split: eight waves, one
+//    launch (700 rows of one sequence, 32/8 heads of 128: 10.5 us against 7.7 + 3
+//    with a merge; 17 tiles: 13.9 against 11.3).
+//  - Slots and heads that fill the chip by themselves are not split either, and take
+//    eight waves from 32 tiles on (32 sequences of up to 4000 rows: 39.2 us,
+//    four waves and three splits 45.7; 64 sequences of 1000 rows: 33.9 against
+//    29.7 of four waves).
+//  - Otherwise the cache is split until there are about 1024 workgroups, for one
+//    sequence 512 (131000 rows: 60.5 us against 73.8 with 1024), of at least 8
+//    tiles, or 4 where the chip would stay empty.
+// 256-wide heads take four waves: their registers leave one to a SIMD.
+// More rows: slots of 128 rows (64 of 256-wide heads), a quarter to each wave; the
+// cache is split only as far as the chip stays empty, since every split's share
+// of every row goes through memory (2048 tokens of two sequences, 14/2 heads of
+// 64: 69 us, with two splits 165).
 AttnPlan plan_attention(int64_t tokens, int64_t batch, int q_heads, int kv_heads, int head_dim, int64_t cache_rows) {
+    constexpr int64_t kFull = 256, kShort = 12, kLong = 32, kMostSplits = 128;
     AttnPlan plan;
     const int64_t rows = tokens * (q_heads / kv_heads);
     plan.shared = rows <= 16 * batch;
     plan.rows = plan.shared ? 16 : own_rows(head_dim);
     plan.slots = static_cast<int>(rows / plan.rows + batch);
     const int64_t tiles = (cache_rows + kTile - 1) / kTile, units = static_cast<int64_t>(plan.slots) * kv_heads;
-    const int64_t target = plan.shared ? (batch > 1 ? 1024 : 512) : 256;
+    const bool full = units >= kFull, narrow = head_dim < 256;
     plan.least = plan.shared && units * ((tiles + 7) / 8) < 512 ? 4 : 8;
-    const int64_t most = (tiles + plan.least - 1) / plan.least;
+    plan.waves = 4;
+    int64_t target = kFull;
+    if (plan.shared) {
+        target = batch > 1 ? 1024 : 512;
+        if (narrow && ((full && tiles >= kLong) || (!full && tiles <= kShort))) plan.waves = 8;
+        if (plan.waves == 8 || (full && narrow)) target = 0;
+    }
     int64_t splits = target / units;
+    const int64_t most = (tiles + plan.least - 1) / plan.least;
     splits = splits < most ? splits : most;
-    plan.splits = static_cast<int>(splits < 1 ? 1 : (splits > 128 ? 128 : splits));
+    plan.splits = static_cast<int>(splits < 1 ? 1 : (splits > kMostSplits ? kMostSplits : splits));
     return plan;
 }
 
