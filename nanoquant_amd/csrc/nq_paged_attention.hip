@@ -87,7 +87,10 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows)
 //  - Slots and heads that fill the chip by themselves are not split either, and take
 //    eight waves from 32 tiles on (32 sequences of up to 4000 rows: 39.2 us,
 //    four waves and three splits 45.7; 64 sequences of 1000 rows: 33.9 against
-//    29.7 of four waves).
+//    29.7 of four waves), unless the table has room for long sequences: then a
+//    split for each 96 tiles, up to 16, so that a long sequence among short ones
+//    does not keep one workgroup (one of 131000 rows and 31 of 500: 86 us, 718
+//    without; 32 of 32000: 356 to 375, 370 without).
 //  - Otherwise the cache is split until there are about 1024 workgroups, for one
 //    sequence 512 (131000 rows: 60.5 us against 73.8 with 1024), of at least 8
 //    tiles, or 4 where the chip would stay empty.
@@ -97,7 +100,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows)
 // of every row goes through memory (2048 tokens of two sequences, 14/2 heads of
 // 64: 69 us, with two splits 165).
 AttnPlan plan_attention(int64_t tokens, int64_t batch, int q_heads, int kv_heads, int head_dim, int64_t cache_rows) {
-    constexpr int64_t kFull = 256, kShort = 12, kLong = 32, kMostSplits = 128;
+    constexpr int64_t kFull = 256, kShort = 12, kLong = 32, kMostSplits = 128, kSkew = 96;
     AttnPlan plan;
     const int64_t rows = tokens * (q_heads / kv_heads);
     plan.shared = rows <= 16 * batch;
@@ -114,6 +117,7 @@ AttnPlan plan_attention(int64_t tokens, int64_t batch, int q_heads, int kv_heads
         if (plan.waves == 8 || (full && narrow)) target = 0;
     }
     int64_t splits = target / units;
+    if (full && plan.shared && tiles / kSkew > splits) splits = tiles / kSkew < 16 ? tiles / kSkew : 16;
     const int64_t most = (tiles + plan.least - 1) / plan.least;
     splits = splits < most ? splits : most;
     plan.splits = static_cast<int>(splits < 1 ? 1 : (splits > kMostSplits ? kMostSplits : splits));
