@@ -1,5 +1,5 @@
 // Log probability of given tokens, entropy of the distribution and its top
-// alternatives from rows of logits, in one read.
+// alternatives from rows of logits, in one read of the logits.
 //
 // A workgroup of four waves takes a part of a row, all of it where there are rows
 // enough. A lane keeps its own running maximum m and, relative to it, s = sum
@@ -7,8 +7,15 @@
 // are on their way while these are worked on. With M the largest of the maxima,
 //   lse = M + log S, S = sum s e^(m - M)
 //   log p(x) = x - lse, entropy = log S - T / S, T = sum (t + s (m - M)) e^(m - M)
-// rounded once from fp64; a row's parts meet in a second launch. Each wave keeps its k largest values in LDS; a block of values costs one
-// comparison unless some value is above the smallest of them.
+// rounded once from fp64; a row's parts meet in a second launch.
+//
+// For alternatives each lane also leaves the largest of its 16 values (a chunk) of
+// every block of 1024. The k-th largest of a row's chunk maxima bounds the k-th
+// largest value from below, fewer than k chunks lie above it, and only those
+// chunks, and the first ones that touch the bound, are read again: selecting
+// costs the first pass one 4-byte store for 16 values. (The maxima of 16 chunks
+// each are kept too, so that few chunk maxima have to be looked at.) (Lists of k kept by each
+// wave took 21.5 us instead of 12.4 for 48 rows of 50257, k = 20.)
 #include <math.h>
 
 #include "nq_common.h"
@@ -18,10 +25,12 @@ namespace {
 
 constexpr int kWave = 64;
 constexpr int kWaves = 4;
+constexpr int kJoinWaves = 8;
 constexpr int kMostTop = 32;
-constexpr int kRoom = kWave;  // values that a list takes in at once
 constexpr int kValues = 16;   // of a lane at once
-constexpr int kMostParts = 64;  // of a row: one to a lane of the joining wave
+constexpr int kBlock = kWave * kValues;
+constexpr int kGroup = 16;  // chunks whose largest value is kept too
+constexpr int kMostParts = 64;  // of a row: one to a lane of the joining waves
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
 
@@ -29,9 +38,10 @@ struct Args {
     const void* logits;
     const int64_t* tokens;
     int64_t row_stride;
-    int32_t vocab, top, parts;
+    int32_t vocab, top, parts, blocks;  // blocks of a row; chunks = 64 blocks
     float* sums;       // [rows][parts][4]: M, S, T of a part (parts > 1)
-    uint64_t* lists;   // [rows][parts][top]: its keys, largest first, 0 where there is none
+    uint32_t* maxima;  // [rows][chunks]: the order of each chunk's largest value (top > 0)
+    uint32_t* groups;  // [rows][chunks / 16]: of 16 chunks' largest value
     float *logprobs, *entropy, *top_logprobs;
     int64_t* top_ids;
 };
@@ -57,6 +67,11 @@ __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t index) {
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x, float identity) {
     return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(identity), __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, 0xf, 0xf, false));
 }
 
 __device__ __forceinline__ float lane_of(float v, int lane) {
@@ -90,129 +105,10 @@ __device__ __forceinline__ double wave_sum(double v) {
 
 __device__ __forceinline__ int count(bool on) { return __popcll(__ballot(on)); }
 
-__device__ __forceinline__ int lanes_before(uint64_t mask) {
-    return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
-                                     __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
-}
-
-template <int DT>
-__device__ __forceinline__ float element(const void* p, int64_t i) { return nq::load_f32(p, DT, i); }
-
-// A wave's LDS operations stay in order; this keeps the compiler to it.
-__device__ __forceinline__ void wave_lds_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-__device__ __forceinline__ uint64_t lane_key(uint64_t key, int lane) {
-    return (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(key >> 32), lane))) << 32) |
-           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(key & 0xffffffffu), lane));
-}
-
-// How many of the k keys of a list, largest first, are above `key`.
-__device__ __forceinline__ int above_in(const uint64_t* list, int k, uint64_t key) {
-    int low = 0;
+__device__ __forceinline__ int wave_total(int v) {
 #pragma unroll
-    for (int step = kMostTop; step >= 1; step /= 2)
-        if (low + step <= k && list[low + step - 1] > key) low += step;
-    return low;
-}
-
-// The wave's list of its k largest keys so far, largest first (0 where there is
-// none), and the order of the smallest of them.
-struct Best {
-    uint64_t* list;  // LDS, [kMostTop + kRoom]: the list, then room for what comes in
-    uint32_t last;
-};
-
-// Takes a block of values into the list: key[e] is the order of the value with
-// index first + (e / VEC) 64 VEC + lane VEC + e % VEC, 0 for none. Blocks come in
-// index order, so a value equal to the last one stays out. When more than
-// kRoom values are above it, the k-th largest of the lanes' maxima bounds
-// from below what can get in; when that leaves too many, the block's own k-th
-// largest value is found bit by bit, and of those equal to it the lowest
-// indexes are taken.
-template <int VEC>
-__device__ __forceinline__ void take(Best& best, const uint32_t (&key)[kValues], int k, int64_t first) {
-    const int lane = threadIdx.x & (kWave - 1);
-    uint32_t bound = best.last + 1;
-    int chosen = 0;
-#pragma unroll
-    for (int e = 0; e < kValues; ++e) chosen += count(key[e] >= bound);
-    if (chosen > kRoom) {
-        uint32_t most = 0;
-#pragma unroll
-        for (int e = 0; e < kValues; ++e) most = max(most, key[e]);
-        uint32_t least = 0;
-        for (int bit = 31; bit >= 8; --bit) {  // a bound from below need not be exact
-            const uint32_t next = least | (1u << bit);
-            if (count(most >= next) >= k) least = next;
-        }
-        bound = max(bound, least);
-        chosen = 0;
-#pragma unroll
-        for (int e = 0; e < kValues; ++e) chosen += count(key[e] >= bound);
-    }
-    int at = 0;
-    const auto put = [&](int e, bool in) {
-        const uint64_t mask = __ballot(in);
-        if (!mask) return;
-        if (in)
-            best.list[kMostTop + at + lanes_before(mask)] =
-                key_of(key[e], static_cast<uint32_t>(first + (e / VEC) * (kWave * VEC) + lane * VEC + e % VEC));
-        at += __popcll(mask);
-    };
-    if (chosen <= kRoom) {
-#pragma unroll
-        for (int e = 0; e < kValues; ++e) put(e, key[e] >= bound);
-    } else {
-        // More than k values are at or above the last bound, so the k-th largest is no less.
-        bound = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t next = bound | (1u << bit);
-            int n = 0;
-#pragma unroll
-            for (int e = 0; e < kValues; ++e) n += count(key[e] >= next);
-            if (n >= k) bound = next;
-        }
-        int ties = k, tied = 0;  // of the values equal to it: taken, seen so far
-#pragma unroll
-        for (int e = 0; e < kValues; ++e) ties -= count(key[e] > bound);
-#pragma unroll
-        for (int c = 0; c < kValues / VEC; ++c) {
-            // Places in index order: lanes before this one, then its own values.
-            int tie_rank = tied;
-#pragma unroll
-            for (int e = c * VEC; e < (c + 1) * VEC; ++e) {
-                const uint64_t mask = __ballot(key[e] == bound);
-                tie_rank += lanes_before(mask);
-                tied += __popcll(mask);
-            }
-#pragma unroll
-            for (int e = c * VEC; e < (c + 1) * VEC; ++e) {
-                const bool tie = key[e] == bound;
-                put(e, key[e] > bound || (tie && tie_rank < ties));
-                tie_rank += tie;
-            }
-        }
-    }
-    wave_lds_sync();
-    // Lane i holds the list's i-th key and the i-th that came in: their ranks.
-    const uint64_t had = lane < k ? best.list[lane] : 0, came = lane < at ? best.list[kMostTop + lane] : 0;
-    const int held = count(had != 0);
-    int had_rank = lane, came_rank = 0;
-    for (int i = 0; i < held; ++i) came_rank += lane_key(had, i) > came;
-    for (int i = 0; i < at; ++i) {
-        const uint64_t key = lane_key(came, i);
-        had_rank += key > had;
-        came_rank += key > came;
-    }
-    wave_lds_sync();
-    if (had && had_rank < k) best.list[had_rank] = had;
-    if (came && came_rank < k) best.list[came_rank] = came;
-    wave_lds_sync();
-    best.last = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(best.list[k - 1] >> 32));
+    for (int m = 1; m < kWave; m *= 2) v += __shfl_xor(v, m, kWave);
+    return v;
 }
 
 template <int DT>
@@ -308,40 +204,28 @@ __device__ __forceinline__ float logit_of(const Args& a, int dtype, int64_t row)
     return token >= 0 && token < a.vocab ? nq::load_f32(a.logits, dtype, row * a.row_stride + token) : __builtin_nanf("");
 }
 
-template <int DT, bool TOP>
+template <int DT>
 __global__ __launch_bounds__(kWaves* kWave) void k_token_logprobs(const Args a) {
     constexpr int VEC = Block<DT>::kVec, kBytes = Block<DT>::kBytes;
-    constexpr int kBlock = kWave * kValues;
-    __shared__ uint64_t lists[TOP ? kWaves : 1][kMostTop + kRoom];
     __shared__ Sums sums[kWaves];
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int64_t row = blockIdx.x / a.parts;
     const int part = blockIdx.x - static_cast<int>(row) * a.parts;
     const char* base = static_cast<const char*>(a.logits) + row * a.row_stride * kBytes;
-    const int blocks = (a.vocab + kBlock - 1) / kBlock, each = (blocks + a.parts - 1) / a.parts;
-    const int begin = part * each + wave, end = min(blocks, (part + 1) * each);
-    const auto first_of = [&](int block) { return static_cast<int64_t>(block) * kBlock; };
-    Best best{lists[TOP ? wave : 0], 0};
-    if (TOP) {
-        if (lane < kMostTop) best.list[lane] = 0;
-        wave_lds_sync();
-    }
+    const int each = (a.blocks + a.parts - 1) / a.parts;
+    const int begin = part * each + wave, end = min(a.blocks, (part + 1) * each);
 
     float m = -INFINITY, s = 0.0f, t = 0.0f;
     Block<DT> next;
-    if (begin < end) load_block<DT>(next, base, first_of(begin), a.vocab);
+    if (begin < end) load_block<DT>(next, base, static_cast<int64_t>(begin) * kBlock, a.vocab);
     for (int block = begin; block < end; block += kWaves) {
         float x[kValues];
         unpack<DT>(next, x);
-        if (block + kWaves < end) load_block<DT>(next, base, first_of(block + kWaves), a.vocab);
+        if (block + kWaves < end) load_block<DT>(next, base, static_cast<int64_t>(block + kWaves) * kBlock, a.vocab);
         float high = x[0];
-        bool nan = x[0] != x[0];
 #pragma unroll
-        for (int e = 1; e < kValues; ++e) {
-            high = fmaxf(high, x[e]);
-            if (TOP) nan |= x[e] != x[e];
-        }
+        for (int e = 1; e < kValues; ++e) high = fmaxf(high, x[e]);
         const float m_new = fmaxf(m, high);
         const float m_use = m_new == -INFINITY ? 0.0f : m_new;
         // What was summed so far moves to the new maximum.
@@ -356,27 +240,31 @@ __global__ __launch_bounds__(kWaves* kWave) void k_token_logprobs(const Args a) 
             bs += w;
             bt = fmaf(w, fmaxf(d, -1000.0f), bt);  // w is 0 there: 0 * -inf is not meant
         }
+        if (a.top) {
+            bool nan = false;
+#pragma unroll
+            for (int e = 0; e < kValues; ++e) nan |= x[e] != x[e];
+            const bool any = static_cast<int64_t>(block) * kBlock + lane * VEC < a.vocab;  // the chunk's first value is in the row
+            const int64_t chunk = (row * a.blocks + block) * kWave + lane;
+            const uint32_t order = !any ? 0 : (nan ? 0xffffffffu : ordered(high));
+            a.maxima[chunk] = order;
+            uint32_t most = max(order, dpp<0xB1>(order));
+            most = max(most, dpp<0x4E>(most));
+            most = max(most, dpp<0x141>(most));
+            most = max(most, dpp<0x140>(most));
+            if (lane % kGroup == 0) a.groups[chunk / kGroup] = most;
+        }
         s += bs;
         t += bt;
         m = m_new;
-        if (TOP && __ballot(nan || ordered(high) > best.last)) {
-            const int64_t first = first_of(block);
-            uint32_t key[kValues];
-#pragma unroll
-            for (int e = 0; e < kValues; ++e) {
-                const int64_t i = first + (e / VEC) * (kWave * VEC) + lane * VEC + e % VEC;
-                key[e] = i < a.vocab ? ordered(x[e]) : 0;  // outside the row: -inf for the sums, nothing here
-            }
-            take<VEC>(best, key, a.top, first);
-        }
     }
 
     const float wave_m = wave_max(m);
     const Sums mine = moved({m, s, t}, wave_m);
     const Sums joined{wave_m, wave_sum(mine.s), wave_sum(mine.t)};
     if (lane == 0) sums[wave] = joined;
-    const float x = wave == 0 && a.parts == 1 ? logit_of(a, DT, row) : 0.0f;
     __syncthreads();
+    if (wave > 0) return;
     float high = sums[0].m;
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) high = fmaxf(high, sums[w].m);
@@ -387,87 +275,182 @@ __global__ __launch_bounds__(kWaves* kWave) void k_token_logprobs(const Args a) 
         all.s += b.s;
         all.t += b.t;
     }
-    const int64_t at = row * a.parts + part;
-    double lse = 0.0;
-    if (a.parts == 1) {
-        lse = finish(a, row, all.m, all.s, all.t, x, threadIdx.x == 0);
-    } else if (threadIdx.x == 0) {
-        a.sums[4 * at] = all.m;
-        a.sums[4 * at + 1] = all.s;
-        a.sums[4 * at + 2] = all.t;
-    }
-    if (!TOP) return;
-    // The waves' lists as one: a key's rank is its place in its own and what the others have above it.
-    for (int i = threadIdx.x; i < kWaves * kMostTop; i += kWaves * kWave) {
-        const int w0 = i / kMostTop, j = i % kMostTop;
-        if (j >= a.top) continue;
-        const uint64_t key = lists[w0][j];
-        int rank = j;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w)
-            if (w != w0) rank += above_in(lists[w], a.top, key);
-        if (a.parts == 1) {
-            put_top(a, row, key, rank, lse);
-        } else if (key) {
-            if (rank < a.top) a.lists[at * a.top + rank] = key;
-        } else {
-            // Empty places follow all lists' keys (rank counts the others' and j its
-            // own): those of the lists before this one come first.
-            for (int w = 0; w < w0; ++w) rank += a.top - above_in(lists[w], a.top, 0);
-            if (rank < a.top) a.lists[at * a.top + rank] = 0;
+    if (a.sums) {
+        if (lane == 0) {
+            float* at = a.sums + 4 * (row * a.parts + part);
+            at[0] = all.m;
+            at[1] = all.s;
+            at[2] = all.t;
         }
+    } else {
+        finish(a, row, all.m, all.s, all.t, logit_of(a, DT, row), lane == 0);
     }
 }
 
-// A row's parts: one to a lane for the sums; the lists in LDS.
-__global__ __launch_bounds__(kWaves* kWave) void k_token_logprobs_join(const Args a, int dtype) {
-    __shared__ uint64_t lists[kMostParts * kMostTop], reach[kMostParts * kMostTop];
-    __shared__ int reached;
+// A row's parts and its alternatives.
+__global__ __launch_bounds__(kJoinWaves* kWave) void k_token_logprobs_join(const Args a, int dtype) {
+    constexpr int kThreads = kJoinWaves * kWave;
+    constexpr int kList = 1024;  // chunks that may hold alternatives
+    // Keys: of fewer than kMostTop chunks above the bound, fewer than kMostTop that
+    // touch it in blocks before the last one taken, and 64 of that block.
+    constexpr int kKeys = (2 * kMostTop + kWave) * kValues;
+    __shared__ uint32_t bests[kThreads], list_id[kList], list_max[kList], bound_at;
+    __shared__ uint64_t keys[kKeys];
+    __shared__ uint32_t group_id[kList];
+    __shared__ int grouped, listed, taken;
+    __shared__ double lse_at;
     const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int64_t row = blockIdx.x;
-    const int keys = a.parts * a.top;
-    for (int i = threadIdx.x; i < keys; i += kWaves * kWave) lists[i] = a.lists[row * keys + i];
-    if (threadIdx.x == 0) reached = 0;
-    const float* at = a.sums + 4 * (row * a.parts + (lane < a.parts ? lane : 0));
-    Sums mine{at[0], at[1], at[2]};
-    const float x = logit_of(a, dtype, row);
-    if (lane >= a.parts) mine = {-INFINITY, 0.0f, 0.0f};
-    const float high = wave_max(mine.m);
-    const double d = mine.m == -INFINITY ? -INFINITY : static_cast<double>(mine.m) - static_cast<double>(high);
-    const double f = exp(d);
-    const double s = wave_sum(mine.s * f), t = wave_sum((mine.t + mine.s * fmax(d, -1000.0)) * f);
-    const double lse = finish(a, row, high, s, t, x, threadIdx.x == 0);
+    const int chunks = a.blocks * kWave;
+    const uint32_t* maxima = a.maxima + (a.top ? row * chunks : 0);
+    if (threadIdx.x == 0) {
+        grouped = listed = taken = 0;
+        bound_at = 0;
+    }
+    const int groups = chunks / kGroup;
+    const uint32_t* group_max = a.groups + (a.top ? row * groups : 0);
+    uint32_t best = 0;
+    if (a.top)
+#pragma unroll 4
+        for (int i = threadIdx.x; i < groups; i += kThreads) best = max(best, group_max[i]);
+    bests[threadIdx.x] = best;
+    if (wave == 0) {
+        const float* at = a.sums + 4 * (row * a.parts + (lane < a.parts ? lane : 0));
+        Sums mine{at[0], at[1], at[2]};
+        const float x = logit_of(a, dtype, row);
+        if (lane >= a.parts) mine = {-INFINITY, 0.0f, 0.0f};
+        const float high = wave_max(mine.m);
+        const double d = mine.m == -INFINITY ? -INFINITY : static_cast<double>(mine.m) - static_cast<double>(high);
+        const double f = exp(d);
+        const double s = wave_sum(mine.s * f), t = wave_sum((mine.t + mine.s * fmax(d, -1000.0)) * f);
+        const double of_row = finish(a, row, high, s, t, x, lane == 0);
+        if (lane == 0) lse_at = of_row;
+    }
     if (a.top == 0) return;
     __syncthreads();
-    // The r-th largest of the lists' j-th keys, with r lists of j keys each at
-    // least top together, bounds the top-th largest key from below.
-    const int j = (a.top + a.parts - 1) / a.parts, r = (a.top + j - 1) / j;
-    const uint32_t best = lane < a.parts ? static_cast<uint32_t>(lists[lane * a.top + j - 1] >> 32) : 0;
-    uint32_t bound = 0;
+
+    // The k-th largest of 64 maxima over a 64th of the groups each: a first bound,
+    // usually little below the chunks' own k-th largest. (Its last bits are left 0.)
+    best = 0;
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) best = max(best, bests[w * kWave + lane]);
+    uint32_t first = 0;
     for (int bit = 31; bit >= 8; --bit) {
-        const uint32_t next = bound | (1u << bit);
-        if (count(best >= next) >= r) bound = next;
+        const uint32_t next = first | (1u << bit);
+        if (count(best >= next) >= a.top) first = next;
     }
-    // The keys that reach it, in any order: a rank is a count of larger keys.
-    for (int i = threadIdx.x; i < keys; i += kWaves * kWave) {
-        const uint64_t key = lists[i];
-        if (key && static_cast<uint32_t>(key >> 32) >= bound) reach[atomicAdd(&reached, 1)] = key;
+    first = max(first, 1u);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < groups; i += kThreads)
+        if (group_max[i] >= first) {
+            const int place = atomicAdd(&grouped, 1);
+            if (place < kList) group_id[place] = i;
+        }
+    __syncthreads();
+    const int near = min(grouped, kList);
+    for (int i = threadIdx.x / kGroup; i < near; i += kThreads / kGroup) {
+        const int chunk = group_id[i] * kGroup + lane % kGroup;
+        const uint32_t value = maxima[chunk];
+        if (value >= first) {
+            const int place = atomicAdd(&listed, 1);
+            if (place < kList) {
+                list_id[place] = chunk;
+                list_max[place] = value;
+            }
+        }
     }
     __syncthreads();
-    const int n = reached;
-    for (int i = threadIdx.x; i < n; i += kWaves * kWave) {
-        const uint64_t key = reach[i];
+    const int found = listed;
+    const bool fits = found <= kList && grouped <= kList;
+    const int n = min(found, kList);
+
+    // The chunks' k-th largest, exactly; 1 (every value) where there are fewer.
+    uint32_t bound = 1;
+    if (fits) {
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const uint32_t value = list_max[i];
+            int above = 0, same = 0;
+#pragma unroll 4
+            for (int c = 0; c < n; ++c) {
+                above += list_max[c] > value;
+                same += list_max[c] == value;
+            }
+            if (above < a.top && above + same >= a.top) bound_at = value;  // all that write, write the same
+        }
+        __syncthreads();
+        bound = max(bound_at, 1u);
+    } else {  // many chunks near the top, such as equal ones
+        uint32_t value = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t next = value | (1u << bit);
+            int more = 0;
+            for (int i = threadIdx.x; i < chunks; i += kThreads) more += maxima[i] >= next;
+            more = wave_total(more);
+            __syncthreads();
+            if (lane == 0) bests[wave] = more;
+            __syncthreads();
+            more = 0;
+#pragma unroll
+            for (int w = 0; w < kJoinWaves; ++w) more += bests[w];
+            if (more >= a.top) value = next;
+        }
+        bound = max(value, 1u);
+    }
+
+    // Values at or above the bound, of the chunks above it and of those that touch
+    // it, block by block (a block's values follow the ones of the blocks before)
+    // until there are k of those. Any order: a rank is a count of larger keys.
+    const auto take = [&](int chunk) {  // the chunk's values by 16 lanes
+        const int c = lane & (kValues - 1), vec = dtype == NQ_DTYPE_F32 ? 4 : 8;
+        const int64_t i = static_cast<int64_t>(chunk / kWave) * kBlock + (c / vec) * (kWave * vec) + (chunk % kWave) * vec + c % vec;
+        if (i >= a.vocab) return;
+        const uint32_t order = ordered(nq::load_f32(a.logits, dtype, row * a.row_stride + i));
+        if (order < bound) return;
+        const int place = atomicAdd(&taken, 1);
+        if (place < kKeys) keys[place] = key_of(order, static_cast<uint32_t>(i));
+    };
+    if (fits) {
+        for (int i = threadIdx.x / kValues; i < n; i += kThreads / kValues) {
+            const int chunk = list_id[i];
+            const uint32_t value = list_max[i];
+            if (value < bound) continue;
+            int before = 0;  // chunks that touch the bound, of the blocks before
+            if (value == bound)
+#pragma unroll 4
+                for (int c = 0; c < n; ++c) before += list_max[c] == bound && list_id[c] / kWave < chunk / kWave;
+            if (before < a.top) take(chunk);
+        }
+    } else {
+        int touching = 0;
+        for (int block = 0; block < a.blocks; ++block) {
+            const uint32_t value = maxima[block * kWave + lane];
+            const uint64_t touch = __ballot(value == bound);
+            const uint64_t in = __ballot(value > bound) | (touching < a.top ? touch : 0);
+            touching += __popcll(touch);
+            int c = 0;  // the in-th chunks, 16 lanes each
+            for (uint64_t rest = in; rest; rest &= rest - 1, ++c)
+                if (c % (kThreads / kValues) == threadIdx.x / kValues) take(block * kWave + __builtin_ctzll(rest));
+        }
+    }
+    __syncthreads();
+    const int reached = min(taken, kKeys);
+    const double lse = lse_at;
+    for (int i = threadIdx.x; i < reached; i += kThreads) {
+        const uint64_t key = keys[i];
         int rank = 0;
 #pragma unroll 8
-        for (int c = 0; c < n; ++c) rank += reach[c] > key;
+        for (int c = 0; c < reached; ++c) rank += keys[c] > key;
         put_top(a, row, key, rank, lse);
     }
 }
 
+int64_t blocks_for(int64_t vocab) { return (vocab + kBlock - 1) / kBlock; }
+
 // Parts of a row: enough workgroups for the chip, but a block for each wave.
 int parts_for(int64_t rows, int64_t vocab) {
     constexpr int64_t kWorkgroups = 1024;
-    const int64_t blocks = (vocab + kWave * kValues - 1) / (kWave * kValues);
+    const int64_t blocks = blocks_for(vocab);
     int64_t parts = (kWorkgroups + rows - 1) / rows;
     const int64_t most = (blocks + kWaves - 1) / kWaves;
     parts = parts < most ? parts : most;
@@ -480,7 +463,7 @@ extern "C" int64_t nq_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab
     if (rows <= 0 || rows > 0xffffff || vocab <= 0 || vocab > 0x7fffff00 || top < 0 || top > kMostTop || top > vocab)
         return -1;
     const int parts = parts_for(rows, vocab);
-    return parts == 1 ? 0 : rows * parts * (16 + 8 * static_cast<int64_t>(top));
+    return parts == 1 && top == 0 ? 0 : rows * (parts * int64_t{16} + (top ? blocks_for(vocab) * (kWave + kWave / kGroup) * int64_t{4} : 0));
 }
 
 extern "C" int nq_token_logprobs(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,
@@ -497,21 +480,20 @@ extern "C" int nq_token_logprobs(const void* logits, int32_t dtype, int64_t rows
     if (reinterpret_cast<uintptr_t>(logits) % nq::dtype_bytes(dtype) || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return NQ_ERR_ALIGNMENT;
     const int parts = parts_for(rows, vocab);
-    float* sums = static_cast<float*>(workspace);
-    const Args a = {logits, tokens, row_stride, static_cast<int32_t>(vocab), top, parts, sums,
-                    reinterpret_cast<uint64_t*>(sums + 4 * rows * parts), logprobs, entropy, top_logprobs, top_ids};
+    const bool joins = parts > 1 || top > 0;
+    float* sums = joins ? static_cast<float*>(workspace) : nullptr;
+    uint32_t* maxima = top ? reinterpret_cast<uint32_t*>(sums + 4 * rows * parts) : nullptr;
+    const Args a = {logits, tokens, row_stride, static_cast<int32_t>(vocab), top, parts,
+                    static_cast<int32_t>(blocks_for(vocab)), sums, maxima,
+                    top ? maxima + rows * blocks_for(vocab) * kWave : nullptr, logprobs, entropy, top_logprobs, top_ids};
     const dim3 grid(static_cast<unsigned>(rows * parts)), block(kWaves * kWave);
     hipStream_t st = static_cast<hipStream_t>(stream);
-#define NQ_LOGPROBS(DT)                                                                  \
-    if (top) hipLaunchKernelGGL((k_token_logprobs<DT, true>), grid, block, 0, st, a);    \
-    else hipLaunchKernelGGL((k_token_logprobs<DT, false>), grid, block, 0, st, a)
     switch (dtype) {
-        case NQ_DTYPE_F32: NQ_LOGPROBS(NQ_DTYPE_F32); break;
-        case NQ_DTYPE_F16: NQ_LOGPROBS(NQ_DTYPE_F16); break;
-        default: NQ_LOGPROBS(NQ_DTYPE_BF16); break;
+        case NQ_DTYPE_F32: hipLaunchKernelGGL(k_token_logprobs<NQ_DTYPE_F32>, grid, block, 0, st, a); break;
+        case NQ_DTYPE_F16: hipLaunchKernelGGL(k_token_logprobs<NQ_DTYPE_F16>, grid, block, 0, st, a); break;
+        default: hipLaunchKernelGGL(k_token_logprobs<NQ_DTYPE_BF16>, grid, block, 0, st, a); break;
     }
-#undef NQ_LOGPROBS
-    if (const int status = nq::launch_status(); status != NQ_OK || parts == 1) return status;
-    hipLaunchKernelGGL(k_token_logprobs_join, dim3(static_cast<unsigned>(rows)), block, 0, st, a, dtype);
+    if (const int status = nq::launch_status(); status != NQ_OK || !joins) return status;
+    hipLaunchKernelGGL(k_token_logprobs_join, dim3(static_cast<unsigned>(rows)), dim3(kJoinWaves * kWave), 0, st, a, dtype);
     return nq::launch_status();
 }

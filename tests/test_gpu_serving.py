@@ -474,6 +474,26 @@ def test_token_logprobs_rows_apart(stride, offset):
     _check_logprobs(ops.launch_token_logprobs(x, tokens.to(DEV), top=5), x, tokens, 5)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_token_logprobs_ties_in_plenty(dtype):
+    """More equal values than are ranked at once: the lowest ids come first, also
+    where the values above them lie behind."""
+
+    vocab = 40003
+    x = torch.zeros(7, vocab)
+    x[1, 39990:40000] = 1.0                        # a few above, at the end
+    x[2, ::2] = -math.inf                          # every other banned
+    x[3] = torch.randint(-2, 3, (vocab,), generator=_g(47)).float()
+    x[4] = -math.inf
+    x[4, 17::1024] = 2.0                           # one to a block of 1024, and these alone
+    x[5, 5:] = -math.inf                           # five equal ones, the rest banned
+    x[6] = torch.arange(vocab) // 2000             # steps
+    x = x.to(dtype)
+    tokens = torch.tensor([0, 1, 3, 4, 17, 2, vocab - 1])
+    for top in (1, 20, 32):
+        _check_logprobs(ops.launch_token_logprobs(x.to(DEV), tokens.to(DEV), top=top), x, tokens, top)
+
+
 def test_token_logprobs_special_rows():
     x = torch.randn(12, 5000, generator=_g(46))
     x[0, :4990] = -math.inf                 # few tokens allowed
