@@ -258,7 +258,8 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 ? 1 : 2) void k_paged_attent
     constexpr int kChunks = D / 64, kDims = D / 16;
     constexpr int kBlock = TILE / 4;   // consecutive cache rows of a lane: of V, and of the scores
     constexpr int kScores = TILE / 16, kSteps = TILE / 32, kWords = kBlock / 4;
-    constexpr bool kEarly = SHARED || D == 256;  // the next K before the softmax, with registers of its own
+    constexpr bool kEarly = NT == 1 || D == 256;  // the next K before the softmax, with registers of its own
+    constexpr bool kInLds = !SHARED || NT > 1;     // where q's parts wait
     const Pages& p = a.p;
     const int lane = threadIdx.x & (kWave - 1), n = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -275,8 +276,12 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 ? 1 : 2) void k_paged_attent
 
     // This wave's query rows: row numbers, positions (-1: sees nothing), q.
     constexpr int QP = Query<QT>::kParts, kQSteps = 2 * kChunks;
-    __shared__ u32x4 q_lds[SHARED ? 1 : WAVES][SHARED ? 1 : kQSteps * NT * QP][kWave];
-    u32x4 q_regs[SHARED ? NT : 1][kQSteps][QP];
+    // LDS: q's parts, of the wave or of all; where the waves share rows, their shares later.
+    constexpr int kQFrags = kInLds ? kQSteps * NT * QP : 0, kQCopies = SHARED ? 1 : WAVES;
+    constexpr int kJoinFrags = SHARED ? WAVES * kDims * NT : 0;
+    __shared__ u32x4 lds[kQFrags * kQCopies > kJoinFrags ? kQFrags * kQCopies : kJoinFrags][kWave];
+    u32x4(*q_lds)[kWave] = lds + (SHARED ? 0 : wave * kQFrags);
+    u32x4 q_regs[kQSteps][QP];
     const int wave_row = SHARED ? 0 : wave * 16 * NT;
     int row[NT], pos[NT];
     float q_scale[NT];
@@ -290,12 +295,12 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 ? 1 : 2) void k_paged_attent
         const int place = r / a.group, head = g * a.group + r - place * a.group;
         pos[t] = on ? row_of(s.context, place, cache_rows) : -1;
         out_at[t] = (static_cast<int64_t>(s.begin + place) * a.q_heads + head) * D;
-        q_scale[t] = a.scale * load_query<QT, kQSteps>(a.q, out_at[t] + 16 * grp, on, q_regs[SHARED ? t : 0]);
-        if constexpr (!SHARED) {
+        q_scale[t] = a.scale * load_query<QT, kQSteps>(a.q, out_at[t] + 16 * grp, on, q_regs);
+        if (kInLds && (!SHARED || wave == 0)) {
 #pragma unroll
             for (int c = 0; c < kQSteps; ++c)
 #pragma unroll
-                for (int x = 0; x < QP; ++x) q_lds[wave][(c * NT + t) * QP + x][lane] = q_regs[0][c][x];
+                for (int x = 0; x < QP; ++x) q_lds[(c * NT + t) * QP + x][lane] = q_regs[c][x];
         }
         int lo = on ? pos[t] : 0x7fffffff, hi = pos[t];
 #pragma unroll
@@ -306,7 +311,8 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 ? 1 : 2) void k_paged_attent
         low_pos = min(low_pos, __builtin_amdgcn_readfirstlane(lo));
         high_pos = max(high_pos, __builtin_amdgcn_readfirstlane(hi));
     }
-    // A lane reads back what it wrote itself: nothing to wait for but the LDS.
+    // Rows of its own: a lane reads back what it wrote itself.
+    if constexpr (kInLds && SHARED) __syncthreads();
 
     f32x4 acc[kDims][NT];
     float m_run[NT], l_run[NT];
@@ -397,7 +403,7 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 ? 1 : 2) void k_paged_attent
             for (int u = 0; u < NT; ++u)
 #pragma unroll
                 for (int x = 0; x < QP; ++x)
-                    qf[u][x] = SHARED ? q_regs[SHARED ? u : 0][c][x] : q_lds[SHARED ? 0 : wave][SHARED ? 0 : (c * NT + u) * QP + x][lane];
+                    qf[u][x] = kInLds ? q_lds[kInLds ? (c * NT + u) * QP + x : 0][lane] : q_regs[c][x];
 #pragma unroll
             for (int t = 0; t < kScores; ++t) {
                 const u32x4 k = widen_k<QT>(kf[t][c / 2][2 * (c & 1)], kf[t][c / 2][2 * (c & 1) + 1]);
@@ -570,7 +576,7 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 ? 1 : 2) void k_paged_attent
         // The waves' shares of the same rows meet in LDS; each wave joins some of the
         // dimensions, the shares in wave order.
         __shared__ float join_ml[WAVES][2][16 * NT];
-        __shared__ f32x4 join_o[WAVES][kDims * NT][kWave];
+        if constexpr (kInLds) __syncthreads();  // q's parts are read
         if (grp == 0) {
 #pragma unroll
             for (int u = 0; u < NT; ++u) {
@@ -581,7 +587,7 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 ? 1 : 2) void k_paged_attent
 #pragma unroll
         for (int d = 0; d < kDims; ++d)
 #pragma unroll
-            for (int u = 0; u < NT; ++u) join_o[wave][d * NT + u][lane] = acc[d][u];
+            for (int u = 0; u < NT; ++u) lds[(wave * kDims + d) * NT + u][lane] = __builtin_bit_cast(u32x4, acc[d][u]);
         __syncthreads();
         if (wave >= kDims) return;
 #pragma unroll
@@ -599,7 +605,7 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 ? 1 : 2) void k_paged_attent
             for (int d = wave; d < kDims; d += WAVES) {
                 f32x4 o = {0, 0, 0, 0};
 #pragma unroll
-                for (int w = 0; w < WAVES; ++w) o += weight[w] * join_o[w][d * NT + u][lane];
+                for (int w = 0; w < WAVES; ++w) o += weight[w] * __builtin_bit_cast(f32x4, lds[(w * kDims + d) * NT + u][lane]);
                 put(u, d, o, m_all, l_all);
             }
         }
@@ -638,6 +644,8 @@ int launch_attention_as(const AttnArgs& a, const AttnPlan& plan, hipStream_t str
     if (plan.waves == 8) {
         if constexpr (D < 256)
             hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 1, kTileRows, true, 8>), grid, block, 0, stream, a);
+    } else if (plan.shared && plan.rows == 32) {
+        hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 2, kTileRows, true, 4>), grid, block, 0, stream, a);
     } else if (plan.shared) {
         hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 1, kTileRows, true, 4>), grid, block, 0, stream, a);
     } else {

@@ -77,44 +77,53 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows)
 }
 
 // How a call is laid out. All rules go by sizes that the host knows: the page
-// table's width stands for the cache's length.
+// table's width stands for the cache's length, the mean for the query rows of a
+// sequence (its tokens times the q heads of a kv head). Times: 32/8 heads of 128.
 //
-// Few query rows to a sequence (at most 16): a slot of 16 rows whose waves share
-// them and take the cache's tiles in turn.
-//  - Short caches (up to 12 tiles of 64 rows) are not split: eight waves, one
-//    launch (700 rows of one sequence, 32/8 heads of 128: 10.5 us against 7.7 + 3
-//    with a merge; 17 tiles: 13.9 against 11.3).
-//  - Slots and heads that fill the chip by themselves are not split either, and take
-//    eight waves from 32 tiles on (32 sequences of up to 4000 rows: 39.2 us,
-//    four waves and three splits 45.7; 64 sequences of 1000 rows: 33.9 against
-//    29.7 of four waves), unless the table has room for long sequences: then a
-//    split for each 96 tiles, up to 16, so that a long sequence among short ones
-//    does not keep one workgroup (one of 131000 rows and 31 of 500: 86 us, 718
-//    without; 32 of 32000: 356 to 375, 370 without).
+// Up to 64 query rows: a slot's waves share its rows and take the cache's tiles in
+// turn. Slots of 16 rows up to a mean of 16 (4 tokens after 3000 rows: 12 us, 18 in
+// a slot of 32), otherwise of 32, which read the cache half as often (16 sequences
+// of 12 tokens: 56 us, 100 with rows of their own; 16 sequences of 6 tokens of 16/4
+// heads of 256: 52 us, 76 in slots of 16).
+//  - Short caches (up to 12 tiles of 64 rows) of 16-row slots are not split: eight
+//    waves, one launch (700 rows of one sequence: 10.5 us against 7.7 + 3 with a
+//    merge; 17 tiles: 13.9 against 11.3).
+//  - Slots and heads that fill the chip by themselves are not split either, and
+//    16-row ones take eight waves from 32 tiles on (32 sequences of up to 4000
+//    rows: 39.2 us, four waves and three splits 45.7; 64 sequences of 1000 rows:
+//    33.9 against 29.7 of four waves), unless the table has room for long
+//    sequences: then a split for each 96 tiles, up to 16, so that a long sequence
+//    among short ones does not keep one workgroup (one of 131000 rows and 31 of
+//    500: 86 us, 718 without; 32 of 32000: 356 to 375, 370 without).
 //  - Otherwise the cache is split until there are about 1024 workgroups, for one
 //    sequence 512 (131000 rows: 60.5 us against 73.8 with 1024), of at least 8
 //    tiles, or 4 where the chip would stay empty.
 // 256-wide heads take four waves: their registers leave one to a SIMD.
-// More rows: slots of 128 rows (64 of 256-wide heads), a quarter to each wave; the
-// cache is split only as far as the chip stays empty, since every split's share
-// of every row goes through memory (2048 tokens of two sequences, 14/2 heads of
-// 64: 69 us, with two splits 165).
+// More rows: slots of 128 rows (64 of 256-wide heads), a quarter to each wave. Every
+// split's share of every row goes through memory, so the cache is split (to 512
+// workgroups) only into as many parts as it has rows for each query row (256
+// tokens after 8000 rows: 97 us, 150 with two splits; 2048 tokens of two sequences,
+// 14/2 heads of 64, not split: 69 us, 165 with two).
 AttnPlan plan_attention(int64_t tokens, int64_t batch, int q_heads, int kv_heads, int head_dim, int64_t cache_rows) {
-    constexpr int64_t kFull = 256, kShort = 12, kLong = 32, kMostSplits = 128, kSkew = 96;
+    constexpr int64_t kMostNarrow = 16, kMostShared = 64, kFull = 256, kShort = 12, kLong = 32, kMostSplits = 128, kSkew = 96;
     AttnPlan plan;
     const int64_t rows = tokens * (q_heads / kv_heads);
-    plan.shared = rows <= 16 * batch;
-    plan.rows = plan.shared ? 16 : own_rows(head_dim);
+    plan.shared = rows <= kMostShared * batch;
+    plan.rows = !plan.shared ? own_rows(head_dim) : rows <= kMostNarrow * batch ? 16 : 32;
     plan.slots = static_cast<int>(rows / plan.rows + batch);
     const int64_t tiles = (cache_rows + kTile - 1) / kTile, units = static_cast<int64_t>(plan.slots) * kv_heads;
     const bool full = units >= kFull, narrow = head_dim < 256;
     plan.least = plan.shared && units * ((tiles + 7) / 8) < 512 ? 4 : 8;
     plan.waves = 4;
-    int64_t target = kFull;
+    int64_t target = 0;
     if (plan.shared) {
         target = batch > 1 ? 1024 : 512;
-        if (narrow && ((full && tiles >= kLong) || (!full && tiles <= kShort))) plan.waves = 8;
+        if (narrow && plan.rows == 16 && ((full && tiles >= kLong) || (!full && tiles <= kShort))) plan.waves = 8;
         if (plan.waves == 8 || (full && narrow)) target = 0;
+    } else {
+        const int64_t worth = batch * cache_rows / rows;
+        target = worth < 2 ? 0 : 512;
+        if (target / units > worth) target = worth * units;
     }
     int64_t splits = target / units;
     if (full && plan.shared && tiles / kSkew > splits) splits = tiles / kSkew < 16 ? tiles / kSkew : 16;

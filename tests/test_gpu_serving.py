@@ -280,6 +280,12 @@ ATTENTIONS = [
     ([(129, 2), (200, 1)], 34, 2, 64, 16),     # more heads to a group than an MFMA has columns
     ([(300, 17)], 4, 4, 256, 64),
     ([(5, 66)], 2, 2, 256, 16),
+    # Caches long enough to be split, few query rows and many.
+    ([(1500, 1), (20, 1)], 8, 2, 128, 64),
+    ([(1300, 6), (40, 2), (0, 1)], 8, 2, 128, 32),
+    ([(900, 3), (1000, 1)], 8, 2, 256, 64),
+    ([(1100, 40)], 4, 1, 64, 32),
+    ([(1000, 30)], 4, 2, 256, 16),
 ]
 
 
@@ -303,6 +309,56 @@ def test_paged_attention(lengths, q_heads, kv, d, page, q_dtype, out_dtype):
     _check_attention(out[mine.to(DEV)], expected[mine], spread[mine], reach[mine], q_dtype=q_dtype, rows=rows, d=d)
     again = ops.launch_paged_attention(q.to(DEV), cache, scaling=d**-0.5, out_dtype=out_dtype, **batch)
     assert torch.equal(again[mine.to(DEV)], out[mine.to(DEV)])  # a fixed order
+
+
+@pytest.mark.parametrize("batch,kv,d,page,extra", [(140, 2, 64, 16, 0), (140, 2, 128, 64, 40), (70, 4, 64, 128, 100),
+                                                   (150, 1, 128, 16, 3), (200, 2, 256, 16, 1)])
+def test_paged_attention_many_sequences(batch, kv, d, page, extra):
+    """More sequences than a wave looks up at once, enough to fill the chip, with
+    page tables much wider than the caches."""
+
+    _say("many sequences", batch, kv, d, page, extra)
+    g = _g(60)
+    lengths = [(int(c), int(n)) for c, n in zip(torch.randint(0, 90, (batch,), generator=g), torch.randint(0, 3, (batch,), generator=g))]
+    lengths[batch // 2] = (600, 1)
+    b = Batch(lengths, kv=kv, d=d, page=page, seed=61, extra_entries=extra)
+    _filled(b, 62)
+    b.scales *= 2.0**-3
+    q = torch.randn(b.tokens, 2 * kv, d, generator=_g(63)).to(torch.bfloat16)
+    expected, spread, reach = osv.attention(q, b.host(), b.table, b.spans, page=page, scaling=d**-0.5)
+    cache, at = b.device()
+    out = ops.launch_paged_attention(q.to(DEV), cache, scaling=d**-0.5, out_dtype=torch.float32, **at)
+    _check_attention(out, expected, spread, reach, q_dtype=torch.bfloat16, rows=601, d=d)
+
+
+def test_paged_append_many_sequences():
+    g = _g(64)
+    lengths = [(int(c), int(n)) for c, n in zip(torch.randint(0, 40, (4200,), generator=g), torch.randint(0, 3, (4200,), generator=g))]
+    b = Batch(lengths, kv=1, d=64, page=16, seed=65)
+    q, k, v = (torch.randn(b.tokens, 1, 64, generator=_g(s)) for s in (66, 67, 68))
+    cos, sin = _rope_tables(48, 64)
+    _, expected = osv.append(q, k, v, b.host(), b.table, b.spans, page=16, q_norm=None, k_norm=None, eps=EPS, cos=cos, sin=sin)
+    cache, at = b.device()
+    ops.launch_paged_append(q.to(DEV), k.to(DEV), v.to(DEV), cache, q_heads=1, q_norm=None, k_norm=None, eps=EPS,
+                            cos=cos.to(DEV), sin=sin.to(DEV), **at)
+    assert torch.equal(cache.k_scales.cpu().double(), expected["k_scales"])
+    _same_bytes(cache.k, expected["k"])
+    _same_bytes(cache.v, expected["v"])
+
+
+@pytest.mark.parametrize("lengths", [[(70, 1)], [(200, 30)]])
+def test_paged_attention_scales_of_any_kind(lengths):
+    """A cache from elsewhere: scales that are no powers of two, and zeros."""
+
+    b = Batch(lengths, kv=2, d=128, page=16, seed=69)
+    _filled(b, 70)
+    b.scales = 0.01 * torch.rand(b.scales.shape, generator=_g(71))
+    b.scales[:, b.table[0][1]] = 0.0
+    q = torch.randn(b.tokens, 4, 128, generator=_g(72))
+    expected, spread, reach = osv.attention(q, b.host(), b.table, b.spans, page=16, scaling=0.1)
+    cache, at = b.device()
+    out = ops.launch_paged_attention(q.to(DEV), cache, scaling=0.1, out_dtype=torch.float32, **at)
+    _check_attention(out, expected, spread, reach, q_dtype=torch.float32, rows=230, d=128)
 
 
 def test_paged_attention_every_byte_is_its_value():
@@ -561,6 +617,37 @@ def test_a_captured_serving_step_replays_with_other_lengths():
             assert torch.equal(got, expected), i
         assert torch.equal(cache.k.view(torch.uint8), eager_cache.k.view(torch.uint8))
         assert torch.equal(cache.v.view(torch.uint8), eager_cache.v.view(torch.uint8))
+
+
+def test_offsets_beyond_32_bits():
+    """Pages that lie more than 2^32 bytes into the pool."""
+
+    kv, d, page, pages = 8, 128, 64, 66000
+    k = torch.empty(pages, kv, page, d, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    v = torch.empty(pages, kv, d, page, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    scales = torch.ones(2, pages, kv, device=DEV)
+    far = ops.PagedCache(k, v, scales[0], scales[1])
+    near = ops.paged_cache(4, kv, page, d, DEV)
+    q, kn, vn = (torch.randn(70, h * d, generator=_g(s)).to(DEV) for h, s in ((16, 73), (kv, 74), (kv, 75)))
+    cos, sin = (x.to(DEV) for x in _rope_tables(80, d))
+    out = []
+    for cache, table in ((far, [65999, 65990]), (near, [3, 1])):
+        at = {"page_table": torch.tensor([table], dtype=torch.int32, device=DEV),
+              "query_starts": torch.tensor([0, 70], dtype=torch.int32, device=DEV),
+              "context_lens": torch.zeros(1, dtype=torch.int32, device=DEV)}
+        rotated = ops.launch_paged_append(q, kn, vn, cache, q_heads=16, q_norm=None, k_norm=None, eps=EPS, cos=cos, sin=sin, **at)
+        out.append(ops.launch_paged_attention(rotated, cache, scaling=0.1, **at))
+        out.append(ops.launch_paged_attention(rotated[69:], cache, scaling=0.1, **{
+            **at, "query_starts": torch.tensor([0, 1], dtype=torch.int32, device=DEV),
+            "context_lens": torch.full((1,), 69, dtype=torch.int32, device=DEV)}))
+    assert torch.equal(out[0], out[2]) and torch.equal(out[1], out[3])
+    del k, v, far
+    stride = (1 << 31) + 5
+    wide = torch.empty(2 * stride, dtype=torch.bfloat16, device=DEV).as_strided((2, 5000), (stride, 1))
+    rows = torch.randn(2, 5000, generator=_g(76)).to(torch.bfloat16)
+    wide.copy_(rows)
+    tokens = torch.tensor([4999, 3])
+    _check_logprobs(ops.launch_token_logprobs(wide, tokens.to(DEV), top=8), rows, tokens, 8)
 
 
 def test_work_on_another_stream():
