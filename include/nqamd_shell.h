@@ -211,7 +211,8 @@ typedef struct nq_paged_kv {
  * q, k, v F32/F16/BF16 of one type, [tokens, heads * head_dim]; tables
  * [rope_positions, head_dim / 2]. A token whose row lies outside the page table
  * or the RoPE tables writes nothing; one whose table entry names no page writes
- * q_out alone. A page that the call writes to belongs to one sequence.
+ * q_out alone. A page that the call writes to belongs to one sequence and stands
+ * once in its part of the table. q_out may be q.
  * K is normed and rotated in fp64, so a stored byte is the rounding of the exact
  * value. Replaces launch_decode_rope and launch_cache_prefix_update
  * (src/nanoquant/runtime/cuda_kernels.py:401-447,546-587,715-815) for many
@@ -229,11 +230,13 @@ int64_t nq_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int32_
  * with the same arrays): the token at cache row r attends rows [0, r] of its
  * sequence, kv head h / (q_heads / kv_heads):
  *   out[t, h, :] = softmax(scaling * q[t, h, :] . K) . V
- * q F32/F16/BF16 [tokens, q_heads, head_dim], read exactly; out F32/F16/BF16
- * [tokens, q_heads * head_dim]; both 16-byte aligned, q_heads a multiple of
- * kv_heads. Scores and softmax in fp32, results joined in a fixed order
- * (deterministic). A token whose row lies outside the page table gives zeros.
- * A table entry in use that names no page counts as NaN rows. NaN in the cache,
+ * q F32/F16/BF16 [tokens, q_heads, head_dim] of any magnitude (F16 and BF16 read
+ * exactly, F32 to 24 bits of every value down to 2^-28 of its head's largest); out
+ * F32/F16/BF16 [tokens, q_heads * head_dim]; both 16-byte aligned, q_heads a
+ * multiple of kv_heads. Scores and softmax in fp32, the weights to 16 bits for
+ * 16-bit outputs and 24 for fp32, results joined in a fixed order (deterministic).
+ * A token whose row lies outside the page table gives zeros. A table entry in use
+ * that names no page counts as NaN rows. NaN in the cache,
  * infinities and NaN in q do what fp32 arithmetic does with them, for the tokens
  * that see them alone; rows that nobody sees may hold anything. Replaces
  * launch_decode_attention (src/nanoquant/runtime/cuda_kernels.py:448-544) for

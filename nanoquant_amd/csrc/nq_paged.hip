@@ -15,6 +15,9 @@
 namespace nq {
 namespace paged {
 
+// Cache rows of a sequence at most: row numbers a few tiles further fit 32 bits.
+constexpr int64_t kMostRows = 0x3fffffff;
+
 int check_pages(const nq_paged_kv* kv, int64_t tokens, Pages& out) {
     if (!kv || !kv->k_pages || !kv->v_pages || !kv->k_scales || !kv->v_scales || !kv->page_table ||
         !kv->query_starts || !kv->context_lens)
@@ -24,7 +27,7 @@ int check_pages(const nq_paged_kv* kv, int64_t tokens, Pages& out) {
     while (shift < 7 && (1 << shift) != kv->page_size) ++shift;
     if ((1 << shift) != kv->page_size) return NQ_ERR_SHAPE;
     if (kv->num_pages <= 0 || kv->num_pages > 0x7fffffff || kv->kv_heads <= 0 || kv->kv_heads > 65535 ||
-        kv->batch <= 0 || kv->batch > 0xffffff || kv->table_pages <= 0 || kv->table_pages > (0x7fffff00 >> shift) ||
+        kv->batch <= 0 || kv->batch > 0xffffff || kv->table_pages <= 0 || kv->table_pages > (kMostRows >> shift) ||
         tokens <= 0 || tokens > 0xffffff)
         return NQ_ERR_SHAPE;
     if ((reinterpret_cast<uintptr_t>(kv->k_pages) | reinterpret_cast<uintptr_t>(kv->v_pages)) & 15)

@@ -439,15 +439,15 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 ? 1 : 2) void k_paged_attent
 
         const bool masked = base + TILE > low_pos + 1;  // uniform: some row of the wave does not see them all
         if (masked) {
-            // A block that a row does not see may have any scale; one that it sees in
-            // part has a page.
+            // Rows that nobody sees may have any scale: the scores are multiplied here.
 #pragma unroll
             for (int u = 0; u < NT; ++u) {
                 const int seen = pos[u] + 1 - (base + kBlock * grp);
-                if (seen <= 0) f[u] = weight_up[u] = 1.0f;
 #pragma unroll
                 for (int j = 0; j < kBlock; ++j)
-                    if (j >= seen) sc[j >> 2][u][j & 3] = -INFINITY;
+                    sc[j >> 2][u][j & 3] = j < seen ? sc[j >> 2][u][j & 3] * f[u] : -INFINITY;
+                f[u] = 1.0f;
+                if (seen <= 0) weight_up[u] = 1.0f;
             }
         }
 

@@ -143,7 +143,7 @@ extern "C" int64_t nq_paged_attention_workspace_bytes(int64_t tokens, int64_t ba
                                                       int32_t head_dim, int32_t page_size, int64_t table_pages) {
     if (tokens <= 0 || tokens > 0xffffff || batch <= 0 || batch > 0xffffff || kv_heads <= 0 || q_heads <= 0 ||
         q_heads > 65535 || q_heads % kv_heads || page_size <= 0 || page_size > 128 || table_pages <= 0 ||
-        table_pages > 0x7fffffff / page_size || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+        table_pages > 0x3fffffff / page_size || (head_dim != 64 && head_dim != 128 && head_dim != 256))
         return -1;
     if (tokens * q_heads > 0x3fffffff) return -1;
     const AttnPlan plan = plan_attention(tokens, batch, q_heads, kv_heads, head_dim, table_pages * page_size);

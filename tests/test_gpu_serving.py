@@ -346,9 +346,10 @@ def test_paged_append_many_sequences():
     _same_bytes(cache.v, expected["v"])
 
 
-@pytest.mark.parametrize("lengths", [[(70, 1)], [(200, 30)]])
+@pytest.mark.parametrize("lengths", [[(70, 1)], [(200, 30)], [(18, 5)], [(20, 1)]])
 def test_paged_attention_scales_of_any_kind(lengths):
-    """A cache from elsewhere: scales that are no powers of two, and zeros."""
+    """A cache from elsewhere: scales that are no powers of two, and zeros, also in
+    the last page."""
 
     b = Batch(lengths, kv=2, d=128, page=16, seed=69)
     _filled(b, 70)

@@ -36,7 +36,7 @@ def _attend(kv, *, q=A, dtype=0, tokens=3, q_heads=4, scaling=0.1, out=A, out_dt
     ({"k_pages": None}, -1), ({"v_scales": None}, -1), ({"page_table": None}, -1), ({"query_starts": None}, -1),
     ({"context_lens": None}, -1), ({"head_dim": 96}, -3), ({"page_size": 8}, -3), ({"page_size": 48}, -3),
     ({"page_size": 256}, -3), ({"num_pages": 0}, -3), ({"kv_heads": 0}, -3), ({"kv_heads": 3}, -3), ({"batch": 0}, -3),
-    ({"table_pages": 0}, -3), ({"table_pages": 1 << 28}, -3), ({"v_pages": A + 8}, -4),
+    ({"table_pages": 0}, -3), ({"table_pages": 1 << 28}, -3), ({"table_pages": 1 << 26}, -3), ({"v_pages": A + 8}, -4),
 ])
 def test_cache_and_batch(call, changes, status):
     assert call(_kv(**changes)) == status
