@@ -3,6 +3,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "nq_common.h"
 #include "../../include/nqamd_shell.h"
 
@@ -66,6 +68,22 @@ __device__ __forceinline__ Found sequence_at(const Pages& p, int64_t slot, const
     const int hit = below ? 63 - __builtin_clzll(below) : 0;
     return {__builtin_amdgcn_readfirstlane(low + hit), __builtin_amdgcn_readlane(context, hit),
             {__builtin_amdgcn_readlane(begin, hit), __builtin_amdgcn_readlane(end, hit)}};
+}
+
+// Sum of a lane's value and those of the lanes before it (DPP).
+__device__ __forceinline__ uint32_t running_sum(uint32_t v) {
+    const auto add = [&](auto ctrl, auto rows) {
+        v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ctrl)::value,
+                                                               decltype(rows)::value, 0xf, false));
+    };
+    using std::integral_constant;
+    add(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // row_shr:1
+    add(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+    add(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+    add(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+    add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast:15 to rows 1 and 3
+    add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // row_bcast:31 to rows 2 and 3
+    return v;
 }
 
 // A token's cache row: its sequence's context plus its place, or -1 outside

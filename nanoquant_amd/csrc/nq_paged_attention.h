@@ -37,29 +37,94 @@ struct AttnArgs {
     Pages p;
     const void* q;
     void* out;
-    float* partial;    // [slots][splits][kv_heads][rows][2] (max, sum), then the same of [head_dim]
+    float* partial;    // [items][kv_heads][rows][2] (max, sum), then the same of [head_dim]
     float* partial_o;
     float scale;       // scaling * log2(e): scores are kept in base 2
     int32_t out_dtype, q_heads, group, slots, splits, least;  // least: cache tiles a split takes at least
 };
 
-// What a slot of `rows` query rows holds, the same for the attention and the merge.
+// Cache tiles of each split, and splits that have any, of a sequence whose last
+// token sees `visible` rows.
+struct SplitPlan {
+    int per, active;
+};
+
+__device__ __forceinline__ SplitPlan split_plan(int visible, int splits, int least) {
+    if (splits == 1) return {0x1ffffff, 1};
+    const int tiles = (visible + kTile - 1) / kTile;
+    const int per = max((tiles + splits - 1) / splits, least);
+    return {per, max((tiles + per - 1) / per, 1)};
+}
+
+// A sequence's share of the work: items of `rows` query rows (a slot) and one of
+// its splits, the splits of a slot next to each other.
+struct Work {
+    Found f;
+    SplitPlan plan;
+    int64_t first, local;  // the sequence's first item; the item's (a token's slot's first item's) place in it
+};
+
+// The work that item `at`, or (TOKEN) token `at` and its q head `head` of a group,
+// belongs to. Up to 64 sequences' items follow each other without gaps, a lane
+// counting each sequence's: workgroups go to the chip's dies and to their parts in
+// turn, so that empty ones among the others leave parts with nothing to do
+// (16 ragged sequences of up to 6 tokens after 3000 rows: 21.3 us, 30.8 with
+// the search's empty ones; 16 of 12 tokens: 41, 58). More sequences have one slot
+// more each than they may need, and all of a slot's splits, found by search.
+template <bool TOKEN>
+__device__ __forceinline__ Work find(const Pages& p, int64_t at, int head, int group, int rows, int splits, int least) {
+    const int cache_rows = p.table_pages << p.page_shift;
+    const auto plan_of = [&](int context, int begin, int end) {
+        const int64_t seen = static_cast<int64_t>(context) + (end - begin);
+        return split_plan(static_cast<int>(min(max(seen, int64_t{0}), static_cast<int64_t>(cache_rows))), splits, least);
+    };
+    Work w;
+    int stride;
+    if (p.batch > kWave) {
+        const auto slot_of = [&](int i, int begin) { return static_cast<int64_t>(begin) * group / rows + i; };
+        const int64_t slot = TOKEN ? at : static_cast<uint32_t>(at) / static_cast<uint32_t>(splits);
+        w.f = sequence_at(p, slot, [&](int i, int begin) { return TOKEN ? static_cast<int64_t>(begin) : slot_of(i, begin); });
+        w.plan = plan_of(w.f.context, w.f.span.begin, w.f.span.end);
+        w.first = slot_of(w.f.b, w.f.span.begin) * splits;
+        stride = splits;
+    } else {
+        const int lane = threadIdx.x & (kWave - 1), b = min(lane, p.batch - 1);
+        const int start = p.starts[b], stop = p.starts[b + 1], context = p.contexts[b];
+        const int begin = min(max(start, 0), p.tokens), end = min(max(stop, begin), p.tokens);
+        const SplitPlan plan = plan_of(context, begin, end);
+        const uint32_t slots = static_cast<uint32_t>((end - begin) * group + rows - 1) / static_cast<uint32_t>(rows);
+        const uint32_t count = lane < p.batch ? slots * plan.active : 0, upto = running_sum(count);
+        // Of a prompt's rows the last see the most: the last items go first.
+        if (!TOKEN) at = static_cast<uint32_t>(__builtin_amdgcn_readlane(upto, kWave - 1)) - 1 - at;
+        const uint64_t before = __ballot(lane < p.batch && (TOKEN ? begin <= at : static_cast<int64_t>(upto) <= at));
+        const int hit = TOKEN ? (before ? 63 - __builtin_clzll(before) : 0) : min(__popcll(before), p.batch - 1);
+        const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, hit); };
+        w.f = {hit, of(context), {of(begin), of(end)}};
+        w.plan = {of(plan.per), of(plan.active)};
+        w.first = static_cast<uint32_t>(of(static_cast<int>(upto - count)));
+        stride = w.plan.active;
+    }
+    if constexpr (TOKEN) {
+        const uint32_t row = static_cast<uint32_t>(max(static_cast<int>(at) - w.f.span.begin, 0)) * group + head;
+        w.local = static_cast<int64_t>(row / static_cast<uint32_t>(rows)) * stride;
+    } else {
+        w.local = at - w.first;
+    }
+    return w;
+}
+
+// What a slot of a sequence, from query row `row0` on, holds.
 struct SlotSpan {
     int b, begin, context;  // sequence, its first token, rows cached before the call
     int row0, rows;         // the slot's first query row in its sequence; rows it holds
     int visible;            // cache rows [0, visible) that some row of the slot sees
 };
 
-__device__ __forceinline__ int64_t first_slot_of(int b, int begin, int group, int rows) {
-    return static_cast<int64_t>(begin) * group / rows + b;
-}
-
-__device__ __forceinline__ SlotSpan slot_span(const Pages& p, const Found& f, int64_t slot, int group, int rows) {
+__device__ __forceinline__ SlotSpan slot_span(const Pages& p, const Found& f, int64_t row0, int group, int rows) {
     SlotSpan o;
     o.b = f.b;
     o.begin = f.span.begin;
     o.context = f.context;
-    const int64_t row0 = (slot - first_slot_of(f.b, f.span.begin, group, rows)) * rows;
     const int64_t all = static_cast<int64_t>(f.span.end - f.span.begin) * group;
     o.row0 = static_cast<int>(row0 < 0 || row0 >= all ? 0 : row0);
     o.rows = static_cast<int>(row0 < 0 || row0 >= all ? 0 : min(static_cast<int64_t>(rows), all - row0));
@@ -67,19 +132,6 @@ __device__ __forceinline__ SlotSpan slot_span(const Pages& p, const Found& f, in
     o.visible = o.rows == 0 || last < 0
                     ? 0 : static_cast<int>(min(last + 1, static_cast<int64_t>(p.table_pages) << p.page_shift));
     return o;
-}
-
-// Cache tiles of each split, and splits that have any.
-struct SplitPlan {
-    int tiles, per, active;
-};
-
-__device__ __forceinline__ SplitPlan split_plan(int visible, int splits, int least) {
-    SplitPlan s;
-    s.tiles = (visible + kTile - 1) / kTile;
-    s.per = max((s.tiles + splits - 1) / splits, least);
-    s.active = (s.tiles + s.per - 1) / s.per;
-    return s;
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -248,31 +300,40 @@ __device__ __forceinline__ void store4(void* out, int dtype, int64_t at, const f
 
 // One workgroup of WAVES waves: a slot of query rows of one kv head over one
 // split of the cache. SHARED: the waves hold the same 16 NT rows and take the
-// split's tiles in turn (few query rows: the cache's bytes are the work);
-// otherwise each wave has 16 NT rows of its own, whose parts wait in LDS (in
-// registers they would leave room for one wave to a SIMD, and nothing would fill
-// the matrix unit during a softmax), and all take every tile.
+// split's tiles in turn; otherwise each wave has 16 NT rows of its own and all take
+// every tile. Where registers are short, q's parts wait in LDS (in registers they
+// would leave room for one wave to a SIMD, and nothing would fill the matrix unit
+// during a softmax).
+//
+// Single tokens are bound by the cache's bytes: 268 MB of one sequence at 5.1 TB/s
+// (a copy reaches 5.04), 153 MB of 64 sequences at 4.5 with the launch. Prompts are
+// bound by the vector unit, which widens K and V, and takes exponentials and parts of
+// the weights (4096 tokens of 32/8 heads of 128: 231 us for 1.4e11 multiplications
+// and additions; vector instructions issue in 64% of the cycles, the matrix unit
+// works in 35%).
 template <int D, int QT, int PP, int NT, int TILE, bool SHARED, int WAVES>
-__global__ __launch_bounds__(WAVES* kWave, D == 256 ? 1 : 2) void k_paged_attention(const AttnArgs a) {
+__global__ __launch_bounds__(WAVES* kWave, D == 256 && NT == 2 ? 1 : 2) void k_paged_attention(const AttnArgs a) {
     constexpr int kRows = (SHARED ? 1 : WAVES) * 16 * NT;
     constexpr int kChunks = D / 64, kDims = D / 16;
     constexpr int kBlock = TILE / 4;   // consecutive cache rows of a lane: of V, and of the scores
     constexpr int kScores = TILE / 16, kSteps = TILE / 32, kWords = kBlock / 4;
-    constexpr bool kEarly = NT == 1 || D == 256;  // the next K before the softmax, with registers of its own
-    constexpr bool kInLds = !SHARED || NT > 1;     // where q's parts wait
+    constexpr bool kEarly = SHARED;    // the next K before the softmax, with registers of its own
+    constexpr bool kInLds = !SHARED || NT > 1 || D == 256;  // where q's parts wait
     const Pages& p = a.p;
     const int lane = threadIdx.x & (kWave - 1), n = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int g = blockIdx.x % p.kv_heads;
-    const int rest = blockIdx.x / p.kv_heads;
-    // Of a prompt's rows the last see the most: their slots go first.
-    const int split = rest % a.splits, slot = SHARED ? rest / a.splits : a.slots - 1 - rest / a.splits;
-    const Found found = sequence_at(p, slot, [&](int i, int begin) { return first_slot_of(i, begin, a.group, kRows); });
-    const SlotSpan s = slot_span(p, found, slot, a.group, kRows);
+    const Work w = find<false>(p, blockIdx.x / p.kv_heads, 0, a.group, kRows, a.splits, a.least);
+    const int64_t item = w.first + w.local;
+    if (w.local < 0 || item >= static_cast<int64_t>(a.slots) * a.splits) return;  // none, or query_starts out of order
+    const uint32_t local = static_cast<uint32_t>(w.local), stride = p.batch > kWave ? a.splits : w.plan.active;
+    const uint32_t nth = local / stride;
+    const int split = static_cast<int>(local - nth * stride);
+    if (split >= w.plan.active) return;
+    const SplitPlan plan = w.plan;
+    const SlotSpan s = slot_span(p, w.f, static_cast<int64_t>(nth) * kRows, a.group, kRows);
     if (s.rows == 0) return;
     const int page = 1 << p.page_shift, cache_rows = p.table_pages << p.page_shift;
-    const SplitPlan plan = split_plan(s.visible, a.splits, a.least);
-    if (split > 0 && split >= plan.active) return;
 
     // This wave's query rows: row numbers, positions (-1: sees nothing), q.
     constexpr int QP = Query<QT>::kParts, kQSteps = 2 * kChunks;
@@ -564,7 +625,7 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 ? 1 : 2) void k_paged_attent
             for (int i = 0; i < 4; ++i) v[i] = pos[t] < 0 ? 0.0f : o[i] * inv;
             store4(a.out, a.out_dtype, out_at[t] + 16 * d + 4 * grp, v);
         } else {
-            const int64_t at = ((static_cast<int64_t>(slot) * a.splits + split) * p.kv_heads + g) * kRows + row[t];
+            const int64_t at = (item * p.kv_heads + g) * kRows + row[t];
             if (d == 0 && grp == 0) {
                 a.partial[2 * at] = m;
                 a.partial[2 * at + 1] = l;
@@ -623,14 +684,11 @@ struct AttnPlan {
     bool shared;
 };
 
-// Query rows of a wave where each has its own: 32, of 256-wide heads 16.
-template <int D>
-constexpr int kOwnTiles = D == 256 ? 1 : 2;
-// Cache rows that a wave takes at once.
+// Cache rows that a wave takes at once where the registers hold them.
 template <int D>
 constexpr int kRowsAtOnce = D == 256 ? 32 : 64;
 
-constexpr int own_rows(int head_dim) { return 64 * (head_dim == 256 ? 1 : 2); }
+constexpr int kOwnRows = 128;  // of a slot whose waves have rows of their own, 32 each
 
 template <int D>
 int launch_paged_attention(const AttnArgs& a, const AttnPlan& plan, int q_dtype, hipStream_t stream);
@@ -641,15 +699,16 @@ int launch_attention_as(const AttnArgs& a, const AttnPlan& plan, hipStream_t str
     if (blocks > 0x7fffffff) return NQ_ERR_SHAPE;
     const dim3 grid(static_cast<unsigned>(blocks)), block(static_cast<unsigned>(plan.waves * kWave));
     constexpr int kTileRows = kRowsAtOnce<D>;
-    if (plan.waves == 8) {
-        if constexpr (D < 256)
+    if (plan.shared && plan.waves == 4) {
+        if (plan.rows == 32)
+            hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 2, 32, true, 4>), grid, block, 0, stream, a);
+        else
+            hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 1, kTileRows, true, 4>), grid, block, 0, stream, a);
+    } else if constexpr (D < 256) {
+        if (plan.shared)
             hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 1, kTileRows, true, 8>), grid, block, 0, stream, a);
-    } else if (plan.shared && plan.rows == 32) {
-        hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 2, kTileRows, true, 4>), grid, block, 0, stream, a);
-    } else if (plan.shared) {
-        hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 1, kTileRows, true, 4>), grid, block, 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((k_paged_attention<D, QT, PP, kOwnTiles<D>, kTileRows, false, 4>), grid, block, 0, stream, a);
+        else
+            hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 2, kTileRows, false, 4>), grid, block, 0, stream, a);
     }
     return nq::launch_status();
 }

@@ -25,15 +25,16 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows)
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int token = blockIdx.x / a.q_heads, head = blockIdx.x - token * a.q_heads;
-    const Found f = sequence_at(p, token, [](int, int begin) { return static_cast<int64_t>(begin); });
-    if (token < f.span.begin || token >= f.span.end) return;
     const int g = head / a.group;
-    const int64_t r = static_cast<int64_t>(token - f.span.begin) * a.group + head - g * a.group;
-    const int64_t slot = first_slot_of(f.b, f.span.begin, a.group, rows) + r / rows;
-    const SlotSpan s = slot_span(p, f, slot, a.group, rows);
-    const SplitPlan plan = split_plan(s.visible, a.splits, a.least);
+    const Work work = find<true>(p, token, head - g * a.group, a.group, rows, a.splits, a.least);
+    const Found& f = work.f;
+    if (token < f.span.begin || token >= f.span.end) return;
+    const SplitPlan plan = work.plan;
     if (plan.active <= 1) return;  // the attention wrote the output itself
-    const int64_t first = (slot * a.splits * p.kv_heads + g) * rows + r % rows;
+    const int64_t item = work.first + work.local;
+    if (item < 0 || item + plan.active > static_cast<int64_t>(a.slots) * a.splits) return;  // query_starts out of order
+    const uint32_t r = static_cast<uint32_t>(token - f.span.begin) * a.group + head - g * a.group;
+    const int64_t first = (item * p.kv_heads + g) * rows + r % static_cast<uint32_t>(rows);
     const int64_t next = static_cast<int64_t>(p.kv_heads) * rows;  // from one split's row to the next split's
     float w[kMost], l[kMost], m = -INFINITY;
 #pragma unroll
@@ -69,7 +70,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows)
 #pragma unroll
     for (int j = 0; j < E; ++j) join[wave][lane + kWave * j] = o[j];
     __syncthreads();
-    const bool off = row_of(s.context, token - s.begin, p.table_pages << p.page_shift) < 0;
+    const bool off = row_of(f.context, token - f.span.begin, p.table_pages << p.page_shift) < 0;
     for (int d = threadIdx.x; d < D; d += kWaves * kWave) {
         const float all = (join[0][d] + join[1][d]) + (join[2][d] + join[3][d]);
         nq::store_f32_as(a.out, a.out_dtype, static_cast<int64_t>(blockIdx.x) * D + d, off ? 0.0f : all / sum);
@@ -78,54 +79,63 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows)
 
 // How a call is laid out. All rules go by sizes that the host knows: the page
 // table's width stands for the cache's length, the mean for the query rows of a
-// sequence (its tokens times the q heads of a kv head). Times: 32/8 heads of 128.
+// sequence (its tokens times the q heads of a kv head). Times: 32/8 heads of 128,
+// after that many cached rows.
 //
-// Up to 64 query rows: a slot's waves share its rows and take the cache's tiles in
-// turn. Slots of 16 rows up to a mean of 16 (4 tokens after 3000 rows: 12 us, 18 in
-// a slot of 32), otherwise of 32, which read the cache half as often (16 sequences
-// of 12 tokens: 56 us, 100 with rows of their own; 16 sequences of 6 tokens of 16/4
-// heads of 256: 52 us, 76 in slots of 16).
-//  - Short caches (up to 12 tiles of 64 rows) of 16-row slots are not split: eight
-//    waves, one launch (700 rows of one sequence: 10.5 us against 7.7 + 3 with a
-//    merge; 17 tiles: 13.9 against 11.3).
-//  - Slots and heads that fill the chip by themselves are not split either, and
-//    16-row ones take eight waves from 32 tiles on (32 sequences of up to 4000
-//    rows: 39.2 us, four waves and three splits 45.7; 64 sequences of 1000 rows:
-//    33.9 against 29.7 of four waves), unless the table has room for long
-//    sequences: then a split for each 96 tiles, up to 16, so that a long sequence
-//    among short ones does not keep one workgroup (one of 131000 rows and 31 of
-//    500: 86 us, 718 without; 32 of 32000: 356 to 375, 370 without).
-//  - Otherwise the cache is split until there are about 1024 workgroups, for one
-//    sequence 512 (131000 rows: 60.5 us against 73.8 with 1024), of at least 8
+// Usually a slot's waves share its rows and take the cache's tiles in turn; slots
+// have 32 rows, which read the cache half as often as 16 (16 sequences of 12 tokens
+// after 3000 rows: 40 us, 50 with 16), but 16
+//  - up to a mean of 16 (4 tokens after 3000: 12 us, 15 with 32);
+//  - where those do not fill the chip and the cache is short (4 sequences of 12
+//    tokens after 500: 11 us, 17 with 32; one of 64 after 30000: 81, 98 with 16;
+//    256-wide heads, 40 tokens after 30: 10 us, 16 with 32, but 16 sequences of 6
+//    after 3000: 38, 43 with 16).
+// Slots of 128 rows, a quarter to each wave, read the cache still less, but leave a
+// chip that they do not fill to one after the other: they are taken from a size on
+// (4096 tokens: 231 us, 286 shared, but 1531 after 517: 98 and 100, 512 after 3500:
+// 94 and 75, 8 sequences of up to 128 after 600: 41 and 19; 4096 of 32/8 heads of
+// 64: 147 and 165, but 2 times 2048 of 14/2: 68 and 50) and after very long caches
+// (512 after 20000: 290, 352 shared). 256-wide heads have them never (4096 tokens
+// of 16/4: 366 us shared, 508 in slots of 64).
+//
+// Splits of the cache, joined in a second launch:
+//  - Short caches (up to 12 tiles of 64 rows) and few 16-row slots have none: eight
+//    waves (one sequence of 700 rows: 10.5 us, as with splits, but a launch less).
+//  - Slots and heads that fill the chip have none (32 sequences of up to 4000 rows:
+//    37.5 us, 44 split), unless the table has room for long sequences: then a split
+//    for each 96 tiles, up to 16, so that a long sequence among short ones does not
+//    keep one workgroup (one of 131000 rows and 31 of 500: 67 us, 718 without; 32
+//    of 32000: 372, 363 without).
+//  - Otherwise as many as make the workgroups that the chip holds at once (8
+//    sequences of 5000 rows: 22.4 us with 512 workgroups, 25.9 with 1024; one of
+//    131000: 60.3, 66.0; 32-row slots of 256-wide heads have a compute unit each:
+//    38 us for 16 sequences of 6 tokens with 256, 52 with 384), of at least 8
 //    tiles, or 4 where the chip would stay empty.
-// 256-wide heads take four waves: their registers leave one to a SIMD.
-// More rows: slots of 128 rows (64 of 256-wide heads), a quarter to each wave. Every
-// split's share of every row goes through memory, so the cache is split (to 512
-// workgroups) only into as many parts as it has rows for each query row (256
-// tokens after 8000 rows: 97 us, 150 with two splits; 2048 tokens of two sequences,
-// 14/2 heads of 64, not split: 69 us, 165 with two).
 AttnPlan plan_attention(int64_t tokens, int64_t batch, int q_heads, int kv_heads, int head_dim, int64_t cache_rows) {
-    constexpr int64_t kMostNarrow = 16, kMostShared = 64, kFull = 256, kShort = 12, kLong = 32, kMostSplits = 128, kSkew = 96;
+    constexpr int64_t kMostNarrow = 16, kMostShared = 64, kFull = 256, kShort = 12, kMedium = 64, kVeryLong = 256;
+    constexpr int64_t kMostSplits = 128, kSkew = 96;
     AttnPlan plan;
-    const int64_t rows = tokens * (q_heads / kv_heads);
-    plan.shared = rows <= kMostShared * batch;
-    plan.rows = !plan.shared ? own_rows(head_dim) : rows <= kMostNarrow * batch ? 16 : 32;
+    const int64_t rows = tokens * (q_heads / kv_heads), mean = (rows + batch - 1) / batch;
+    const int64_t tiles = (cache_rows + kTile - 1) / kTile;
+    const bool narrow = head_dim < 256;
+    // Slots in use, if all sequences have the mean.
+    const auto work_of = [&](int64_t of) { return batch * ((mean + of - 1) / of) * kv_heads; };
+    plan.shared = !narrow || rows <= kMostShared * batch ||
+                  (work_of(kOwnRows) < (head_dim == 64 ? 1024 : 352) && (mean <= kOwnRows || tiles < kVeryLong));
+    plan.rows = !plan.shared ? kOwnRows
+                : rows <= kMostNarrow * batch || (work_of(16) < kFull && tiles <= (narrow ? kMedium : kShort)) ? 16 : 32;
     plan.slots = static_cast<int>(rows / plan.rows + batch);
-    const int64_t tiles = (cache_rows + kTile - 1) / kTile, units = static_cast<int64_t>(plan.slots) * kv_heads;
-    const bool full = units >= kFull, narrow = head_dim < 256;
+    const int64_t units = static_cast<int64_t>(plan.slots) * kv_heads;
+    const int64_t work = work_of(plan.rows);
+    const bool full = units >= kFull;
     plan.least = plan.shared && units * ((tiles + 7) / 8) < 512 ? 4 : 8;
     plan.waves = 4;
-    int64_t target = 0;
+    int64_t target = !narrow && plan.rows == 32 ? 256 : 512;  // workgroups that the chip holds at once
     if (plan.shared) {
-        target = batch > 1 ? 1024 : 512;
-        if (narrow && plan.rows == 16 && ((full && tiles >= kLong) || (!full && tiles <= kShort))) plan.waves = 8;
+        if (narrow && plan.rows == 16 && !full && tiles <= kShort) plan.waves = 8;
         if (plan.waves == 8 || (full && narrow)) target = 0;
-    } else {
-        const int64_t worth = batch * cache_rows / rows;
-        target = worth < 2 ? 0 : 512;
-        if (target / units > worth) target = worth * units;
     }
-    int64_t splits = target / units;
+    int64_t splits = target / work;
     if (full && plan.shared && tiles / kSkew > splits) splits = tiles / kSkew < 16 ? tiles / kSkew : 16;
     const int64_t most = (tiles + plan.least - 1) / plan.least;
     splits = splits < most ? splits : most;

@@ -380,6 +380,28 @@ def test_paged_attention_every_byte_is_its_value():
     assert torch.equal(out[0].cpu()[~nan], expected[~nan])
 
 
+@pytest.mark.parametrize("batch,d,new", [(63, 64, (0, 1, 1, 3)), (64, 128, (1, 0, 9, 2, 33)), (64, 256, (6, 1, 0, 4, 9)),
+                                         (65, 64, (0, 1, 9, 2)), (5, 64, (40, 0, 25, 18, 50)), (5, 256, (30, 0, 25, 18, 50))])
+def test_paged_attention_uneven_batches(batch, d, new):
+    """Sequences without tokens or rows, of one slot and several, among ones that are split."""
+
+    _say("uneven", batch, d, new)
+    contexts = (700, 0, 33, 2000 if batch < 6 else 900, 1)
+    lengths = [(contexts[i * i % 5] if i % 3 else 0, new[i % len(new)]) for i in range(batch - 1)] + [(1200, new[0])]
+    b = Batch(lengths, kv=2, d=d, page=32, seed=83, ahead=2, behind=1)
+    _filled(b, 84)
+    b.scales *= 2.0**-3
+    q = torch.randn(b.tokens, 8, d, generator=_g(85)).to(torch.bfloat16)
+    expected, spread, reach = osv.attention(q, b.host(), b.table, b.spans, page=32, scaling=d**-0.5)
+    cache, at = b.device()
+    out = torch.full((b.tokens, 8 * d), 9.0, dtype=torch.float32, device=DEV)
+    ops.launch_paged_attention(q.to(DEV), cache, scaling=d**-0.5, out=out, **at)
+    mine = ~torch.isnan(expected[:, 0, 0])
+    assert (out.cpu()[~mine] == 9.0).all()
+    rows = max(c + n for c, n in lengths)
+    _check_attention(out[mine.to(DEV)], expected[mine], spread[mine], reach[mine], q_dtype=torch.bfloat16, rows=rows, d=d)
+
+
 @pytest.mark.parametrize("what", ["k", "v"])
 @pytest.mark.parametrize("lengths,row", [([(0, 70)], 40), ([(90, 6)], 93), ([(10, 3)], 12), ([(200, 2)], 17)])
 def test_paged_attention_nan_reaches_those_who_see_it(lengths, row, what):

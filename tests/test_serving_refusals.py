@@ -105,3 +105,10 @@ def test_wrappers_refuse_host_tensors_and_bad_geometry():
     for geometry in ((0, 1, 16, 64), (1, 1, 24, 64), (1, 1, 16, 80), (1, 0, 16, 64)):
         with pytest.raises(ValueError, match="geometry"):
             ops.paged_cache(*geometry, "cpu")
+
+
+@pytest.mark.parametrize("tokens,batch", [(1, 2), (3, 70), (64, 65), (1, 100000)])
+def test_a_batch_may_have_more_sequences_than_tokens(tokens, batch):
+    for head_dim in (64, 128, 256):
+        for table_pages in (1, 100, 4000):
+            assert _native.load().nq_paged_attention_workspace_bytes(tokens, batch, 4, 4, head_dim, 64, table_pages) >= 0
