@@ -212,7 +212,7 @@ typedef struct nq_paged_kv {
  * [rope_positions, head_dim / 2]. A token whose row lies outside the page table
  * or the RoPE tables writes nothing; one whose table entry names no page writes
  * q_out alone. A page that the call writes to belongs to one sequence and stands
- * once in its part of the table. q_out may be q.
+ * once in its part of the table. q_out may be q where both have one type.
  * K is normed and rotated in fp64, so a stored byte is the rounding of the exact
  * value. Replaces launch_decode_rope and launch_cache_prefix_update
  * (src/nanoquant/runtime/cuda_kernels.py:401-447,546-587,715-815) for many
@@ -230,15 +230,15 @@ int64_t nq_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int32_
  * with the same arrays): the token at cache row r attends rows [0, r] of its
  * sequence, kv head h / (q_heads / kv_heads):
  *   out[t, h, :] = softmax(scaling * q[t, h, :] . K) . V
- * q F32/F16/BF16 [tokens, q_heads, head_dim] of any magnitude (F16 and BF16 read
- * exactly, F32 to 24 bits of every value down to 2^-28 of its head's largest); out
+ * q F32/F16/BF16 [tokens, q_heads, head_dim] (F16 and BF16 read exactly, F32 to
+ * 24 bits of every value down to 2^-28 of its head's largest, or of 2^-100); out
  * F32/F16/BF16 [tokens, q_heads * head_dim]; both 16-byte aligned, q_heads a
  * multiple of kv_heads. Scores and softmax in fp32, the weights to 16 bits for
  * 16-bit outputs and 24 for fp32, results joined in a fixed order (deterministic).
  * A token whose row lies outside the page table gives zeros. A table entry in use
- * that names no page counts as NaN rows. NaN in the cache,
- * infinities and NaN in q do what fp32 arithmetic does with them, for the tokens
- * that see them alone; rows that nobody sees may hold anything. Replaces
+ * that names no page counts as NaN rows. NaN in the cache, infinities and NaN in q
+ * do what fp32 arithmetic does with them, for the tokens that see them alone; rows
+ * that nobody sees may hold anything. Replaces
  * launch_decode_attention (src/nanoquant/runtime/cuda_kernels.py:448-544) for
  * many sequences and pages. */
 int nq_paged_attention(const void* q, int32_t q_dtype, int64_t tokens, int32_t q_heads, const nq_paged_kv* kv,
@@ -253,10 +253,10 @@ int64_t nq_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t t
  *   entropy[r]  = -sum p log p over the row, 0 log 0 = 0
  *   top_ids[r, :], top_logprobs[r, :] = the `top` likeliest tokens, likeliest first,
  *     the lowest index first among equals, NaN above all
- * top 0 to 32 (top_ids and top_logprobs may be NULL for 0). Logits of -inf have probability 0; a row that holds NaN or +inf, or
- * -inf alone, has NaN for every log probability and for the entropy. Beside
- * nq_greedy_select for callers that report how likely an answer is; the
- * reference's engine returns tokens alone (src/nanoquant/runtime/generation.py:240-246). */
+ * top 0 to 32 (top_ids and top_logprobs may be NULL for 0). Logits of -inf have
+ * probability 0; a row that holds NaN or +inf, or -inf alone, has NaN for every
+ * log probability and for the entropy. Beside nq_greedy_select for callers that
+ * report how likely an answer is; the reference's engine returns tokens alone (src/nanoquant/runtime/generation.py:240-246). */
 int nq_token_logprobs(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,
                       const int64_t* tokens, int32_t top, float* logprobs, float* entropy, int64_t* top_ids,
                       float* top_logprobs, void* workspace, int64_t workspace_bytes, void* stream);

@@ -262,6 +262,11 @@ __device__ __forceinline__ uint32_t moved4(uint32_t w, float ratio) {
 // / page + 2 pages with new rows, and its slots begin at starts[b] / page + 2 b:
 // the grid follows from the host's counts alone. The rest: q, one wave per token
 // and kQHeads of its heads.
+//
+// Long prompts are bound by bytes (8192 fp32 tokens of 32/8 heads of 128: 356 MB in
+// 74 us, 4.8 TB/s, where a copy reaches 5.04; q with 4 heads a wave took 82, with
+// 16 75.5), decode steps by the chain of dependent loads (starts, table, row,
+// scale: one token 4.6 us, one of 48 sequences each 5.0).
 template <int D, int DT, int WAVES>
 __global__ __launch_bounds__(WAVES* kWave) void k_paged_append(const AppendArgs a) {
     constexpr int kPage = WAVES * kPageTokens, kThreads = WAVES * kWave, H = kHeads<D>;

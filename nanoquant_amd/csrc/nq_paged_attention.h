@@ -306,7 +306,7 @@ __device__ __forceinline__ void store4(void* out, int dtype, int64_t at, const f
 // during a softmax).
 //
 // Single tokens are bound by the cache's bytes: 268 MB of one sequence at 5.1 TB/s
-// (a copy reaches 5.04), 153 MB of 64 sequences at 4.5 with the launch. Prompts are
+// (a copy reaches 5.04), 153 MB of 32 ragged sequences at 4.1 with the launch. Prompts are
 // bound by the vector unit, which widens K and V, and takes exponentials and parts of
 // the weights (4096 tokens of 32/8 heads of 128: 231 us for 1.4e11 multiplications
 // and additions; vector instructions issue in 64% of the cycles, the matrix unit
