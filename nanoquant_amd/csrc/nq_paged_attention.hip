@@ -94,11 +94,11 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows)
 //    after 3000: 38, 43 with 16).
 // Slots of 128 rows, a quarter to each wave, read the cache still less, but leave a
 // chip that they do not fill to one after the other: they are taken from a size on
-// (4096 tokens: 231 us, 286 shared, but 1531 after 517: 98 and 100, 512 after 3500:
+// (4096 tokens: 231 us, 286 shared, but 1531 after 517: 97 and 99, 512 after 3500:
 // 94 and 75, 8 sequences of up to 128 after 600: 41 and 19; 4096 of 32/8 heads of
 // 64: 147 and 165, but 2 times 2048 of 14/2: 68 and 50) and after very long caches
 // (512 after 20000: 290, 352 shared). 256-wide heads have them never (4096 tokens
-// of 16/4: 366 us shared, 508 in slots of 64).
+// of 16/4: 366 us shared, 508 in slots of 64, before a step that made both faster).
 //
 // Splits of the cache, joined in a second launch:
 //  - Short caches (up to 12 tiles of 64 rows) and few 16-row slots have none: eight
