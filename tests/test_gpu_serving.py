@@ -381,12 +381,13 @@ def test_paged_attention_every_byte_is_its_value():
 
 
 @pytest.mark.parametrize("batch,d,new", [(63, 64, (0, 1, 1, 3)), (64, 128, (1, 0, 9, 2, 33)), (64, 256, (6, 1, 0, 4, 9)),
-                                         (65, 64, (0, 1, 9, 2)), (5, 64, (40, 0, 25, 18, 50)), (5, 256, (30, 0, 25, 18, 50))])
+                                         (65, 64, (0, 1, 9, 2)), (5, 64, (40, 0, 25, 18, 50)), (5, 256, (30, 0, 25, 18, 50)),
+                                         (129, 64, (0, 1, 1, 9)), (200, 128, (1, 1, 0, 1)), (4098, 64, (1, 0, 0, 0, 0, 0, 2))])
 def test_paged_attention_uneven_batches(batch, d, new):
     """Sequences without tokens or rows, of one slot and several, among ones that are split."""
 
     _say("uneven", batch, d, new)
-    contexts = (700, 0, 33, 2000 if batch < 6 else 900, 1)
+    contexts = (700, 0, 33, 2000 if batch < 6 else 900, 1) if batch < 1000 else (20, 0, 33, 9, 1)
     lengths = [(contexts[i * i % 5] if i % 3 else 0, new[i % len(new)]) for i in range(batch - 1)] + [(1200, new[0])]
     b = Batch(lengths, kv=2, d=d, page=32, seed=83, ahead=2, behind=1)
     _filled(b, 84)
