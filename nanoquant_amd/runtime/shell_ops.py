@@ -571,7 +571,7 @@ def launch_paged_append(
             or table[1] * 2 != head_dim or not table[0] or sin.shape != table:
         raise ValueError("RoPE tables must be fp32 [positions, head_dim / 2]")
     if q_out is None:
-        q_out = torch.empty((tokens, q_heads, head_dim), dtype=q_dtype, device=device)
+        q_out = torch.empty(tokens, q_heads, head_dim, dtype=q_dtype, device=device)
     elif q_out.numel() != tokens * q_heads * head_dim:
         raise ValueError("q_out must be [tokens, q_heads, head_dim]")
     if q_out.dtype not in _FLOAT:
@@ -627,7 +627,7 @@ def launch_paged_attention(
     if not 0.0 < scaling < float("inf"):
         raise ValueError("paged attention scaling must be positive and finite")
     if out is None:
-        out = torch.empty((tokens, q_heads * head_dim), dtype=out_dtype, device=device)
+        out = torch.empty(tokens, q_heads * head_dim, dtype=out_dtype, device=device)
     elif out.numel() != q.numel():
         raise ValueError("paged attention output geometry is incompatible")
     if out.dtype not in _FLOAT:
@@ -640,7 +640,8 @@ def launch_paged_attention(
     if workspace is None and need:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
     status = lib.nq_paged_attention(
-        q.data_ptr(), _native.DTYPE_CODES[q.dtype], tokens, q_heads, ctypes.byref(kv), scaling, out.data_ptr(), _native.DTYPE_CODES[out.dtype], _ptr(workspace),
+        q.data_ptr(), _native.DTYPE_CODES[q.dtype], tokens, q_heads, ctypes.byref(kv), scaling, out.data_ptr(),
+        _native.DTYPE_CODES[out.dtype], _ptr(workspace),
         0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(device),
     )
     _native.check("nq_paged_attention", status)
@@ -698,10 +699,8 @@ def launch_token_logprobs(
         raise ValueError("token logprobs require CUDA/HIP tensors on one device")
     if out is None:
         _check_device("token logprobs", device, tokens, workspace)
-        out = TokenLogprobs(torch.empty(rows, dtype=torch.float32, device=device),
-                            torch.empty(rows, dtype=torch.float32, device=device),
-                            torch.empty((rows, top), dtype=torch.int64, device=device),
-                            torch.empty((rows, top), dtype=torch.float32, device=device))
+        logprobs = torch.empty(rows, dtype=torch.float32, device=device)
+        out = TokenLogprobs(logprobs, torch.empty_like(logprobs), tokens.new_empty(rows, top), logprobs.new_empty(rows, top))
     else:
         _check_device("token logprobs", device, tokens, *out, workspace)
         if out.logprobs.dtype != torch.float32 or out.entropy.dtype != torch.float32 or out.top_ids.dtype != torch.int64 \
@@ -716,7 +715,8 @@ def launch_token_logprobs(
     if workspace is None and need:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
     status = lib.nq_token_logprobs(
-        logits.data_ptr(), _native.DTYPE_CODES[logits.dtype], rows, vocab, stride, tokens.data_ptr(), top, out.logprobs.data_ptr(), out.entropy.data_ptr(), _ptr(out.top_ids if top else None),
+        logits.data_ptr(), _native.DTYPE_CODES[logits.dtype], rows, vocab, stride, tokens.data_ptr(), top,
+        out.logprobs.data_ptr(), out.entropy.data_ptr(), _ptr(out.top_ids if top else None),
         _ptr(out.top_logprobs if top else None), _ptr(workspace),
         0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(device),
     )
