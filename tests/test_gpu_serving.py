@@ -403,6 +403,57 @@ def test_paged_attention_uneven_batches(batch, d, new):
     _check_attention(out[mine.to(DEV)], expected[mine], spread[mine], reach[mine], q_dtype=torch.bfloat16, rows=rows, d=d)
 
 
+@pytest.mark.parametrize("q_dtype,out_dtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
+                                               (torch.float16, torch.float32)])
+@pytest.mark.parametrize("what", ["numbers", "k", "v", "scales"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_paged_attention_chunks_under_a_very_wide_table(d, what, q_dtype, out_dtype):
+    """Slots whose waves have rows of their own, split and not, with NaN that some of
+    their rows see and with scales that are no powers of two."""
+
+    _say("wide table", d, what, q_dtype, out_dtype)
+    page, lengths = 128, [(2600, 70), (0, 41), (100, 130)]
+    b = Batch(lengths, kv=2, d=d, page=page, seed=86, ahead=1, behind=1, extra_entries=110)
+    _filled(b, 87)
+    b.scales *= 2.0**-3
+    if what == "k":
+        b.k_bytes[b.table[0][2620 // page], 1, 2620 % page, 3] = 0x7f
+    if what == "v":
+        b.v_bytes[b.table[0][2620 // page], 0, d - 5, 2620 % page] = 0xff
+        b.v_bytes[b.table[2][0], 1, 7, 101] = 0x7f
+    if what == "scales":
+        b.scales *= 1 + torch.rand(b.scales.shape, generator=_g(88))
+    q = torch.randn(b.tokens, 8, d, generator=_g(89)).to(q_dtype)
+    expected, spread, reach = osv.attention(q, b.host(), b.table, b.spans, page=page, scaling=d**-0.5)
+    cache, at = b.device()
+    out = torch.full((b.tokens, 8 * d), 9.0, dtype=out_dtype, device=DEV)
+    ops.launch_paged_attention(q.to(DEV), cache, scaling=d**-0.5, out=out, **at)
+    mine = torch.arange(b.tokens)[1:-1]
+    assert (out[0] == 9.0).all() and (out[-1] == 9.0).all()
+    assert torch.isnan(expected[mine]).any() == (what in ("k", "v"))
+    _check_attention(out[mine.to(DEV)], expected[mine], spread[mine], reach[mine], q_dtype=q_dtype, rows=2670, d=d)
+
+
+@pytest.mark.parametrize("rise", [0.5, 2.0, 4.0, 5.0, -3.0])
+@pytest.mark.parametrize("tokens,extra", [(1, 1), (9, 1), (70, 250)])
+def test_paged_attention_scores_that_rise_from_tile_to_tile(tokens, extra, rise):
+    """By less than a running maximum may lag behind, and by more."""
+
+    d, page = 64, 64
+    b = Batch([(1000, tokens)], kv=1, d=d, page=page, seed=90, extra_entries=extra)
+    _filled(b, 91)
+    b.k_bytes.zero_()
+    b.scales[0] = 1.0
+    for i, at in enumerate(b.table[0][:-(-(1000 + tokens) // page)]):
+        b.k_bytes[at, :, :, 0] = torch.tensor(min(i, 16), dtype=torch.float32).to(torch.float8_e4m3fn).view(torch.uint8)
+    q = torch.randn(tokens, 4, d, generator=_g(92))
+    q[:, :, 0] = rise
+    expected, spread, reach = osv.attention(q, b.host(), b.table, b.spans, page=page, scaling=1.0)
+    cache, at = b.device()
+    out = ops.launch_paged_attention(q.to(DEV), cache, scaling=1.0, out_dtype=torch.float32, **at)
+    _check_attention(out, expected, spread, reach, q_dtype=torch.float32, rows=1000 + tokens, d=d)
+
+
 @pytest.mark.parametrize("what", ["k", "v"])
 @pytest.mark.parametrize("lengths,row", [([(0, 70)], 40), ([(90, 6)], 93), ([(10, 3)], 12), ([(200, 2)], 17)])
 def test_paged_attention_nan_reaches_those_who_see_it(lengths, row, what):
