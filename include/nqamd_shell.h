@@ -232,9 +232,10 @@ int64_t nq_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int32_
  *   out[t, h, :] = softmax(scaling * q[t, h, :] . K) . V
  * q F32/F16/BF16 [tokens, q_heads, head_dim] (F16 and BF16 read exactly, F32 to
  * 2^-23 of every value down to 2^-28 of its head's largest, or of 2^-100, and to
- * 2^-51 of that below); out F32/F16/BF16 [tokens, q_heads * head_dim]; both 16-byte aligned, q_heads a
- * multiple of kv_heads. Scores and softmax in fp32, the weights to 16 bits for
- * 16-bit outputs and 24 for fp32, results joined in a fixed order (deterministic).
+ * 2^-51 of that below); out F32/F16/BF16 [tokens, q_heads * head_dim]; both
+ * 16-byte aligned, q_heads a multiple of kv_heads. Scores and softmax in fp32, the
+ * weights to 16 bits for 16-bit outputs and 24 for fp32, results joined in a fixed
+ * order (deterministic).
  * A token whose row lies outside the page table gives zeros. A table entry in use
  * that names no page counts as NaN rows. NaN in the cache, infinities and NaN in q
  * do what fp32 arithmetic does with them, for the tokens that see them alone; rows

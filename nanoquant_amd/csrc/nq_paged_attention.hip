@@ -1,4 +1,6 @@
 // Attention over the 8-bit paged cache: plan, merge of the splits, entry points.
+#include <algorithm>
+
 #include "nq_paged_attention.h"
 
 namespace nq {
@@ -107,15 +109,22 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows)
 //    37.5 us, 44 split), unless the table has room for long sequences: then a split
 //    for each 96 tiles, up to 16, so that a long sequence among short ones does not
 //    keep one workgroup (one of 131000 rows and 31 of 500: 67 us, 718 without; 32
-//    of 32000: 372, 363 without).
+//    of 32000: 372, 363 without). Not more than a sequence of the mean length
+//    needs to fill the chip by itself, and none for one sequence: long prompts have
+//    slots enough (16/4 heads of 256 under a table of 131072 rows, one prompt of 4096
+//    tokens: 345 us, 1273 in 16 splits; two of 2048, table 32768: 235 us, 670 in 5;
+//    8 of 100 after 500 rows: 101 us, 103 in 16, and with one of them after 130000:
+//    534 and 609).
 //  - Otherwise as many as make the workgroups that the chip holds at once (8
 //    sequences of 5000 rows: 22.4 us with 512 workgroups, 25.9 with 1024; one of
 //    131000: 60.3, 66.0; 32-row slots of 256-wide heads have a compute unit each:
 //    38 us for 16 sequences of 6 tokens with 256, 52 with 384), of at least 8
 //    tiles, or 4 where the chip would stay empty.
+//  - Never more than 1 GiB of partial results holds (256 sequences of 16 tokens
+//    after 300 rows, table 131072: 462 us in 10 splits, 693 in 16 and 1.7 GB).
 AttnPlan plan_attention(int64_t tokens, int64_t batch, int q_heads, int kv_heads, int head_dim, int64_t cache_rows) {
     constexpr int64_t kMostNarrow = 16, kMostShared = 64, kFull = 256, kShort = 12, kMedium = 64, kVeryLong = 256;
-    constexpr int64_t kMostSplits = 128, kSkew = 96;
+    constexpr int64_t kMostSplits = 128, kSkew = 96, kMostPartials = int64_t{1} << 30;
     AttnPlan plan;
     const int64_t rows = tokens * (q_heads / kv_heads), mean = (rows + batch - 1) / batch;
     const int64_t tiles = (cache_rows + kTile - 1) / kTile;
@@ -138,10 +147,15 @@ AttnPlan plan_attention(int64_t tokens, int64_t batch, int q_heads, int kv_heads
         if (plan.waves == 8 || (full && narrow)) target = 0;
     }
     int64_t splits = target / work;
-    if (full && plan.shared && tiles / kSkew > splits) splits = tiles / kSkew < 16 ? tiles / kSkew : 16;
-    const int64_t most = (tiles + plan.least - 1) / plan.least;
-    splits = splits < most ? splits : most;
-    plan.splits = static_cast<int>(splits < 1 ? 1 : (splits > kMostSplits ? kMostSplits : splits));
+    // Workgroups of one sequence: from kFull on it fills the chip by itself.
+    const int64_t alone = (mean + plan.rows - 1) / plan.rows * kv_heads;
+    if (full && plan.shared && batch > 1 && alone < kFull) {
+        const int64_t skew = std::min({tiles / kSkew, int64_t{16}, 512 / alone});
+        splits = std::max(splits, skew);
+    }
+    const int64_t each = units * plan.rows * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+    splits = std::min({splits, (tiles + plan.least - 1) / plan.least, kMostSplits, kMostPartials / each});
+    plan.splits = static_cast<int>(std::max(splits, int64_t{1}));
     return plan;
 }
 

@@ -1,0 +1,53 @@
+"""The layout of paged attention calls, on the CPU: the restated plan is the library's,
+and a call's workspace is bounded."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+from serving_plan import MOST_PARTIALS, plan, workspace_bytes
+
+from nanoquant_amd.runtime import _native
+
+GEOMETRIES = [(32, 8, 128), (16, 8, 128), (8, 1, 128), (32, 32, 128), (64, 64, 128), (14, 2, 64), (4, 4, 64), (34, 2, 64),
+              (16, 4, 256), (8, 8, 256), (64, 8, 256)]
+
+
+def _bytes(tokens, batch, q_heads, kv_heads, head_dim, page, entries):
+    return _native.load().nq_paged_attention_workspace_bytes(tokens, batch, q_heads, kv_heads, head_dim, page, entries)
+
+
+def test_the_restated_plan_is_the_librarys():
+    rng = random.Random(5)
+    for _ in range(20000):
+        q_heads, kv, d = rng.choice(GEOMETRIES)
+        batch = round(2 ** rng.uniform(0, 10))
+        tokens = min(round(batch * 2 ** rng.uniform(-1, 13)) + 1, 0x3FFFFFFF // q_heads)
+        page = rng.choice([16, 32, 64, 128])
+        entries = round(2 ** rng.uniform(0, 20 - (page.bit_length() - 1)))
+        p = plan(tokens, batch, q_heads, kv, d, page * entries)
+        got = _bytes(tokens, batch, q_heads, kv, d, page, entries)
+        assert got == -1 or got == workspace_bytes(p, kv), (tokens, batch, q_heads, kv, d, page, entries, p)
+
+
+@pytest.mark.parametrize("tokens,batch,q_heads,kv,d,rows,most", [
+    (32768, 1, 16, 4, 256, 131072, 0),             # one long prompt of 256-wide heads: its slots fill the chip
+    (32768, 1, 16, 4, 256, 32768, 0),
+    (32768, 1, 32, 8, 128, 131072, 0),
+    (8192, 4, 16, 4, 256, 131072, 0),              # each of four prompts does
+    (4096, 256, 32, 8, 128, 131072, MOST_PARTIALS),  # 16 tokens each
+    (512, 512, 32, 8, 128, 131072, MOST_PARTIALS),   # a decode step
+    (4096, 4096, 64, 64, 128, 1 << 20, MOST_PARTIALS),
+])
+def test_workspace_of_calls_that_fill_the_chip(tokens, batch, q_heads, kv, d, rows, most):
+    assert 0 <= _bytes(tokens, batch, q_heads, kv, d, 64, rows // 64) <= most
+
+
+def test_no_workspace_is_larger_than_the_bound():
+    rng = random.Random(6)
+    for _ in range(20000):
+        q_heads, kv, d = rng.choice(GEOMETRIES)
+        batch = round(2 ** rng.uniform(0, 16))
+        tokens = min(round(2 ** rng.uniform(0, 22)), 0x3FFFFFFF // q_heads)
+        assert _bytes(tokens, batch, q_heads, kv, d, 64, round(2 ** rng.uniform(0, 16))) <= MOST_PARTIALS
