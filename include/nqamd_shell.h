@@ -222,7 +222,9 @@ int nq_paged_append(const void* q, const void* k, const void* v, int32_t dtype, 
                     const float* cos_table, const float* sin_table, int64_t rope_positions,
                     const nq_paged_kv* kv, void* q_out, int32_t q_out_dtype, void* stream);
 
-/* Workspace bytes of nq_paged_attention (0: none needed). */
+/* Workspace bytes of nq_paged_attention (0: none needed; at most 1 GiB), or -1 for
+ * sizes that it refuses: among others a grid of 2^32 threads or more, as the
+ * append and the log probabilities refuse too (NQ_ERR_SHAPE). */
 int64_t nq_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int32_t q_heads, int32_t kv_heads,
                                            int32_t head_dim, int32_t page_size, int64_t table_pages);
 
@@ -246,7 +248,7 @@ int nq_paged_attention(const void* q, int32_t q_dtype, int64_t tokens, int32_t q
                        float scaling, void* out, int32_t out_dtype, void* workspace, int64_t workspace_bytes,
                        void* stream);
 
-/* Workspace bytes of nq_token_logprobs (0: none needed). */
+/* Workspace bytes of nq_token_logprobs (0: none needed; -1: refused sizes). */
 int64_t nq_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top);
 
 /* For each row of logits (F32/F16/BF16, row_stride >= vocab elements apart):

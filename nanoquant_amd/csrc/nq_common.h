@@ -80,6 +80,9 @@ inline int dtype_bytes(int d) {
     }
 }
 
+// A grid's threads are counted in 32 bits.
+inline bool launchable(int64_t blocks, int64_t threads) { return blocks <= 0x7fffffff && blocks * threads <= 0xffffffff; }
+
 inline int launch_status() {
     return hipGetLastError() == hipSuccess ? NQ_OK : NQ_ERR_LAUNCH;
 }

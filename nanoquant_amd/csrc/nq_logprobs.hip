@@ -467,6 +467,7 @@ extern "C" int64_t nq_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab
     if (rows <= 0 || rows > 0xffffff || vocab <= 0 || vocab > 0x7fffff00 || top < 0 || top > kMostTop || top > vocab)
         return -1;
     const int parts = parts_for(rows, vocab);
+    if (!nq::launchable(rows * parts, kWaves * kWave) || (top && !nq::launchable(rows, kJoinWaves * kWave))) return -1;
     return parts == 1 && top == 0 ? 0 : rows * (parts * int64_t{16} + (top ? blocks_for(vocab) * (kWave + kWave / kGroup) * int64_t{4} : 0));
 }
 

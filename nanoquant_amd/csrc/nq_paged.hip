@@ -441,7 +441,7 @@ int launch_append(AppendArgs& a, int64_t tokens, int kv_heads, int64_t batch, hi
     const int waves = (1 << a.p.page_shift) / kPageTokens;
     const int64_t kv_blocks = ((tokens >> a.p.page_shift) + 2 * batch) * kv_heads;
     const int64_t blocks = kv_blocks + (tokens * a.q_groups + waves - 1) / waves;
-    if (blocks > 0x7fffffff) return NQ_ERR_SHAPE;
+    if (!nq::launchable(blocks, waves * kWave)) return NQ_ERR_SHAPE;
     a.kv_blocks = static_cast<int32_t>(kv_blocks);
     const dim3 grid(static_cast<unsigned>(blocks)), block(static_cast<unsigned>(waves * kWave));
     switch (waves) {

@@ -722,8 +722,7 @@ int launch_paged_attention(const AttnArgs& a, const AttnPlan& plan, int q_dtype,
 
 template <int D, int QT, int PP>
 int launch_attention_as(const AttnArgs& a, const AttnPlan& plan, hipStream_t stream) {
-    const int64_t blocks = static_cast<int64_t>(plan.slots) * plan.splits * a.p.kv_heads;
-    if (blocks > 0x7fffffff) return NQ_ERR_SHAPE;
+    const int64_t blocks = static_cast<int64_t>(plan.slots) * plan.splits * a.p.kv_heads;  // launchable: checked with the workspace
     const dim3 grid(static_cast<unsigned>(blocks)), block(static_cast<unsigned>(plan.waves * kWave));
     constexpr int kTileRows = kRowsAtOnce<D>;
     if (plan.shared && plan.waves == 4) {

@@ -173,6 +173,8 @@ extern "C" int64_t nq_paged_attention_workspace_bytes(int64_t tokens, int64_t ba
         return -1;
     if (tokens * q_heads > 0x3fffffff) return -1;
     const AttnPlan plan = plan_attention(tokens, batch, q_heads, kv_heads, head_dim, table_pages * page_size);
+    // (The merge has a workgroup for each partial row of a split at most: 1 GiB holds 2^22.)
+    if (!nq::launchable(static_cast<int64_t>(plan.slots) * plan.splits * kv_heads, plan.waves * kWave)) return -1;
     return partial_rows(plan, kv_heads) * (2 + head_dim) * static_cast<int64_t>(sizeof(float));
 }
 

@@ -3,6 +3,7 @@ and a call's workspace is bounded."""
 
 from __future__ import annotations
 
+import ctypes
 import random
 
 import pytest
@@ -51,3 +52,47 @@ def test_no_workspace_is_larger_than_the_bound():
         batch = round(2 ** rng.uniform(0, 16))
         tokens = min(round(2 ** rng.uniform(0, 22)), 0x3FFFFFFF // q_heads)
         assert _bytes(tokens, batch, q_heads, kv, d, 64, round(2 ** rng.uniform(0, 16))) <= MOST_PARTIALS
+
+
+# -- launches: at most 2^32 - 1 threads --------------------------------------------
+
+A = 4096  # an address: checks end before it is read
+
+
+def _kv(**changes):
+    kv = _native.PagedKv(A, A, A, A, 8, 2, 128, 16, 0, A, 4, A, A, 3)
+    for name, value in changes.items():
+        setattr(kv, name, value)
+    return kv
+
+
+@pytest.mark.parametrize("changes,tokens,q_heads", [
+    ({"batch": 1 << 21, "page_size": 128, "head_dim": 64}, 3, 4),      # slots of pages, 1024 threads each
+    ({"batch": 1 << 23, "page_size": 16}, 3, 4),                       # 128 threads each
+    ({"batch": 1, "page_size": 16}, 0xFFFFFF, 64),                     # groups of q heads
+])
+def test_append_refuses_what_no_launch_holds(changes, tokens, q_heads):
+    status = _native.load().nq_paged_append(A, A, A, 0, tokens, q_heads, None, None, 0, 1e-6, A, A, 64,
+                                            ctypes.byref(_kv(**changes)), A, 0, None)
+    assert status == -3
+
+
+@pytest.mark.parametrize("changes,tokens,q_heads", [
+    ({"batch": 1 << 23}, 3, 4),
+    ({"batch": 1 << 23, "head_dim": 256}, 3, 4),
+    ({"batch": 1 << 18, "kv_heads": 64}, 3, 64),
+])
+def test_attention_refuses_what_no_launch_holds(changes, tokens, q_heads):
+    kv = _kv(**changes)
+    assert _bytes(tokens, kv.batch, q_heads, kv.kv_heads, kv.head_dim, 16, 4) == -1
+    status = _native.load().nq_paged_attention(A, 0, tokens, q_heads, ctypes.byref(kv), 0.1, A, 0, A, 1 << 40, None)
+    assert status == -3
+
+
+def test_token_logprobs_refuse_what_no_launch_holds():
+    lib = _native.load()
+    assert lib.nq_token_logprobs_workspace_bytes(8388607, 64, 1) > 0  # 512 threads to a row's join
+    assert lib.nq_token_logprobs_workspace_bytes(0xFFFFFF, 64, 0) == 0  # 256, and no join
+    for rows in (8388608, 0xFFFFFF):
+        assert lib.nq_token_logprobs_workspace_bytes(rows, 64, 1) == -1
+        assert lib.nq_token_logprobs(A, 0, rows, 64, 64, A, 1, A, A, A, A, A, 1 << 50, None) == -3
