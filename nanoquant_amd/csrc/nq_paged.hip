@@ -148,10 +148,11 @@ __device__ __forceinline__ float round_to_odd(double x) {
 
 // x as fp32 for an e4m3 rounding: the nearest fp32 value does, unless it lies
 // where e4m3 rounds to even or where a scale ends. All of those have 0 in their
-// last 19 bits.
+// last 19 bits, but for subnormal ones (at the smallest scales).
 __device__ __forceinline__ float for_e4m3(double x) {
     float f = static_cast<float>(x);
-    if (__ballot((__float_as_uint(f) & 0x7ffffu) == 0 && f != 0.0f)) f = round_to_odd(x);
+    const uint32_t u = __float_as_uint(f);
+    if (__ballot(f != 0.0f && ((u & 0x7ffffu) == 0 || (u & 0x7f800000u) == 0))) f = round_to_odd(x);
     return f;
 }
 

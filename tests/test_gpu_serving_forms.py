@@ -17,7 +17,7 @@ import torch
 from conftest import gpu_available
 from nanoquant_amd.runtime import shell_ops as ops
 from oracle import serving as osv
-from test_gpu_serving import DEV, Batch, _filled, _g, _say
+from test_gpu_serving import DEV, Batch, _filled, _g, _same_bytes, _say
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a HIP device")]
 
@@ -46,3 +46,29 @@ def test_paged_attention_light_query_values_beside_a_heavy_one(d, tokens, extra,
     # A weight: its score's error and the maximum's, an exponential's and a part's step; sums over the rows.
     bound = (2 * u * 8 * reach[..., None] + u * ((100 + tokens) / 16 + 64 + 2)) * spread + u * expected.abs()
     assert ((out.view(expected.shape) - expected).abs() / bound).max() <= 1
+
+
+def test_paged_append_rounds_k_once_below_the_least_normal_number():
+    """At the smallest scale, 2^-126, e4m3's borders between bytes 0, 1, 2 and 3 are
+    fp32 subnormals. K = x + y of fp64, its rotation's sum: x on such a border, y too
+    little for fp32 to hold beside it, on either side. The byte is that of the exact sum."""
+
+    d, page = 64, 16
+    borders = [2.0**-136, 3 * 2.0**-136, 5 * 2.0**-136, 2.0**-135 + 2.0**-137]  # the last is no border
+    b = Batch([(0, 8)], kv=1, d=d, page=page, seed=96)
+    k = torch.zeros(8, 1, d, dtype=torch.float64)
+    sin = torch.zeros(8, d // 2)
+    for t in range(8):
+        for j, border in enumerate(borders):
+            k[t, 0, j] = border * (1 if t % 4 < 2 else -1)
+            k[t, 0, j + d // 2] = 2.0**-140
+            sin[t, j] = 2.0**-30 * (1 if t % 2 else -1)  # K = border -+ 2^-170
+    k = k.float()
+    v = torch.zeros(8, 1, d)
+    cos = torch.ones(8, d // 2)
+    _, expected = osv.append(k, k, v, b.host(), b.table, b.spans, page=page, q_norm=None, k_norm=None, eps=0.0, cos=cos, sin=sin)
+    cache, batch = b.device()
+    ops.launch_paged_append(k.to(DEV), k.to(DEV), v.to(DEV), cache, q_heads=1, q_norm=None, k_norm=None, eps=0.0,
+                            cos=cos.to(DEV), sin=sin.to(DEV), **batch)
+    _same_bytes(cache.k, expected["k"])
+    assert len(set(expected["k"][b.table[0][0], 0, :8, 0].abs().tolist())) == 2  # both sides of the first border
