@@ -19,6 +19,12 @@ class Plan(NamedTuple):
     waves: int
     slots: int
     splits: int
+    least: int     # cache tiles that a split takes at least
+
+    def active(self, visible: int) -> int:
+        """Splits of a sequence whose last token sees that many rows."""
+        tiles = _up(visible, TILE)
+        return 1 if self.splits == 1 else max(_up(tiles, max(_up(tiles, self.splits), self.least)), 1)
 
     @property
     def form(self) -> tuple[int, int, bool, int, bool]:
@@ -56,7 +62,14 @@ def plan(tokens: int, batch: int, q_heads: int, kv_heads: int, head_dim: int, ca
     if full and shared and batch > 1 and alone < FULL:
         splits = max(splits, min(tiles // SKEW, 16, 512 // alone))
     splits = min(splits, _up(tiles, least), MOST_SPLITS, MOST_PARTIALS // (units * slot * (head_dim + 2) * 4))
-    return Plan(head_dim, slot, shared, waves, slots, max(splits, 1))
+    return Plan(head_dim, slot, shared, waves, slots, max(splits, 1), least)
+
+
+# (head_dim, rows, shared, waves, joined): all that calls can reach.
+FORMS = {(d, *form) for d in (64, 128) for form in (
+    (16, True, 8, False), (16, True, 4, False), (16, True, 4, True), (32, True, 4, False), (32, True, 4, True),
+    (128, False, 4, False), (128, False, 4, True))} | {
+    (256, rows, True, 4, joined) for rows in (16, 32) for joined in (False, True)}
 
 
 def workspace_bytes(p: Plan, kv_heads: int) -> int:

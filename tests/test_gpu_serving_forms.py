@@ -11,15 +11,109 @@ of its scales and of the subtraction: 2^-24 * 8 of it.
 
 from __future__ import annotations
 
+import functools
+
 import pytest
 import torch
 
 from conftest import gpu_available
 from nanoquant_amd.runtime import shell_ops as ops
 from oracle import serving as osv
-from test_gpu_serving import DEV, Batch, _filled, _g, _same_bytes, _say
+from test_gpu_serving import DEV, EPS, HALF_STEP, Batch, _check_attention, _filled, _g, _rope_tables, _same_bytes, _say
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a HIP device")]
+
+
+# One call or more for each form that a call can take (tests/serving_plan.py; test_serving_plan.py
+# holds this list to it): rows of a slot, waves that share them or not, one launch or two.
+ATTENTIONS = [
+    # lengths, q heads, kv heads, head_dim, page, table entries behind the longest sequence
+    *(case for d in (64, 128) for case in (
+        ([(130, 1), (63, 2), (0, 1)], 8, 2, d, 16, 1),                             # 16 rows, eight waves
+        ([(i * 7 % 300, 1 + i % 3) for i in range(70)], 8, 4, d, 32, 1),           # 16 rows, the chip is full
+        ([(1500, 2), (20, 3), (0, 1)], 8, 2, d, 64, 1),                            # ... split
+        ([(i * 11 % 200, 5 + i % 3) for i in range(40)], 16, 4, d, 32, 1),         # 32 rows
+        ([(1500, 10), (20, 12), (0, 8)], 8, 2, d, 64, 50),                         # ... split
+        ([(37, 70), (0, 65), (5, 66), (100, 65)], 66, 33, d, 128, 128),            # 128 rows
+        ([(700, 90), (0, 70), (33, 65)], 8, 4, d, 128, 122),                       # ... split
+    )),
+    ([(130, 1), (63, 2), (0, 1)], 8, 2, 256, 16, 1),
+    ([(1500, 2), (20, 3), (0, 1)], 8, 2, 256, 64, 1),
+    ([(i * 31 % 300, 39 + i % 3) for i in range(11)], 8, 8, 256, 32, 1),
+    ([(1500, 30), (20, 33), (0, 28)], 8, 2, 256, 64, 1),
+]
+
+DTYPES = [(q, out) for q in (torch.float32, torch.bfloat16, torch.float16) for out in (torch.float32, torch.bfloat16, torch.float16)]
+
+
+@functools.lru_cache(maxsize=2)
+def _case(at: int, full: bool):
+    """The batch, the queries (24 bits, or few enough for every type) and their attention."""
+
+    lengths, q_heads, kv, d, page, extra = ATTENTIONS[at]
+    b = Batch(lengths, kv=kv, d=d, page=page, seed=97, ahead=1, behind=2, extra_entries=extra)
+    _filled(b, 98)
+    b.scales *= 2.0**-3
+    q = torch.randn(b.tokens, q_heads, d, generator=_g(99))
+    if not full:
+        q = (q * 32).round() / 32
+    return b, q, osv.attention(q, b.host(), b.table, b.spans, page=page, scaling=d**-0.5)
+
+
+@pytest.mark.parametrize("at", range(len(ATTENTIONS)))
+@pytest.mark.parametrize("full", [True, False])
+def test_paged_attention_in_every_form(at, full):
+    """Each form with each type of q and of the output."""
+
+    lengths, q_heads, kv, d, page, _ = ATTENTIONS[at]
+    b, q, (expected, spread, reach) = _case(at, full)
+    cache, batch = b.device()
+    mine = ~torch.isnan(expected[:, 0, 0])
+    assert mine.sum() == b.spans[-1][1] - 1
+    for q_dtype, out_dtype in DTYPES:
+        if full != (q_dtype == torch.float32):
+            continue
+        _say("form", at, q_dtype, out_dtype)
+        assert torch.equal(q.to(q_dtype).float(), q)
+        out = torch.full((b.tokens, q_heads * d), 9.0, dtype=out_dtype, device=DEV)
+        ops.launch_paged_attention(q.to(q_dtype).to(DEV), cache, scaling=d**-0.5, out=out, **batch)
+        assert (out.cpu()[~mine] == 9.0).all()
+        _check_attention(out[mine.to(DEV)], expected[mine], spread[mine], reach[mine], q_dtype=q_dtype,
+                         rows=max(c + n for c, n in lengths), d=d)
+
+
+@pytest.mark.parametrize("dtype,norm_dtype,out_dtype,in_place", [
+    (torch.float32, torch.bfloat16, torch.bfloat16, False), (torch.float32, torch.float16, torch.float16, False),
+    (torch.bfloat16, torch.bfloat16, torch.bfloat16, True), (torch.float16, torch.float32, torch.float16, True),
+    (torch.float32, torch.float32, torch.float32, True), (torch.bfloat16, torch.float16, torch.float16, False),
+    (torch.float16, torch.bfloat16, torch.bfloat16, False), (torch.bfloat16, None, torch.bfloat16, True)])
+@pytest.mark.parametrize("d,q_heads,kv,page", [(64, 9, 3, 16), (128, 5, 5, 64), (256, 6, 2, 32)])
+def test_paged_append_with_16_bit_norms_and_outputs(d, q_heads, kv, page, dtype, norm_dtype, out_dtype, in_place):
+    """Norm weights and rotated queries of every type, and queries rotated in place."""
+
+    _say("append", d, dtype, norm_dtype, out_dtype, in_place)
+    b = Batch([(page - 3, 7), (0, 1), (2 * page, page + 2)], kv=kv, d=d, page=page, seed=100, ahead=1, behind=2)
+    q, k, v = (torch.randn(b.tokens, h, d, generator=_g(s)).to(dtype) for h, s in ((q_heads, 101), (kv, 102), (kv, 103)))
+    qn, kn = (None if norm_dtype is None else (1 + 0.1 * torch.randn(d, generator=_g(s))).to(norm_dtype) for s in (104, 105))
+    cos, sin = _rope_tables(4 * page, d)
+    rotated, expected = osv.append(q, k, v, b.host(), b.table, b.spans, page=page, q_norm=qn, k_norm=kn, eps=EPS, cos=cos, sin=sin)
+    cache, batch = b.device()
+    into = q.to(DEV)
+    out = into if in_place else torch.full((b.tokens, q_heads, d), 7.0, dtype=out_dtype, device=DEV)
+    got = ops.launch_paged_append(into, k.to(DEV), v.to(DEV), cache, q_heads=q_heads, q_norm=None if qn is None else qn.to(DEV),
+                                  k_norm=None if kn is None else kn.to(DEV), eps=EPS, cos=cos.to(DEV), sin=sin.to(DEV),
+                                  q_out=out, **batch)
+    assert got is out
+    _same_bytes(cache.k, expected["k"])
+    _same_bytes(cache.v, expected["v"])
+    assert torch.equal(cache.k_scales.cpu().double(), expected["k_scales"])
+    written = ~torch.isnan(rotated[:, 0, 0])
+    assert torch.equal(out.cpu()[~written], q[~written] if in_place else torch.full_like(out.cpu()[~written], 7.0))
+    # 8 fp32 roundings relative to the rotated pair, and the output's own.
+    x, half = rotated[written], d // 2
+    pair = torch.sqrt(x[..., :half].pow(2) + x[..., half:].pow(2)).repeat(1, 1, 2)
+    bound = 8 * 2.0**-24 * 1.5 * pair + HALF_STEP[out_dtype] * x.abs() + (2.0**-25 if out_dtype == torch.float16 else 0.0)
+    assert ((out.cpu()[written].double() - x).abs() <= bound).all()
 
 
 @pytest.mark.parametrize("d,tokens,extra", [(64, 1, 1), (64, 9, 1), (64, 70, 260), (128, 1, 1), (128, 9, 12), (128, 70, 260),

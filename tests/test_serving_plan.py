@@ -7,7 +7,8 @@ import ctypes
 import random
 
 import pytest
-from serving_plan import MOST_PARTIALS, plan, workspace_bytes
+from serving_plan import FORMS, MOST_PARTIALS, plan, workspace_bytes
+from test_gpu_serving_forms import ATTENTIONS, DTYPES
 
 from nanoquant_amd.runtime import _native
 
@@ -21,6 +22,7 @@ def _bytes(tokens, batch, q_heads, kv_heads, head_dim, page, entries):
 
 def test_the_restated_plan_is_the_librarys():
     rng = random.Random(5)
+    forms = set()
     for _ in range(20000):
         q_heads, kv, d = rng.choice(GEOMETRIES)
         batch = round(2 ** rng.uniform(0, 10))
@@ -30,6 +32,20 @@ def test_the_restated_plan_is_the_librarys():
         p = plan(tokens, batch, q_heads, kv, d, page * entries)
         got = _bytes(tokens, batch, q_heads, kv, d, page, entries)
         assert got == -1 or got == workspace_bytes(p, kv), (tokens, batch, q_heads, kv, d, page, entries, p)
+        forms.add(p.form)
+    assert forms == FORMS
+
+
+def test_the_gpu_tests_reach_every_form_with_every_type():
+    forms = set()
+    for lengths, q_heads, kv, d, page, extra in ATTENTIONS:
+        width = max(-(-(c + n) // page) for c, n in lengths) + extra
+        p = plan(sum(n for _, n in lengths) + 3, len(lengths), q_heads, kv, d, width * page)
+        active = {p.active(c + n) for c, n in lengths}
+        assert p.splits == 1 or (max(active) > 1 and min(active) == 1), "some sequences are split, others not"
+        forms.add(p.form)
+    assert forms == FORMS
+    assert {q for q, _ in DTYPES} == {out for _, out in DTYPES} and len(set(DTYPES)) == 9
 
 
 @pytest.mark.parametrize("tokens,batch,q_heads,kv,d,rows,most", [
