@@ -37,7 +37,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 64;  // cache rows that splits are counted in
-constexpr float kSlack = 6.0f;  // weights stay below 2^6: sums as safe as of a few dozen rows more
+constexpr float kSlack = 6.0f;  // what weights are relative to lies this far above a new maximum
 
 struct AttnArgs {
     Pages p;
@@ -541,12 +541,13 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 && NT == 2 ? 1 : 2) void k_p
 #pragma unroll
             for (int j = 1; j < kBlock; ++j) top = fmaxf(top, sc[j >> 2][u][j & 3]);
             // What weights are relative to need not be the largest score: it moves
-            // only where a weight would pass 2^kSlack, seldom after the first tiles,
-            // and the accumulators with it (4096 tokens of 16/4 heads of 256: 343 us,
-            // 364 where they follow every new maximum).
+            // only where a weight would pass 1, seldom after the first tiles, to 2^kSlack
+            // above the score, and the accumulators with it (4096 tokens of 16/4 heads
+            // of 256: 343 us, 364 where they follow every new maximum). Weights
+            // never pass 1, so that values near fp32's largest stay what they are.
             const float m_tile = rows_max(top * f[u]);
-            if (const bool grows = m_tile > m_run[u] + kSlack; __ballot(grows)) {
-                const float m_new = grows ? m_tile : m_run[u];
+            if (const bool grows = m_tile > m_run[u]; __ballot(grows)) {
+                const float m_new = grows ? m_tile + kSlack : m_run[u];
                 const float keep = exp2_hw(m_run[u] - (m_new == -INFINITY ? 0.0f : m_new));
                 l_run[u] *= keep;
 #pragma unroll

@@ -166,3 +166,27 @@ def test_paged_append_rounds_k_once_below_the_least_normal_number():
                             cos=cos.to(DEV), sin=sin.to(DEV), **batch)
     _same_bytes(cache.k, expected["k"])
     assert len(set(expected["k"][b.table[0][0], 0, :8, 0].abs().tolist())) == 2  # both sides of the first border
+
+
+@pytest.mark.parametrize("rise", [2.0, 4.0, -4.0])
+@pytest.mark.parametrize("d,tokens,extra,scale", [(64, 1, 1, 1.0), (128, 9, 12, 1.0), (128, 70, 250, 1.0), (256, 9, 1, 1.0),
+                                                  (64, 70, 250, 1.25)])
+def test_paged_attention_values_near_the_top_of_fp32(d, tokens, extra, scale, rise):
+    """Values of 2^123 with scores that rise from tile to tile by less than a running
+    maximum may lag behind: a weight times its value stays below 2^128."""
+
+    _say("large values", d, tokens, extra, scale, rise)
+    page = 64
+    b = Batch([(1000, tokens)], kv=1, d=d, page=page, seed=106, extra_entries=extra)
+    b.k_bytes.zero_()
+    b.k_bytes[..., 1] = 0x70  # 128: rows that weigh nothing, but for one in each page
+    b.v_bytes[:] = 0x38       # 1.0
+    for i, at in enumerate(b.table[0][:-(-(1000 + tokens) // page)]):
+        b.k_bytes[at, :, 0, :2] = torch.tensor([min(i, 16), 0], dtype=torch.float32).to(torch.float8_e4m3fn).view(torch.uint8)
+    b.scales[0], b.scales[1] = 1.0, scale * 2.0**123
+    q = torch.zeros(tokens, 4, d)
+    q[:, :, 0], q[:, :, 1] = rise, -8.0
+    expected, spread, reach = osv.attention(q, b.host(), b.table, b.spans, page=page, scaling=1.0)
+    cache, at = b.device()
+    out = ops.launch_paged_attention(q.to(DEV), cache, scaling=1.0, out_dtype=torch.float32, **at)
+    _check_attention(out, expected, spread, reach, q_dtype=torch.float32, rows=1000 + tokens, d=d)
