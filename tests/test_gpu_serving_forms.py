@@ -17,9 +17,13 @@ import pytest
 import torch
 
 from conftest import gpu_available
+from nanoquant_amd import synthetic as syn
 from nanoquant_amd.runtime import shell_ops as ops
+from nanoquant_amd.runtime.decoder_shell import PackedDecoder
 from oracle import serving as osv
-from test_gpu_serving import DEV, EPS, HALF_STEP, Batch, _check_attention, _filled, _g, _rope_tables, _same_bytes, _say
+from oracle.nq_oracle import relative_l2
+from test_gpu_serving import (DEV, EPS, HALF_STEP, SMALL, Batch, _check_attention, _filled, _g, _rope_tables, _same_bytes,
+                              _say)
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a HIP device")]
 
@@ -190,3 +194,68 @@ def test_paged_attention_values_near_the_top_of_fp32(d, tokens, extra, scale, ri
     cache, at = b.device()
     out = ops.launch_paged_attention(q.to(DEV), cache, scaling=1.0, out_dtype=torch.float32, **at)
     _check_attention(out, expected, spread, reach, q_dtype=torch.float32, rows=1000 + tokens, d=d)
+
+
+def test_paged_attention_takes_a_narrower_table_as_a_copy():
+    """What a call sees does not hang on the table's width; a view of some of its columns is refused."""
+
+    b = Batch([(300, 3), (20, 1), (0, 9)], kv=2, d=128, page=16, seed=107, extra_entries=900)
+    _filled(b, 108)
+    b.scales *= 2.0**-3
+    q = torch.randn(b.tokens, 8, 128, generator=_g(109))
+    expected, spread, reach = osv.attention(q, b.host(), b.table, b.spans, page=16, scaling=0.1)
+    cache, batch = b.device()
+    narrow = batch["page_table"][:, :20]
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.launch_paged_attention(q.to(DEV), cache, scaling=0.1, **{**batch, "page_table": narrow})
+    for table in (batch["page_table"], narrow.contiguous()):
+        out = ops.launch_paged_attention(q.to(DEV), cache, scaling=0.1, out_dtype=torch.float32, **{**batch, "page_table": table})
+        _check_attention(out, expected, spread, reach, q_dtype=torch.float32, rows=303, d=128)
+
+
+def test_calls_on_two_streams_at_once():
+    """Each call's workspace is its own: splits of two calls in flight do not meet."""
+
+    batches = [Batch([(2000 + 500 * i, 2), (30, 1)], kv=2, d=64, page=64, seed=110 + i) for i in range(2)]
+    inputs = []
+    for i, b in enumerate(batches):
+        _filled(b, 112 + i)
+        b.scales *= 2.0**-3
+        cache, batch = b.device()
+        inputs.append((torch.randn(b.tokens, 8, 64, generator=_g(114 + i)).to(DEV), cache, batch))
+    alone = [ops.launch_paged_attention(q, cache, scaling=0.125, **batch) for q, cache, batch in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in inputs]
+    together = []
+    for _ in range(20):
+        for stream, (q, cache, batch) in zip(streams, inputs):
+            with torch.cuda.stream(stream):
+                together.append(ops.launch_paged_attention(q, cache, scaling=0.125, **batch))
+    torch.cuda.synchronize()
+    for i, out in enumerate(together):
+        assert torch.equal(out, alone[i % 2]), i
+
+
+def test_decoder_protocol_with_the_8_bit_cache():
+    """forward_step, prompt and decode steps, gives the logits of prefill."""
+
+    weights = syn.synthetic_decoder(SMALL, seed=syn.BASE_SEED + 84, random_norms=True)
+    decoder = PackedDecoder(SMALL, weights, device="cuda", max_positions=150, activation_dtype=torch.float32,
+                            cache_dtype=torch.float8_e4m3fn)
+    ids = torch.randint(0, SMALL.vocab, (66,), generator=_g(116)).to(DEV)
+    decoder.reset()
+    expected = [decoder.prefill(ids[:63]).clone()]
+    for i in range(63, 66):
+        expected.append(decoder.prefill(ids[i:i + 1], start=i).clone())
+    cache, got = None, []
+    for at, n in ((0, 63), (63, 1), (64, 1), (65, 1)):
+        where = torch.arange(at, at + n, device=DEV)
+        step = decoder.forward_step(input_ids=ids[None, at:at + n], attention_mask=torch.ones(1, at + n, device=DEV),
+                                    position_ids=where[None], cache_position=where, cache=cache, max_cache_length=150,
+                                    workload="decode" if n == 1 else "prefill", deterministic=True)
+        cache = step.cache
+        got.append(step.logits.view(-1).clone())
+    assert torch.equal(got[0], expected[0])
+    # Decode steps fold norms and sums into the linears: 2e-5 relative a linear, e4m3 steps of K and V (8e-3 over three layers).
+    for a, e in zip(got[1:], expected[1:]):
+        assert relative_l2(a.cpu(), e.cpu()) < 8e-3
