@@ -7,7 +7,9 @@
 // are on their way while these are worked on. With M the largest of the maxima,
 //   lse = M + log S, S = sum s e^(m - M)
 //   log p(x) = x - lse, entropy = log S - T / S, T = sum (t + s (m - M)) e^(m - M)
-// rounded once from fp64; a row's parts meet in a second launch.
+// m, s and t are fp32 up to a part's (a row's, where it has one part), the parts'
+// sum, the logarithm and the differences fp64; results are rounded once from those.
+// A row's parts meet in a second launch.
 //
 // Bound by the logits' bytes: 1531 rows of 151936 fp32 values (930 MB) are read at
 // 6.4 TB/s (145 us; loads that leave the caches alone).
@@ -19,7 +21,9 @@
 // costs the first pass one 4-byte store for 16 values. The maxima of 16 chunks
 // each are kept too, so that few chunk maxima have to be looked at. (48 rows of
 // 50257 bf16, k = 20: 12.4 us; lists of k kept by each wave took 21.5, chunk maxima
-// alone 15.8. One row of 151936 fp32, k = 5: 9.4 us, two launches and their waits.)
+// alone 15.8. One row of 151936 fp32, k = 5: 9.4 us, two launches and their waits. The
+// join, 8 and 5.7 us of these, reads the groups' maxima twice, a bound between, and
+// waits for the row's logarithm before it.)
 #include <math.h>
 
 #include "nq_common.h"

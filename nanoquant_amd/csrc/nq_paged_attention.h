@@ -324,12 +324,14 @@ __device__ __forceinline__ void store4(void* out, int dtype, int64_t at, const f
 // would leave room for one wave to a SIMD, and nothing would fill the matrix unit
 // during a softmax).
 //
-// Single tokens are bound by the cache's bytes: 268 MB of one sequence at 5.1 TB/s
-// (a copy reaches 5.04), 153 MB of 32 ragged sequences at 4.1 with the launch. Prompts are
-// bound by the vector unit, which widens K and V, and takes exponentials and parts of
-// the weights (4096 tokens of 32/8 heads of 128: 231 us for 1.4e11 multiplications
-// and additions; vector instructions issue in 64% of the cycles, the matrix unit
-// works in 35%).
+// Single tokens after long caches are bound by the cache's bytes: 268 MB of one
+// sequence at 4.8 TB/s (a copy reaches 5.04), 153 MB of 32 ragged sequences at 4.1 with the
+// launch. Prompts are bound by the vector unit, which widens K and V, and takes
+// exponentials and parts of the weights (4096 bf16 tokens of 32/8 heads of 128: 231
+// to 237 us for 1.4e11 multiplications and additions; the vector unit works in 71% of the
+// SIMDs' cycles, the matrix unit in 43%). Of some 600 vector instructions a tile 128
+// widen K and V: waves that have rows of their own each do that for themselves,
+// four times a workgroup, and heads of 128 spill 71 to 74 registers there.
 template <int D, int QT, int PP, int NT, int TILE, bool SHARED, int WAVES>
 __global__ __launch_bounds__(WAVES* kWave, D == 256 && NT == 2 ? 1 : 2) void k_paged_attention(const AttnArgs a) {
     constexpr int kRows = (SHARED ? 1 : WAVES) * 16 * NT;

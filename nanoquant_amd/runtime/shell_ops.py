@@ -459,10 +459,14 @@ class PagedCache(NamedTuple):
     v_scales: torch.Tensor
 
 
+_PAGE_SIZES = (16, 32, 64, 128)
+_HEAD_DIMS = (64, 128, 256)
+
+
 def paged_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, device: torch.device | str) -> PagedCache:
     """An empty paged cache. ``page_size`` is 16, 32, 64 or 128, ``head_dim`` 64, 128 or 256."""
 
-    if pages < 1 or kv_heads < 1 or page_size not in _PAGE_SIZES or head_dim not in (64, 128, 256):
+    if pages < 1 or kv_heads < 1 or page_size not in _PAGE_SIZES or head_dim not in _HEAD_DIMS:
         raise ValueError("paged cache geometry is unsupported")
 
     def zeros(*shape: int) -> torch.Tensor:
@@ -471,10 +475,6 @@ def paged_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, device
     scales = torch.zeros((2, pages, kv_heads), dtype=torch.float32, device=device)
     return PagedCache(zeros(pages, kv_heads, page_size, head_dim), zeros(pages, kv_heads, head_dim, page_size),
                       scales[0], scales[1])
-
-
-_PAGE_SIZES = (16, 32, 64, 128)
-_HEAD_DIMS = (64, 128, 256)
 
 
 def _paged_kv(name: str, device: torch.device, cache: PagedCache, page_table: torch.Tensor,
