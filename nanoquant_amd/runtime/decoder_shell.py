@@ -241,7 +241,7 @@ class _Buffers:
     attn_ws: torch.Tensor
     o_slots: torch.Tensor      # fused decode: sums of residual^2 per 16 rows after the o-projection
     down_slots: torch.Tensor   # ... and after the down-projection
-    starts: torch.Tensor       # 8-bit cache: the one sequence's first token and end
+    starts: torch.Tensor | None  # 8-bit cache: the one sequence's first token and end
 
 
 class PackedDecoder:
@@ -383,7 +383,7 @@ class PackedDecoder:
             f32(tokens, c.hidden), f32(tokens, c.hidden),
             torch.empty(workspace, dtype=torch.uint8, device=dev),
             f32(-(-c.hidden // 16)), f32(-(-c.hidden // 16)),
-            torch.tensor([0, tokens], dtype=torch.int32, device=dev),
+            None if self.paged is None else torch.arange(0, 2 * tokens, tokens, dtype=torch.int32, device=dev),
         )
 
     # -- one forward -----------------------------------------------------------------

@@ -259,3 +259,28 @@ def test_decoder_protocol_with_the_8_bit_cache():
     # Decode steps fold norms and sums into the linears: 2e-5 relative a linear, e4m3 steps of K and V (8e-3 over three layers).
     for a, e in zip(got[1:], expected[1:]):
         assert relative_l2(a.cpu(), e.cpu()) < 8e-3
+
+
+@pytest.mark.parametrize("cache", [torch.bfloat16, torch.float8_e4m3fn])
+def test_decoder_passes_wait_for_nothing(cache):
+    """A prompt on the device, its pass, decode steps and their scores: the host waits for none."""
+
+    weights = syn.synthetic_decoder(SMALL, seed=syn.BASE_SEED + 85, random_norms=True)
+    decoder = PackedDecoder(SMALL, weights, device=DEV, max_positions=150, cache_dtype=cache)
+    ids = torch.randint(0, SMALL.vocab, (70,), generator=_g(117)).to(DEV)
+
+    def passes():
+        tokens = decoder.generate_greedy(ids, 20)
+        scored, answer = decoder.generate_greedy_scored(ids, 20, top=2)
+        return tokens, scored, answer, decoder.score(ids, top=2), decoder.prefill(ids[:33]).clone()
+
+    first = passes()
+    before = torch.cuda.get_sync_debug_mode()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        second = passes()
+    finally:
+        torch.cuda.set_sync_debug_mode(before)
+    for a, b in zip(first, second):
+        for x, y in zip(a if isinstance(a, tuple) else (a,), b if isinstance(b, tuple) else (b,)):
+            assert torch.equal(x, y)
