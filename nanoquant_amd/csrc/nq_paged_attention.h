@@ -558,6 +558,14 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 && NT == 2 ? 1 : 2) void k_p
             }
             // Nothing seen so far (or only -inf): subtract 0, the weights are 0.
             const float m_use = m_run[u] == -INFINITY ? 0.0f : m_run[u];
+            // The fused subtraction sees what rounding took off the largest score: half a
+            // step of it, which is no number to raise 2 to where scores pass 2^30. They
+            // are rounded first there, so that the largest has the weight that it has in fp32.
+            if (__ballot(fabsf(m_use) > 0x1p24f)) {
+#pragma unroll
+                for (int j = 0; j < kBlock; ++j) sc[j >> 2][u][j & 3] *= f[u];
+                f[u] = 1.0f;
+            }
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < kBlock; ++j) {
