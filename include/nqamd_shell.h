@@ -248,6 +248,27 @@ int nq_paged_attention(const void* q, int32_t q_dtype, int64_t tokens, int32_t q
                        float scaling, void* out, int32_t out_dtype, void* workspace, int64_t workspace_bytes,
                        void* stream);
 
+/* Workspace bytes of nq_shared_attention (0: none needed; at most 1 GiB), or -1 for
+ * sizes that it refuses. */
+int64_t nq_shared_attention_workspace_bytes(int64_t tokens, int64_t batch, int32_t q_heads, int32_t kv_heads,
+                                            int32_t head_dim, int32_t page_size, int64_t table_pages,
+                                            int64_t shared_rows);
+
+/* nq_paged_attention for sequences that hold the same first rows, which are read
+ * once for many query rows of different sequences where each has few of them:
+ * the first shared_rows / page_size entries of every sequence's part of the page
+ * table stand for the same pages, and the call reads sequence 0's in their
+ * place (as many of them as make whole multiples of 64 rows too). What a token sees is what it sees in
+ * nq_paged_attention, also where a sequence has fewer rows than that. shared_rows
+ * is 0 to page_size * table_pages; it is part of a captured call.
+ * lse (fp32 [tokens, q_heads], NULL: not wanted) gets each query row's
+ *   lse[t, h] = log sum_j exp(scaling * q[t, h, :] . K_j)
+ * over the rows that the token sees; -inf for a token whose row lies outside the
+ * page table. Types, layouts and everything else as in nq_paged_attention. */
+int nq_shared_attention(const void* q, int32_t q_dtype, int64_t tokens, int32_t q_heads, const nq_paged_kv* kv,
+                        int64_t shared_rows, float scaling, void* out, int32_t out_dtype, float* lse,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Workspace bytes of nq_token_logprobs (0: none needed; -1: refused sizes). */
 int64_t nq_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top);
 

@@ -49,6 +49,19 @@ struct AttnArgs {
     int32_t out_dtype, q_heads, group, slots, splits, least;  // least: cache tiles a split takes at least
 };
 
+// A call whose sequences hold the same first rows, or that wants each row's
+// log-sum-exp. Workgroups [0, blocks) take the shared rows [0, skip), a multiple of
+// the page and of kTile, for the query rows of all sequences together; the others take what lies
+// behind them, sequence by sequence. All leave their shares to the join, the shared ones' behind
+// the others' slots * splits items.
+struct SharedArgs : AttnArgs {
+    float* lse;                          // [tokens][q_heads], may be null
+    int32_t skip, blocks, shared_splits, shared_per;  // shared_per: tiles of a split of the shared rows
+};
+
+template <bool SEGMENTS>
+using ArgsOf = std::conditional_t<SEGMENTS, SharedArgs, AttnArgs>;
+
 // Cache tiles of each split, and splits that have any, of a sequence whose last
 // token sees `visible` rows.
 struct SplitPlan {
@@ -78,11 +91,13 @@ struct Work {
 // the search's empty ones; 16 of 12 tokens: 41, 58). More sequences have one slot
 // more each than they may need, and all of a slot's splits, found by search (256 of
 // up to 1000 rows: 73 us; counted in two rounds 77).
+// Cache rows before `skip` are not these items'.
 template <bool TOKEN>
-__device__ __forceinline__ Work find(const Pages& p, int64_t at, int head, int group, int rows, int splits, int least) {
-    const int cache_rows = p.table_pages << p.page_shift;
+__device__ __forceinline__ Work find(const Pages& p, int64_t at, int head, int group, int rows, int splits, int least,
+                                     int skip = 0) {
+    const int cache_rows = (p.table_pages << p.page_shift) - skip;
     const auto plan_of = [&](int context, int begin, int end) {
-        const int64_t seen = static_cast<int64_t>(context) + (end - begin);
+        const int64_t seen = static_cast<int64_t>(context) + (end - begin) - skip;
         return split_plan(static_cast<int>(min(max(seen, int64_t{0}), static_cast<int64_t>(cache_rows))), splits, least);
     };
     Work w;
@@ -141,7 +156,42 @@ __device__ __forceinline__ SlotSpan slot_span(const Pages& p, const Found& f, in
     return o;
 }
 
+// The sequence of a token, for each lane its own: the last one that begins at or
+// before it. With starts that are not in order some sequence comes out; its span
+// decides whether it has the token.
+__device__ __forceinline__ Found lane_sequence(const Pages& p, int token) {
+    const auto span_of = [&](int b) {
+        const int start = p.starts[b], stop = p.starts[b + 1];
+        const int begin = min(max(start, 0), p.tokens);
+        return Span{begin, min(max(stop, begin), p.tokens)};
+    };
+    if (p.batch <= kWave) {
+        const int b = min(static_cast<int>(threadIdx.x & (kWave - 1)), p.batch - 1), context = p.contexts[b];
+        const Span span = span_of(b);
+        int hit = 0;
+#pragma unroll
+        for (int step = kWave / 2; step > 0; step /= 2) {
+            const int begin = __shfl(span.begin, min(hit + step, kWave - 1), kWave);
+            if (hit + step < p.batch && begin <= token) hit += step;
+        }
+        return {hit, __shfl(context, hit, kWave), {__shfl(span.begin, hit, kWave), __shfl(span.end, hit, kWave)}};
+    }
+    int low = 0, high = p.batch;  // the last b in [low, high) whose start is at most `token`
+    while (high - low > 1) {
+        const int mid = (low + high) / 2;
+        if (min(max(p.starts[mid], 0), p.tokens) <= token) low = mid;
+        else high = mid;
+    }
+    return {low, p.contexts[low], span_of(low)};
+}
+
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// log(2^m l): of a sum of weights relative to 2^m. In fp64, or a large m would cost
+// the logarithm's last bits.
+__device__ __forceinline__ float log_of_sum(float m, float l) {
+    return static_cast<float>((static_cast<double>(m) + __builtin_amdgcn_logf(l)) * 0.6931471805599453);
+}
 
 // Max / sum over the four 16-lane rows of a wave (lanes l, l ^ 16, l ^ 32, l ^ 48).
 __device__ __forceinline__ float rows_max(float x) {
@@ -332,8 +382,8 @@ __device__ __forceinline__ void store4(void* out, int dtype, int64_t at, const f
 // SIMDs' cycles, the matrix unit in 43%). Of some 600 vector instructions a tile 128
 // widen K and V: waves that have rows of their own each do that for themselves,
 // four times a workgroup, and heads of 128 spill 71 to 74 registers there.
-template <int D, int QT, int PP, int NT, int TILE, bool SHARED, int WAVES>
-__global__ __launch_bounds__(WAVES* kWave, D == 256 && NT == 2 ? 1 : 2) void k_paged_attention(const AttnArgs a) {
+template <int D, int QT, int PP, int NT, int TILE, bool SHARED, int WAVES, bool SEGMENTS>
+__global__ __launch_bounds__(WAVES* kWave, D == 256 && NT == 2 ? 1 : 2) void k_paged_attention(const ArgsOf<SEGMENTS> a) {
     constexpr int kRows = (SHARED ? 1 : WAVES) * 16 * NT;
     constexpr int kChunks = D / 64, kDims = D / 16;
     constexpr int kBlock = TILE / 4;   // consecutive cache rows of a lane: of V, and of the scores
@@ -344,16 +394,40 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 && NT == 2 ? 1 : 2) void k_p
     const int lane = threadIdx.x & (kWave - 1), n = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int g = blockIdx.x % p.kv_heads;
-    const Work w = find<false>(p, blockIdx.x / p.kv_heads, 0, a.group, kRows, a.splits, a.least);
-    const int64_t item = w.first + w.local;
-    if (w.local < 0 || item >= static_cast<int64_t>(a.slots) * a.splits) return;  // none, or query_starts out of order
-    const uint32_t local = static_cast<uint32_t>(w.local), stride = p.batch > kWave ? a.splits : w.plan.active;
-    const uint32_t nth = local / stride;
-    const int split = static_cast<int>(local - nth * stride);
-    if (split >= w.plan.active) return;
-    const SplitPlan plan = w.plan;
-    const SlotSpan s = slot_span(p, w.f, static_cast<int64_t>(nth) * kRows, a.group, kRows);
-    if (s.rows == 0) return;
+    const int unit = blockIdx.x / p.kv_heads;
+    bool all = false;  // of the shared rows, for all sequences
+    int split, skip = 0;
+    int64_t item;
+    SplitPlan plan;
+    SlotSpan s;
+    if constexpr (SEGMENTS) all = static_cast<int>(blockIdx.x) < a.blocks;
+    if (all) {
+        if constexpr (SEGMENTS) {
+            const int nth = unit / a.shared_splits;
+            split = unit - nth * a.shared_splits;
+            item = static_cast<int64_t>(a.slots) * a.splits + unit;
+            plan = {a.shared_per, a.shared_splits};
+            const int row0 = nth * kRows, rows = p.tokens * a.group;
+            s = {0, 0, 0, row0, min(kRows, rows - row0), a.skip};
+        }
+    } else {
+        Work w;
+        if constexpr (SEGMENTS) {
+            skip = a.skip;
+            w = find<false>(p, unit - a.blocks / p.kv_heads, 0, a.group, kRows, a.splits, a.least, skip);
+        } else {
+            w = find<false>(p, unit, 0, a.group, kRows, a.splits, a.least);
+        }
+        item = w.first + w.local;
+        if (w.local < 0 || item >= static_cast<int64_t>(a.slots) * a.splits) return;  // none, or query_starts out of order
+        const uint32_t local = static_cast<uint32_t>(w.local), stride = p.batch > kWave ? a.splits : w.plan.active;
+        const uint32_t nth = local / stride;
+        split = static_cast<int>(local - nth * stride);
+        if (split >= w.plan.active) return;
+        plan = w.plan;
+        s = slot_span(p, w.f, static_cast<int64_t>(nth) * kRows, a.group, kRows);
+        if (s.rows == 0) return;
+    }
     const int page = 1 << p.page_shift, cache_rows = p.table_pages << p.page_shift;
 
     // This wave's query rows: row numbers, positions (-1: sees nothing), q.
@@ -375,7 +449,13 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 && NT == 2 ? 1 : 2) void k_p
         const bool on = row[t] < s.rows;
         const int r = on ? s.row0 + row[t] : 0;
         const int place = r / a.group, head = g * a.group + r - place * a.group;
-        pos[t] = on ? row_of(s.context, place, cache_rows) : -1;
+        if (all) {
+            const Found f = lane_sequence(p, place);
+            const bool has = on && place >= f.span.begin && place < f.span.end;
+            pos[t] = has ? row_of(f.context, place - f.span.begin, cache_rows) : -1;
+        } else {
+            pos[t] = on ? row_of(s.context, place, cache_rows) : -1;
+        }
         out_at[t] = (static_cast<int64_t>(s.begin + place) * a.q_heads + head) * D;
         q_scale[t] = a.scale * load_query<QT, kQSteps>(a.q, out_at[t] + 16 * grp, on, q_regs);
         if (kInLds && (!SHARED || wave == 0)) {
@@ -407,9 +487,10 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 && NT == 2 ? 1 : 2) void k_p
         for (int d = 0; d < kDims; ++d) acc[d][t] = f32x4{0, 0, 0, 0};
     }
 
-    const int tile_end = min((split + 1) * plan.per * (kTile / TILE), (min(high_pos + 1, s.visible) + TILE - 1) / TILE);
+    const int first_tile = skip / TILE;
+    const int tile_end = min(first_tile + (split + 1) * plan.per * (kTile / TILE), (min(high_pos + 1, s.visible) + TILE - 1) / TILE);
     const int step = SHARED ? WAVES : 1;
-    const int tile_begin = split * plan.per * (kTile / TILE) + (SHARED ? wave : 0);
+    const int tile_begin = first_tile + split * plan.per * (kTile / TILE) + (SHARED ? wave : 0);
     // Table entries of this lane's blocks of kBlock rows: block n / 4 for K, grp
     // for the scores' scales and for V. What no query sees takes the last entry
     // in use. All loads of the loop are unconditional and in one order (entries,
@@ -656,8 +737,13 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 && NT == 2 ? 1 : 2) void k_p
     // Output o of query row t, or its share for the merge.
     const auto put = [&](int t, int d, const f32x4& o, float m, float l) {
         if (row[t] >= s.rows) return;
-        if (plan.active <= 1) {
+        bool whole = plan.active <= 1;
+        if constexpr (SEGMENTS) whole = whole && a.blocks == 0;
+        if (whole) {
             const float inv = pos[t] < 0 ? 0.0f : 1.0f / l;
+            if constexpr (SEGMENTS) {
+                if (a.lse && d == 0 && grp == 0) a.lse[out_at[t] / D] = pos[t] < 0 ? -INFINITY : log_of_sum(m, l);
+            }
             float v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = pos[t] < 0 ? 0.0f : o[i] * inv;
@@ -731,6 +817,22 @@ constexpr int kOwnRows = 128;  // of a slot whose waves have rows of their own, 
 template <int D>
 int launch_paged_attention(const AttnArgs& a, const AttnPlan& plan, int q_dtype, hipStream_t stream);
 
+// The same with shared rows apart or log-sum-exps.
+template <int D, int QT, int PP>
+int launch_shared_as(const SharedArgs& a, const AttnPlan& plan, hipStream_t stream) {
+    const int64_t blocks = static_cast<int64_t>(plan.slots) * plan.splits * a.p.kv_heads + a.blocks;
+    const dim3 grid(static_cast<unsigned>(blocks)), block(4 * kWave);
+    constexpr int kTileRows = kRowsAtOnce<D>;
+    if (plan.rows == 16) {
+        hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 1, kTileRows, true, 4, true>), grid, block, 0, stream, a);
+    } else if (plan.shared) {
+        hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 2, 32, true, 4, true>), grid, block, 0, stream, a);
+    } else if constexpr (D < 256) {
+        hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 2, kTileRows, false, 4, true>), grid, block, 0, stream, a);
+    }
+    return nq::launch_status();
+}
+
 template <int D, int QT, int PP>
 int launch_attention_as(const AttnArgs& a, const AttnPlan& plan, hipStream_t stream) {
     const int64_t blocks = static_cast<int64_t>(plan.slots) * plan.splits * a.p.kv_heads;  // launchable: checked with the workspace
@@ -738,14 +840,14 @@ int launch_attention_as(const AttnArgs& a, const AttnPlan& plan, hipStream_t str
     constexpr int kTileRows = kRowsAtOnce<D>;
     if (plan.shared && plan.waves == 4) {
         if (plan.rows == 32)
-            hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 2, 32, true, 4>), grid, block, 0, stream, a);
+            hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 2, 32, true, 4, false>), grid, block, 0, stream, a);
         else
-            hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 1, kTileRows, true, 4>), grid, block, 0, stream, a);
+            hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 1, kTileRows, true, 4, false>), grid, block, 0, stream, a);
     } else if constexpr (D < 256) {
         if (plan.shared)
-            hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 1, kTileRows, true, 8>), grid, block, 0, stream, a);
+            hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 1, kTileRows, true, 8, false>), grid, block, 0, stream, a);
         else
-            hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 2, kTileRows, false, 4>), grid, block, 0, stream, a);
+            hipLaunchKernelGGL((k_paged_attention<D, QT, PP, 2, kTileRows, false, 4, false>), grid, block, 0, stream, a);
     }
     return nq::launch_status();
 }
@@ -764,6 +866,27 @@ int launch_attention_for(const AttnArgs& a, const AttnPlan& plan, int q_dtype, h
         default: return launch_attention_out<D, NQ_DTYPE_BF16>(a, plan, stream);
     }
 }
+
+template <int D, int QT>
+int launch_shared_out(const SharedArgs& a, const AttnPlan& plan, hipStream_t stream) {
+    return a.out_dtype == NQ_DTYPE_F32 ? launch_shared_as<D, QT, 3>(a, plan, stream)
+                                       : launch_shared_as<D, QT, 2>(a, plan, stream);
+}
+
+template <int D>
+int launch_shared_for(const SharedArgs& a, const AttnPlan& plan, int q_dtype, hipStream_t stream) {
+    switch (q_dtype) {
+        case NQ_DTYPE_F32: return launch_shared_out<D, NQ_DTYPE_F32>(a, plan, stream);
+        case NQ_DTYPE_F16: return launch_shared_out<D, NQ_DTYPE_F16>(a, plan, stream);
+        default: return launch_shared_out<D, NQ_DTYPE_BF16>(a, plan, stream);
+    }
+}
+
+template <int D>
+int launch_shared_attention(const SharedArgs& a, const AttnPlan& plan, int q_dtype, hipStream_t stream);
+
+// The layout of a call without shared rows (nq_paged_attention.hip).
+AttnPlan plan_attention(int64_t tokens, int64_t batch, int q_heads, int kv_heads, int head_dim, int64_t cache_rows);
 
 }  // namespace paged
 }  // namespace nq

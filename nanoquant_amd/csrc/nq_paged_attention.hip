@@ -10,77 +10,6 @@ template <> int launch_paged_attention<64>(const AttnArgs&, const AttnPlan&, int
 template <> int launch_paged_attention<128>(const AttnArgs&, const AttnPlan&, int, hipStream_t);
 template <> int launch_paged_attention<256>(const AttnArgs&, const AttnPlan&, int, hipStream_t);
 
-}  // namespace paged
-}  // namespace nq
-
-namespace {
-
-using namespace nq::paged;
-
-// One workgroup per token and q head: its waves take the splits in turn, eight
-// loads in flight, and meet in LDS:
-//   out = sum_i w_i o_i / sum_i w_i l_i, w_i = 2^(m_i - max m)
-// Bound by the wait for a launch and two rounds of loads: 3.5 to 5 us.
-template <int D>
-__global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows) {
-    constexpr int E = D / kWave, kWaves = 4, kMost = 2;  // kMost: 64 splits each
-    __shared__ float join[kWaves][D], weights[kMost * kWave];
-    const Pages& p = a.p;
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int token = blockIdx.x / a.q_heads, head = blockIdx.x - token * a.q_heads;
-    const int g = head / a.group;
-    const Work work = find<true>(p, token, head - g * a.group, a.group, rows, a.splits, a.least);
-    const Found& f = work.f;
-    if (token < f.span.begin || token >= f.span.end) return;
-    const SplitPlan plan = work.plan;
-    if (plan.active <= 1) return;  // the attention wrote the output itself
-    const int64_t item = work.first + work.local;
-    if (item < 0 || item + plan.active > static_cast<int64_t>(a.slots) * a.splits) return;  // query_starts out of order
-    const uint32_t r = static_cast<uint32_t>(token - f.span.begin) * a.group + head - g * a.group;
-    const int64_t first = (item * p.kv_heads + g) * rows + r % static_cast<uint32_t>(rows);
-    const int64_t next = static_cast<int64_t>(p.kv_heads) * rows;  // from one split's row to the next split's
-    float w[kMost], l[kMost], m = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < kMost; ++c) {
-        const int i = lane + kWave * c;
-        const bool on = i < plan.active;
-        w[c] = on ? a.partial[2 * (first + i * next)] : -INFINITY;
-        l[c] = on ? a.partial[2 * (first + i * next) + 1] : 0.0f;
-        m = fmaxf(m, w[c]);
-    }
-#pragma unroll
-    for (int k = 1; k < kWave; k *= 2) m = fmaxf(m, __shfl_xor(m, k, kWave));
-    const float m_use = m == -INFINITY ? 0.0f : m;
-    float sum = 0.0f, o[E];
-#pragma unroll
-    for (int c = 0; c < kMost; ++c) {
-        w[c] = exp2_hw(w[c] - m_use);
-        if (wave == 0) weights[lane + kWave * c] = w[c];
-        sum += w[c] * l[c];
-    }
-#pragma unroll
-    for (int k = 1; k < kWave; k *= 2) sum += __shfl_xor(sum, k, kWave);
-#pragma unroll
-    for (int j = 0; j < E; ++j) o[j] = 0.0f;
-    __syncthreads();
-#pragma unroll 8
-    for (int i = wave; i < plan.active; i += kWaves) {
-        const float weight = weights[i];
-        const float* at = a.partial_o + (first + i * next) * D + lane;
-#pragma unroll
-        for (int j = 0; j < E; ++j) o[j] += weight * at[kWave * j];
-    }
-#pragma unroll
-    for (int j = 0; j < E; ++j) join[wave][lane + kWave * j] = o[j];
-    __syncthreads();
-    const bool off = row_of(f.context, token - f.span.begin, p.table_pages << p.page_shift) < 0;
-    for (int d = threadIdx.x; d < D; d += kWaves * kWave) {
-        const float all = (join[0][d] + join[1][d]) + (join[2][d] + join[3][d]);
-        nq::store_f32_as(a.out, a.out_dtype, static_cast<int64_t>(blockIdx.x) * D + d, off ? 0.0f : all / sum);
-    }
-}
-
 // How a call is laid out. All rules go by sizes that the host knows: the page
 // table's width stands for the cache's length, the mean for the query rows of a
 // sequence (its tokens times the q heads of a kv head). Times: 32/8 heads of 128,
@@ -165,6 +94,77 @@ AttnPlan plan_attention(int64_t tokens, int64_t batch, int q_heads, int kv_heads
     splits = std::min({splits, (tiles + plan.least - 1) / plan.least, kMostSplits, kMostPartials / each});
     plan.splits = static_cast<int>(std::max(splits, int64_t{1}));
     return plan;
+}
+
+}  // namespace paged
+}  // namespace nq
+
+namespace {
+
+using namespace nq::paged;
+
+// One workgroup per token and q head: its waves take the splits in turn, eight
+// loads in flight, and meet in LDS:
+//   out = sum_i w_i o_i / sum_i w_i l_i, w_i = 2^(m_i - max m)
+// Bound by the wait for a launch and two rounds of loads: 3.5 to 5 us.
+template <int D>
+__global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a, int rows) {
+    constexpr int E = D / kWave, kWaves = 4, kMost = 2;  // kMost: 64 splits each
+    __shared__ float join[kWaves][D], weights[kMost * kWave];
+    const Pages& p = a.p;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int token = blockIdx.x / a.q_heads, head = blockIdx.x - token * a.q_heads;
+    const int g = head / a.group;
+    const Work work = find<true>(p, token, head - g * a.group, a.group, rows, a.splits, a.least);
+    const Found& f = work.f;
+    if (token < f.span.begin || token >= f.span.end) return;
+    const SplitPlan plan = work.plan;
+    if (plan.active <= 1) return;  // the attention wrote the output itself
+    const int64_t item = work.first + work.local;
+    if (item < 0 || item + plan.active > static_cast<int64_t>(a.slots) * a.splits) return;  // query_starts out of order
+    const uint32_t r = static_cast<uint32_t>(token - f.span.begin) * a.group + head - g * a.group;
+    const int64_t first = (item * p.kv_heads + g) * rows + r % static_cast<uint32_t>(rows);
+    const int64_t next = static_cast<int64_t>(p.kv_heads) * rows;  // from one split's row to the next split's
+    float w[kMost], l[kMost], m = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kMost; ++c) {
+        const int i = lane + kWave * c;
+        const bool on = i < plan.active;
+        w[c] = on ? a.partial[2 * (first + i * next)] : -INFINITY;
+        l[c] = on ? a.partial[2 * (first + i * next) + 1] : 0.0f;
+        m = fmaxf(m, w[c]);
+    }
+#pragma unroll
+    for (int k = 1; k < kWave; k *= 2) m = fmaxf(m, __shfl_xor(m, k, kWave));
+    const float m_use = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f, o[E];
+#pragma unroll
+    for (int c = 0; c < kMost; ++c) {
+        w[c] = exp2_hw(w[c] - m_use);
+        if (wave == 0) weights[lane + kWave * c] = w[c];
+        sum += w[c] * l[c];
+    }
+#pragma unroll
+    for (int k = 1; k < kWave; k *= 2) sum += __shfl_xor(sum, k, kWave);
+#pragma unroll
+    for (int j = 0; j < E; ++j) o[j] = 0.0f;
+    __syncthreads();
+#pragma unroll 8
+    for (int i = wave; i < plan.active; i += kWaves) {
+        const float weight = weights[i];
+        const float* at = a.partial_o + (first + i * next) * D + lane;
+#pragma unroll
+        for (int j = 0; j < E; ++j) o[j] += weight * at[kWave * j];
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) join[wave][lane + kWave * j] = o[j];
+    __syncthreads();
+    const bool off = row_of(f.context, token - f.span.begin, p.table_pages << p.page_shift) < 0;
+    for (int d = threadIdx.x; d < D; d += kWaves * kWave) {
+        const float all = (join[0][d] + join[1][d]) + (join[2][d] + join[3][d]);
+        nq::store_f32_as(a.out, a.out_dtype, static_cast<int64_t>(blockIdx.x) * D + d, off ? 0.0f : all / sum);
+    }
 }
 
 int64_t partial_rows(const AttnPlan& plan, int kv_heads) {

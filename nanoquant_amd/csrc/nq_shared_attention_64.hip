@@ -1,0 +1,13 @@
+// Attention over the 8-bit paged cache with shared first rows, heads of 64.
+#include "nq_paged_attention.h"
+
+namespace nq {
+namespace paged {
+
+template <>
+int launch_shared_attention<64>(const SharedArgs& a, const AttnPlan& plan, int q_dtype, hipStream_t stream) {
+    return launch_shared_for<64>(a, plan, q_dtype, stream);
+}
+
+}  // namespace paged
+}  // namespace nq

@@ -648,6 +648,80 @@ def launch_paged_attention(
     return out
 
 
+# -- serving: long conversations in bounded memory and traffic ---------------------
+
+
+def shared_attention_workspace_bytes(tokens: int, batch: int, q_heads: int, cache: PagedCache, table_pages: int,
+                                     shared_rows: int) -> int:
+    _pages, kv_heads, page_size, head_dim = cache.k.shape
+    return int(_native.load().nq_shared_attention_workspace_bytes(tokens, batch, q_heads, kv_heads, head_dim, page_size,
+                                                                  table_pages, shared_rows))
+
+
+def launch_shared_attention(
+    q: torch.Tensor,
+    cache: PagedCache,
+    *,
+    page_table: torch.Tensor,
+    query_starts: torch.Tensor,
+    context_lens: torch.Tensor,
+    shared_rows: int,
+    scaling: float,
+    out: torch.Tensor | None = None,
+    out_dtype: torch.dtype = torch.bfloat16,
+    lse: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``launch_paged_attention`` for a batch whose sequences hold the same first
+    ``shared_rows`` cache rows: the first ``shared_rows // page_size`` entries of
+    every part of the page table name the same pages (sequence 0's are read),
+    and their keys and values are read once for many sequences
+    (nq_shared_attention). ``lse`` (fp32 ``[tokens, q_heads]``) gets each query
+    row's log-sum-exp, which ``launch_attention_weights`` takes. With
+    ``shared_rows=0`` nothing is shared. Mirrors ``launch_decode_attention``
+    (src/nanoquant/runtime/cuda_kernels.py:493-544) for many sequences."""
+
+    device = q.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return launch_shared_attention(
+                q, cache, page_table=page_table, query_starts=query_starts, context_lens=context_lens,
+                shared_rows=shared_rows, scaling=scaling, out=out, out_dtype=out_dtype, lse=lse, workspace=workspace)
+    if q.ndim != 3 or q.dtype not in _FLOAT:
+        raise ValueError("shared attention query must be F32/F16/BF16 [tokens, q_heads, head_dim]")
+    _check_device("shared attention", device, q, out, lse, workspace)
+    kv = _paged_kv("shared attention", device, cache, page_table, query_starts, context_lens)
+    tokens, q_heads, head_dim = q.shape
+    if head_dim != kv.head_dim or not tokens or not q_heads or q_heads % kv.kv_heads:
+        raise ValueError("shared attention query geometry does not match the cache")
+    if not 0.0 < scaling < float("inf"):
+        raise ValueError("shared attention scaling must be positive and finite")
+    if not 0 <= shared_rows <= kv.table_pages * kv.page_size:
+        raise ValueError("shared attention shared_rows must lie within the page table")
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (tokens, q_heads)):
+        raise ValueError("shared attention lse must be fp32 [tokens, q_heads]")
+    if out is None:
+        out = torch.empty(tokens, q_heads * head_dim, dtype=out_dtype, device=device)
+    elif out.numel() != q.numel():
+        raise ValueError("shared attention output geometry is incompatible")
+    if out.dtype not in _FLOAT:
+        raise ValueError("shared attention output must be F32/F16/BF16")
+    lib = _native.load()
+    need = lib.nq_shared_attention_workspace_bytes(tokens, kv.batch, q_heads, kv.kv_heads, head_dim, kv.page_size,
+                                                   kv.table_pages, shared_rows)
+    if need < 0:
+        raise ValueError("shared attention geometry was rejected")
+    if workspace is None and need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    status = lib.nq_shared_attention(
+        q.data_ptr(), _native.DTYPE_CODES[q.dtype], tokens, q_heads, ctypes.byref(kv), shared_rows, scaling,
+        out.data_ptr(), _native.DTYPE_CODES[out.dtype], _ptr(lse), _ptr(workspace),
+        0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(device),
+    )
+    _native.check("nq_shared_attention", status)
+    return out
+
+
 # -- how likely the answers are ---------------------------------------------------
 
 
