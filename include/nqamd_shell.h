@@ -269,6 +269,23 @@ int nq_shared_attention(const void* q, int32_t q_dtype, int64_t tokens, int32_t 
                         int64_t shared_rows, float scaling, void* out, int32_t out_dtype, float* lse,
                         void* workspace, int64_t workspace_bytes, void* stream);
 
+/* The attention that cached rows receive from the call's tokens, summed over the
+ * tokens that see them and the q heads of a kv head g:
+ *   out[page of j, g, row of j] = old + sum_t sum_h exp(scaling * q[t, h, :] . K_j - lse[t, h])
+ * for every row j from `first` on of a sequence that has tokens in the call; old is
+ * weights' value there, or 0 for rows that the call itself brought (j >= context_lens[b]),
+ * so that pages need no clearing. Nothing else of out is written. weights and out
+ * are fp32 [num_pages, kv_heads, page_size] and may be the same; lse as
+ * nq_shared_attention left it for the same call. Pages that the rows from `first` on
+ * lie in belong to one sequence and stand once in its part of the table; rows before
+ * `first` may lie in pages that sequences share. A row whose table entry names no page is left
+ * out. q as in nq_paged_attention; a weight never passes 1, is off by about 2^-22
+ * of lse and of its score relative to itself, and NaN where they are. Sums in fp32
+ * in a fixed order (deterministic). */
+int nq_attention_weights(const void* q, int32_t q_dtype, int64_t tokens, int32_t q_heads, const nq_paged_kv* kv,
+                         float scaling, const float* lse, int64_t first, const float* weights, float* out,
+                         void* stream);
+
 /* Workspace bytes of nq_token_logprobs (0: none needed; -1: refused sizes). */
 int64_t nq_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top);
 

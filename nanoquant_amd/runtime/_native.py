@@ -78,6 +78,7 @@ EXPORTED_SYMBOLS = (
     "nq_paged_attention",
     "nq_shared_attention_workspace_bytes",
     "nq_shared_attention",
+    "nq_attention_weights",
     "nq_token_logprobs_workspace_bytes",
     "nq_token_logprobs",
 )
@@ -266,6 +267,9 @@ def _declare(lib: ctypes.CDLL) -> None:
         "nq_shared_attention_workspace_bytes": (c_i64, [c_i64, c_i64, i32, i32, i32, i32, c_i64, c_i64]),
         "nq_shared_attention": (
             c_int, [vp, i32, c_i64, i32, ctypes.POINTER(PagedKv), c_i64, f32, vp, i32, vp, vp, c_i64, vp],
+        ),
+        "nq_attention_weights": (
+            c_int, [vp, i32, c_i64, i32, ctypes.POINTER(PagedKv), f32, vp, c_i64, vp, vp, vp],
         ),
         "nq_token_logprobs_workspace_bytes": (c_i64, [c_i64, c_i64, i32]),
         "nq_token_logprobs": (c_int, [vp, i32, c_i64, c_i64, c_i64, vp, i32, vp, vp, vp, vp, vp, c_i64, vp]),

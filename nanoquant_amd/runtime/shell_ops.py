@@ -722,6 +722,59 @@ def launch_shared_attention(
     return out
 
 
+def launch_attention_weights(
+    q: torch.Tensor,
+    cache: PagedCache,
+    lse: torch.Tensor,
+    weights: torch.Tensor,
+    *,
+    page_table: torch.Tensor,
+    query_starts: torch.Tensor,
+    context_lens: torch.Tensor,
+    scaling: float,
+    first: int = 0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Adds the attention that each cached row from ``first`` on receives from the
+    call's tokens to ``weights`` (fp32 ``[pages, kv_heads, page_size]``, in place
+    unless ``out`` is given; rows that the call brought start at 0), after
+    ``launch_shared_attention`` with the same arrays, whose ``lse`` it takes
+    (nq_attention_weights). ``launch_paged_evict`` decides by these weights. Pages
+    that sequences share hold rows before ``first`` alone. The reference keeps
+    every row (src/nanoquant/runtime/transformers_generation.py:262-418)."""
+
+    device = q.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return launch_attention_weights(
+                q, cache, lse, weights, page_table=page_table, query_starts=query_starts, context_lens=context_lens,
+                scaling=scaling, first=first, out=out)
+    if q.ndim != 3 or q.dtype not in _FLOAT:
+        raise ValueError("attention weights query must be F32/F16/BF16 [tokens, q_heads, head_dim]")
+    _check_device("attention weights", device, q, lse, weights, out)
+    kv = _paged_kv("attention weights", device, cache, page_table, query_starts, context_lens)
+    tokens, q_heads, head_dim = q.shape
+    if head_dim != kv.head_dim or not tokens or not q_heads or q_heads % kv.kv_heads:
+        raise ValueError("attention weights query geometry does not match the cache")
+    if not 0.0 < scaling < float("inf"):
+        raise ValueError("attention weights scaling must be positive and finite")
+    if lse.dtype is not torch.float32 or lse.shape != (tokens, q_heads):
+        raise ValueError("attention weights lse must be fp32 [tokens, q_heads]")
+    if out is None:
+        out = weights
+    shape = (kv.num_pages, kv.kv_heads, kv.page_size)
+    if weights.dtype is not torch.float32 or out.dtype is not torch.float32 or weights.shape != shape or out.shape != shape:
+        raise ValueError("attention weights must be fp32 [pages, kv_heads, page_size]")
+    if first < 0:
+        raise ValueError("attention weights begin at a row from 0 on")
+    status = _native.load().nq_attention_weights(
+        q.data_ptr(), _native.DTYPE_CODES[q.dtype], tokens, q_heads, ctypes.byref(kv), scaling, lse.data_ptr(), first,
+        weights.data_ptr(), out.data_ptr(), _stream(device),
+    )
+    _native.check("nq_attention_weights", status)
+    return out
+
+
 # -- how likely the answers are ---------------------------------------------------
 
 
