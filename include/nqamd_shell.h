@@ -286,6 +286,34 @@ int nq_attention_weights(const void* q, int32_t q_dtype, int64_t tokens, int32_t
                          float scaling, const float* lse, int64_t first, const float* weights, float* out,
                          void* stream);
 
+/* Workspace bytes of nq_paged_evict (0: none needed; -1: refused sizes). */
+int64_t nq_paged_evict_workspace_bytes(int64_t batch, int32_t kv_heads, int32_t page_size, int64_t table_pages,
+                                       int64_t budget);
+
+/* Cuts every sequence with more than `budget` cached rows to that many. Of such a
+ * sequence's n = context_lens[b] rows stay, for each kv head by itself, rows
+ * [0, first), rows [n - recent, n) and of those between the
+ * budget - first - recent with the greatest weights (nq_attention_weights; fp32
+ * [num_pages, kv_heads, page_size]), the lowest row first among equals, NaN above all. They keep
+ * their order: row i of the cut sequence is row rows_out[b, g, i] of the old one.
+ *   page_table_out [batch, ceil(budget / page_size)]: the first / page_size pages in
+ *     front as they were (nothing of them is written: others may share them), then
+ *     the pages into[b, :] ([batch, ceil(budget / page_size) - first / page_size])
+ *   context_lens_out [batch]: budget
+ *   into's pages: the rows' K and V as an append of them in one call would store
+ *     them (a page's scale is the least power of two that brings its rows within
+ *     448) and their weights; nothing is written behind the last row
+ * A sequence with budget rows or fewer keeps its pages and its length; its entries of into are not
+ * touched, and rows_out has its rows, then -1. Rows in pages that the
+ * table does not name count as NaN; an entry of into that names no page writes nothing but
+ * page_table_out. into's pages stand there once, and in no sequence's part of the page table.
+ * Values beyond fp32 become NaN. kv->query_starts is not read and may be NULL.
+ * first + recent <= budget. Keys keep the rotation of their position: the
+ * tokens appended next have other positions than cache rows (nq_paged_append_at). */
+int nq_paged_evict(const nq_paged_kv* kv, float* weights, const int32_t* into, int64_t budget, int64_t first,
+                   int64_t recent, int32_t* page_table_out, int32_t* context_lens_out, int32_t* rows_out,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Workspace bytes of nq_token_logprobs (0: none needed; -1: refused sizes). */
 int64_t nq_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top);
 

@@ -93,5 +93,44 @@ __device__ __forceinline__ int row_of(int context, int place, int rows) {
     return row >= 0 && row < rows ? static_cast<int>(row) : -1;
 }
 
+// fp64 -> fp32 towards zero with the last bit set where that drops something:
+// a later rounding to fewer bits (e4m3 keeps 4) then rounds the fp64 value.
+__device__ __forceinline__ float round_to_odd(double x) {
+    float f = static_cast<float>(x);
+    if (!(fabsf(f) < INFINITY)) return f;  // beyond fp32, or not finite
+    if (static_cast<double>(f) != x) {
+        uint32_t u = __float_as_uint(f);
+        if (fabs(static_cast<double>(f)) > fabs(x)) u -= 1;
+        f = __uint_as_float(u | 1u);
+    }
+    return f;
+}
+
+// The least power of two 2^e, e >= -126, with amax <= 448 * 2^e = 1.75 * 2^(8 + e).
+__device__ __forceinline__ float scale_for(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    const int e = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return __uint_as_float(static_cast<uint32_t>(max(e, -126) + 127) << 23);
+}
+
+// Four e4m3 bytes that stand for byte * from, as bytes that stand for byte * to (a
+// power of two that holds them); NaN for what fp32 does not hold. A power of two
+// times a byte is exact in fp32; with any other scale the fp32 product would be a first rounding.
+__device__ __forceinline__ uint32_t rescaled4(uint32_t w, float from, float to) {
+    float x[4] = {__builtin_amdgcn_cvt_f32_fp8(w, 0), __builtin_amdgcn_cvt_f32_fp8(w, 1),
+                  __builtin_amdgcn_cvt_f32_fp8(w, 2), __builtin_amdgcn_cvt_f32_fp8(w, 3)};
+    const float inv = 1.0f / to;
+    const bool exact = (__float_as_uint(from) & 0x7fffffu) == 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float y = x[j] * from;
+        if (!(fabsf(y) < INFINITY)) x[j] = __builtin_nanf("");
+        else x[j] = exact ? y * inv : round_to_odd(static_cast<double>(x[j]) * from * inv);
+    }
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], r, true);
+    return static_cast<uint32_t>(r);
+}
+
 }  // namespace paged
 }  // namespace nq

@@ -133,19 +133,6 @@ __device__ __forceinline__ double inverse_root(double x) {
     return y0 > 0.0 && y0 < INFINITY ? y : y0;
 }
 
-// fp64 -> fp32 towards zero with the last bit set where that drops something:
-// a later rounding to fewer bits (e4m3 keeps 4) then rounds the fp64 value.
-__device__ __forceinline__ float round_to_odd(double x) {
-    float f = static_cast<float>(x);
-    if (!(fabsf(f) < INFINITY)) return f;  // beyond fp32, or not finite
-    if (static_cast<double>(f) != x) {
-        uint32_t u = __float_as_uint(f);
-        if (fabs(static_cast<double>(f)) > fabs(x)) u -= 1;
-        f = __uint_as_float(u | 1u);
-    }
-    return f;
-}
-
 // x as fp32 for an e4m3 rounding: the nearest fp32 value does, unless it lies
 // where e4m3 rounds to even or where a scale ends. All of those have 0 in their
 // last 19 bits, but for subnormal ones (at the smallest scales).
@@ -227,13 +214,6 @@ __device__ __forceinline__ void load_weight(const void* w, int dtype, int place,
     if (dtype == NQ_DTYPE_F32) load_values<NQ_DTYPE_F32>(w, place, out);
     else if (dtype == NQ_DTYPE_F16) load_values<NQ_DTYPE_F16>(w, place, out);
     else load_values<NQ_DTYPE_BF16>(w, place, out);
-}
-
-// The least power of two 2^e, e >= -126, with amax <= 448 * 2^e = 1.75 * 2^(8 + e).
-__device__ __forceinline__ float scale_for(float amax) {
-    const uint32_t u = __float_as_uint(amax);
-    const int e = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
-    return __uint_as_float(static_cast<uint32_t>(max(e, -126) + 127) << 23);
 }
 
 __device__ __forceinline__ float finite_or_zero(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; }

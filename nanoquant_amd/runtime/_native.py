@@ -79,6 +79,8 @@ EXPORTED_SYMBOLS = (
     "nq_shared_attention_workspace_bytes",
     "nq_shared_attention",
     "nq_attention_weights",
+    "nq_paged_evict_workspace_bytes",
+    "nq_paged_evict",
     "nq_token_logprobs_workspace_bytes",
     "nq_token_logprobs",
 )
@@ -270,6 +272,10 @@ def _declare(lib: ctypes.CDLL) -> None:
         ),
         "nq_attention_weights": (
             c_int, [vp, i32, c_i64, i32, ctypes.POINTER(PagedKv), f32, vp, c_i64, vp, vp, vp],
+        ),
+        "nq_paged_evict_workspace_bytes": (c_i64, [c_i64, i32, i32, c_i64, c_i64]),
+        "nq_paged_evict": (
+            c_int, [ctypes.POINTER(PagedKv), vp, vp, c_i64, c_i64, c_i64, vp, vp, vp, vp, c_i64, vp],
         ),
         "nq_token_logprobs_workspace_bytes": (c_i64, [c_i64, c_i64, i32]),
         "nq_token_logprobs": (c_int, [vp, i32, c_i64, c_i64, c_i64, vp, i32, vp, vp, vp, vp, vp, c_i64, vp]),

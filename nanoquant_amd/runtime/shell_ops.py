@@ -478,8 +478,9 @@ def paged_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, device
 
 
 def _paged_kv(name: str, device: torch.device, cache: PagedCache, page_table: torch.Tensor,
-              query_starts: torch.Tensor, context_lens: torch.Tensor) -> _native.PagedKv:
-    """Checks of the cache and the batch; the C descriptor of both."""
+              query_starts: torch.Tensor | None, context_lens: torch.Tensor) -> _native.PagedKv:
+    """Checks of the cache and the batch; the C descriptor of both. A call without
+    tokens has no query_starts."""
 
     k, v, k_scales, v_scales = cache
     _check_device(name, device, k, v, k_scales, v_scales, page_table, query_starts, context_lens)
@@ -494,15 +495,15 @@ def _paged_kv(name: str, device: torch.device, cache: PagedCache, page_table: to
     if k_scales.dtype is not torch.float32 or v_scales.dtype is not torch.float32 or k_scales.shape != scales \
             or v_scales.shape != scales:
         raise ValueError(f"{name} cache scales must be fp32 [pages, kv_heads]")
-    if page_table.dtype is not torch.int32 or query_starts.dtype is not torch.int32 \
-            or context_lens.dtype is not torch.int32:
+    if page_table.dtype is not torch.int32 or context_lens.dtype is not torch.int32 \
+            or (query_starts is not None and query_starts.dtype is not torch.int32):
         raise ValueError(f"{name} page_table, query_starts and context_lens must be int32")
     shape = page_table.shape
     if len(shape) != 2 or not shape[0] or not shape[1] or context_lens.shape != (shape[0],) \
-            or query_starts.shape != (shape[0] + 1,):
+            or (query_starts is not None and query_starts.shape != (shape[0] + 1,)):
         raise ValueError(f"{name} takes page_table [batch, pages], query_starts [batch + 1] and context_lens [batch]")
     return _native.PagedKv(k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), pages, kv_heads,
-                           head_dim, page_size, 0, page_table.data_ptr(), shape[1], query_starts.data_ptr(),
+                           head_dim, page_size, 0, page_table.data_ptr(), shape[1], _ptr(query_starts),
                            context_lens.data_ptr(), shape[0])
 
 
@@ -772,6 +773,81 @@ def launch_attention_weights(
         weights.data_ptr(), out.data_ptr(), _stream(device),
     )
     _native.check("nq_attention_weights", status)
+    return out
+
+
+class Evicted(NamedTuple):
+    """``launch_paged_evict``'s result: the sequences' new int32 page table ``[batch,
+    ceil(budget / page_size)]`` and lengths ``[batch]``, and the old row of each
+    row that stayed, int32 ``[batch, kv_heads, budget]`` (-1 behind the last)."""
+
+    page_table: torch.Tensor
+    context_lens: torch.Tensor
+    rows: torch.Tensor
+
+
+def paged_evict_workspace_bytes(batch: int, cache: PagedCache, table_pages: int, budget: int) -> int:
+    _pages, kv_heads, page_size, _head_dim = cache.k.shape
+    return int(_native.load().nq_paged_evict_workspace_bytes(batch, kv_heads, page_size, table_pages, budget))
+
+
+def launch_paged_evict(
+    cache: PagedCache,
+    weights: torch.Tensor,
+    *,
+    page_table: torch.Tensor,
+    context_lens: torch.Tensor,
+    into: torch.Tensor,
+    budget: int,
+    first: int = 0,
+    recent: int = 0,
+    out: Evicted | None = None,
+    workspace: torch.Tensor | None = None,
+) -> Evicted:
+    """Cuts every sequence with more than ``budget`` cached rows to that many: its
+    ``first`` rows, its ``recent`` newest and, for each kv head, of those between
+    the heaviest by ``weights`` (``launch_attention_weights``). The rows that stay
+    move in their order to the free pages ``into`` (int32 ``[batch, ceil(budget /
+    page_size) - first // page_size]``), but for the whole pages of the first rows, which stay where
+    they are (nq_paged_evict). The keys keep the positions they were rotated at:
+    ``launch_paged_append`` takes those of the next tokens as ``rope_starts``. The reference
+    keeps every row (src/nanoquant/runtime/transformers_generation.py:262-418)."""
+
+    device = cache.k.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return launch_paged_evict(cache, weights, page_table=page_table, context_lens=context_lens, into=into,
+                                      budget=budget, first=first, recent=recent, out=out, workspace=workspace)
+    _check_device("paged evict", device, weights, into, workspace)
+    batch = page_table.shape[0] if page_table.ndim == 2 else 0
+    kv = _paged_kv("paged evict", device, cache, page_table, None, context_lens)
+    if weights.dtype is not torch.float32 or weights.shape != (kv.num_pages, kv.kv_heads, kv.page_size):
+        raise ValueError("paged evict weights must be fp32 [pages, kv_heads, page_size]")
+    if budget < 1 or first < 0 or recent < 0 or first + recent > budget:
+        raise ValueError("paged evict keeps at least one row, and first and recent rows within its budget")
+    entries = -(-budget // kv.page_size)
+    slots = entries - first // kv.page_size
+    if into.dtype is not torch.int32 or into.shape != (batch, slots):
+        raise ValueError("paged evict into must be int32 [batch, ceil(budget / page_size) - first // page_size]")
+    if out is None:
+        out = Evicted(into.new_empty(batch, entries), into.new_empty(batch), into.new_empty(batch, kv.kv_heads, budget))
+    else:
+        _check_device("paged evict", device, *out)
+        if any(x.dtype is not torch.int32 for x in out) or out.page_table.shape != (batch, entries) \
+                or out.context_lens.shape != (batch,) or out.rows.shape != (batch, kv.kv_heads, budget):
+            raise ValueError("paged evict outputs must be int32 [batch, pages], [batch] and [batch, kv_heads, budget]")
+    lib = _native.load()
+    need = lib.nq_paged_evict_workspace_bytes(batch, kv.kv_heads, kv.page_size, kv.table_pages, budget)
+    if need < 0:
+        raise ValueError("paged evict geometry was rejected")
+    if workspace is None and need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    status = lib.nq_paged_evict(
+        ctypes.byref(kv), weights.data_ptr(), into.data_ptr() if slots else None, budget, first, recent,
+        out.page_table.data_ptr(), out.context_lens.data_ptr(), out.rows.data_ptr(), _ptr(workspace),
+        0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(device),
+    )
+    _native.check("nq_paged_evict", status)
     return out
 
 
