@@ -222,6 +222,16 @@ int nq_paged_append(const void* q, const void* k, const void* v, int32_t dtype, 
                     const float* cos_table, const float* sin_table, int64_t rope_positions,
                     const nq_paged_kv* kv, void* q_out, int32_t q_out_dtype, void* stream);
 
+/* nq_paged_append for sequences whose tokens have other positions than cache rows,
+ * as after nq_paged_evict: sequence b's tokens are rotated as those at positions
+ * rope_starts[b], rope_starts[b] + 1, ... (int32 [batch], device memory; NULL:
+ * their cache rows). A token whose position lies outside the RoPE tables writes nothing. */
+int nq_paged_append_at(const void* q, const void* k, const void* v, int32_t dtype, int64_t tokens,
+                       int32_t q_heads, const void* q_norm, const void* k_norm, int32_t norm_dtype, float eps,
+                       const float* cos_table, const float* sin_table, int64_t rope_positions,
+                       const nq_paged_kv* kv, const int32_t* rope_starts, void* q_out, int32_t q_out_dtype,
+                       void* stream);
+
 /* Workspace bytes of nq_paged_attention (0: none needed; at most 1 GiB), or -1 for
  * sizes that it refuses: among others a grid of 2^32 threads or more, as the
  * append and the log probabilities refuse too (NQ_ERR_SHAPE). */

@@ -49,6 +49,7 @@ struct AppendArgs {
     Pages p;
     const void *q, *k, *v, *q_norm, *k_norm;
     const float *cos_table, *sin_table;
+    const int32_t* rope_starts;  // [batch] position of each sequence's first token; null: its cache row
     void* q_out;
     float eps;
     int32_t norm_dtype, q_dtype, q_heads, q_groups, rope_rows, kv_blocks;
@@ -270,14 +271,15 @@ __global__ __launch_bounds__(WAVES* kWave) void k_paged_append(const AppendArgs 
         const Found f = sequence_at(p, token, [](int, int begin) { return static_cast<int64_t>(begin); });
         const Span s = f.span;
         const int row = token >= s.begin && token < s.end ? row_of(f.context, token - s.begin, rows) : -1;
-        if (row < 0 || row >= a.rope_rows) return;
+        const int64_t position = a.rope_starts ? static_cast<int64_t>(a.rope_starts[f.b]) + (token - s.begin) : row;
+        if (row < 0 || position < 0 || position >= a.rope_rows) return;
         float cs[E], sn[E], x[kQHeads / H][E];
         const int64_t at = (static_cast<int64_t>(token) * a.q_heads + head) * D + place;
         const int last = a.q_heads - 1 - head;
 #pragma unroll
         for (int i = 0; i < kQHeads / H; ++i) load_values<DT>(a.q, at + min(i * H + sub, last) * D, x[i]);
         load_weight(a.q_norm, a.norm_dtype, place, w);
-        load_rope_row<D>(a, row, place, cs, sn);
+        load_rope_row<D>(a, static_cast<int>(position), place, cs, sn);
 #pragma unroll
         for (int i = 0; i < kQHeads / H; ++i) {
             norm_rope<D>(x[i], w, a.q_norm != nullptr, a.eps, cs, sn);
@@ -294,9 +296,11 @@ __global__ __launch_bounds__(WAVES* kWave) void k_paged_append(const AppendArgs 
     const Span s = f.span;
     const int b = f.b, context = f.context;
     const int64_t slot0 = first_slot(b, s.begin);
-    // New rows of the sequence that have a place: positions [low, high).
-    const int64_t low = max(static_cast<int64_t>(context), int64_t{0});
-    const int64_t high = min(static_cast<int64_t>(context) + (s.end - s.begin), static_cast<int64_t>(min(rows, a.rope_rows)));
+    // New rows of the sequence that have a place and, `turned` further, a row of the RoPE tables: [low, high).
+    const int64_t turned = a.rope_starts ? static_cast<int64_t>(a.rope_starts[b]) - context : 0;
+    const int64_t low = max(max(static_cast<int64_t>(context), int64_t{0}), -turned);
+    const int64_t high = min(static_cast<int64_t>(context) + (s.end - s.begin),
+                             min(static_cast<int64_t>(rows), a.rope_rows - turned));
     const int64_t nth = low / kPage + (slot - slot0);
     const int64_t begin = max(low, nth * kPage), end = min(high, (nth + 1) * kPage);
     if (slot < slot0 || begin >= end) return;
@@ -322,7 +326,7 @@ __global__ __launch_bounds__(WAVES* kWave) void k_paged_append(const AppendArgs 
     for (int i = 0; i < kPageTokens / H; ++i) {
         if (!any_at(i)) break;
         float cs[E], sn[E];
-        load_rope_row<D>(a, static_cast<int>(begin) + min(row_at(i), n - 1), place, cs, sn);
+        load_rope_row<D>(a, static_cast<int>(begin + turned) + min(row_at(i), n - 1), place, cs, sn);
         double y[E];
 #pragma unroll
         for (int j = 0; j < E; ++j) y[j] = static_cast<double>(kf[i][j]);
@@ -447,10 +451,11 @@ bool float_code(int d) { return nq::is_float_dtype(d); }
 
 }  // namespace
 
-extern "C" int nq_paged_append(const void* q, const void* k, const void* v, int32_t dtype, int64_t tokens,
-                               int32_t q_heads, const void* q_norm, const void* k_norm, int32_t norm_dtype, float eps,
-                               const float* cos_table, const float* sin_table, int64_t rope_positions,
-                               const nq_paged_kv* kv, void* q_out, int32_t q_out_dtype, void* stream) {
+extern "C" int nq_paged_append_at(const void* q, const void* k, const void* v, int32_t dtype, int64_t tokens,
+                                  int32_t q_heads, const void* q_norm, const void* k_norm, int32_t norm_dtype, float eps,
+                                  const float* cos_table, const float* sin_table, int64_t rope_positions,
+                                  const nq_paged_kv* kv, const int32_t* rope_starts, void* q_out, int32_t q_out_dtype,
+                                  void* stream) {
     if (!q || !k || !v || !cos_table || !sin_table || !q_out || (q_norm == nullptr) != (k_norm == nullptr))
         return NQ_ERR_ARGUMENT;
     if (!float_code(dtype) || !float_code(q_out_dtype) || (q_norm && !float_code(norm_dtype))) return NQ_ERR_DTYPE;
@@ -459,7 +464,7 @@ extern "C" int nq_paged_append(const void* q, const void* k, const void* v, int3
     if (q_heads <= 0 || q_heads > 65535 || q_heads % kv->kv_heads || rope_positions <= 0) return NQ_ERR_SHAPE;
     if (!(eps >= 0.0f)) return NQ_ERR_ARGUMENT;
     a.q = q; a.k = k; a.v = v; a.q_norm = q_norm; a.k_norm = k_norm;
-    a.cos_table = cos_table; a.sin_table = sin_table; a.q_out = q_out;
+    a.cos_table = cos_table; a.sin_table = sin_table; a.rope_starts = rope_starts; a.q_out = q_out;
     a.eps = eps; a.norm_dtype = norm_dtype; a.q_dtype = q_out_dtype; a.q_heads = q_heads;
     a.rope_rows = static_cast<int32_t>(rope_positions < 0x7fffffff ? rope_positions : 0x7fffffff);
     a.q_groups = (q_heads + kQHeads - 1) / kQHeads;
@@ -469,4 +474,12 @@ extern "C" int nq_paged_append(const void* q, const void* k, const void* v, int3
         case 128: return launch_append<128>(a, dtype, tokens, kv->kv_heads, kv->batch, st);
         default: return launch_append<256>(a, dtype, tokens, kv->kv_heads, kv->batch, st);
     }
+}
+
+extern "C" int nq_paged_append(const void* q, const void* k, const void* v, int32_t dtype, int64_t tokens,
+                               int32_t q_heads, const void* q_norm, const void* k_norm, int32_t norm_dtype, float eps,
+                               const float* cos_table, const float* sin_table, int64_t rope_positions,
+                               const nq_paged_kv* kv, void* q_out, int32_t q_out_dtype, void* stream) {
+    return nq_paged_append_at(q, k, v, dtype, tokens, q_heads, q_norm, k_norm, norm_dtype, eps, cos_table, sin_table,
+                              rope_positions, kv, nullptr, q_out, q_out_dtype, stream);
 }

@@ -74,6 +74,7 @@ EXPORTED_SYMBOLS = (
     "nq_output_projection",
     "nq_greedy_select",
     "nq_paged_append",
+    "nq_paged_append_at",
     "nq_paged_attention_workspace_bytes",
     "nq_paged_attention",
     "nq_shared_attention_workspace_bytes",
@@ -261,6 +262,10 @@ def _declare(lib: ctypes.CDLL) -> None:
         "nq_paged_append": (
             c_int,
             [vp, vp, vp, i32, c_i64, i32, vp, vp, i32, f32, vp, vp, c_i64, ctypes.POINTER(PagedKv), vp, i32, vp],
+        ),
+        "nq_paged_append_at": (
+            c_int,
+            [vp, vp, vp, i32, c_i64, i32, vp, vp, i32, f32, vp, vp, c_i64, ctypes.POINTER(PagedKv), vp, vp, i32, vp],
         ),
         "nq_paged_attention_workspace_bytes": (c_i64, [c_i64, c_i64, i32, i32, i32, i32, c_i64]),
         "nq_paged_attention": (

@@ -531,12 +531,15 @@ def launch_paged_append(
     context_lens: torch.Tensor,
     q_out: torch.Tensor | None = None,
     q_dtype: torch.dtype = torch.float32,
+    rope_starts: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Per-head RMSNorm + RoPE of a ragged batch's q and k and the append of k and
     v to an 8-bit paged cache; returns the rotated q ``[tokens, q_heads,
     head_dim]``. Tokens ``query_starts[b] .. query_starts[b + 1]`` are sequence
     b's, at cache rows ``context_lens[b] ..``, in the pages ``page_table[b]``
-    (nq_paged_append). Mirrors ``launch_decode_rope`` and
+    (nq_paged_append). ``rope_starts`` (int32 ``[batch]``) are the positions that
+    the sequences' tokens begin at where those are not their cache rows, as after
+    ``launch_paged_evict`` (nq_paged_append_at). Mirrors ``launch_decode_rope`` and
     ``launch_cache_prefix_update`` (src/nanoquant/runtime/cuda_kernels.py:715-815)
     for many sequences."""
 
@@ -545,8 +548,9 @@ def launch_paged_append(
         with torch.cuda.device(device):
             return launch_paged_append(
                 q, k, v, cache, q_heads=q_heads, q_norm=q_norm, k_norm=k_norm, eps=eps, cos=cos, sin=sin,
-                page_table=page_table, query_starts=query_starts, context_lens=context_lens, q_out=q_out, q_dtype=q_dtype)
-    _check_device("paged append", device, q, k, v, q_norm, k_norm, cos, sin, q_out)
+                page_table=page_table, query_starts=query_starts, context_lens=context_lens, q_out=q_out, q_dtype=q_dtype,
+                rope_starts=rope_starts)
+    _check_device("paged append", device, q, k, v, q_norm, k_norm, cos, sin, q_out, rope_starts)
     kv = _paged_kv("paged append", device, cache, page_table, query_starts, context_lens)
     kv_heads, head_dim = kv.kv_heads, kv.head_dim
     if q_heads < 1 or q_heads % kv_heads:
@@ -571,18 +575,20 @@ def launch_paged_append(
     if cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or len(table) != 2 \
             or table[1] * 2 != head_dim or not table[0] or sin.shape != table:
         raise ValueError("RoPE tables must be fp32 [positions, head_dim / 2]")
+    if rope_starts is not None and (rope_starts.dtype is not torch.int32 or rope_starts.shape != context_lens.shape):
+        raise ValueError("paged append rope_starts must be int32 [batch]")
     if q_out is None:
         q_out = torch.empty(tokens, q_heads, head_dim, dtype=q_dtype, device=device)
     elif q_out.numel() != tokens * q_heads * head_dim:
         raise ValueError("q_out must be [tokens, q_heads, head_dim]")
     if q_out.dtype not in _FLOAT:
         raise ValueError("q_out must be F32/F16/BF16")
-    status = _native.load().nq_paged_append(
+    status = _native.load().nq_paged_append_at(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), _native.DTYPE_CODES[dtype], tokens, q_heads, _ptr(q_norm),
-        _ptr(k_norm), norm_code, eps, cos.data_ptr(), sin.data_ptr(), table[0], ctypes.byref(kv), q_out.data_ptr(),
-        _native.DTYPE_CODES[q_out.dtype], _stream(device),
+        _ptr(k_norm), norm_code, eps, cos.data_ptr(), sin.data_ptr(), table[0], ctypes.byref(kv), _ptr(rope_starts),
+        q_out.data_ptr(), _native.DTYPE_CODES[q_out.dtype], _stream(device),
     )
-    _native.check("nq_paged_append", status)
+    _native.check("nq_paged_append_at", status)
     return q_out
 
 

@@ -61,8 +61,9 @@ def finite_amax(x: torch.Tensor) -> torch.Tensor:
     return torch.where(torch.isfinite(x), x.abs(), 0.0).amax((1, 2))
 
 
-def append(q, k, v, cache, table, spans, *, page, q_norm, k_norm, eps, cos, sin):
-    """Rotated q (fp64, NaN rows where no token writes) and the cache afterwards."""
+def append(q, k, v, cache, table, spans, *, page, q_norm, k_norm, eps, cos, sin, rope_starts=None):
+    """Rotated q (fp64, NaN rows where no token writes) and the cache afterwards;
+    `rope_starts` are the sequences' first positions where those are not cache rows."""
 
     cache = {name: x.clone().double() for name, x in cache.items()}
     pages, d = cache["k"].shape[0], cache["k"].shape[3]
@@ -73,11 +74,12 @@ def append(q, k, v, cache, table, spans, *, page, q_norm, k_norm, eps, cos, sin)
         new: dict[int, list[tuple[int, torch.Tensor, torch.Tensor]]] = {}
         for t in range(begin, end):
             row = context + t - begin
-            if row < 0 or row >= rows_held or row >= cos.shape[0]:
+            at = row if rope_starts is None else rope_starts[b] + t - begin
+            if row < 0 or row >= rows_held or at < 0 or at >= cos.shape[0]:
                 continue
-            q_out[t] = norm_rope(q[t], q_norm, eps, cos[row], sin[row])
+            q_out[t] = norm_rope(q[t], q_norm, eps, cos[at], sin[at])
             new.setdefault(row // page, []).append(
-                (row % page, norm_rope(k[t], k_norm, eps, cos[row], sin[row]), v[t].double()))
+                (row % page, norm_rope(k[t], k_norm, eps, cos[at], sin[at]), v[t].double()))
         for slot, rows in new.items():
             at = table[b][slot]
             if at < 0 or at >= pages:
