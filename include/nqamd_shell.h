@@ -164,6 +164,35 @@ int nq_greedy_select(const void* workspace, int64_t vocab, int64_t hidden, int64
                      int64_t* history, int64_t history_capacity, int32_t* step,
                      int32_t* position, void* stream);
 
+/* nq_greedy_select from `count` partials of another projection (nq_int4_projection). */
+int nq_greedy_select_partials(const void* partials, int64_t count, int64_t* token_out, int64_t* history,
+                              int64_t history_capacity, int32_t* step, int32_t* position, void* stream);
+
+/* Workspace bytes of nq_int4_projection (-1: refused sizes). */
+int64_t nq_int4_projection_workspace_bytes(int64_t tokens, int64_t out_features, int64_t in_features, int32_t group);
+
+/* Partials (8 bytes each) that nq_int4_projection leaves for one token. */
+int64_t nq_int4_projection_partials(int64_t out_features);
+
+/* Products with 4-bit weights and group scales:
+ *   y[t, o] = sum_i scales[o, i / group] * (w[o, i] - zeros[o, i / group]) * x[t, i]
+ * x F32/F16/BF16 [tokens, in_features] (1 to 65535 tokens; the form is that of a few: the weights
+ * are read once for up to 5 tokens with groups of 128, 2 with 64 and 1 with 32); packed
+ * [out_features, in_features / 2], byte j of a row holding column 2 j in its low
+ * four bits and 2 j + 1 in its high ones, 16-byte aligned; scales F32/F16/BF16 [out_features,
+ * ceil(in_features / group)], zeros uint8 of the same shape (NULL: 8), any value
+ * from 0 to 255; y F32/F16/BF16 [tokens, out_features]. group 32, 64 or 128,
+ * in_features a multiple of 32. x is read to 2^-23 of its largest value in a group (or of 2^-100), sums
+ * within a group are exact, those of groups fp32 in a fixed order. A token that
+ * holds an infinity or a NaN gives NaN. partials, for one token (NULL: not
+ * wanted), get the largest value of each 16 rows for nq_greedy_select_partials.
+ * Stands beside nq_output_projection for a weight of a quarter of its bytes
+ * (the reference's is bf16: src/nanoquant/runtime/cuda_kernels.py:588-618,684-712). */
+int nq_int4_projection(const void* x, int32_t x_dtype, int64_t tokens, const void* packed, const void* scales,
+                       int32_t scale_dtype, const uint8_t* zeros, int64_t out_features, int64_t in_features,
+                       int32_t group, void* y, int32_t y_dtype, void* partials, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
 /* ---- Serving: ragged batches over an 8-bit paged KV cache ------------------ */
 
 /* An 8-bit paged KV cache and the batch that a call runs on it.

@@ -2187,17 +2187,21 @@ extern "C" int nq_output_projection(const void* x, int32_t x_dtype, const void* 
     return nq::launch_status();
 }
 
+extern "C" int nq_greedy_select_partials(const void* partials, int64_t count, int64_t* token_out, int64_t* history,
+                                         int64_t history_capacity, int32_t* step, int32_t* position, void* stream) {
+    if (!partials || !token_out) return NQ_ERR_ARGUMENT;
+    if ((history != nullptr) != (step != nullptr) || history_capacity < 0) return NQ_ERR_ARGUMENT;
+    if (count <= 0) return NQ_ERR_SHAPE;
+    hipLaunchKernelGGL(k_greedy_select, dim3(1), dim3(1024), 0, as_stream(stream),
+                       static_cast<const uint64_t*>(partials), count, token_out, history, history_capacity, step, position);
+    return nq::launch_status();
+}
+
 extern "C" int nq_greedy_select(const void* workspace, int64_t vocab, int64_t hidden, int64_t* token_out,
                                 int64_t* history, int64_t history_capacity, int32_t* step, int32_t* position,
                                 void* stream) {
-    if (!workspace || !token_out) return NQ_ERR_ARGUMENT;
-    if ((history != nullptr) != (step != nullptr) || history_capacity < 0) return NQ_ERR_ARGUMENT;
     const int64_t wgs = vocab > 0 && vocab <= 0x7fffffffLL && hidden > 0 && hidden % 8 == 0 ? proj_workgroups(vocab, hidden) : -1;
-    if (wgs <= 0) return NQ_ERR_SHAPE;
-    hipLaunchKernelGGL(k_greedy_select, dim3(1), dim3(1024), 0, as_stream(stream),
-                       static_cast<const uint64_t*>(workspace), wgs, token_out, history, history_capacity, step,
-                       position);
-    return nq::launch_status();
+    return nq_greedy_select_partials(workspace, wgs, token_out, history, history_capacity, step, position, stream);
 }
 
 extern "C" int64_t nq_decode_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,

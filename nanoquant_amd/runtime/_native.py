@@ -73,6 +73,10 @@ EXPORTED_SYMBOLS = (
     "nq_output_projection_workspace_bytes",
     "nq_output_projection",
     "nq_greedy_select",
+    "nq_greedy_select_partials",
+    "nq_int4_projection_workspace_bytes",
+    "nq_int4_projection_partials",
+    "nq_int4_projection",
     "nq_paged_append",
     "nq_paged_append_at",
     "nq_paged_attention_workspace_bytes",
@@ -259,6 +263,12 @@ def _declare(lib: ctypes.CDLL) -> None:
         "nq_output_projection_workspace_bytes": (c_i64, [c_i64, c_i64]),
         "nq_output_projection": (c_int, [vp, i32, vp, c_i64, c_i64, vp, vp, c_i64, vp]),
         "nq_greedy_select": (c_int, [vp, c_i64, c_i64, vp, vp, c_i64, vp, vp, vp]),
+        "nq_greedy_select_partials": (c_int, [vp, c_i64, vp, vp, c_i64, vp, vp, vp]),
+        "nq_int4_projection_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64, i32]),
+        "nq_int4_projection_partials": (c_i64, [c_i64]),
+        "nq_int4_projection": (
+            c_int, [vp, i32, c_i64, vp, vp, i32, vp, c_i64, c_i64, i32, vp, i32, vp, vp, c_i64, vp],
+        ),
         "nq_paged_append": (
             c_int,
             [vp, vp, vp, i32, c_i64, i32, vp, vp, i32, f32, vp, vp, c_i64, ctypes.POINTER(PagedKv), vp, i32, vp],

@@ -424,7 +424,8 @@ def launch_greedy_select(
 ) -> torch.Tensor:
     """Greedy token (lowest index among equal maxima, like ``torch.argmax``) from
     the partials of ``launch_output_projection``, written to ``token_out[0]``;
-    optionally appended to ``history`` at ``step`` and advancing ``position``."""
+    optionally appended to ``history`` at ``step`` and advancing ``position``.
+    The partials of ``launch_int4_projection`` are an int64 tensor, and are known by that."""
 
     device = workspace.device
     if token_out.dtype != torch.int64 or token_out.numel() < 1:
@@ -436,12 +437,139 @@ def launch_greedy_select(
     if position is not None:
         _position("greedy select", position, device)
     _check_device("greedy select", device, workspace, token_out, history, step, position)
-    status = _native.load().nq_greedy_select(
-        workspace.data_ptr(), vocab, hidden, token_out.data_ptr(), _ptr(history),
-        0 if history is None else history.numel(), _ptr(step), _ptr(position), _stream(device),
-    )
+    after = (token_out.data_ptr(), _ptr(history), 0 if history is None else history.numel(), _ptr(step), _ptr(position),
+             _stream(device))
+    if workspace.dtype is torch.int64:
+        if workspace.numel() != int4_projection_partials(vocab):
+            raise ValueError("greedy select takes the partials of a projection to the vocabulary")
+        status = _native.load().nq_greedy_select_partials(workspace.data_ptr(), workspace.numel(), *after)
+        _native.check("nq_greedy_select_partials", status)
+        return token_out
+    status = _native.load().nq_greedy_select(workspace.data_ptr(), vocab, hidden, *after)
     _native.check("nq_greedy_select", status)
     return token_out
+
+
+# -- 4-bit weights ---------------------------------------------------------------
+
+
+class Int4Matrix(NamedTuple):
+    """A ``[out, in]`` matrix of 4-bit weights: uint8 ``packed`` ``[out, in / 2]``, byte j of a
+    row holding column 2 j in its low bits and 2 j + 1 in its high ones, ``scales`` F32/F16/BF16
+    ``[out, ceil(in / group)]`` with groups of 32, 64 or 128 columns, and uint8
+    ``zeros`` of that shape (None: 8). A weight is ``scale * (nibble - zero)``."""
+
+    packed: torch.Tensor
+    scales: torch.Tensor
+    zeros: torch.Tensor | None = None
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.packed.shape[0], 2 * self.packed.shape[1]
+
+    def to(self, device: torch.device | str) -> "Int4Matrix":
+        return Int4Matrix(*(None if t is None else t.to(device).contiguous() for t in self))
+
+
+_INT4_GROUPS = (32, 64, 128)
+
+
+def int4_matrix(weight: torch.Tensor, group: int = 128, scale_dtype: torch.dtype = torch.float16) -> Int4Matrix:
+    """``weight`` ``[out, in]`` rounded to 4 bits: for each group of columns the scale
+    that brings its largest value to 7, or its lowest to -8 where that is the smaller scale.
+    Once, before serving."""
+
+    if weight.ndim != 2 or weight.shape[1] % 32 or group not in _INT4_GROUPS or scale_dtype not in _FLOAT:
+        raise ValueError("4-bit weights need [out, in] with in a multiple of 32 and groups of 32, 64 or 128")
+    outs, ins = weight.shape
+    groups = -(-ins // group)
+    packed = torch.empty(outs, ins // 2, dtype=torch.uint8, device=weight.device)
+    scales = torch.empty(outs, groups, dtype=scale_dtype, device=weight.device)
+    for first in range(0, outs, 8192):
+        w = torch.nn.functional.pad(weight[first:first + 8192].float(), (0, groups * group - ins)).view(-1, groups, group)
+        scale = torch.maximum(w.amax(-1) / 7, -w.amin(-1) / 8).to(scale_dtype)
+        scales[first:first + 8192] = scale
+        scale = scale.float()
+        q = torch.where(scale[..., None] > 0, w / scale[..., None], 0.0).round_().clamp_(-8, 7).add_(8).to(torch.uint8)
+        q = q.view(q.shape[0], -1)[:, :ins]
+        packed[first:first + 8192] = q[:, 0::2] | (q[:, 1::2] << 4)
+    return Int4Matrix(packed, scales)
+
+
+def int4_projection_workspace_bytes(tokens: int, weight: Int4Matrix) -> int:
+    outs, ins = weight.shape
+    return int(_native.load().nq_int4_projection_workspace_bytes(tokens, outs, ins, _int4_group(weight)))
+
+
+def int4_projection_partials(out_features: int) -> int:
+    return int(_native.load().nq_int4_projection_partials(out_features))
+
+
+def _int4_group(weight: Int4Matrix) -> int:
+    """The group that the scales' shape says (the widest, where a narrower one would be the same)."""
+
+    ins, groups = 2 * weight.packed.shape[1], weight.scales.shape[1]
+    for group in reversed(_INT4_GROUPS):
+        if -(-ins // group) == groups:
+            return group
+    raise ValueError("4-bit scales must be [out, ceil(in / group)] with groups of 32, 64 or 128")
+
+
+def launch_int4_projection(
+    x: torch.Tensor,
+    weight: Int4Matrix,
+    *,
+    out: torch.Tensor | None = None,
+    out_dtype: torch.dtype = torch.float32,
+    partials: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``x @ W.T`` of F32/F16/BF16 ``x`` ``[tokens, in]`` and 4-bit weights, for a few
+    tokens (nq_int4_projection): fp32 sums, rounded once to ``out``. For one
+    token ``partials`` (int64 ``[int4_projection_partials(out)]``) get what
+    ``launch_greedy_select`` chooses by. Beside ``launch_output_projection``, at a
+    quarter of its weight's bytes (src/nanoquant/runtime/cuda_kernels.py:684-712)."""
+
+    device = x.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return launch_int4_projection(x, weight, out=out, out_dtype=out_dtype, partials=partials, workspace=workspace)
+    packed, scales, zeros = weight
+    if packed.dtype is not torch.uint8 or packed.ndim != 2 or packed.shape[1] % 16 or not packed.numel():
+        raise ValueError("4-bit weights must be uint8 [out, in / 2] with in a multiple of 32")
+    outs, ins = weight.shape
+    if scales.dtype not in _FLOAT or scales.ndim != 2 or scales.shape[0] != outs:
+        raise ValueError("4-bit scales must be F32/F16/BF16 [out, ceil(in / group)]")
+    group = _int4_group(weight)
+    if zeros is not None and (zeros.dtype is not torch.uint8 or zeros.shape != scales.shape):
+        raise ValueError("4-bit zeros must be uint8 of the scales' shape")
+    if x.ndim != 2 or x.dtype not in _FLOAT or not x.shape[0] or x.shape[1] != ins:
+        raise ValueError("4-bit projection input must be F32/F16/BF16 [tokens, in]")
+    _check_device("4-bit projection", device, x, packed, scales, zeros, out, partials, workspace)
+    tokens = x.shape[0]
+    if out is None:
+        out = torch.empty(tokens, outs, dtype=out_dtype, device=device)
+    elif out.shape != (tokens, outs):
+        raise ValueError("4-bit projection output must be [tokens, out]")
+    if out.dtype not in _FLOAT:
+        raise ValueError("4-bit projection output must be F32/F16/BF16")
+    lib = _native.load()
+    if partials is not None and (tokens != 1 or partials.dtype is not torch.int64
+                                 or partials.shape != (lib.nq_int4_projection_partials(outs),)):
+        raise ValueError("4-bit projection partials are those of one token: int64 [int4_projection_partials(out)]")
+    need = lib.nq_int4_projection_workspace_bytes(tokens, outs, ins, group)
+    if need < 0:
+        raise ValueError("4-bit projection geometry was rejected")
+    if workspace is None and need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    status = lib.nq_int4_projection(
+        x.data_ptr(), _native.DTYPE_CODES[x.dtype], tokens, packed.data_ptr(), scales.data_ptr(),
+        _native.DTYPE_CODES[scales.dtype], _ptr(zeros), outs, ins, group, out.data_ptr(), _native.DTYPE_CODES[out.dtype],
+        _ptr(partials), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
+        _stream(device),
+    )
+    _native.check("nq_int4_projection", status)
+    return out
 
 
 # -- serving: ragged batches over an 8-bit paged cache ---------------------------
