@@ -24,6 +24,14 @@ constexpr int kWave = 64, kChunk = 128, kDigits = 3;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// How a call is laid out: `blocks` blocks of tokens at once, of each row's chunks a
+// `slice` for a workgroup, in stages of `stage` that LDS holds the digits of.
+struct Int4Plan {
+    int blocks, passes, share, slices, slice, stage;
+    int64_t groups;  // workgroups of a pass and slice
+};
 
 struct Int4Args {
     const void* x;
@@ -31,14 +39,11 @@ struct Int4Args {
     const void* scales;      // [outs][groups]
     const uint8_t* zeros;    // the same, or null: 8
     void* y;
+    float* partial;          // [slices][tokens][outs] where the slices are joined in a second launch
     uint64_t* best;          // [tiles] largest value and its row, of one token; may be null
-    // The tokens' digits: bytes [tokens][3][chunks][2][64], for each token, chunk and group of it 2^e
-    // ([tokens][chunks][4]), and the digits' sums ([tokens][3][chunks][4]).
-    uint8_t* digits;
-    float* units;
-    int32_t* sums;
-    int64_t outs, ins;
+    int64_t outs, ins, tiles, step;  // step: tiles from one of a wave's to its next
     int32_t tokens, chunks, groups, x_dtype, scale_dtype, y_dtype;
+    int32_t share, slice, stage;
 };
 
 // Groups of a chunk, columns of B that one of them has, and tokens of these.
@@ -47,18 +52,55 @@ struct Shape {
     static constexpr int kGroups = kChunk / G, kColumns = 16 / kGroups, kTokens = kColumns / kDigits;
 };
 
-// One thread per 8 columns of a token.
+__device__ __forceinline__ uint64_t order_of(float v, uint32_t row) {
+    const uint32_t u = __float_as_uint(v == 0.0f ? 0.0f : v);
+    return static_cast<uint64_t>(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (0xffffffffu - row);
+}
+
+// The largest (value, row) of a tile's 16 rows, which 16 lanes hold.
+__device__ __forceinline__ uint64_t best_of_tile(uint64_t key) {
+#pragma unroll
+    for (int m = 1; m < 16; m *= 2) {
+        const uint32_t low = __shfl_xor(static_cast<uint32_t>(key), m, kWave);
+        const uint32_t high = __shfl_xor(static_cast<uint32_t>(key >> 32), m, kWave);
+        const uint64_t other = static_cast<uint64_t>(high) << 32 | low;
+        key = other > key ? other : key;
+    }
+    return key;
+}
+
+// What a wave's lanes wrote to LDS is what its lanes read after this.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+constexpr int kWaves = 4, kThreads = kWaves * kWave;
+constexpr int kAtOnce = 4;  // chunks whose weights a wave loads at once
+
+// Digits in LDS: a line of `stage` chunks, [2][64] bytes each (even and odd columns), for each token and
+// digit; 64 bytes more a line, so that a product's columns lie in different banks.
+__host__ __device__ constexpr int line_bytes(int stage) { return stage * kChunk + 64; }
+
+// A column of B in a chunk: what a product with it is multiplied by, but for the
+// row's scale, and the sum of its digits.
+struct Column {
+    float unit, sum;
+};
+
+// Eight adjacent columns of a token as digits.
 template <int G>
-__global__ __launch_bounds__(256) void k_int4_digits(const Int4Args a) {
-    constexpr int kGroup = G / 8;  // threads of a group
-    const int token = blockIdx.y, at = blockIdx.x * 256 + threadIdx.x, chunk = at / 16, t = at & 15;
-    if (chunk >= a.chunks) return;  // whole groups of lanes
+__device__ __forceinline__ void digits_of(const Int4Args& a, int token, int chunk, int t, uint32_t (&even)[kDigits],
+                                          uint32_t (&odd)[kDigits], int (&sum)[kDigits], float& unit) {
+    constexpr int kGroup = G / 8;  // lanes of a group
     float x[8], most = 0.0f;
     bool finite = true;
+    const int64_t at = static_cast<int64_t>(chunk) * kChunk + 8 * t;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = at < a.ins ? nq::load_f32(a.x, a.x_dtype, token * a.ins + at + j) : 0.0f;  // ins: a multiple of 32
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const int64_t i = static_cast<int64_t>(at) * 8 + j;
-        x[j] = i < a.ins ? nq::load_f32(a.x, a.x_dtype, token * a.ins + i) : 0.0f;
         finite = finite && fabsf(x[j]) < INFINITY;
         most = fmaxf(most, fabsf(x[j]));
     }
@@ -70,8 +112,8 @@ __global__ __launch_bounds__(256) void k_int4_digits(const Int4Args a) {
     const uint32_t bits = __float_as_uint(most);
     const int k = max(static_cast<int>(bits >> 23) - 127 + ((bits & 0x7fffffu) > 0x7e0000u ? 1 : 0), -100);
     const float up = finite ? __uint_as_float(static_cast<uint32_t>(22 - k + 127) << 23) : 0.0f;
-    uint32_t even[kDigits] = {}, odd[kDigits] = {};
-    int sum[kDigits] = {};
+#pragma unroll
+    for (int d = 0; d < kDigits; ++d) even[d] = odd[d] = sum[d] = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         int n = finite ? static_cast<int>(rintf(x[j] * up)) : 0;
@@ -84,104 +126,241 @@ __global__ __launch_bounds__(256) void k_int4_digits(const Int4Args a) {
         }
     }
 #pragma unroll
-    for (int d = 0; d < kDigits; ++d) {
-        uint32_t* to = reinterpret_cast<uint32_t*>(a.digits + ((static_cast<int64_t>(token) * kDigits + d) * a.chunks + chunk) * kChunk);
-        to[t] = even[d];
-        to[16 + t] = odd[d];
+    for (int d = 0; d < kDigits; ++d)
 #pragma unroll
         for (int m = 1; m < kGroup; m *= 2) sum[d] += __shfl_xor(sum[d], m, kWave);
-        if (t % kGroup == 0) a.sums[((static_cast<int64_t>(token) * kDigits + d) * a.chunks + chunk) * 4 + t / kGroup] = sum[d];
-    }
-    if (t % kGroup == 0)
-        a.units[(static_cast<int64_t>(token) * a.chunks + chunk) * 4 + t / kGroup] =
-            finite ? __uint_as_float(static_cast<uint32_t>(k - 22 + 127) << 23) : __builtin_nanf("");
+    unit = finite ? __uint_as_float(static_cast<uint32_t>(k - 22 + 127) << 23) : __builtin_nanf("");
 }
 
-__device__ __forceinline__ uint64_t order_of(float v, uint32_t row) {
-    const uint32_t u = __float_as_uint(v == 0.0f ? 0.0f : v);
-    return static_cast<uint64_t>(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (0xffffffffu - row);
-}
-
-constexpr int kWaves = 4;
-
-// A workgroup has 16 rows; its waves take the chunks in turn.
-template <int G>
-__global__ __launch_bounds__(kWaves* kWave) void k_int4_product(const Int4Args a) {
+// A workgroup has a slice of the chunks and, share waves to a tile of 16 rows, kWaves / share tiles
+// at a time; the waves of a tile each take a part of a stage's chunks. NB blocks of tokens.
+template <int G, int NB>
+__global__ __launch_bounds__(kThreads) void k_int4_product(const Int4Args a) {
     using S = Shape<G>;
-    __shared__ float join[kWaves][16][17];
-    __shared__ uint64_t keys[16];
-    const int lane = threadIdx.x & (kWave - 1), c = lane & 15, q = lane >> 4, wave = threadIdx.x / kWave;
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * 16;
+    constexpr int kMost = kAtOnce * S::kGroups;  // groups whose scales a wave holds in LDS
+    extern __shared__ u32x4 lds[];
+    // Zeros, digits, columns; for each wave scales [kMost][16], zeros [kMost][16] and sums [16][17].
+    uint8_t* digits = reinterpret_cast<uint8_t*>(lds) + 64;
+    const int first = blockIdx.z * NB * S::kTokens, tokens = min(NB * S::kTokens, a.tokens - first);
+    const int line = line_bytes(a.stage);
+    Column* columns = reinterpret_cast<Column*>(digits + tokens * kDigits * line);  // [stage][NB][16]
+    float* mine_f = reinterpret_cast<float*>(columns + a.stage * NB * 16);
+    const int lane = threadIdx.x & (kWave - 1), c = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    constexpr int kEach = kMost * 16 + kMost * 4 + 16 * 17;
+    float* sums = mine_f + wave * kEach;
+    float* scales = sums + 16 * 17;
+    uint8_t* zeros = reinterpret_cast<uint8_t*>(scales + kMost * 16);
+    // (sums lie at 16 * 17 words, so that scales are 16-byte aligned.)
+    if (threadIdx.x < 16) reinterpret_cast<uint32_t*>(lds)[threadIdx.x] = 0;
+
+    const int chunk0 = blockIdx.y * a.slice, chunk1 = min(chunk0 + a.slice, a.chunks);
+    const int part = wave % a.share;
     const int64_t half = a.ins / 2;
-    const uint8_t* row = a.packed + min(row0 + c, a.outs - 1) * half;
-    // This lane's column of B.
     const int group = c / S::kColumns, in_group = c % S::kColumns, local = in_group / kDigits, digit = in_group % kDigits;
-    const float power = digit == 0 ? 1.0f : digit == 1 ? 256.0f : 65536.0f;
-    const bool mine = q * S::kGroups / 4 == group;
-    for (int first = 0; first < a.tokens; first += S::kTokens) {
-        const int token = first + local;
-        const bool on = local < S::kTokens && token < a.tokens;
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int chunk = wave; chunk < a.chunks; chunk += kWaves) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(row + min(static_cast<int64_t>(chunk) * 64 + 16 * q, half - 16));
-            const int64_t at = (static_cast<int64_t>(on ? token : 0) * kDigits + (on ? digit : 0)) * a.chunks + chunk;
-            u32x4 b[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-            if (on && mine) {
-                const u32x4* from = reinterpret_cast<const u32x4*>(a.digits + at * kChunk);
-                b[0] = from[q];
-                b[1] = from[4 + q];
-            }
-            const u32x4 low = w & 0x0f0f0f0fu, high = (w >> 4) & 0x0f0f0f0fu;
-            i32x4 dot = {0, 0, 0, 0};
-            dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, low), __builtin_bit_cast(i32x4, b[0]), dot, 0, 0, 0);
-            dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, high), __builtin_bit_cast(i32x4, b[1]), dot, 0, 0, 0);
-            if (on) {
-                const float unit = power * a.units[(static_cast<int64_t>(token) * a.chunks + chunk) * 4 + group];
-                const int sum = a.sums[at * 4 + group];
-                const int64_t g = min(chunk * S::kGroups + group, a.groups - 1);
+    const bool mine = q * S::kGroups / 4 == group && local < S::kTokens;
+
+    // The digits of chunks [begin, begin + n).
+    const auto fill = [&](int begin, int n) {
+        for (int i = threadIdx.x; i < tokens * n * 16; i += kThreads) {  // whole rows of 16 lanes
+            const int t = i & 15, token = i / (16 * n), at = (i >> 4) - token * n;
+            uint32_t even[kDigits], odd[kDigits];
+            int sum[kDigits];
+            float unit;
+            digits_of<G>(a, first + token, begin + at, t, even, odd, sum, unit);
+            const int block = token / S::kTokens, in_block = token - block * S::kTokens;
+            float power = 1.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int64_t s = min(row0 + 4 * q + i, a.outs - 1) * a.groups + g;
-                    const int zero = a.zeros ? a.zeros[s] : 8;
-                    acc[i] += nq::load_f32(a.scales, a.scale_dtype, s) * unit * static_cast<float>(dot[i] - zero * sum);
+            for (int d = 0; d < kDigits; ++d) {
+                uint32_t* to = reinterpret_cast<uint32_t*>(digits + (token * kDigits + d) * line + at * kChunk);
+                to[t] = even[d];
+                to[16 + t] = odd[d];
+                if (t % (G / 8) == 0)
+                    columns[(at * NB + block) * 16 + t / (G / 8) * S::kColumns + in_block * kDigits + d] =
+                        Column{unit * power, static_cast<float>(sum[d])};
+                power *= 256.0f;
+            }
+        }
+    };
+    // Columns that no token has.
+    for (int i = threadIdx.x; i < a.stage * NB * 16; i += kThreads) {
+        const int at = i & 15, t = at % S::kColumns / kDigits;
+        if (t >= S::kTokens || (i >> 4) % NB * S::kTokens + t >= tokens) columns[i] = Column{0.0f, 0.0f};
+    }
+
+    for (int64_t tile0 = static_cast<int64_t>(blockIdx.x) * (kWaves / a.share); tile0 < a.tiles; tile0 += a.step) {
+        const int64_t tile = tile0 + wave / a.share, row0 = min(tile, a.tiles - 1) * 16;
+        const uint8_t* row = a.packed + min(row0 + c, a.outs - 1) * half;
+        const int64_t scale_row = min(row0 + c, a.outs - 1) * a.groups;
+        float acc[NB][4];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[b][i] = 0.0f;
+        for (int begin = chunk0; begin < chunk1; begin += a.stage) {
+            const int n = min(a.stage, chunk1 - begin);
+            if (tile0 == static_cast<int64_t>(blockIdx.x) * (kWaves / a.share) || a.stage < a.slice) {
+                if (begin != chunk0 || a.stage < a.slice) __syncthreads();  // the stage before is read
+                fill(begin, n);
+                __syncthreads();
+            }
+            // This wave's chunks [at, end) of the stage.
+            const int per = (n + a.share - 1) / a.share, end = min(n, (part + 1) * per);
+            u32x4 w[kAtOnce];
+            const auto load = [&](int at) {
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j)
+                    w[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(
+                        row + min(static_cast<int64_t>(begin + at + j) * 64 + 16 * q, half - 16)));
+            };
+            if (part * per < end) load(part * per);
+            for (int at = part * per; at < end; at += kAtOnce) {
+                // Scales and zeros of these chunks: lane 16 q + r loads a quarter of row r's.
+#pragma unroll
+                for (int j = 0; j < kMost / 4; ++j) {
+                    const int k = q * (kMost / 4) + j, g = min((begin + at) * S::kGroups + k, a.groups - 1);
+                    scales[k * 16 + c] = nq::load_f32(a.scales, a.scale_dtype, scale_row + g);
+                    if (a.zeros) zeros[k * 16 + c] = a.zeros[scale_row + g];
+                }
+                u32x4 now[kAtOnce];
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) now[j] = w[j];
+                if (at + kAtOnce < end) load(at + kAtOnce);
+                wave_sync();
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    if (at + j >= end) break;
+                    const u32x4 low = now[j] & 0x0f0f0f0fu, high = (now[j] >> 4) & 0x0f0f0f0fu;
+                    const f32x4 s = *reinterpret_cast<const f32x4*>(scales + (j * S::kGroups + group) * 16 + 4 * q);
+                    const uint32_t z = a.zeros ? *reinterpret_cast<const uint32_t*>(zeros + (j * S::kGroups + group) * 16 + 4 * q)
+                                               : 0x08080808u;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const int token = b * S::kTokens + local;
+                        const uint8_t* from = mine && token < tokens ? digits + (token * kDigits + digit) * line + (at + j) * kChunk + 16 * q
+                                                                     : reinterpret_cast<const uint8_t*>(lds);
+                        const int odd = mine && token < tokens ? 64 : 0;
+                        i32x4 dot = {0, 0, 0, 0};
+                        dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, low),
+                                                                    *reinterpret_cast<const i32x4*>(from), dot, 0, 0, 0);
+                        dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, high),
+                                                                    *reinterpret_cast<const i32x4*>(from + odd), dot, 0, 0, 0);
+                        const Column col = columns[((at + j) * NB + b) * 16 + c];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            // Whole numbers below 2^24: exact.
+                            const float zero = static_cast<float>(z >> (8 * i) & 255u);
+                            const float t = fmaf(-zero, col.sum, static_cast<float>(dot[i]));
+                            acc[b][i] = fmaf(s[i] * col.unit, t, acc[b][i]);
+                        }
+                    }
+                }
+                wave_sync();
+            }
+        }
+        // A token's columns meet in LDS: lane 16 t + r sums token t's of row r.
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (a.share > 1) __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[(4 * q + i) * 17 + c] = acc[b][i];
+            if (a.share > 1) __syncthreads();
+            else wave_sync();
+            if (part == 0) {
+                for (int t = q; t < S::kTokens; t += 4) {
+                    const int token = b * S::kTokens + t;
+                    if (token >= tokens) break;
+                    float y = 0.0f;
+                    for (int d = kDigits - 1; d >= 0; --d)
+                        for (int k = 0; k < S::kGroups; ++k)
+                            for (int o = 0; o < a.share; ++o) y += sums[o * kEach + c * 17 + k * S::kColumns + t * kDigits + d];
+                    const bool there = tile < a.tiles && row0 + c < a.outs;
+                    if (a.partial) {
+                        if (there) a.partial[(static_cast<int64_t>(blockIdx.y) * a.tokens + first + token) * a.outs + row0 + c] = y;
+                    } else {
+                        if (there) nq::store_f32_as(a.y, a.y_dtype, static_cast<int64_t>(first + token) * a.outs + row0 + c, y);
+                        if (a.best) {
+                            const uint64_t top = best_of_tile(there ? order_of(y, static_cast<uint32_t>(row0 + c)) : 0);
+                            if (c == 0 && tile < a.tiles) a.best[tile] = top;
+                        }
+                    }
                 }
             }
+            wave_sync();
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) join[wave][4 * q + i][c] = on ? acc[i] : 0.0f;
-        __syncthreads();
-        // Thread 16 t + r: token first + t, row r.
-        const int r = threadIdx.x & 15, t = threadIdx.x >> 4;
-        if (t < S::kTokens && first + t < a.tokens) {
-            float y = 0.0f;
-#pragma unroll
-            for (int d = kDigits - 1; d >= 0; --d)
-#pragma unroll
-                for (int s = 0; s < S::kGroups; ++s)
-#pragma unroll
-                    for (int w = 0; w < kWaves; ++w) y += join[w][r][s * S::kColumns + t * kDigits + d];
-            const bool there = row0 + r < a.outs;
-            if (there) nq::store_f32_as(a.y, a.y_dtype, static_cast<int64_t>(first + t) * a.outs + row0 + r, y);
-            if (a.best && t == 0) keys[r] = there ? order_of(y, static_cast<uint32_t>(row0 + r)) : 0;
-        }
-        __syncthreads();
     }
-    if (a.best && threadIdx.x == 0) {
-        uint64_t top = keys[0];
-        for (int r = 1; r < 16; ++r) top = keys[r] > top ? keys[r] : top;
-        a.best[blockIdx.x] = top;
+}
+
+// The slices' sums, in order; 16 lanes have a tile.
+__global__ __launch_bounds__(256) void k_int4_join(const Int4Args a, int slices) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int token = blockIdx.y;
+    float y = 0.0f;
+    if (row < a.outs) {
+        for (int i = 0; i < slices; ++i) y += a.partial[(static_cast<int64_t>(i) * a.tokens + token) * a.outs + row];
+        nq::store_f32_as(a.y, a.y_dtype, token * a.outs + row, y);
+    }
+    if (a.best) {
+        const uint64_t top = best_of_tile(row < a.outs ? order_of(y, static_cast<uint32_t>(row)) : 0);
+        if ((threadIdx.x & 15) == 0 && row < a.outs) a.best[row / 16] = top;
     }
 }
 
 int64_t chunks_of(int64_t ins) { return (ins + kChunk - 1) / kChunk; }
 
-template <int G>
-int launch_for(const Int4Args& a, hipStream_t stream) {
-    const dim3 pre(static_cast<unsigned>((a.chunks + 15) / 16), static_cast<unsigned>(a.tokens));
-    hipLaunchKernelGGL(k_int4_digits<G>, pre, dim3(256), 0, stream, a);
-    if (const int st = nq::launch_status(); st != NQ_OK) return st;
-    hipLaunchKernelGGL(k_int4_product<G>, dim3(static_cast<unsigned>((a.outs + 15) / 16)), dim3(kWaves * kWave), 0, stream, a);
+size_t lds_bytes(int tokens, int blocks, int groups, int stage) {
+    const int most = kAtOnce * groups;
+    return 64 + static_cast<size_t>(tokens) * kDigits * line_bytes(stage) + static_cast<size_t>(stage) * blocks * 16 * sizeof(Column) +
+           kWaves * (most * 16 + most * 4 + 16 * 17) * sizeof(float);
+}
+
+Int4Plan plan_int4(int64_t tokens, int64_t outs, int64_t ins, int group) {
+    constexpr size_t kBudget = 60 * 1024;
+    const int groups = kChunk / group, each = 16 / groups / kDigits;
+    const int64_t blocks = (tokens + each - 1) / each, chunks = chunks_of(ins), tiles = (outs + 15) / 16;
+    Int4Plan p{};
+    p.passes = static_cast<int>((blocks + 5) / 6);
+    const int64_t at_once = (blocks + p.passes - 1) / p.passes;
+    p.blocks = at_once <= 3 ? static_cast<int>(at_once) : 6;
+    p.passes = static_cast<int>((blocks + p.blocks - 1) / p.blocks);
+    const int held = static_cast<int>(std::min<int64_t>(tokens, int64_t{p.blocks} * each));
+    // Chunks whose digits LDS holds at once.
+    const size_t fixed = lds_bytes(held, p.blocks, groups, 0), each_chunk = lds_bytes(held, p.blocks, groups, 1) - fixed;
+    const int most = static_cast<int>(std::min<int64_t>(chunks, std::max<int64_t>(1, static_cast<int64_t>((kBudget - std::min(fixed, kBudget)) / each_chunk))));
+    p.slices = 1;
+    p.share = tiles * p.passes >= 2048 ? 1 : 4;
+    if (most < chunks && tiles * p.passes < 2048) {
+        // Digits that LDS does not hold at once, and few tiles: slices.
+        p.share = 1;
+        const int64_t want = (2048 + tiles * p.passes - 1) / (tiles * p.passes);
+        p.slices = static_cast<int>(std::min<int64_t>({16, chunks, std::max<int64_t>(want, 1)}));
+    }
+    p.slice = static_cast<int>((chunks + p.slices - 1) / p.slices);
+    p.slices = static_cast<int>((chunks + p.slice - 1) / p.slice);
+    const int stages = (p.slice + most - 1) / most;
+    p.stage = (p.slice + stages - 1) / stages;
+    const int64_t per = kWaves / p.share, all = (tiles + per - 1) / per;
+    // Digits made once serve several tiles.
+    p.groups = stages == 1 ? std::min<int64_t>(all, std::max<int64_t>(1, 1024 / (int64_t{p.passes} * p.slices))) : all;
+    return p;
+}
+
+template <int G, int NB>
+int launch_as(const Int4Args& a, const Int4Plan& p, hipStream_t stream) {
+    const int held = std::min(a.tokens, NB * Shape<G>::kTokens);
+    const dim3 grid(static_cast<unsigned>(p.groups), static_cast<unsigned>(p.slices), static_cast<unsigned>(p.passes));
+    hipLaunchKernelGGL((k_int4_product<G, NB>), grid, dim3(kThreads), lds_bytes(held, NB, Shape<G>::kGroups, a.stage), stream, a);
     return nq::launch_status();
+}
+
+template <int G>
+int launch_for(const Int4Args& a, const Int4Plan& p, hipStream_t stream) {
+    switch (p.blocks) {
+        case 1: return launch_as<G, 1>(a, p, stream);
+        case 2: return launch_as<G, 2>(a, p, stream);
+        case 3: return launch_as<G, 3>(a, p, stream);
+        default: return launch_as<G, 6>(a, p, stream);
+    }
 }
 
 }  // namespace
@@ -190,10 +369,9 @@ extern "C" int64_t nq_int4_projection_workspace_bytes(int64_t tokens, int64_t ou
     if (tokens <= 0 || tokens > 65535 || out_features <= 0 || out_features > 0x7fffffff || in_features <= 0 || in_features % 32 ||
         in_features > (1 << 24) || (group != 32 && group != 64 && group != 128))
         return -1;
-    if (!nq::launchable((out_features + 15) / 16, kWaves * kWave)) return -1;
-    if (!nq::launchable((chunks_of(in_features) + 15) / 16 * tokens, 256)) return -1;
-    // Digits, their sums, and an exponent for each token and group.
-    return tokens * chunks_of(in_features) * (kDigits * kChunk + (kDigits + 1) * 4 * 4);
+    const Int4Plan p = plan_int4(tokens, out_features, in_features, group);
+    if (!nq::launchable(p.groups * p.slices * p.passes, kThreads)) return -1;
+    return p.slices == 1 ? 0 : p.slices * tokens * out_features * static_cast<int64_t>(sizeof(float));
 }
 
 extern "C" int64_t nq_int4_projection_partials(int64_t out_features) { return out_features <= 0 ? -1 : (out_features + 15) / 16; }
@@ -202,35 +380,45 @@ extern "C" int nq_int4_projection(const void* x, int32_t x_dtype, int64_t tokens
                                   int32_t scale_dtype, const uint8_t* zeros, int64_t out_features, int64_t in_features,
                                   int32_t group, void* y, int32_t y_dtype, void* partials, void* workspace,
                                   int64_t workspace_bytes, void* stream) {
-    if (!x || !packed || !scales || !y || !workspace) return NQ_ERR_ARGUMENT;
+    if (!x || !packed || !scales || !y) return NQ_ERR_ARGUMENT;
     if (!nq::is_float_dtype(x_dtype) || !nq::is_float_dtype(scale_dtype) || !nq::is_float_dtype(y_dtype)) return NQ_ERR_DTYPE;
     const int64_t need = nq_int4_projection_workspace_bytes(tokens, out_features, in_features, group);
     if (need < 0 || (partials && tokens != 1)) return NQ_ERR_SHAPE;
+    if (need > 0 && !workspace) return NQ_ERR_ARGUMENT;
     if (workspace_bytes < need) return NQ_ERR_WORKSPACE;
     if ((reinterpret_cast<uintptr_t>(packed) | reinterpret_cast<uintptr_t>(workspace)) & 15) return NQ_ERR_ALIGNMENT;
     if (reinterpret_cast<uintptr_t>(partials) & 7) return NQ_ERR_ALIGNMENT;
+    const Int4Plan p = plan_int4(tokens, out_features, in_features, group);
     Int4Args a{};
     a.x = x;
     a.packed = static_cast<const uint8_t*>(packed);
     a.scales = scales;
     a.zeros = zeros;
     a.y = y;
+    a.partial = p.slices > 1 ? static_cast<float*>(workspace) : nullptr;
     a.best = static_cast<uint64_t*>(partials);
     a.outs = out_features;
     a.ins = in_features;
+    a.tiles = (out_features + 15) / 16;
+    a.step = p.groups * (kWaves / p.share);
     a.tokens = static_cast<int32_t>(tokens);
     a.chunks = static_cast<int32_t>(chunks_of(in_features));
     a.groups = static_cast<int32_t>((in_features + group - 1) / group);
     a.x_dtype = x_dtype;
     a.scale_dtype = scale_dtype;
     a.y_dtype = y_dtype;
-    a.digits = static_cast<uint8_t*>(workspace);
-    a.units = reinterpret_cast<float*>(a.digits + tokens * a.chunks * kDigits * kChunk);
-    a.sums = reinterpret_cast<int32_t*>(a.units + tokens * a.chunks * 4);
+    a.share = p.share;
+    a.slice = p.slice;
+    a.stage = p.stage;
     hipStream_t st = static_cast<hipStream_t>(stream);
+    int status;
     switch (group) {
-        case 32: return launch_for<32>(a, st);
-        case 64: return launch_for<64>(a, st);
-        default: return launch_for<128>(a, st);
+        case 32: status = launch_for<32>(a, p, st); break;
+        case 64: status = launch_for<64>(a, p, st); break;
+        default: status = launch_for<128>(a, p, st); break;
     }
+    if (status != NQ_OK || p.slices == 1) return status;
+    const dim3 grid(static_cast<unsigned>((out_features + 255) / 256), static_cast<unsigned>(tokens));
+    hipLaunchKernelGGL(k_int4_join, grid, dim3(256), 0, st, a, p.slices);
+    return nq::launch_status();
 }
