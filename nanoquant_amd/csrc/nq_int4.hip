@@ -42,7 +42,7 @@ struct Int4Args {
     float* partial;          // [slices][tokens][outs] where the slices are joined in a second launch
     uint64_t* best;          // [tiles] largest value and its row, of one token; may be null
     int64_t outs, ins, tiles, step;  // step: tiles from one of a wave's to its next
-    int32_t tokens, chunks, groups, x_dtype, scale_dtype, y_dtype;
+    int32_t tokens, chunks, groups, x_dtype, y_dtype;
     int32_t share, slice, stage;
 };
 
@@ -77,11 +77,16 @@ __device__ __forceinline__ void wave_sync() {
 }
 
 constexpr int kWaves = 4, kThreads = kWaves * kWave;
-constexpr int kAtOnce = 4;  // chunks whose weights a wave loads at once
+constexpr int kAhead = 2;   // rounds of x
+constexpr int kAtOnce = 4;  // chunks whose weights a wave loads at once: 256 bytes of each of 16 rows
 
 // Digits in LDS: a line of `stage` chunks, [2][64] bytes each (even and odd columns), for each token and
 // digit; 64 bytes more a line, so that a product's columns lie in different banks.
 __host__ __device__ constexpr int line_bytes(int stage) { return stage * kChunk + 64; }
+
+// Words of LDS that each wave has for itself.
+template <int GROUPS>
+constexpr int kEachWave = 16 * 16 * 4 + 16 * 17 + kAtOnce * GROUPS * (16 + 4);
 
 // A column of B in a chunk: what a product with it is multiplied by, but for the
 // row's scale, and the sum of its digits.
@@ -89,16 +94,51 @@ struct Column {
     float unit, sum;
 };
 
+// A 16-bit value's bits as fp32.
+__device__ __forceinline__ float from_half(uint32_t bits, int dtype) {
+    return dtype == NQ_DTYPE_BF16 ? __uint_as_float(bits << 16)
+                                  : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+}
+
+// Eight adjacent values' bits, at any address that fits their type.
+struct Eight {
+    uint32_t w[8];
+};
+
+__device__ __forceinline__ Eight load8(const void* p, int dtype, int64_t i) {
+    Eight v;
+    if (dtype == NQ_DTYPE_F32) {
+        typedef uint32_t vec __attribute__((ext_vector_type(4), aligned(4)));
+        const vec* from = reinterpret_cast<const vec*>(static_cast<const uint32_t*>(p) + i);
+        const vec x0 = from[0], x1 = from[1];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v.w[j] = j < 4 ? x0[j & 3] : x1[j & 3];
+    } else {
+        typedef uint32_t vec __attribute__((ext_vector_type(4), aligned(2)));
+        const vec x = *reinterpret_cast<const vec*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v.w[j] = x[j & 3];
+    }
+    return v;
+}
+
+__device__ __forceinline__ void widen8(const Eight& v, int dtype, float (&x)[8]) {
+    if (dtype == NQ_DTYPE_F32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(v.w[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = from_half(v.w[j / 2] >> (16 * (j & 1)) & 0xffffu, dtype);
+    }
+}
+
 // Eight adjacent columns of a token as digits.
 template <int G>
-__device__ __forceinline__ void digits_of(const Int4Args& a, int token, int chunk, int t, uint32_t (&even)[kDigits],
-                                          uint32_t (&odd)[kDigits], int (&sum)[kDigits], float& unit) {
+__device__ __forceinline__ void digits_of(const float (&x)[8], uint32_t (&even)[kDigits], uint32_t (&odd)[kDigits],
+                                          int (&sum)[kDigits], float& unit) {
     constexpr int kGroup = G / 8;  // lanes of a group
-    float x[8], most = 0.0f;
+    float most = 0.0f;
     bool finite = true;
-    const int64_t at = static_cast<int64_t>(chunk) * kChunk + 8 * t;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = at < a.ins ? nq::load_f32(a.x, a.x_dtype, token * a.ins + at + j) : 0.0f;  // ins: a multiple of 32
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         finite = finite && fabsf(x[j]) < INFINITY;
@@ -134,12 +174,12 @@ __device__ __forceinline__ void digits_of(const Int4Args& a, int token, int chun
 
 // A workgroup has a slice of the chunks and, share waves to a tile of 16 rows, kWaves / share tiles
 // at a time; the waves of a tile each take a part of a stage's chunks. NB blocks of tokens.
-template <int G, int NB>
-__global__ __launch_bounds__(kThreads) void k_int4_product(const Int4Args a) {
+template <int G, int NB, int ST>
+__global__ __launch_bounds__(kThreads, NB <= 3 ? 3 : 2) void k_int4_product(const Int4Args a) {
     using S = Shape<G>;
     constexpr int kMost = kAtOnce * S::kGroups;  // groups whose scales a wave holds in LDS
     extern __shared__ u32x4 lds[];
-    // Zeros, digits, columns; for each wave scales [kMost][16], zeros [kMost][16] and sums [16][17].
+    // Zeros, digits, columns; for each wave 16 rows' units, sums [16][17], scales [kMost][16] and zeros [kMost][16].
     uint8_t* digits = reinterpret_cast<uint8_t*>(lds) + 64;
     const int first = blockIdx.z * NB * S::kTokens, tokens = min(NB * S::kTokens, a.tokens - first);
     const int line = line_bytes(a.stage);
@@ -147,11 +187,12 @@ __global__ __launch_bounds__(kThreads) void k_int4_product(const Int4Args a) {
     float* mine_f = reinterpret_cast<float*>(columns + a.stage * NB * 16);
     const int lane = threadIdx.x & (kWave - 1), c = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    constexpr int kEach = kMost * 16 + kMost * 4 + 16 * 17;
-    float* sums = mine_f + wave * kEach;
+    constexpr int kRow = S::kColumns + 1;  // a row's sums, in another bank than the next one's
+    constexpr int kEach = kEachWave<S::kGroups>;
+    u32x4* units = reinterpret_cast<u32x4*>(mine_f + wave * kEach);
+    float* sums = reinterpret_cast<float*>(units + 16 * 16);
     float* scales = sums + 16 * 17;
     uint8_t* zeros = reinterpret_cast<uint8_t*>(scales + kMost * 16);
-    // (sums lie at 16 * 17 words, so that scales are 16-byte aligned.)
     if (threadIdx.x < 16) reinterpret_cast<uint32_t*>(lds)[threadIdx.x] = 0;
 
     const int chunk0 = blockIdx.y * a.slice, chunk1 = min(chunk0 + a.slice, a.chunks);
@@ -160,14 +201,25 @@ __global__ __launch_bounds__(kThreads) void k_int4_product(const Int4Args a) {
     const int group = c / S::kColumns, in_group = c % S::kColumns, local = in_group / kDigits, digit = in_group % kDigits;
     const bool mine = q * S::kGroups / 4 == group && local < S::kTokens;
 
-    // The digits of chunks [begin, begin + n).
+    // The digits of chunks [begin, begin + n), eight columns of a token to a thread and round. The
+    // first rounds' columns are loaded before the weights, which take longer.
+    Eight ahead[kAhead];
+    const auto bits_at = [&](int begin, int n, int i) {
+        const int token = tokens == 1 ? 0 : i / (16 * n);
+        const int64_t at = static_cast<int64_t>(begin + (i >> 4) - token * n) * kChunk + 8 * (i & 15);
+        Eight v = {};
+        if (i < tokens * n * 16 && at < a.ins) v = load8(a.x, a.x_dtype, (first + token) * a.ins + at);  // ins is a multiple of 32
+        return v;
+    };
     const auto fill = [&](int begin, int n) {
-        for (int i = threadIdx.x; i < tokens * n * 16; i += kThreads) {  // whole rows of 16 lanes
-            const int t = i & 15, token = i / (16 * n), at = (i >> 4) - token * n;
+        const auto round = [&](int i, const Eight& bits) {
+            const int t = i & 15, token = tokens == 1 ? 0 : i / (16 * n), at = (i >> 4) - token * n;
+            float x[8];
             uint32_t even[kDigits], odd[kDigits];
             int sum[kDigits];
             float unit;
-            digits_of<G>(a, first + token, begin + at, t, even, odd, sum, unit);
+            widen8(bits, a.x_dtype, x);
+            digits_of<G>(x, even, odd, sum, unit);
             const int block = token / S::kTokens, in_block = token - block * S::kTokens;
             float power = 1.0f;
 #pragma unroll
@@ -180,7 +232,14 @@ __global__ __launch_bounds__(kThreads) void k_int4_product(const Int4Args a) {
                         Column{unit * power, static_cast<float>(sum[d])};
                 power *= 256.0f;
             }
+        };
+        const int all = tokens * n * 16;  // whole rows of 16 lanes
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int i = threadIdx.x + j * kThreads;
+            if (i < all) round(i, ahead[j]);
         }
+        for (int i = threadIdx.x + kAhead * kThreads; i < all; i += kThreads) round(i, bits_at(begin, n, i));
     };
     // Columns that no token has.
     for (int i = threadIdx.x; i < a.stage * NB * 16; i += kThreads) {
@@ -190,7 +249,9 @@ __global__ __launch_bounds__(kThreads) void k_int4_product(const Int4Args a) {
 
     for (int64_t tile0 = static_cast<int64_t>(blockIdx.x) * (kWaves / a.share); tile0 < a.tiles; tile0 += a.step) {
         const int64_t tile = tile0 + wave / a.share, row0 = min(tile, a.tiles - 1) * 16;
-        const uint8_t* row = a.packed + min(row0 + c, a.outs - 1) * half;
+        const uint8_t* row[4];  // lane 16 g + u loads 16-byte unit u of rows g, 4 + g, 8 + g and 12 + g
+#pragma unroll
+        for (int j = 0; j < 4; ++j) row[j] = a.packed + min(row0 + 4 * j + q, a.outs - 1) * half;
         const int64_t scale_row = min(row0 + c, a.outs - 1) * a.groups;
         float acc[NB][4];
 #pragma unroll
@@ -199,41 +260,61 @@ __global__ __launch_bounds__(kThreads) void k_int4_product(const Int4Args a) {
             for (int i = 0; i < 4; ++i) acc[b][i] = 0.0f;
         for (int begin = chunk0; begin < chunk1; begin += a.stage) {
             const int n = min(a.stage, chunk1 - begin);
-            if (tile0 == static_cast<int64_t>(blockIdx.x) * (kWaves / a.share) || a.stage < a.slice) {
+            // This wave's chunks [at, end) of the stage. Weights, scales and zeros (lane 16 q + r
+            // loads a quarter of row r's) are on their way while those before are worked on.
+            const int per = (n + a.share - 1) / a.share, end = min(n, (part + 1) * per);
+            u32x4 w[4];
+            uint32_t s_next[kMost / 4];
+            uint8_t z_next[kMost / 4] = {};
+            const auto load = [&](int at) {
+                const auto g = [&](int j) { return scale_row + min((begin + at) * S::kGroups + q * (kMost / 4) + j, a.groups - 1); };
+                if constexpr (ST == NQ_DTYPE_F32) {
+#pragma unroll
+                    for (int j = 0; j < kMost / 4; ++j) s_next[j] = static_cast<const uint32_t*>(a.scales)[g(j)];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kMost / 4; ++j) s_next[j] = static_cast<const uint16_t*>(a.scales)[g(j)];
+                }
+                if (a.zeros) {
+#pragma unroll
+                    for (int j = 0; j < kMost / 4; ++j) z_next[j] = a.zeros[g(j)];
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    w[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(
+                        row[j] + min(static_cast<int64_t>(begin + at) * 64 + 16 * c, half - 16)));
+            };
+            const bool fills = tile0 == static_cast<int64_t>(blockIdx.x) * (kWaves / a.share) || a.stage < a.slice;
+            if (fills) {
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) ahead[j] = bits_at(begin, n, threadIdx.x + j * kThreads);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (part * per < end) load(part * per);
+            if (fills) {
                 if (begin != chunk0 || a.stage < a.slice) __syncthreads();  // the stage before is read
                 fill(begin, n);
                 __syncthreads();
             }
-            // This wave's chunks [at, end) of the stage.
-            const int per = (n + a.share - 1) / a.share, end = min(n, (part + 1) * per);
-            u32x4 w[kAtOnce];
-            const auto load = [&](int at) {
-#pragma unroll
-                for (int j = 0; j < kAtOnce; ++j)
-                    w[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(
-                        row + min(static_cast<int64_t>(begin + at + j) * 64 + 16 * q, half - 16)));
-            };
-            if (part * per < end) load(part * per);
             for (int at = part * per; at < end; at += kAtOnce) {
-                // Scales and zeros of these chunks: lane 16 q + r loads a quarter of row r's.
 #pragma unroll
                 for (int j = 0; j < kMost / 4; ++j) {
-                    const int k = q * (kMost / 4) + j, g = min((begin + at) * S::kGroups + k, a.groups - 1);
-                    scales[k * 16 + c] = nq::load_f32(a.scales, a.scale_dtype, scale_row + g);
-                    if (a.zeros) zeros[k * 16 + c] = a.zeros[scale_row + g];
+                    scales[(q * (kMost / 4) + j) * 16 + c] =
+                        ST == NQ_DTYPE_F32 ? __uint_as_float(s_next[j]) : from_half(s_next[j], ST);
+                    zeros[(q * (kMost / 4) + j) * 16 + c] = a.zeros ? z_next[j] : 8;
                 }
-                u32x4 now[kAtOnce];
+                // Unit u of row r lies at r's place u ^ r: the products' lanes read 16 rows from 16 places.
 #pragma unroll
-                for (int j = 0; j < kAtOnce; ++j) now[j] = w[j];
+                for (int j = 0; j < 4; ++j) units[(4 * j + q) * 16 + (c ^ (4 * j + q))] = w[j];
                 if (at + kAtOnce < end) load(at + kAtOnce);
                 wave_sync();
 #pragma unroll
                 for (int j = 0; j < kAtOnce; ++j) {
                     if (at + j >= end) break;
-                    const u32x4 low = now[j] & 0x0f0f0f0fu, high = (now[j] >> 4) & 0x0f0f0f0fu;
+                    const u32x4 now = units[c * 16 + ((4 * j + q) ^ c)];
+                    const u32x4 low = now & 0x0f0f0f0fu, high = (now >> 4) & 0x0f0f0f0fu;
                     const f32x4 s = *reinterpret_cast<const f32x4*>(scales + (j * S::kGroups + group) * 16 + 4 * q);
-                    const uint32_t z = a.zeros ? *reinterpret_cast<const uint32_t*>(zeros + (j * S::kGroups + group) * 16 + 4 * q)
-                                               : 0x08080808u;
+                    const uint32_t z = *reinterpret_cast<const uint32_t*>(zeros + (j * S::kGroups + group) * 16 + 4 * q);
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
                         const int token = b * S::kTokens + local;
@@ -258,22 +339,33 @@ __global__ __launch_bounds__(kThreads) void k_int4_product(const Int4Args a) {
                 wave_sync();
             }
         }
-        // A token's columns meet in LDS: lane 16 t + r sums token t's of row r.
+        // The groups' columns are added in registers, a token's digits and the waves of a tile in
+        // LDS: lane 16 t + r has token t's of row r.
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            if (a.share > 1) __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sums[(4 * q + i) * 17 + c] = acc[b][i];
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int m = S::kColumns; m < 16; m *= 2) acc[b][i] += __shfl_xor(acc[b][i], m, kWave);
+            if (a.share > 1) __syncthreads();
+            if (c < S::kColumns) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sums[(4 * q + i) * kRow + c] = acc[b][i];
+            }
             if (a.share > 1) __syncthreads();
             else wave_sync();
             if (part == 0) {
-                for (int t = q; t < S::kTokens; t += 4) {
-                    const int token = b * S::kTokens + t;
-                    if (token >= tokens) break;
+#pragma unroll
+                for (int t0 = 0; t0 < S::kTokens; t0 += 4) {
+                    const int t = t0 + q, token = b * S::kTokens + t;
+                    if (t >= S::kTokens || token >= tokens) break;
                     float y = 0.0f;
-                    for (int d = kDigits - 1; d >= 0; --d)
-                        for (int k = 0; k < S::kGroups; ++k)
-                            for (int o = 0; o < a.share; ++o) y += sums[o * kEach + c * 17 + k * S::kColumns + t * kDigits + d];
+#pragma unroll
+                    for (int o = 0; o < kWaves; ++o) {
+                        if (o >= a.share) break;
+#pragma unroll
+                        for (int d = kDigits - 1; d >= 0; --d) y += sums[o * kEach + c * kRow + t * kDigits + d];
+                    }
                     const bool there = tile < a.tiles && row0 + c < a.outs;
                     if (a.partial) {
                         if (there) a.partial[(static_cast<int64_t>(blockIdx.y) * a.tokens + first + token) * a.outs + row0 + c] = y;
@@ -309,9 +401,9 @@ __global__ __launch_bounds__(256) void k_int4_join(const Int4Args a, int slices)
 int64_t chunks_of(int64_t ins) { return (ins + kChunk - 1) / kChunk; }
 
 size_t lds_bytes(int tokens, int blocks, int groups, int stage) {
-    const int most = kAtOnce * groups;
+    const int wave = groups == 1 ? kEachWave<1> : groups == 2 ? kEachWave<2> : kEachWave<4>;
     return 64 + static_cast<size_t>(tokens) * kDigits * line_bytes(stage) + static_cast<size_t>(stage) * blocks * 16 * sizeof(Column) +
-           kWaves * (most * 16 + most * 4 + 16 * 17) * sizeof(float);
+           static_cast<size_t>(kWaves) * wave * sizeof(float);
 }
 
 Int4Plan plan_int4(int64_t tokens, int64_t outs, int64_t ins, int group) {
@@ -341,25 +433,34 @@ Int4Plan plan_int4(int64_t tokens, int64_t outs, int64_t ins, int group) {
     p.stage = (p.slice + stages - 1) / stages;
     const int64_t per = kWaves / p.share, all = (tiles + per - 1) / per;
     // Digits made once serve several tiles.
-    p.groups = stages == 1 ? std::min<int64_t>(all, std::max<int64_t>(1, 1024 / (int64_t{p.passes} * p.slices))) : all;
+    p.groups = stages == 1 ? std::min<int64_t>(all, std::max<int64_t>(1, 768 / (int64_t{p.passes} * p.slices))) : all;
     return p;
 }
 
-template <int G, int NB>
+template <int G, int NB, int ST>
 int launch_as(const Int4Args& a, const Int4Plan& p, hipStream_t stream) {
     const int held = std::min(a.tokens, NB * Shape<G>::kTokens);
     const dim3 grid(static_cast<unsigned>(p.groups), static_cast<unsigned>(p.slices), static_cast<unsigned>(p.passes));
-    hipLaunchKernelGGL((k_int4_product<G, NB>), grid, dim3(kThreads), lds_bytes(held, NB, Shape<G>::kGroups, a.stage), stream, a);
+    hipLaunchKernelGGL((k_int4_product<G, NB, ST>), grid, dim3(kThreads), lds_bytes(held, NB, Shape<G>::kGroups, a.stage), stream, a);
     return nq::launch_status();
 }
 
+template <int G, int NB>
+int launch_with(const Int4Args& a, const Int4Plan& p, int scale_dtype, hipStream_t stream) {
+    switch (scale_dtype) {
+        case NQ_DTYPE_F32: return launch_as<G, NB, NQ_DTYPE_F32>(a, p, stream);
+        case NQ_DTYPE_F16: return launch_as<G, NB, NQ_DTYPE_F16>(a, p, stream);
+        default: return launch_as<G, NB, NQ_DTYPE_BF16>(a, p, stream);
+    }
+}
+
 template <int G>
-int launch_for(const Int4Args& a, const Int4Plan& p, hipStream_t stream) {
+int launch_for(const Int4Args& a, const Int4Plan& p, int scale_dtype, hipStream_t stream) {
     switch (p.blocks) {
-        case 1: return launch_as<G, 1>(a, p, stream);
-        case 2: return launch_as<G, 2>(a, p, stream);
-        case 3: return launch_as<G, 3>(a, p, stream);
-        default: return launch_as<G, 6>(a, p, stream);
+        case 1: return launch_with<G, 1>(a, p, scale_dtype, stream);
+        case 2: return launch_with<G, 2>(a, p, scale_dtype, stream);
+        case 3: return launch_with<G, 3>(a, p, scale_dtype, stream);
+        default: return launch_with<G, 6>(a, p, scale_dtype, stream);
     }
 }
 
@@ -405,7 +506,6 @@ extern "C" int nq_int4_projection(const void* x, int32_t x_dtype, int64_t tokens
     a.chunks = static_cast<int32_t>(chunks_of(in_features));
     a.groups = static_cast<int32_t>((in_features + group - 1) / group);
     a.x_dtype = x_dtype;
-    a.scale_dtype = scale_dtype;
     a.y_dtype = y_dtype;
     a.share = p.share;
     a.slice = p.slice;
@@ -413,9 +513,9 @@ extern "C" int nq_int4_projection(const void* x, int32_t x_dtype, int64_t tokens
     hipStream_t st = static_cast<hipStream_t>(stream);
     int status;
     switch (group) {
-        case 32: status = launch_for<32>(a, p, st); break;
-        case 64: status = launch_for<64>(a, p, st); break;
-        default: status = launch_for<128>(a, p, st); break;
+        case 32: status = launch_for<32>(a, p, scale_dtype, st); break;
+        case 64: status = launch_for<64>(a, p, scale_dtype, st); break;
+        default: status = launch_for<128>(a, p, scale_dtype, st); break;
     }
     if (status != NQ_OK || p.slices == 1) return status;
     const dim3 grid(static_cast<unsigned>((out_features + 255) / 256), static_cast<unsigned>(tokens));
