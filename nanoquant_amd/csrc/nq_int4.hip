@@ -14,6 +14,7 @@
 // 128 / G groups; a group's columns are a few tokens' digits, and zero in the lanes of
 // other groups, so that one product keeps the groups apart.
 #include <algorithm>
+#include <type_traits>
 
 #include "nq_common.h"
 #include "../../include/nqamd_shell.h"
@@ -152,18 +153,22 @@ __device__ __forceinline__ void digits_of(const float (&x)[8], uint32_t (&even)[
     const uint32_t bits = __float_as_uint(most);
     const int k = max(static_cast<int>(bits >> 23) - 127 + ((bits & 0x7fffffu) > 0x7e0000u ? 1 : 0), -100);
     const float up = finite ? __uint_as_float(static_cast<uint32_t>(22 - k + 127) << 23) : 0.0f;
+    // n + 0x808080 has the digits plus 128 each as its bytes: n is at least -2^23 and at
+    // most 2^22 * 1.984375 = 0x7f0000.
+    uint32_t u[8];
 #pragma unroll
-    for (int d = 0; d < kDigits; ++d) even[d] = odd[d] = sum[d] = 0;
+    for (int j = 0; j < 8; ++j) u[j] = static_cast<uint32_t>(finite ? static_cast<int>(rintf(x[j] * up)) : 0) + 0x808080u;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        int n = finite ? static_cast<int>(rintf(x[j] * up)) : 0;
-#pragma unroll
-        for (int d = 0; d < kDigits; ++d) {
-            const int digit = static_cast<int8_t>(n);
-            n = (n - digit) >> 8;
-            sum[d] += digit;
-            (j & 1 ? odd : even)[d] |= static_cast<uint32_t>(digit & 255) << (8 * (j / 2));
-        }
+    for (int d = 0; d < kDigits; ++d) {
+        // Byte d of four values in a word.
+        const uint32_t pair = 0x0c0c0400u + 0x0101u * d;
+        const auto four = [&](uint32_t a, uint32_t b, uint32_t e, uint32_t f) {
+            return (__builtin_amdgcn_perm(b, a, pair) | __builtin_amdgcn_perm(f, e, pair) << 16) ^ 0x80808080u;
+        };
+        even[d] = four(u[0], u[2], u[4], u[6]);
+        odd[d] = four(u[1], u[3], u[5], u[7]);
+        sum[d] = __builtin_amdgcn_sdot4(static_cast<int>(even[d]), 0x01010101,
+                                        __builtin_amdgcn_sdot4(static_cast<int>(odd[d]), 0x01010101, 0, false), false);
     }
 #pragma unroll
     for (int d = 0; d < kDigits; ++d)
@@ -177,6 +182,7 @@ __device__ __forceinline__ void digits_of(const float (&x)[8], uint32_t (&even)[
 template <int G, int NB, int ST>
 __global__ __launch_bounds__(kThreads, NB <= 3 ? 3 : 2) void k_int4_product(const Int4Args a) {
     using S = Shape<G>;
+    constexpr int kTogether = NB <= 2 ? 2 : 1;
     constexpr int kMost = kAtOnce * S::kGroups;  // groups whose scales a wave holds in LDS
     extern __shared__ u32x4 lds[];
     // Zeros, digits, columns; for each wave 16 rows' units, sums [16][17], scales [kMost][16] and zeros [kMost][16].
@@ -200,6 +206,15 @@ __global__ __launch_bounds__(kThreads, NB <= 3 ? 3 : 2) void k_int4_product(cons
     const int64_t half = a.ins / 2;
     const int group = c / S::kColumns, in_group = c % S::kColumns, local = in_group / kDigits, digit = in_group % kDigits;
     const bool mine = q * S::kGroups / 4 == group && local < S::kTokens;
+    // Where this lane's operand of a block begins in LDS, and its odd columns' behind; 0: zeros.
+    int from_at[NB], odd_at[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int token = b * S::kTokens + local;
+        const bool on = mine && token < tokens;
+        from_at[b] = on ? 64 + (token * kDigits + digit) * line + 16 * q : 0;
+        odd_at[b] = on ? 64 : 0;
+    }
 
     // The digits of chunks [begin, begin + n), eight columns of a token to a thread and round. The
     // first rounds' columns are loaded before the weights, which take longer.
@@ -264,7 +279,7 @@ __global__ __launch_bounds__(kThreads, NB <= 3 ? 3 : 2) void k_int4_product(cons
             // loads a quarter of row r's) are on their way while those before are worked on.
             const int per = (n + a.share - 1) / a.share, end = min(n, (part + 1) * per);
             u32x4 w[4];
-            uint32_t s_next[kMost / 4];
+            std::conditional_t<ST == NQ_DTYPE_F32, uint32_t, uint16_t> s_next[kMost / 4];
             uint8_t z_next[kMost / 4] = {};
             const auto load = [&](int at) {
                 const auto g = [&](int j) { return scale_row + min((begin + at) * S::kGroups + q * (kMost / 4) + j, a.groups - 1); };
@@ -308,32 +323,52 @@ __global__ __launch_bounds__(kThreads, NB <= 3 ? 3 : 2) void k_int4_product(cons
                 for (int j = 0; j < 4; ++j) units[(4 * j + q) * 16 + (c ^ (4 * j + q))] = w[j];
                 if (at + kAtOnce < end) load(at + kAtOnce);
                 wave_sync();
+                // Everything that LDS has for a few chunks, then their products: what waits in between
+                // waits once for all.
 #pragma unroll
-                for (int j = 0; j < kAtOnce; ++j) {
-                    if (at + j >= end) break;
-                    const u32x4 now = units[c * 16 + ((4 * j + q) ^ c)];
-                    const u32x4 low = now & 0x0f0f0f0fu, high = (now >> 4) & 0x0f0f0f0fu;
-                    const f32x4 s = *reinterpret_cast<const f32x4*>(scales + (j * S::kGroups + group) * 16 + 4 * q);
-                    const uint32_t z = *reinterpret_cast<const uint32_t*>(zeros + (j * S::kGroups + group) * 16 + 4 * q);
+                for (int j0 = 0; j0 < kAtOnce; j0 += kTogether) {
+                    if (at + j0 >= end) break;
+                    u32x4 now[kTogether];
+                    f32x4 s[kTogether];
+                    uint32_t z[kTogether];
+                    i32x4 x[kTogether][NB][2];
+                    Column col[kTogether][NB];
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const int token = b * S::kTokens + local;
-                        const uint8_t* from = mine && token < tokens ? digits + (token * kDigits + digit) * line + (at + j) * kChunk + 16 * q
-                                                                     : reinterpret_cast<const uint8_t*>(lds);
-                        const int odd = mine && token < tokens ? 64 : 0;
-                        i32x4 dot = {0, 0, 0, 0};
-                        dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, low),
-                                                                    *reinterpret_cast<const i32x4*>(from), dot, 0, 0, 0);
-                        dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, high),
-                                                                    *reinterpret_cast<const i32x4*>(from + odd), dot, 0, 0, 0);
-                        const Column col = columns[((at + j) * NB + b) * 16 + c];
+                    for (int k = 0; k < kTogether; ++k) {
+                        const int j = j0 + k, chunk = min(at + j, end - 1);
+                        now[k] = units[c * 16 + ((4 * j + q) ^ c)];
+                        s[k] = *reinterpret_cast<const f32x4*>(scales + (j * S::kGroups + group) * 16 + 4 * q);
+                        z[k] = *reinterpret_cast<const uint32_t*>(zeros + (j * S::kGroups + group) * 16 + 4 * q);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            // Whole numbers below 2^24: exact.
-                            const float zero = static_cast<float>(z >> (8 * i) & 255u);
-                            const float t = fmaf(-zero, col.sum, static_cast<float>(dot[i]));
-                            acc[b][i] = fmaf(s[i] * col.unit, t, acc[b][i]);
+                        for (int b = 0; b < NB; ++b) {
+                            const uint8_t* from = reinterpret_cast<const uint8_t*>(lds) + (from_at[b] ? from_at[b] + chunk * kChunk : 0);
+                            x[k][b][0] = *reinterpret_cast<const i32x4*>(from);
+                            x[k][b][1] = *reinterpret_cast<const i32x4*>(from + odd_at[b]);
+                            col[k][b] = columns[(chunk * NB + b) * 16 + c];
                         }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int k = 0; k < kTogether; ++k) {
+                        if (at + j0 + k >= end) break;
+                        const u32x4 low = now[k] & 0x0f0f0f0fu, high = (now[k] >> 4) & 0x0f0f0f0fu;
+                        i32x4 dot[NB];
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+                            dot[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, low), x[k][b][0],
+                                                                          i32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+                            dot[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, high), x[k][b][1], dot[b], 0, 0, 0);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                // Whole numbers below 2^24: exact.
+                                const float zero = static_cast<float>(z[k] >> (8 * i) & 255u);
+                                const float t = fmaf(-zero, col[k][b].sum, static_cast<float>(dot[b][i]));
+                                acc[b][i] = fmaf(s[k][i] * col[k][b].unit, t, acc[b][i]);
+                            }
                     }
                 }
                 wave_sync();
