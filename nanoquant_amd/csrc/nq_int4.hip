@@ -30,7 +30,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // How a call is laid out: `blocks` blocks of tokens at once, of each row's chunks a
 // `slice` for a workgroup, in stages of `stage` that LDS holds the digits of.
 struct Int4Plan {
-    int blocks, passes, share, slices, slice, stage;
+    int waves, blocks, passes, share, slices, slice, stage;
     int64_t groups;  // workgroups of a pass and slice
 };
 
@@ -77,7 +77,6 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-constexpr int kWaves = 4, kThreads = kWaves * kWave;
 constexpr int kAhead = 2;   // rounds of x
 constexpr int kAtOnce = 4;  // chunks whose weights a wave loads at once: 256 bytes of each of 16 rows
 
@@ -179,8 +178,9 @@ __device__ __forceinline__ void digits_of(const float (&x)[8], uint32_t (&even)[
 
 // A workgroup has a slice of the chunks and, share waves to a tile of 16 rows, kWaves / share tiles
 // at a time; the waves of a tile each take a part of a stage's chunks. NB blocks of tokens.
-template <int G, int NB, int ST>
-__global__ __launch_bounds__(kThreads, NB <= 3 ? 3 : 2) void k_int4_product(const Int4Args a) {
+template <int G, int NB, int ST, int kWaves>
+__global__ __launch_bounds__(kWaves* kWave, kWaves == 8 ? 1 : NB <= 3 ? 3 : 2) void k_int4_product(const Int4Args a) {
+    constexpr int kThreads = kWaves * kWave;
     using S = Shape<G>;
     constexpr int kTogether = NB <= 2 ? 2 : 1;
     constexpr int kMost = kAtOnce * S::kGroups;  // groups whose scales a wave holds in LDS
@@ -424,7 +424,12 @@ __global__ __launch_bounds__(256) void k_int4_join(const Int4Args a, int slices)
     const int token = blockIdx.y;
     float y = 0.0f;
     if (row < a.outs) {
-        for (int i = 0; i < slices; ++i) y += a.partial[(static_cast<int64_t>(i) * a.tokens + token) * a.outs + row];
+        constexpr int kMost = 16;
+        float part[kMost];
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) part[i] = i < slices ? a.partial[(static_cast<int64_t>(i) * a.tokens + token) * a.outs + row] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) y += part[i];
         nq::store_f32_as(a.y, a.y_dtype, token * a.outs + row, y);
     }
     if (a.best) {
@@ -435,10 +440,10 @@ __global__ __launch_bounds__(256) void k_int4_join(const Int4Args a, int slices)
 
 int64_t chunks_of(int64_t ins) { return (ins + kChunk - 1) / kChunk; }
 
-size_t lds_bytes(int tokens, int blocks, int groups, int stage) {
+size_t lds_bytes(int waves, int tokens, int blocks, int groups, int stage) {
     const int wave = groups == 1 ? kEachWave<1> : groups == 2 ? kEachWave<2> : kEachWave<4>;
     return 64 + static_cast<size_t>(tokens) * kDigits * line_bytes(stage) + static_cast<size_t>(stage) * blocks * 16 * sizeof(Column) +
-           static_cast<size_t>(kWaves) * wave * sizeof(float);
+           static_cast<size_t>(waves) * wave * sizeof(float);
 }
 
 Int4Plan plan_int4(int64_t tokens, int64_t outs, int64_t ins, int group) {
@@ -452,13 +457,15 @@ Int4Plan plan_int4(int64_t tokens, int64_t outs, int64_t ins, int group) {
     p.passes = static_cast<int>((blocks + p.blocks - 1) / p.blocks);
     const int held = static_cast<int>(std::min<int64_t>(tokens, int64_t{p.blocks} * each));
     // Chunks whose digits LDS holds at once.
-    const size_t fixed = lds_bytes(held, p.blocks, groups, 0), each_chunk = lds_bytes(held, p.blocks, groups, 1) - fixed;
+    const size_t fixed = lds_bytes(4, held, p.blocks, groups, 0), each_chunk = lds_bytes(4, held, p.blocks, groups, 1) - fixed;
     const int most = static_cast<int>(std::min<int64_t>(chunks, std::max<int64_t>(1, static_cast<int64_t>((kBudget - std::min(fixed, kBudget)) / each_chunk))));
     p.slices = 1;
+    p.waves = 4;
     p.share = tiles * p.passes >= 2048 ? 1 : 4;
     if (most < chunks && tiles * p.passes < 2048) {
         // Digits that LDS does not hold at once, and few tiles: slices.
         p.share = 1;
+        p.waves = p.blocks == 6 ? 8 : 4;
         const int64_t want = (2048 + tiles * p.passes - 1) / (tiles * p.passes);
         p.slices = static_cast<int>(std::min<int64_t>({16, chunks, std::max<int64_t>(want, 1)}));
     }
@@ -466,18 +473,26 @@ Int4Plan plan_int4(int64_t tokens, int64_t outs, int64_t ins, int group) {
     p.slices = static_cast<int>((chunks + p.slice - 1) / p.slice);
     const int stages = (p.slice + most - 1) / most;
     p.stage = (p.slice + stages - 1) / stages;
-    const int64_t per = kWaves / p.share, all = (tiles + per - 1) / per;
+    const int64_t per = p.waves / p.share, all = (tiles + per - 1) / per;
     // Digits made once serve several tiles.
     p.groups = stages == 1 ? std::min<int64_t>(all, std::max<int64_t>(1, 768 / (int64_t{p.passes} * p.slices))) : all;
     return p;
 }
 
-template <int G, int NB, int ST>
-int launch_as(const Int4Args& a, const Int4Plan& p, hipStream_t stream) {
+template <int G, int NB, int ST, int WV>
+int launch_on(const Int4Args& a, const Int4Plan& p, hipStream_t stream) {
     const int held = std::min(a.tokens, NB * Shape<G>::kTokens);
     const dim3 grid(static_cast<unsigned>(p.groups), static_cast<unsigned>(p.slices), static_cast<unsigned>(p.passes));
-    hipLaunchKernelGGL((k_int4_product<G, NB, ST>), grid, dim3(kThreads), lds_bytes(held, NB, Shape<G>::kGroups, a.stage), stream, a);
+    hipLaunchKernelGGL((k_int4_product<G, NB, ST, WV>), grid, dim3(WV * kWave), lds_bytes(WV, held, NB, Shape<G>::kGroups, a.stage), stream, a);
     return nq::launch_status();
+}
+
+template <int G, int NB, int ST>
+int launch_as(const Int4Args& a, const Int4Plan& p, hipStream_t stream) {
+    if constexpr (NB == 6) {
+        if (p.waves == 8) return launch_on<G, NB, ST, 8>(a, p, stream);
+    }
+    return launch_on<G, NB, ST, 4>(a, p, stream);
 }
 
 template <int G, int NB>
@@ -506,7 +521,7 @@ extern "C" int64_t nq_int4_projection_workspace_bytes(int64_t tokens, int64_t ou
         in_features > (1 << 24) || (group != 32 && group != 64 && group != 128))
         return -1;
     const Int4Plan p = plan_int4(tokens, out_features, in_features, group);
-    if (!nq::launchable(p.groups * p.slices * p.passes, kThreads)) return -1;
+    if (!nq::launchable(p.groups * p.slices * p.passes, p.waves * kWave)) return -1;
     return p.slices == 1 ? 0 : p.slices * tokens * out_features * static_cast<int64_t>(sizeof(float));
 }
 
@@ -536,7 +551,7 @@ extern "C" int nq_int4_projection(const void* x, int32_t x_dtype, int64_t tokens
     a.outs = out_features;
     a.ins = in_features;
     a.tiles = (out_features + 15) / 16;
-    a.step = p.groups * (kWaves / p.share);
+    a.step = p.groups * (p.waves / p.share);
     a.tokens = static_cast<int32_t>(tokens);
     a.chunks = static_cast<int32_t>(chunks_of(in_features));
     a.groups = static_cast<int32_t>((in_features + group - 1) / group);
