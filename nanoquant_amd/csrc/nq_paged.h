@@ -113,19 +113,25 @@ __device__ __forceinline__ float scale_for(float amax) {
     return __uint_as_float(static_cast<uint32_t>(max(e, -126) + 127) << 23);
 }
 
-// Four e4m3 bytes that stand for byte * from, as bytes that stand for byte * to (a
+// Four e4m3 bytes that stand for byte * from[.], as bytes that stand for byte * to (a
 // power of two that holds them); NaN for what fp32 does not hold. A power of two
 // times a byte is exact in fp32; with any other scale the fp32 product would be a first rounding.
-__device__ __forceinline__ uint32_t rescaled4(uint32_t w, float from, float to) {
-    float x[4] = {__builtin_amdgcn_cvt_f32_fp8(w, 0), __builtin_amdgcn_cvt_f32_fp8(w, 1),
-                  __builtin_amdgcn_cvt_f32_fp8(w, 2), __builtin_amdgcn_cvt_f32_fp8(w, 3)};
+__device__ __forceinline__ uint32_t rescaled4(uint32_t w, const float (&from)[4], float to) {
+    const float v[4] = {__builtin_amdgcn_cvt_f32_fp8(w, 0), __builtin_amdgcn_cvt_f32_fp8(w, 1),
+                        __builtin_amdgcn_cvt_f32_fp8(w, 2), __builtin_amdgcn_cvt_f32_fp8(w, 3)};
     const float inv = 1.0f / to;
-    const bool exact = (__float_as_uint(from) & 0x7fffffu) == 0;
+    float x[4];
+    bool exact = true;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float y = x[j] * from;
-        if (!(fabsf(y) < INFINITY)) x[j] = __builtin_nanf("");
-        else x[j] = exact ? y * inv : round_to_odd(static_cast<double>(x[j]) * from * inv);
+        const float y = v[j] * from[j];
+        x[j] = fabsf(y) < INFINITY ? y * inv : __builtin_nanf("");
+        exact = exact && (__float_as_uint(from[j]) & 0x7fffffu) == 0;
+    }
+    if (__ballot(!exact)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (x[j] == x[j]) x[j] = round_to_odd(static_cast<double>(v[j]) * from[j] * inv);
     }
     int r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
     r = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], r, true);

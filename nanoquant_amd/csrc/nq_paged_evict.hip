@@ -21,7 +21,8 @@ struct EvictArgs {
     float* weights;        // [pages][kv_heads][page]
     const int32_t* into;   // [batch][slots]
     int32_t *table, *lens, *rows;  // [batch][entries], [batch], [batch][kv_heads][budget]
-    int32_t budget, first, recent, entries, kept, slots;  // kept: pages in front that stay; slots = entries - kept
+    uint32_t* bins;
+    int32_t budget, first, recent, entries, kept, slots, parts;  // kept: pages in front that stay; slots = entries - kept
 };
 
 // The weights in an order of whole numbers: NaN above all, -0 as 0.
@@ -32,113 +33,346 @@ __device__ __forceinline__ uint32_t key_of(float w) {
 }
 
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / kWave;
+constexpr int kBins = 2048, kLevels = 3;  // of 11, 11 and 10 bits of a key, the highest first
 
-// One workgroup per sequence and kv head.
-__global__ __launch_bounds__(kSelectThreads) void k_evict_select(const EvictArgs a) {
-    __shared__ uint32_t bins[256], counts[2][kSelectWaves], found[2];
+__host__ __device__ constexpr int shift_of(int level) { return level == 0 ? 21 : level == 1 ? 10 : 0; }
+__device__ __forceinline__ uint32_t bin_of(uint32_t key, int level) { return key >> shift_of(level) & (level == 2 ? 1023u : 2047u); }
+// Whether a key has the threshold's bits above a level's.
+__device__ __forceinline__ bool in_reach(uint32_t key, uint32_t prefix, int level) {
+    return level == 0 || key >> shift_of(level - 1) == prefix >> shift_of(level - 1);
+}
+
+// What all workgroups of a sequence and kv head know.
+struct Sequence {
+    const int32_t* table;
+    int32_t* rows;
+    int g, n, end, keep;  // of rows [first, end) the `keep` heaviest
+    bool longer;
+};
+
+__device__ __forceinline__ Sequence sequence_of(const EvictArgs& a, int unit) {
     const Pages& p = a.p;
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int b = blockIdx.x / p.kv_heads, g = blockIdx.x - b * p.kv_heads;
-    const int page = 1 << p.page_shift, held = p.table_pages << p.page_shift;
-    const int context = p.contexts[b], n = min(max(context, 0), held);
-    const bool longer = n > a.budget;
-    const int32_t* table = p.table + static_cast<int64_t>(b) * p.table_pages;
-    int32_t* rows = a.rows + static_cast<int64_t>(blockIdx.x) * a.budget;
-    if (g == 0) {
+    const int b = unit / p.kv_heads;
+    Sequence s;
+    s.g = unit - b * p.kv_heads;
+    s.table = p.table + static_cast<int64_t>(b) * p.table_pages;
+    s.rows = a.rows + static_cast<int64_t>(unit) * a.budget;
+    s.n = min(max(p.contexts[b], 0), p.table_pages << p.page_shift);
+    s.longer = s.n > a.budget;
+    s.end = s.n - a.recent;
+    s.keep = a.budget - a.first - a.recent;
+    return s;
+}
+
+// The rows that stay whatever their weight, the new table and length.
+__device__ __forceinline__ void write_frame(const EvictArgs& a, const Sequence& s, int unit) {
+    const Pages& p = a.p;
+    const int b = unit / p.kv_heads;
+    if (s.g == 0) {
         for (int i = threadIdx.x; i < a.entries; i += kSelectThreads)
             a.table[static_cast<int64_t>(b) * a.entries + i] =
-                longer && i >= a.kept ? a.into[static_cast<int64_t>(b) * a.slots + i - a.kept] : i < p.table_pages ? table[i] : -1;
-        if (threadIdx.x == 0) a.lens[b] = longer ? a.budget : context;
+                s.longer && i >= a.kept ? a.into[static_cast<int64_t>(b) * a.slots + i - a.kept] : i < p.table_pages ? s.table[i] : -1;
+        if (threadIdx.x == 0) a.lens[b] = s.longer ? a.budget : p.contexts[b];
     }
-    if (!longer) {
-        for (int i = threadIdx.x; i < a.budget; i += kSelectThreads) rows[i] = i < n ? i : -1;
+    if (!s.longer) {
+        for (int i = threadIdx.x; i < a.budget; i += kSelectThreads) s.rows[i] = i < s.n ? i : -1;
         return;
     }
-    for (int i = threadIdx.x; i < a.first; i += kSelectThreads) rows[i] = i;
-    for (int i = threadIdx.x; i < a.recent; i += kSelectThreads) rows[a.budget - a.recent + i] = n - a.recent + i;
-    // Of rows [a.first, end) the `keep` heaviest.
-    const int end = n - a.recent, keep = a.budget - a.first - a.recent;
-    if (keep == 0) return;
-    const auto key_at = [&](int row) {
-        const int32_t id = table[row >> p.page_shift];
-        if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.pages)) return 0xffffffffu;
-        return key_of(a.weights[(static_cast<int64_t>(id) * p.kv_heads + g) * page + (row & (page - 1))]);
-    };
-    // The keep-th greatest key, 8 bits at a time: `above` keys have a greater prefix.
-    uint32_t prefix = 0, above = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (threadIdx.x < 256) bins[threadIdx.x] = 0;
-        __syncthreads();
-        for (int row = a.first + static_cast<int>(threadIdx.x); row < end; row += kSelectThreads) {
-            const uint32_t key = key_at(row);
-            if (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&bins[key >> shift & 255u], 1u);
-        }
-        __syncthreads();
-        if (wave == 0) {
-            // Lane l has bins 255 - 4 l down to 252 - 4 l.
-            uint32_t c[4], sum = 0;
+    for (int i = threadIdx.x; i < a.first; i += kSelectThreads) s.rows[i] = i;
+    for (int i = threadIdx.x; i < a.recent; i += kSelectThreads) s.rows[a.budget - a.recent + i] = s.end + i;
+}
+
+__device__ __forceinline__ uint32_t key_at(const EvictArgs& a, const Sequence& s, int row) {
+    const Pages& p = a.p;
+    const int32_t id = s.table[row >> p.page_shift];
+    const bool on = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.pages);
+    const int64_t at = (static_cast<int64_t>(on ? id : 0) * p.kv_heads + s.g << p.page_shift) + (row & ((1 << p.page_shift) - 1));
+    const uint32_t key = key_of(a.weights[at]);
+    return on ? key : 0xffffffffu;
+}
+
+// The bin of a level that the keep-th greatest key lies in, and how many keys are
+// greater than all of it: `above` of higher levels and those of this level's higher
+// bins. Thread t has bins kBins - 1 - 2 t and the one below. All threads get the answer.
+struct Bin {
+    uint32_t bin, above;
+};
+
+__device__ __forceinline__ Bin find_bin(const uint32_t (&c)[2], uint32_t keep, uint32_t above, uint32_t (&waves)[kSelectWaves],
+                                        uint32_t (&found)[2]) {
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const uint32_t mine = c[0] + c[1], upto = running_sum(mine);
+    if (lane == kWave - 1) waves[wave] = upto;
+    __syncthreads();
+    uint32_t before = above + upto - mine;
+    for (int w = 0; w < wave; ++w) before += waves[w];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum += c[j] = bins[255 - 4 * lane - j];
-            const uint32_t upto = running_sum(sum);
-            uint32_t before = above + upto - sum;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (before < static_cast<uint32_t>(keep) && before + c[j] >= static_cast<uint32_t>(keep)) {
-                    found[0] = prefix | static_cast<uint32_t>(255 - 4 * lane - j) << shift;
-                    found[1] = before;
-                }
-                before += c[j];
-            }
+    for (int j = 0; j < 2; ++j) {
+        if (before < keep && before + c[j] >= keep) {
+            found[0] = kBins - 1 - 2 * threadIdx.x - j;
+            found[1] = before;
         }
-        __syncthreads();
-        prefix = found[0];
-        above = found[1];
-        __syncthreads();
+        before += c[j];
     }
-    // Keys above `prefix` are chosen, and the first keep - above of those that equal it.
-    const uint32_t ties = static_cast<uint32_t>(keep) - above;
-    const int per = ((end - a.first + kSelectWaves - 1) / kSelectWaves + kWave - 1) & ~(kWave - 1);
-    const int begin = a.first + wave * per, stop = min(end, begin + per);
+    __syncthreads();
+    const Bin b = {found[0], found[1]};
+    __syncthreads();  // found and waves are read
+    return b;
+}
+
+// Writes the rows of a wave, 64 at a time from `begin` on, whose keys are above the threshold, and
+// the first `ties` of those that equal it; `more` and `same` of these lie before it.
+struct Writer {
+    uint32_t threshold, ties, more, same;
+
+    __device__ __forceinline__ void operator()(const EvictArgs& a, const Sequence& s, int row, bool on, uint32_t key) {
+        const int lane = threadIdx.x & (kWave - 1);
+        const uint64_t greater = __ballot(on && key > threshold), equal = __ballot(on && key == threshold);
+        const uint64_t before = (uint64_t{1} << lane) - 1;
+        const uint32_t my_same = same + __popcll(equal & before), my_more = more + __popcll(greater & before);
+        if ((greater >> lane & 1) || ((equal >> lane & 1) && my_same < ties)) s.rows[a.first + my_more + min(my_same, ties)] = row;
+        more += __popcll(greater);
+        same += __popcll(equal);
+    }
+};
+
+// One workgroup per sequence and kv head. Up to 1024 R rows wait in registers as
+// their keys; more are read again for each level. 24 sequences of up to 6001 rows: see
+// the entry point.
+template <int R>
+__global__ __launch_bounds__(kSelectThreads) void k_evict_select(const EvictArgs a) {
+    __shared__ uint32_t bins[kBins], counts[2][kSelectWaves], found[2];
+    const Sequence s = sequence_of(a, blockIdx.x);
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int all = s.end - a.first;
+    const bool held = s.longer && s.keep > 0 && all <= kSelectThreads * R;
+    const int per = ((all + kSelectWaves - 1) / kSelectWaves + kWave - 1) & ~(kWave - 1);
+    const int begin = a.first + wave * per, stop = min(s.end, begin + per);
+    uint32_t keys[R];
+    if (held) {
+#pragma unroll
+        for (int j = 0; j < R; ++j) keys[j] = key_at(a, s, min(begin + kWave * j + lane, s.end - 1));
+    }
+    write_frame(a, s, blockIdx.x);
+    if (!s.longer || s.keep == 0) return;
+    const auto for_each = [&](auto&& f) {
+        if (held) {
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                if (begin + kWave * j >= stop) break;
+                f(begin + kWave * j + lane, keys[j]);
+            }
+        } else {
+            for (int row = begin + lane; row - lane < stop; row += kWave) f(row, key_at(a, s, min(row, s.end - 1)));
+        }
+    };
+    uint32_t prefix = 0, above = 0;
+    for (int level = 0; level < kLevels; ++level) {
+        for (int i = threadIdx.x; i < kBins; i += kSelectThreads) bins[i] = 0;
+        __syncthreads();
+        for_each([&](int row, uint32_t key) {
+            if (row < stop && in_reach(key, prefix, level)) atomicAdd(&bins[bin_of(key, level)], 1u);
+        });
+        __syncthreads();
+        const uint32_t c[2] = {bins[kBins - 1 - 2 * threadIdx.x], bins[kBins - 2 - 2 * threadIdx.x]};
+        const Bin b = find_bin(c, s.keep, above, counts[0], found);
+        prefix |= b.bin << shift_of(level);
+        above = b.above;
+    }
     uint32_t more = 0, same = 0;
-    for (int row = begin + lane; row - lane < stop; row += kWave) {
-        const uint32_t key = row < stop ? key_at(row) : 0u;
+    for_each([&](int row, uint32_t key) {
         more += __popcll(__ballot(row < stop && key > prefix));
         same += __popcll(__ballot(row < stop && key == prefix));
-    }
+    });
     if (lane == 0) {
         counts[0][wave] = more;
         counts[1][wave] = same;
     }
     __syncthreads();
-    more = same = 0;
+    Writer write = {prefix, static_cast<uint32_t>(s.keep) - above, 0, 0};
     for (int w = 0; w < wave; ++w) {
-        more += counts[0][w];
-        same += counts[1][w];
+        write.more += counts[0][w];
+        write.same += counts[1][w];
     }
-    for (int row = begin + lane; row - lane < stop; row += kWave) {
-        const uint32_t key = row < stop ? key_at(row) : 0u;
-        const uint64_t greater = __ballot(row < stop && key > prefix), equal = __ballot(row < stop && key == prefix);
-        const uint64_t before = (uint64_t{1} << lane) - 1;
-        const uint32_t my_same = same + __popcll(equal & before), my_more = more + __popcll(greater & before);
-        const bool mine = (greater >> lane & 1) || ((equal >> lane & 1) && my_same < ties);
-        if (mine) rows[a.first + my_more + min(my_same, ties)] = row;
-        more += __popcll(greater);
-        same += __popcll(equal);
+    for_each([&](int row, uint32_t key) { write(a, s, row, row < stop, key); });
+}
+
+// The same with a long sequence's rows in parts of kPart, a workgroup each: a launch
+// counts each level's bins (a.bins: [sequence and head][level][part][kBins]), the last
+// one writes. Every workgroup adds the parts' counts up for itself.
+constexpr int kPartKeys = 8, kPart = kSelectThreads * kPartKeys;
+
+template <int LEVEL>
+__global__ __launch_bounds__(kSelectThreads) void k_evict_part(const EvictArgs a) {
+    __shared__ uint32_t bins[kBins], counts[2][kSelectWaves], found[2], passed[2];
+    const int unit = blockIdx.x / a.parts, part = blockIdx.x - unit * a.parts;
+    const Sequence s = sequence_of(a, unit);
+    if (LEVEL == 0 && part == 0) write_frame(a, s, unit);
+    if (!s.longer || s.keep == 0) return;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int from = a.first + part * kPart, parts = (s.end - a.first + kPart - 1) / kPart;
+    if (part >= parts) return;
+    const int begin = from + wave * (kPart / kSelectWaves), stop = min(s.end, begin + kPart / kSelectWaves);
+    uint32_t keys[kPartKeys];
+#pragma unroll
+    for (int j = 0; j < kPartKeys; ++j) keys[j] = key_at(a, s, min(begin + kWave * j + lane, s.end - 1));
+    uint32_t* mine = a.bins + static_cast<int64_t>(unit) * kLevels * a.parts * kBins;
+    uint32_t prefix = 0, above = 0;
+    if (threadIdx.x < 2) passed[threadIdx.x] = 0;
+#pragma unroll
+    for (int level = 0; level < LEVEL; ++level) {
+        // All parts' counts, and those of the parts before this one.
+        uint32_t c[2] = {0, 0}, before[2] = {0, 0};
+        const uint32_t* at = mine + static_cast<int64_t>(level) * a.parts * kBins + kBins - 2 - 2 * threadIdx.x;
+#pragma unroll 8
+        for (int i = 0; i < parts; ++i) {
+            const uint2 v = *reinterpret_cast<const uint2*>(at + static_cast<int64_t>(i) * kBins);
+            c[0] += v.y;
+            c[1] += v.x;
+            if (i < part) {
+                before[0] += v.y;
+                before[1] += v.x;
+            }
+        }
+        const Bin b = find_bin(c, s.keep, above, counts[0], found);
+        prefix |= b.bin << shift_of(level);
+        above = b.above;
+        if constexpr (LEVEL == kLevels) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t bin = kBins - 1 - 2 * threadIdx.x - j;
+                if (bin > b.bin && before[j]) atomicAdd(&passed[0], before[j]);
+                if (level == kLevels - 1 && bin == b.bin) passed[1] = before[j];
+            }
+        }
+    }
+    if constexpr (LEVEL < kLevels) {
+        for (int i = threadIdx.x; i < kBins; i += kSelectThreads) bins[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kPartKeys; ++j)
+            if (begin + kWave * j + lane < stop && in_reach(keys[j], prefix, LEVEL)) atomicAdd(&bins[bin_of(keys[j], LEVEL)], 1u);
+        __syncthreads();
+        uint32_t* to = mine + (static_cast<int64_t>(LEVEL) * a.parts + part) * kBins;
+        for (int i = threadIdx.x; i < kBins; i += kSelectThreads) to[i] = bins[i];
+    } else {
+        uint32_t more = 0, same = 0;
+#pragma unroll
+        for (int j = 0; j < kPartKeys; ++j) {
+            const bool on = begin + kWave * j + lane < stop;
+            more += __popcll(__ballot(on && keys[j] > prefix));
+            same += __popcll(__ballot(on && keys[j] == prefix));
+        }
+        if (lane == 0) {
+            counts[0][wave] = more;
+            counts[1][wave] = same;
+        }
+        __syncthreads();
+        Writer write = {prefix, static_cast<uint32_t>(s.keep) - above, passed[0], passed[1]};
+        for (int w = 0; w < wave; ++w) {
+            write.more += counts[0][w];
+            write.same += counts[1][w];
+        }
+#pragma unroll
+        for (int j = 0; j < kPartKeys; ++j) {
+            const int row = begin + kWave * j + lane;
+            write(a, s, row, row < stop, keys[j]);
+        }
     }
 }
 
 constexpr int kMoveThreads = 256;
 
-// One workgroup per sequence, fresh page, kv head and K or V: the rows' bytes wait
-// in LDS until the page's scale is known.
+// One workgroup per sequence, fresh page, kv head and K or V. A thread holds its
+// share of the page's bytes in registers until the page's scale is known: 16-byte
+// pieces of K's rows, words of four rows of V's lines, whose bytes it gathers.
+template <int D, bool IS_V>
+__device__ __forceinline__ void move_page(const EvictArgs& a, int b, int slot, int g, int64_t to, const int64_t* source,
+                                          const float* scales, uint32_t& top, int count) {
+    // Source of row r: an offset into K, or into V's line 0; -1: no page.
+    constexpr int kUnits = IS_V ? D / 8 : D / 32;  // of a page of 128 rows and 256 threads
+    constexpr int kWords = IS_V ? 1 : 4;
+    const Pages& p = a.p;
+    const int shift = p.page_shift, page = 1 << shift;
+    const int units = IS_V ? D << (shift - 2) : (D / 16) << shift;
+    uint32_t w[kUnits][kWords];
+    // Unit i is line i / (page / 4), rows 4 (i % (page / 4)) of V; row i / (D / 16) of K.
+    const auto row_of_unit = [&](int i) { return IS_V ? 4 * (i & (page / 4 - 1)) : i / (D / 16); };
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+        const int i = threadIdx.x + k * kMoveThreads, row = row_of_unit(i);
+        if constexpr (IS_V) {
+            uint32_t bytes[4] = {0, 0, 0, 0};
+            if (i < units) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (row + j < count) bytes[j] = source[row + j] < 0 ? 0x7fu : p.v[source[row + j] + (static_cast<int64_t>(i >> (shift - 2)) << shift)];
+            }
+            w[k][0] = bytes[0] | bytes[1] << 8 | bytes[2] << 16 | bytes[3] << 24;
+        } else {
+            u32x4 v = {0, 0, 0, 0};
+            if (i < units && row < count) {
+                v = u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+                if (source[row] >= 0) v = *reinterpret_cast<const u32x4*>(p.k + source[row] + 16 * (i % (D / 16)));
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[k][j] = v[j];
+        }
+    }
+    float most = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+        const int i = threadIdx.x + k * kMoveThreads, row = row_of_unit(i);
+        if (i >= units) break;
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) {
+            const float x[4] = {__builtin_amdgcn_cvt_f32_fp8(w[k][j], 0), __builtin_amdgcn_cvt_f32_fp8(w[k][j], 1),
+                                __builtin_amdgcn_cvt_f32_fp8(w[k][j], 2), __builtin_amdgcn_cvt_f32_fp8(w[k][j], 3)};
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const float y = fabsf(x[m] * scales[IS_V ? row + m : row]);
+                most = fmaxf(most, y < INFINITY ? y : 0.0f);
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 1; m < kWave; m *= 2) most = fmaxf(most, __shfl_xor(most, m, kWave));
+    if ((threadIdx.x & (kWave - 1)) == 0) atomicMax(&top, __float_as_uint(most));  // values >= 0: ordered as their bits
+    __syncthreads();
+    const float scale = scale_for(__uint_as_float(top));
+    if (threadIdx.x == 0) (IS_V ? p.v_scales : p.k_scales)[to] = scale;
+    uint8_t* out = (IS_V ? p.v : p.k) + to * page * D;
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+        const int i = threadIdx.x + k * kMoveThreads, row = row_of_unit(i);
+        if (i >= units || row >= count) continue;
+        if constexpr (IS_V) {
+            const float from[4] = {scales[row], scales[row + 1], scales[row + 2], scales[row + 3]};
+            const uint32_t v = rescaled4(w[k][0], from, scale);
+            uint8_t* at = out + (static_cast<int64_t>(i >> (shift - 2)) << shift) + row;
+            if (row + 4 <= count) {
+                *reinterpret_cast<uint32_t*>(at) = v;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 3; ++j)
+                    if (row + j < count) at[j] = static_cast<uint8_t>(v >> (8 * j));
+            }
+        } else {
+            const float from[4] = {scales[row], scales[row], scales[row], scales[row]};
+            u32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = rescaled4(w[k][j], from, scale);
+            *reinterpret_cast<u32x4*>(out + static_cast<int64_t>(row) * D + 16 * (i % (D / 16))) = v;
+        }
+    }
+}
+
 template <int D>
 __global__ __launch_bounds__(kMoveThreads) void k_evict_move(const EvictArgs a) {
-    constexpr int kWords = D / 4, kLine = kWords + 1, kMost = 128;
-    __shared__ int64_t source[kMost];  // each row's page and head, or -1
-    __shared__ float scales[kMost];
-    __shared__ int offset[kMost];      // the row in its page
+    constexpr int kMost = 128;
+    __shared__ int64_t source[kMost];
+    __shared__ float scales[kMost];  // 0 behind the last row
     __shared__ uint32_t top;
-    extern __shared__ uint32_t bytes[];
     const Pages& p = a.p;
     const int page = 1 << p.page_shift, held = p.table_pages << p.page_shift;
     const int g = blockIdx.x % p.kv_heads;
@@ -150,70 +384,37 @@ __global__ __launch_bounds__(kMoveThreads) void k_evict_move(const EvictArgs a) 
     const int32_t id = a.into[static_cast<int64_t>(b) * a.slots + slot];
     if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.pages)) return;
     const int first = (a.kept + slot) << p.page_shift, count = min(page, a.budget - first);
-    const int32_t* rows = a.rows + (static_cast<int64_t>(b) * p.kv_heads + g) * a.budget + first;
     const int64_t to = static_cast<int64_t>(id) * p.kv_heads + g;
     if (threadIdx.x == 0) top = 0;
-    if (static_cast<int>(threadIdx.x) < count) {
-        const int row = rows[threadIdx.x];
-        const int32_t from = p.table[static_cast<int64_t>(b) * p.table_pages + (row >> p.page_shift)];
+    if (threadIdx.x < kMost) {
+        const bool there = static_cast<int>(threadIdx.x) < count;
+        const int row = there ? a.rows[(static_cast<int64_t>(b) * p.kv_heads + g) * a.budget + first + threadIdx.x] : 0;
+        const int32_t from = there ? p.table[static_cast<int64_t>(b) * p.table_pages + (row >> p.page_shift)] : -1;
         const bool on = static_cast<uint32_t>(from) < static_cast<uint32_t>(p.pages);
-        const int64_t at = on ? static_cast<int64_t>(from) * p.kv_heads + g : -1;
-        source[threadIdx.x] = at;
-        offset[threadIdx.x] = row & (page - 1);
-        scales[threadIdx.x] = on ? (is_v ? p.v_scales : p.k_scales)[at] : 1.0f;
-        if (!is_v) a.weights[to * page + threadIdx.x] = on ? a.weights[at * page + (row & (page - 1))] : __builtin_nanf("");
+        const int64_t at = static_cast<int64_t>(on ? from : 0) * p.kv_heads + g;
+        const int offset = row & (page - 1);
+        source[threadIdx.x] = !on ? -1 : is_v ? at * D * page + offset : (at * page + offset) * D;
+        scales[threadIdx.x] = !there ? 0.0f : on ? (is_v ? p.v_scales : p.k_scales)[at] : 1.0f;
+        if (!is_v && there) a.weights[to * page + threadIdx.x] = on ? a.weights[at * page + offset] : __builtin_nanf("");
     }
     __syncthreads();
-    float most = 0.0f;
-    const auto hold = [&](int row, int c, uint32_t w) {
-        bytes[row * kLine + c] = w;
-        const float scale = scales[row];
-        const float x[4] = {__builtin_amdgcn_cvt_f32_fp8(w, 0) * scale, __builtin_amdgcn_cvt_f32_fp8(w, 1) * scale,
-                            __builtin_amdgcn_cvt_f32_fp8(w, 2) * scale, __builtin_amdgcn_cvt_f32_fp8(w, 3) * scale};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[j]) < INFINITY ? fabsf(x[j]) : 0.0f);
-    };
-    if (!is_v) {
-        for (int i = threadIdx.x; i < count * kWords; i += kMoveThreads) {
-            const int row = i / kWords, c = i - row * kWords;
-            const int64_t at = source[row];
-            hold(row, c, at < 0 ? 0x7f7f7f7fu : *reinterpret_cast<const uint32_t*>(p.k + (at * page + offset[row]) * D + 4 * c));
-        }
-    } else {
-        for (int i = threadIdx.x; i < count * kWords; i += kMoveThreads) {
-            const int c = i / count, row = i - c * count;  // neighbours read neighbouring bytes of V's lines
-            const int64_t at = source[row];
-            uint32_t w = 0x7f7f7f7fu;
-            if (at >= 0) {
-                w = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w |= static_cast<uint32_t>(p.v[(at * D + 4 * c + j) * page + offset[row]]) << (8 * j);
-            }
-            hold(row, c, w);
-        }
-    }
-    atomicMax(&top, __float_as_uint(most));  // values >= 0: ordered as their bits
-    __syncthreads();
-    const float scale = scale_for(__uint_as_float(top));
-    if (threadIdx.x == 0) (is_v ? p.v_scales : p.k_scales)[to] = scale;
-    for (int i = threadIdx.x; i < count * kWords; i += kMoveThreads) {
-        const int row = is_v ? i % count : i / kWords, c = is_v ? i / count : i - row * kWords;
-        const uint32_t w = rescaled4(bytes[row * kLine + c], scales[row], scale);
-        if (!is_v) {
-            *reinterpret_cast<uint32_t*>(p.k + (to * page + row) * D + 4 * c) = w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) p.v[(to * D + 4 * c + j) * page + row] = static_cast<uint8_t>(w >> (8 * j));
-        }
-    }
+    if (is_v) move_page<D, true>(a, b, slot, g, to, source, scales, top, count);
+    else move_page<D, false>(a, b, slot, g, to, source, scales, top, count);
 }
 
 template <int D>
 int launch_move(const EvictArgs& a, hipStream_t stream) {
-    const size_t bytes = static_cast<size_t>(D + 4) << a.p.page_shift;  // 33 KB at most
     const dim3 grid(static_cast<unsigned>(2 * static_cast<int64_t>(a.p.batch) * a.slots * a.p.kv_heads)), block(kMoveThreads);
-    hipLaunchKernelGGL(k_evict_move<D>, grid, block, bytes, stream, a);
+    hipLaunchKernelGGL(k_evict_move<D>, grid, block, 0, stream, a);
     return nq::launch_status();
+}
+
+constexpr int kFewKeys = 8, kManyKeys = 32;
+
+// Parts of a sequence's rows, or 0 where a workgroup takes a sequence and head alone.
+int64_t parts_of(int64_t units, int64_t rows) {
+    if (rows <= kSelectThreads * kFewKeys || units >= 128) return 0;
+    return (rows + kPart - 1) / kPart;
 }
 
 }  // namespace
@@ -223,9 +424,10 @@ extern "C" int64_t nq_paged_evict_workspace_bytes(int64_t batch, int32_t kv_head
     if (batch <= 0 || batch > 0xffffff || kv_heads <= 0 || kv_heads > 65535 || page_size <= 0 || page_size > 128 ||
         table_pages <= 0 || table_pages > 0x3fffffff / page_size || budget <= 0 || budget > 0x3fffffff)
         return -1;
-    if (!nq::launchable(batch * kv_heads, kSelectThreads)) return -1;
+    const int64_t parts = parts_of(batch * kv_heads, table_pages * page_size);
+    if (!nq::launchable(batch * kv_heads * std::max<int64_t>(parts, 1), kSelectThreads)) return -1;
     if (!nq::launchable(2 * batch * kv_heads * ((budget + page_size - 1) / page_size), kMoveThreads)) return -1;
-    return 0;
+    return batch * kv_heads * parts * kLevels * kBins * static_cast<int64_t>(sizeof(uint32_t));
 }
 
 extern "C" int nq_paged_evict(const nq_paged_kv* kv, float* weights, const int32_t* into, int64_t budget, int64_t first,
@@ -240,6 +442,7 @@ extern "C" int nq_paged_evict(const nq_paged_kv* kv, float* weights, const int32
     if (need < 0 || first < 0 || recent < 0 || first > budget || recent > budget - first) return NQ_ERR_SHAPE;
     if (need > 0 && !workspace) return NQ_ERR_ARGUMENT;
     if (workspace_bytes < need) return NQ_ERR_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return NQ_ERR_ALIGNMENT;
     a.weights = weights;
     a.into = into;
     a.table = page_table_out;
@@ -253,8 +456,20 @@ extern "C" int nq_paged_evict(const nq_paged_kv* kv, float* weights, const int32
     a.slots = a.entries - a.kept;
     if (a.slots > 0 && !into) return NQ_ERR_ARGUMENT;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid(static_cast<unsigned>(kv->batch * kv->kv_heads));
-    hipLaunchKernelGGL(k_evict_select, grid, dim3(kSelectThreads), 0, st, a);
+    const int64_t units = kv->batch * kv->kv_heads;
+    a.parts = static_cast<int32_t>(parts_of(units, kv->table_pages * kv->page_size));
+    a.bins = static_cast<uint32_t*>(workspace);
+    const dim3 block(kSelectThreads), grid(static_cast<unsigned>(units * std::max(a.parts, 1)));
+    if (a.parts > 0) {
+        hipLaunchKernelGGL(k_evict_part<0>, grid, block, 0, st, a);
+        hipLaunchKernelGGL(k_evict_part<1>, grid, block, 0, st, a);
+        hipLaunchKernelGGL(k_evict_part<2>, grid, block, 0, st, a);
+        hipLaunchKernelGGL(k_evict_part<3>, grid, block, 0, st, a);
+    } else if (kv->table_pages * kv->page_size <= kSelectThreads * kFewKeys) {
+        hipLaunchKernelGGL(k_evict_select<kFewKeys>, grid, block, 0, st, a);
+    } else {
+        hipLaunchKernelGGL(k_evict_select<kManyKeys>, grid, block, 0, st, a);
+    }
     if (const int status = nq::launch_status(); status != NQ_OK || a.slots == 0) return status;
     switch (kv->head_dim) {
         case 64: return launch_move<64>(a, st);

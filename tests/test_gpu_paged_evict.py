@@ -177,3 +177,66 @@ def test_captured_calls_replay_with_other_lengths_and_weights():
         assert all(torch.equal(x, y) for x, y in zip(out, eager))
         after = [x.view(torch.uint8) for x in cache[:2]] + [*cache[2:], w]
         assert all(torch.equal(x, y) for x, y in zip(pages, after))
+
+
+@pytest.mark.parametrize("contexts,kv,page,budget,first,recent,kind", [
+    ([20000, 9000, 8193], 2, 64, 5000, 10, 300, "spread"),     # parts of a sequence's rows
+    ([70001], 3, 128, 20000, 4, 64, "spread"),
+    ([70001], 3, 128, 20000, 4, 64, "equal"),
+    ([40000, 100], 1, 16, 39999, 0, 0, "few"),
+    ([33000], 128, 64, 1000, 0, 20, "spread"),                 # more rows than registers hold keys
+    ([30000], 130, 64, 900, 7, 0, "few"),
+    ([8192], 2, 32, 4000, 0, 0, "spread"),
+])
+def test_long_sequences(contexts, kv, page, budget, first, recent, kind):
+    """Rows against torch's stable sort; the values that moved are the values they were."""
+
+    _say("evict long", contexts, kv, page, budget, first, recent, kind)
+    d = 64
+    g = torch.Generator(device=DEV).manual_seed(381)
+    used = [-(-c // page) for c in contexts]
+    slots = -(-budget // page) - first // page
+    pages = sum(used) + len(contexts) * slots
+    order = torch.randperm(pages, generator=g, device=DEV).to(torch.int32)
+    table = torch.full((len(contexts), max(used)), -1, dtype=torch.int32, device=DEV)
+    at = 0
+    for i, n in enumerate(used):
+        table[i, :n] = order[at:at + n]
+        at += n
+    into = order[at:].view(len(contexts), slots).contiguous()
+    cache = ops.paged_cache(pages, kv, page, d, DEV)
+    for x, scale in ((cache.k, cache.k_scales), (cache.v, cache.v_scales)):
+        x.view(torch.uint8).copy_(torch.randint(0x20, 0x70, x.shape, generator=g, device=DEV, dtype=torch.uint8))
+        scale.fill_(2.0**-5)
+    weights = torch.rand(pages, kv, page, generator=g, device=DEV)
+    if kind == "equal":
+        weights.fill_(1.0)
+    elif kind == "few":
+        weights = torch.randint(0, 3, weights.shape, generator=g, device=DEV).float()
+    before, old = ops.PagedCache(*(x.clone() for x in cache)), weights.clone()
+    lens = torch.tensor(contexts, dtype=torch.int32, device=DEV)
+    got = ops.launch_paged_evict(cache, weights, page_table=table, context_lens=lens, into=into, budget=budget, first=first,
+                                 recent=recent)
+
+    def rows_of(c, w, line, n):
+        """A sequence's rows as values and weights: [kv, n, d] twice, [kv, n]."""
+        at = line[:-(-n // page)].long()
+        k = c.k.view(torch.uint8)[at].view(torch.float8_e4m3fn).float() * c.k_scales[at][..., None, None]
+        v = c.v.view(torch.uint8)[at].view(torch.float8_e4m3fn).float() * c.v_scales[at][..., None, None]
+        return (k.transpose(0, 1).reshape(kv, -1, d)[:, :n], v.permute(1, 0, 3, 2).reshape(kv, -1, d)[:, :n],
+                w[at].transpose(0, 1).reshape(kv, -1)[:, :n])
+
+    for b, n in enumerate(contexts):
+        cut = min(n, budget)
+        k, v, w = rows_of(before, old, table[b], n)
+        keep = torch.arange(n, device=DEV).expand(kv, n)
+        if n > budget:
+            mid = torch.sort(w[:, first:n - recent], dim=1, descending=True, stable=True).indices[:, :budget - first - recent] + first
+            keep = torch.cat((keep[:, :first], mid.sort(1).values, keep[:, n - recent:]), 1)
+        assert torch.equal(got.rows[b, :, :cut].long(), keep)
+        assert (got.rows[b, :, cut:] == -1).all()
+        new = rows_of(cache, weights, got.page_table[b], cut)
+        index = keep[..., None].expand(kv, cut, d)
+        assert torch.equal(new[0], k.gather(1, index)) and torch.equal(new[1], v.gather(1, index))
+        assert torch.equal(new[2], w.gather(1, keep))
+    assert got.context_lens.tolist() == [min(n, budget) for n in contexts]
