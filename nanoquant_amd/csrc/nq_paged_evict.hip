@@ -200,6 +200,7 @@ __global__ __launch_bounds__(kSelectThreads) void k_evict_select(const EvictArgs
 // The same with a long sequence's rows in parts of kPart, a workgroup each: a launch
 // counts each level's bins (a.bins: [sequence and head][level][part][kBins]), the last
 // one writes. Every workgroup adds the parts' counts up for itself.
+constexpr int kPartsAtOnce = 8;  // counts of parts that a thread loads at once
 constexpr int kPartKeys = 8, kPart = kSelectThreads * kPartKeys;
 
 template <int LEVEL>
@@ -217,33 +218,44 @@ __global__ __launch_bounds__(kSelectThreads) void k_evict_part(const EvictArgs a
 #pragma unroll
     for (int j = 0; j < kPartKeys; ++j) keys[j] = key_at(a, s, min(begin + kWave * j + lane, s.end - 1));
     uint32_t* mine = a.bins + static_cast<int64_t>(unit) * kLevels * a.parts * kBins;
+    // All parts' counts, and those of the parts before this one.
+    uint32_t c[LEVEL + 1][2] = {}, before[LEVEL + 1][2] = {};
+    const uint32_t* at = mine + kBins - 2 - 2 * threadIdx.x;
+    for (int i0 = 0; i0 < parts; i0 += kPartsAtOnce) {
+        uint2 v[LEVEL + 1][kPartsAtOnce];
+#pragma unroll
+        for (int level = 0; level < LEVEL; ++level)
+#pragma unroll
+            for (int i = 0; i < kPartsAtOnce; ++i)
+                v[level][i] = *reinterpret_cast<const uint2*>(at + (static_cast<int64_t>(level) * a.parts + min(i0 + i, parts - 1)) * kBins);
+#pragma unroll
+        for (int level = 0; level < LEVEL; ++level)
+#pragma unroll
+            for (int i = 0; i < kPartsAtOnce; ++i) {
+                const uint32_t on = i0 + i < parts, ahead = i0 + i < part;
+                c[level][0] += on ? v[level][i].y : 0u;
+                c[level][1] += on ? v[level][i].x : 0u;
+                before[level][0] += ahead ? v[level][i].y : 0u;
+                before[level][1] += ahead ? v[level][i].x : 0u;
+            }
+    }
     uint32_t prefix = 0, above = 0;
     if (threadIdx.x < 2) passed[threadIdx.x] = 0;
 #pragma unroll
     for (int level = 0; level < LEVEL; ++level) {
-        // All parts' counts, and those of the parts before this one.
-        uint32_t c[2] = {0, 0}, before[2] = {0, 0};
-        const uint32_t* at = mine + static_cast<int64_t>(level) * a.parts * kBins + kBins - 2 - 2 * threadIdx.x;
-#pragma unroll 8
-        for (int i = 0; i < parts; ++i) {
-            const uint2 v = *reinterpret_cast<const uint2*>(at + static_cast<int64_t>(i) * kBins);
-            c[0] += v.y;
-            c[1] += v.x;
-            if (i < part) {
-                before[0] += v.y;
-                before[1] += v.x;
-            }
-        }
-        const Bin b = find_bin(c, s.keep, above, counts[0], found);
+        const Bin b = find_bin(c[level], s.keep, above, counts[0], found);
         prefix |= b.bin << shift_of(level);
         above = b.above;
         if constexpr (LEVEL == kLevels) {
+            uint32_t more = 0;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const uint32_t bin = kBins - 1 - 2 * threadIdx.x - j;
-                if (bin > b.bin && before[j]) atomicAdd(&passed[0], before[j]);
-                if (level == kLevels - 1 && bin == b.bin) passed[1] = before[j];
+                if (bin > b.bin) more += before[level][j];
+                if (level == kLevels - 1 && bin == b.bin) passed[1] = before[level][j];
             }
+            more = running_sum(more);
+            if (lane == kWave - 1 && more) atomicAdd(&passed[0], more);
         }
     }
     if constexpr (LEVEL < kLevels) {
@@ -281,49 +293,62 @@ __global__ __launch_bounds__(kSelectThreads) void k_evict_part(const EvictArgs a
     }
 }
 
-constexpr int kMoveThreads = 256;
+// Threads that move a page: 64 bytes to each, or as many as a workgroup should have.
+template <int D, int SHIFT>
+constexpr int kMoveThreads = (D << SHIFT) <= 4096 ? 64 : (D << SHIFT) <= 8192 ? 128 : 256;
 
 // One workgroup per sequence, fresh page, kv head and K or V. A thread holds its
 // share of the page's bytes in registers until the page's scale is known: 16-byte
-// pieces of K's rows, words of four rows of V's lines, whose bytes it gathers.
-template <int D, bool IS_V>
-__device__ __forceinline__ void move_page(const EvictArgs& a, int b, int slot, int g, int64_t to, const int64_t* source,
-                                          const float* scales, uint32_t& top, int count) {
-    // Source of row r: an offset into K, or into V's line 0; -1: no page.
-    constexpr int kUnits = IS_V ? D / 8 : D / 32;  // of a page of 128 rows and 256 threads
-    constexpr int kWords = IS_V ? 1 : 4;
+// pieces of K's rows, words of four rows of V's lines, whose bytes it gathers. A page
+// waits for its rows' numbers, their pages and their bytes one after the other and
+// does little in between, so small pages take one wave: as many of them as possible wait at once.
+template <int D, int SHIFT, bool IS_V>
+__device__ __forceinline__ void move_page(const EvictArgs& a, int64_t to, const int64_t* source, const float* scales,
+                                          const uint32_t* keep, uint32_t& top, int count) {
+    constexpr int kThreads = kMoveThreads<D, SHIFT>, kPage = 1 << SHIFT, kBytes = D << SHIFT;
+    constexpr int kUnits = kBytes / (IS_V ? 4 : 16) / kThreads, kWords = IS_V ? 1 : 4;
+    constexpr int kAtOnce = IS_V && kUnits > 16 ? 16 : kUnits;
+    // Unit i is line i / (page / 4), rows 4 (i % (page / 4)) of V (a thread has the same rows of every
+    // line); row i / (D / 16) of K.
     const Pages& p = a.p;
-    const int shift = p.page_shift, page = 1 << shift;
-    const int units = IS_V ? D << (shift - 2) : (D / 16) << shift;
+    const int quad = threadIdx.x & (kPage / 4 - 1);
+    const auto row_of_unit = [&](int i) { return IS_V ? 4 * quad : i / (D / 16); };
     uint32_t w[kUnits][kWords];
-    // Unit i is line i / (page / 4), rows 4 (i % (page / 4)) of V; row i / (D / 16) of K.
-    const auto row_of_unit = [&](int i) { return IS_V ? 4 * (i & (page / 4 - 1)) : i / (D / 16); };
+    if constexpr (IS_V) {
+        const uint8_t* from[4];
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-        const int i = threadIdx.x + k * kMoveThreads, row = row_of_unit(i);
-        if constexpr (IS_V) {
-            uint32_t bytes[4] = {0, 0, 0, 0};
-            if (i < units) {
+        for (int j = 0; j < 4; ++j) from[j] = p.v + source[4 * quad + j];
+        const uint32_t kept = keep[quad];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (row + j < count) bytes[j] = source[row + j] < 0 ? 0x7fu : p.v[source[row + j] + (static_cast<int64_t>(i >> (shift - 2)) << shift)];
-            }
-            w[k][0] = bytes[0] | bytes[1] << 8 | bytes[2] << 16 | bytes[3] << 24;
-        } else {
-            u32x4 v = {0, 0, 0, 0};
-            if (i < units && row < count) {
-                v = u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
-                if (source[row] >= 0) v = *reinterpret_cast<const u32x4*>(p.k + source[row] + 16 * (i % (D / 16)));
-            }
+        for (int k0 = 0; k0 < kUnits; k0 += kAtOnce) {
+            uint32_t bytes[kAtOnce][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[k][j] = v[j];
+            for (int k = 0; k < kAtOnce; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) bytes[k][j] = from[j][((threadIdx.x + (k0 + k) * kThreads) / (kPage / 4)) * kPage];
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k)
+                w[k0 + k][0] = ((bytes[k][0] | bytes[k][1] << 8 | bytes[k][2] << 16 | bytes[k][3] << 24) & kept) | (~kept & 0x7f7f7f7fu);
+        }
+    } else {
+        u32x4 v[kUnits];
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+            const int i = threadIdx.x + k * kThreads;
+            v[k] = *reinterpret_cast<const u32x4*>(p.k + source[row_of_unit(i)] + 16 * (i % (D / 16)));
+        }
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+            const int row = row_of_unit(threadIdx.x + k * kThreads);
+            const bool on = keep[row / 4] >> (8 * (row & 3)) & 1u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[k][j] = on ? v[k][j] : 0x7f7f7f7fu;
         }
     }
     float most = 0.0f;
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
-        const int i = threadIdx.x + k * kMoveThreads, row = row_of_unit(i);
-        if (i >= units) break;
+        const int row = row_of_unit(threadIdx.x + k * kThreads);
 #pragma unroll
         for (int j = 0; j < kWords; ++j) {
             const float x[4] = {__builtin_amdgcn_cvt_f32_fp8(w[k][j], 0), __builtin_amdgcn_cvt_f32_fp8(w[k][j], 1),
@@ -341,15 +366,15 @@ __device__ __forceinline__ void move_page(const EvictArgs& a, int b, int slot, i
     __syncthreads();
     const float scale = scale_for(__uint_as_float(top));
     if (threadIdx.x == 0) (IS_V ? p.v_scales : p.k_scales)[to] = scale;
-    uint8_t* out = (IS_V ? p.v : p.k) + to * page * D;
+    uint8_t* out = (IS_V ? p.v : p.k) + to * kBytes;
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
-        const int i = threadIdx.x + k * kMoveThreads, row = row_of_unit(i);
-        if (i >= units || row >= count) continue;
+        const int i = threadIdx.x + k * kThreads, row = row_of_unit(i);
+        if (row >= count) continue;
         if constexpr (IS_V) {
             const float from[4] = {scales[row], scales[row + 1], scales[row + 2], scales[row + 3]};
             const uint32_t v = rescaled4(w[k][0], from, scale);
-            uint8_t* at = out + (static_cast<int64_t>(i >> (shift - 2)) << shift) + row;
+            uint8_t* at = out + i / (kPage / 4) * kPage + row;
             if (row + 4 <= count) {
                 *reinterpret_cast<uint32_t*>(at) = v;
             } else {
@@ -362,51 +387,64 @@ __device__ __forceinline__ void move_page(const EvictArgs& a, int b, int slot, i
             u32x4 v;
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = rescaled4(w[k][j], from, scale);
-            *reinterpret_cast<u32x4*>(out + static_cast<int64_t>(row) * D + 16 * (i % (D / 16))) = v;
+            *reinterpret_cast<u32x4*>(out + row * D + 16 * (i % (D / 16))) = v;
         }
     }
 }
 
-template <int D>
-__global__ __launch_bounds__(kMoveThreads) void k_evict_move(const EvictArgs a) {
-    constexpr int kMost = 128;
-    __shared__ int64_t source[kMost];
-    __shared__ float scales[kMost];  // 0 behind the last row
+template <int D, int SHIFT>
+__global__ __launch_bounds__((kMoveThreads<D, SHIFT>)) void k_evict_move(const EvictArgs a) {
+    constexpr int kPage = 1 << SHIFT;
+    __shared__ int64_t source[kPage];    // each row's offset in K, or in line 0 of V; any page's where there is none
+    __shared__ float scales[kPage];      // 0 behind the last row
+    __shared__ uint32_t keep[kPage / 4];  // a byte for each row, 0 where its page is none
     __shared__ uint32_t top;
     const Pages& p = a.p;
-    const int page = 1 << p.page_shift, held = p.table_pages << p.page_shift;
     const int g = blockIdx.x % p.kv_heads;
     int unit = blockIdx.x / p.kv_heads;
     const bool is_v = unit & 1;
     unit >>= 1;
     const int b = unit / a.slots, slot = unit - b * a.slots;
-    if (min(max(p.contexts[b], 0), held) <= a.budget) return;
+    const int first = (a.kept + slot) << SHIFT, count = min(kPage, a.budget - first);
+    const bool there = static_cast<int>(threadIdx.x) < count;
+    // What does not wait for anything is loaded together.
+    const int context = p.contexts[b];
     const int32_t id = a.into[static_cast<int64_t>(b) * a.slots + slot];
+    const int row = a.rows[(static_cast<int64_t>(b) * p.kv_heads + g) * a.budget + first + min(static_cast<int>(threadIdx.x), count - 1)];
+    if (min(max(context, 0), p.table_pages << SHIFT) <= a.budget) return;
     if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.pages)) return;
-    const int first = (a.kept + slot) << p.page_shift, count = min(page, a.budget - first);
     const int64_t to = static_cast<int64_t>(id) * p.kv_heads + g;
     if (threadIdx.x == 0) top = 0;
-    if (threadIdx.x < kMost) {
-        const bool there = static_cast<int>(threadIdx.x) < count;
-        const int row = there ? a.rows[(static_cast<int64_t>(b) * p.kv_heads + g) * a.budget + first + threadIdx.x] : 0;
-        const int32_t from = there ? p.table[static_cast<int64_t>(b) * p.table_pages + (row >> p.page_shift)] : -1;
+    if (threadIdx.x < kPage) {
+        const int32_t from = p.table[static_cast<int64_t>(b) * p.table_pages + (row >> SHIFT)];
         const bool on = static_cast<uint32_t>(from) < static_cast<uint32_t>(p.pages);
         const int64_t at = static_cast<int64_t>(on ? from : 0) * p.kv_heads + g;
-        const int offset = row & (page - 1);
-        source[threadIdx.x] = !on ? -1 : is_v ? at * D * page + offset : (at * page + offset) * D;
+        const int offset = row & (kPage - 1);
+        source[threadIdx.x] = is_v ? at * (D << SHIFT) + offset : ((at << SHIFT) + offset) * D;
+        reinterpret_cast<uint8_t*>(keep)[threadIdx.x] = on ? 0xff : 0;
         scales[threadIdx.x] = !there ? 0.0f : on ? (is_v ? p.v_scales : p.k_scales)[at] : 1.0f;
-        if (!is_v && there) a.weights[to * page + threadIdx.x] = on ? a.weights[at * page + offset] : __builtin_nanf("");
+        if (!is_v && there) a.weights[(to << SHIFT) + threadIdx.x] = on ? a.weights[(at << SHIFT) + offset] : __builtin_nanf("");
     }
     __syncthreads();
-    if (is_v) move_page<D, true>(a, b, slot, g, to, source, scales, top, count);
-    else move_page<D, false>(a, b, slot, g, to, source, scales, top, count);
+    if (is_v) move_page<D, SHIFT, true>(a, to, source, scales, keep, top, count);
+    else move_page<D, SHIFT, false>(a, to, source, scales, keep, top, count);
+}
+
+template <int D, int SHIFT>
+int launch_move_as(const EvictArgs& a, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(2 * static_cast<int64_t>(a.p.batch) * a.slots * a.p.kv_heads));
+    hipLaunchKernelGGL((k_evict_move<D, SHIFT>), grid, dim3(kMoveThreads<D, SHIFT>), 0, stream, a);
+    return nq::launch_status();
 }
 
 template <int D>
 int launch_move(const EvictArgs& a, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(2 * static_cast<int64_t>(a.p.batch) * a.slots * a.p.kv_heads)), block(kMoveThreads);
-    hipLaunchKernelGGL(k_evict_move<D>, grid, block, 0, stream, a);
-    return nq::launch_status();
+    switch (a.p.page_shift) {
+        case 4: return launch_move_as<D, 4>(a, stream);
+        case 5: return launch_move_as<D, 5>(a, stream);
+        case 6: return launch_move_as<D, 6>(a, stream);
+        default: return launch_move_as<D, 7>(a, stream);
+    }
 }
 
 constexpr int kFewKeys = 8, kManyKeys = 32;
@@ -426,7 +464,7 @@ extern "C" int64_t nq_paged_evict_workspace_bytes(int64_t batch, int32_t kv_head
         return -1;
     const int64_t parts = parts_of(batch * kv_heads, table_pages * page_size);
     if (!nq::launchable(batch * kv_heads * std::max<int64_t>(parts, 1), kSelectThreads)) return -1;
-    if (!nq::launchable(2 * batch * kv_heads * ((budget + page_size - 1) / page_size), kMoveThreads)) return -1;
+    if (!nq::launchable(2 * batch * kv_heads * ((budget + page_size - 1) / page_size), 256)) return -1;
     return batch * kv_heads * parts * kLevels * kBins * static_cast<int64_t>(sizeof(uint32_t));
 }
 
