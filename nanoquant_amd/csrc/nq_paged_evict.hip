@@ -91,6 +91,13 @@ __device__ __forceinline__ uint32_t key_at(const EvictArgs& a, const Sequence& s
     return on ? key : 0xffffffffu;
 }
 
+// The sum of the values of the waves before this one.
+__device__ __forceinline__ uint32_t waves_before(const uint32_t (&of)[kSelectWaves]) {
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const uint32_t v = lane < wave ? of[lane] : 0u;
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(running_sum(v)), kWave - 1));
+}
+
 // The bin of a level that the keep-th greatest key lies in, and how many keys are
 // greater than all of it: `above` of higher levels and those of this level's higher
 // bins. Thread t has bins kBins - 1 - 2 t and the one below. All threads get the answer.
@@ -104,8 +111,7 @@ __device__ __forceinline__ Bin find_bin(const uint32_t (&c)[2], uint32_t keep, u
     const uint32_t mine = c[0] + c[1], upto = running_sum(mine);
     if (lane == kWave - 1) waves[wave] = upto;
     __syncthreads();
-    uint32_t before = above + upto - mine;
-    for (int w = 0; w < wave; ++w) before += waves[w];
+    uint32_t before = above + upto - mine + waves_before(waves);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         if (before < keep && before + c[j] >= keep) {
@@ -189,11 +195,7 @@ __global__ __launch_bounds__(kSelectThreads) void k_evict_select(const EvictArgs
         counts[1][wave] = same;
     }
     __syncthreads();
-    Writer write = {prefix, static_cast<uint32_t>(s.keep) - above, 0, 0};
-    for (int w = 0; w < wave; ++w) {
-        write.more += counts[0][w];
-        write.same += counts[1][w];
-    }
+    Writer write = {prefix, static_cast<uint32_t>(s.keep) - above, waves_before(counts[0]), waves_before(counts[1])};
     for_each([&](int row, uint32_t key) { write(a, s, row, row < stop, key); });
 }
 
@@ -280,11 +282,8 @@ __global__ __launch_bounds__(kSelectThreads) void k_evict_part(const EvictArgs a
             counts[1][wave] = same;
         }
         __syncthreads();
-        Writer write = {prefix, static_cast<uint32_t>(s.keep) - above, passed[0], passed[1]};
-        for (int w = 0; w < wave; ++w) {
-            write.more += counts[0][w];
-            write.same += counts[1][w];
-        }
+        Writer write = {prefix, static_cast<uint32_t>(s.keep) - above, passed[0] + waves_before(counts[0]),
+                        passed[1] + waves_before(counts[1])};
 #pragma unroll
         for (int j = 0; j < kPartKeys; ++j) {
             const int row = begin + kWave * j + lane;
