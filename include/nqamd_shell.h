@@ -318,8 +318,8 @@ int nq_shared_attention(const void* q, int32_t q_dtype, int64_t tokens, int32_t 
  * nq_shared_attention left it for the same call. Pages that the rows from `first` on
  * lie in belong to one sequence and stand once in its part of the table; rows before
  * `first` may lie in pages that sequences share. A row whose table entry names no page is left
- * out. q as in nq_paged_attention; a weight never passes 1, is off by about 2^-22
- * of lse and of its score relative to itself, and NaN where they are. Sums in fp32
+ * out. q as in nq_paged_attention; a weight is off by about 2^-22 of lse and of its
+ * score relative to itself (never above 1 where lse is beyond 710), and NaN where they are. Sums in fp32
  * in a fixed order (deterministic). */
 int nq_attention_weights(const void* q, int32_t q_dtype, int64_t tokens, int32_t q_heads, const nq_paged_kv* kv,
                          float scaling, const float* lse, int64_t first, const float* weights, float* out,

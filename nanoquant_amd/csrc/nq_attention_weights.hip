@@ -17,7 +17,7 @@ namespace {
 
 using namespace nq::paged;
 
-constexpr int kWaves = 4;
+constexpr float kLarge = 1024.0f;  // log-sum-exps beyond this have weights held to 1
 
 struct WeightArgs {
     Pages p;
@@ -43,11 +43,17 @@ __device__ __forceinline__ float sum_rows(float (&w)[16], int n) {
     return w[0];
 }
 
+template <bool TURNS>
+constexpr int kWavesOf = TURNS ? 8 : 4;
+
 // TURNS: the waves of a workgroup hold the same cache rows and take the query rows in
 // turn; otherwise each wave has cache rows of its own and takes all query rows.
 template <int D, int QT, bool TURNS>
-__global__ __launch_bounds__(kWaves* kWave) void k_attention_weights(const WeightArgs a) {
+__global__ __launch_bounds__(kWavesOf<TURNS>* kWave) void k_attention_weights(const WeightArgs a) {
+    constexpr int kWaves = kWavesOf<TURNS>;
     constexpr int kChunks = D / 64, kQSteps = 2 * kChunks, QP = Query<QT>::kParts, kBlock = 16;
+    // Many query rows: K is widened once, and the next rows of q are on their way, where there are registers for it.
+    constexpr bool kHeld = TURNS && QT != NQ_DTYPE_F32 && D <= 128;
     __shared__ float join[TURNS ? kWaves : 1][kTile];
     const Pages& p = a.p;
     const int lane = threadIdx.x & (kWave - 1), n = lane & 15, grp = lane >> 4;
@@ -84,54 +90,100 @@ __global__ __launch_bounds__(kWaves* kWave) void k_attention_weights(const Weigh
         // Query rows before this see none of the tile's rows.
         const int64_t blind = static_cast<int64_t>(base) - context;
         const int from = blind > 0 ? static_cast<int>(min(blind * a.group, static_cast<int64_t>(all))) & ~15 : 0;
+        const int row = base + kBlock * grp + n;
+        const bool mine = row >= a.first && row < rows && static_cast<uint32_t>(id) < static_cast<uint32_t>(p.pages);
+        const int64_t place_of_row = base_of(id) * page + (row & (page - 1));
+        float old = 0.0f;
+        if (!TURNS || wave == 0) old = a.before[place_of_row];  // a page's row, whatever it is
+        u32x4 wide[kHeld ? 4 : 1][kHeld ? kQSteps : 1];
+        if constexpr (kHeld) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int c = 0; c < kQSteps; ++c) wide[t][c] = widen_k<QT>(kf[t][c / 2][2 * (c & 1)], kf[t][c / 2][2 * (c & 1) + 1]);
+        }
+        // 16 query rows: this lane's one, as the products take it.
+        struct Rows {
+            u32x4 part[kQSteps][QP];
+            float up, lse;
+            int pos;
+        };
+        const auto load = [&](int r0) {
+            Rows x;
+            const int r = r0 + n;
+            const bool on = r < all;
+            const int place = on ? r / a.group : 0, head = on ? g * a.group + r - place * a.group : 0;
+            x.pos = on ? row_of(context, place, cache_rows) : -1;
+            const int64_t at = static_cast<int64_t>(begin + place) * a.q_heads + head;
+            x.lse = on ? a.lse[at] : 0.0f;
+            x.up = load_query<QT, kQSteps>(a.q, at * D + 16 * grp, on, x.part);
+            return x;
+        };
         if (tile < tiles) {
-            for (int r0 = from + (TURNS ? 16 * wave : 0); r0 < all; r0 += TURNS ? 16 * kWaves : 16) {
-                const int r = r0 + n;
-                const bool on = r < all;
-                const int place = on ? r / a.group : 0, head = on ? g * a.group + r - place * a.group : 0;
-                const int pos = on ? row_of(context, place, cache_rows) : -1;
-                const int64_t row = static_cast<int64_t>(begin + place) * a.q_heads + head;
-                u32x4 part[kQSteps][QP];
-                const float f = k_scale * a.scale * load_query<QT, kQSteps>(a.q, row * D + 16 * grp, on, part);
-                const float lse = on ? a.lse[row] * 1.4426950408889634f : 0.0f;
+            constexpr int kStep = TURNS ? 16 * kWaves : 16;
+            int r0 = from + (TURNS ? 16 * wave : 0);
+            Rows x;
+            if (r0 < all) x = load(r0);
+            for (; r0 < all; r0 += kStep) {
+                Rows next;
+                if constexpr (kHeld) {
+                    next = load(min(r0 + kStep, all));  // behind the last one: nothing
+                } else {
+                    // K's bytes as the compiler may not know them: it would widen them all ahead of the
+                    // loop and take the registers of other waves (32 sequences: 33.6 us, 42.5 so).
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int c = 0; c < kChunks; ++c) asm volatile("" : "+v"(kf[t][c]));
+                }
                 f32x4 sc[4];
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     sc[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
                     for (int c = 0; c < kQSteps; ++c) {
-                        const u32x4 k = widen_k<QT>(kf[t][c / 2][2 * (c & 1)], kf[t][c / 2][2 * (c & 1) + 1]);
-                        if constexpr (QP == 2) sc[t] = mfma_k<QT>(lowered(k), part[c][1], sc[t]);
-                        sc[t] = mfma_k<QT>(k, part[c][0], sc[t]);
+                        u32x4 k;
+                        if constexpr (kHeld) k = wide[t][c];
+                        else k = widen_k<QT>(kf[t][c / 2][2 * (c & 1)], kf[t][c / 2][2 * (c & 1) + 1]);
+                        if constexpr (QP == 2) sc[t] = mfma_k<QT>(lowered(k), x.part[c][1], sc[t]);
+                        sc[t] = mfma_k<QT>(k, x.part[c][0], sc[t]);
                     }
                 }
-                const int seen = pos + 1 - (base + kBlock * grp);
+                const float f = k_scale * a.scale * x.up, lse = x.lse * 1.4426950408889634f;
+                const int seen = x.pos + 1 - (base + kBlock * grp);
+                const bool large = __ballot(fabsf(lse) > kLarge);
+                if (__ballot(seen < kBlock) || large) {
 #pragma unroll
-                for (int j = 0; j < kBlock; ++j) {
-                    float x = fmaf(sc[j >> 2][j & 3], f, -lse);
-                    x = x > 0.0f ? 0.0f : x;  // what rounding leaves above 0; NaN stays
-                    w[j] += j < seen ? exp2_hw(x) : 0.0f;
+                    for (int j = 0; j < kBlock; ++j) {
+                        float y = fmaf(sc[j >> 2][j & 3], f, -lse);
+                        if (large) y = y > 0.0f ? 0.0f : y;  // what rounding leaves above 0; NaN stays
+                        w[j] += j < seen ? exp2_hw(y) : 0.0f;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kBlock; ++j) w[j] += exp2_hw(fmaf(sc[j >> 2][j & 3], f, -lse));
                 }
+                if constexpr (kHeld) x = next;
+                else if (r0 + kStep < all) x = load(r0 + kStep);
             }
         }
         float total = sum_rows(w, n);
-        const int row = base + kBlock * grp + n;
         if constexpr (TURNS) {
             join[wave][lane] = total;
             __syncthreads();
-            if (wave == 0) total = (join[0][lane] + join[1][lane]) + (join[2][lane] + join[3][lane]);
+            total = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) total += join[i][lane];
         }
-        if ((!TURNS || wave == 0) && row >= a.first && row < rows && static_cast<uint32_t>(id) < static_cast<uint32_t>(p.pages)) {
-            const int64_t i = base_of(id) * page + (row & (page - 1));
-            a.out[i] = row < context ? a.before[i] + total : total;
-        }
+        if ((!TURNS || wave == 0) && mine) a.out[place_of_row] = row < context ? old + total : total;
         if constexpr (TURNS) __syncthreads();  // join is read
     }
 }
 
 template <int D, int QT>
 int launch_as(WeightArgs& a, bool turns, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.p.batch) * a.slots * a.p.kv_heads)), block(kWaves * kWave);
+    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.p.batch) * a.slots * a.p.kv_heads));
+    const dim3 block(static_cast<unsigned>((turns ? kWavesOf<true> : kWavesOf<false>) * kWave));
     if (turns) hipLaunchKernelGGL((k_attention_weights<D, QT, true>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((k_attention_weights<D, QT, false>), grid, block, 0, stream, a);
     return nq::launch_status();
@@ -171,9 +223,9 @@ extern "C" int nq_attention_weights(const void* q, int32_t q_dtype, int64_t toke
     a.first = static_cast<int32_t>(first);
     const bool turns = tokens * a.group > 64 * kv->batch;
     const int64_t tiles = (cache_rows + kTile - 1) / kTile - first / kTile, units = kv->batch * kv->kv_heads;
-    const int64_t most = turns ? tiles : (tiles + kWaves - 1) / kWaves;
+    const int64_t most = turns ? tiles : (tiles + kWavesOf<false> - 1) / kWavesOf<false>;
     a.slots = static_cast<int32_t>(std::max(int64_t{1}, std::min(most, (4096 + units - 1) / units)));
-    if (!nq::launchable(units * a.slots, kWaves * kWave)) return NQ_ERR_SHAPE;
+    if (!nq::launchable(units * a.slots, kWavesOf<true> * kWave)) return NQ_ERR_SHAPE;
     hipStream_t st = static_cast<hipStream_t>(stream);
     switch (kv->head_dim) {
         case 64: return launch_for<64>(a, q_dtype, turns, st);
