@@ -35,6 +35,8 @@ each PAGE_ROWS rows and head): every pass then appends with
 ``launch_paged_append`` and attends with ``launch_paged_attention``. It is there
 for the memory: a step takes 1.97 ms on the 36-layer Qwen3-8B geometry with 640 positions,
 1.66 with the bf16 cache, and 2.06 against 1.91 with 4096.
+With 4-bit ``lm_head`` weights (``shell_ops.int4_matrix``) the output projection is
+``launch_int4_projection``, which reads a quarter of the bf16 matrix's bytes.
 ``generate_greedy_scored`` and ``score`` report how likely an answer or a given
 text is (``launch_token_logprobs``).
 
@@ -135,7 +137,7 @@ class DecoderLayerWeights:
 @dataclass
 class DecoderShellWeights:
     embed: torch.Tensor  # [vocab, hidden] bf16
-    lm_head: torch.Tensor  # [vocab, hidden] bf16
+    lm_head: torch.Tensor | ops.Int4Matrix  # [vocab, hidden] bf16, or 4-bit (``ops.int4_matrix``)
     final_norm: torch.Tensor  # [hidden]
     layers: list[DecoderLayerWeights] = field(default_factory=list)
 
@@ -197,7 +199,10 @@ def load_decoder_weights(
 
 def dense_tensors(weights: DecoderShellWeights, dense_names: dict[str, str] = QWEN3_DENSE_NAMES) -> dict[str, torch.Tensor]:
     """The dense tensors of `weights` under checkpoint names (inverse of the
-    dense part of ``load_decoder_weights``)."""
+    dense part of ``load_decoder_weights``). A 4-bit ``lm_head`` is none of them."""
+
+    if isinstance(weights.lm_head, ops.Int4Matrix):
+        raise DecoderShellError("a 4-bit lm_head is not a dense checkpoint tensor")
 
     out = {dense_names["embed"]: weights.embed, dense_names["lm_head"]: weights.lm_head,
            dense_names["final_norm"]: weights.final_norm}
@@ -287,7 +292,12 @@ class PackedDecoder:
         self.backend = backend or HipPackedBackend(prefill_operands=operands)
         dev = self.device
         self.embed = weights.embed.to(dev, torch.bfloat16).contiguous()
-        self.lm_head = weights.lm_head.to(dev, torch.bfloat16).contiguous()
+        if isinstance(weights.lm_head, ops.Int4Matrix):
+            if weights.lm_head.shape != (c.vocab, c.hidden):
+                raise DecoderShellError("lm_head shape does not match the configuration")
+            self.lm_head = weights.lm_head.to(dev)
+        else:
+            self.lm_head = weights.lm_head.to(dev, torch.bfloat16).contiguous()
         self.final_norm = weights.final_norm.to(dev).contiguous()
         self.layers: list[dict[str, PreparedLayer]] = []
         self.norms: list[tuple[torch.Tensor, torch.Tensor, torch.Tensor | None, torch.Tensor | None]] = []
@@ -339,7 +349,10 @@ class PackedDecoder:
         self.ids = torch.zeros(1, dtype=torch.int64, device=dev)
         self.history = torch.zeros(history_capacity, dtype=torch.int64, device=dev)
         self.logits = torch.empty(c.vocab, dtype=torch.float32, device=dev)
-        self.proj_ws = torch.empty(ops.output_projection_workspace_bytes(c.vocab, c.hidden), dtype=torch.uint8, device=dev)
+        if isinstance(self.lm_head, ops.Int4Matrix):
+            self.proj_ws = torch.empty(ops.int4_projection_partials(c.vocab), dtype=torch.int64, device=dev)
+        else:
+            self.proj_ws = torch.empty(ops.output_projection_workspace_bytes(c.vocab, c.hidden), dtype=torch.uint8, device=dev)
         self._decode_bufs: _Buffers | None = None
         self._graphs: dict[int, torch.cuda.CUDAGraph] = {}
         self.host_position = 0
@@ -463,7 +476,15 @@ class PackedDecoder:
             ops.launch_silu_mul(b.gate, b.up, out=b.act)
             self._linears([b.act], [prepared["down_proj"]], [b.down], t)
         ops.launch_add_rmsnorm(b.residual, self.final_norm, c.eps, delta=None if fused else b.down, out=b.final)
-        ops.launch_output_projection(b.final[t - 1], self.lm_head, logits=self.logits, workspace=self.proj_ws)
+        self._project(b.final[t - 1], self.logits, self.proj_ws)
+
+    def _project(self, x: torch.Tensor, logits: torch.Tensor, partials: torch.Tensor) -> None:
+        """Logits of one row and what the greedy selection chooses by."""
+
+        if isinstance(self.lm_head, ops.Int4Matrix):
+            ops.launch_int4_projection(x[None], self.lm_head, out=logits[None], partials=partials)
+        else:
+            ops.launch_output_projection(x, self.lm_head, logits=logits, workspace=partials)
 
     def _decode_body(self) -> None:
         assert self._decode_bufs is not None
@@ -537,7 +558,8 @@ class PackedDecoder:
         the ids before it, the entropy of that distribution and its `top`
         likeliest tokens. One prompt pass, then the output projection row by row
         (the logits that a decode step at that row would see, 0.18 ms each at
-        151936 x 4096) and one ``launch_token_logprobs`` for SCORE_ROWS rows. Leaves the decoder as
+        151936 x 4096; with a 4-bit ``lm_head`` SCORE_ROWS rows at once) and one
+        ``launch_token_logprobs`` for SCORE_ROWS rows. Leaves the decoder as
         ``prefill(ids)`` does."""
 
         c = self.config
@@ -553,8 +575,11 @@ class PackedDecoder:
         partials = torch.empty_like(self.proj_ws)  # proj_ws keeps the last row's
         for first in range(0, rows, SCORE_ROWS):
             n = min(SCORE_ROWS, rows - first)
-            for i in range(n):
-                ops.launch_output_projection(b.final[first + i], self.lm_head, logits=logits[i], workspace=partials)
+            if isinstance(self.lm_head, ops.Int4Matrix):  # many rows at once: each reads the matrix less often
+                ops.launch_int4_projection(b.final[first:first + n], self.lm_head, out=logits[:n])
+            else:
+                for i in range(n):
+                    self._project(b.final[first + i], logits[i], partials)
             ops.launch_token_logprobs(logits[:n], ids[first + 1:first + 1 + n], top=top,
                                       out=ops.TokenLogprobs(*(x[first:first + n] for x in out)))
         return out
