@@ -168,7 +168,7 @@ int nq_greedy_select(const void* workspace, int64_t vocab, int64_t hidden, int64
 int nq_greedy_select_partials(const void* partials, int64_t count, int64_t* token_out, int64_t* history,
                               int64_t history_capacity, int32_t* step, int32_t* position, void* stream);
 
-/* Workspace bytes of nq_int4_projection (-1: refused sizes). */
+/* Workspace bytes of nq_int4_projection (0: none needed; -1: refused sizes). */
 int64_t nq_int4_projection_workspace_bytes(int64_t tokens, int64_t out_features, int64_t in_features, int32_t group);
 
 /* Partials (8 bytes each) that nq_int4_projection leaves for one token. */
@@ -177,7 +177,7 @@ int64_t nq_int4_projection_partials(int64_t out_features);
 /* Products with 4-bit weights and group scales:
  *   y[t, o] = sum_i scales[o, i / group] * (w[o, i] - zeros[o, i / group]) * x[t, i]
  * x F32/F16/BF16 [tokens, in_features] (1 to 65535 tokens; the form is that of a few: the weights
- * are read once for up to 5 tokens with groups of 128, 2 with 64 and 1 with 32); packed
+ * are read once for up to 30 tokens with groups of 128, 12 with 64 and 6 with 32); packed
  * [out_features, in_features / 2], byte j of a row holding column 2 j in its low
  * four bits and 2 j + 1 in its high ones, 16-byte aligned; scales F32/F16/BF16 [out_features,
  * ceil(in_features / group)], zeros uint8 of the same shape (NULL: 8), any value
@@ -346,7 +346,7 @@ int64_t nq_paged_evict_workspace_bytes(int64_t batch, int32_t kv_heads, int32_t 
  * touched, and rows_out has its rows, then -1. Rows in pages that the
  * table does not name count as NaN; an entry of into that names no page writes nothing but
  * page_table_out. into's pages stand there once, and in no sequence's part of the page table.
- * Values beyond fp32 become NaN. kv->query_starts is not read and may be NULL.
+ * Values beyond fp32 become NaN. Outputs lie apart from the arrays that the call reads. kv->query_starts is not read and may be NULL.
  * first + recent <= budget. Keys keep the rotation of their position: the
  * tokens appended next have other positions than cache rows (nq_paged_append_at). */
 int nq_paged_evict(const nq_paged_kv* kv, float* weights, const int32_t* into, int64_t budget, int64_t first,

@@ -492,6 +492,8 @@ extern "C" int nq_paged_evict(const nq_paged_kv* kv, float* weights, const int32
     a.kept = static_cast<int32_t>(first / kv->page_size);
     a.slots = a.entries - a.kept;
     if (a.slots > 0 && !into) return NQ_ERR_ARGUMENT;
+    // Other workgroups still read what one would write there.
+    if (page_table_out == kv->page_table || context_lens_out == kv->context_lens) return NQ_ERR_ARGUMENT;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int64_t units = kv->batch * kv->kv_heads;
     a.parts = static_cast<int32_t>(parts_of(units, kv->table_pages * kv->page_size));

@@ -486,11 +486,19 @@ class PackedDecoder:
         else:
             ops.launch_output_projection(x, self.lm_head, logits=logits, workspace=partials)
 
+    def _select(self, position: torch.Tensor | None = None) -> None:
+        """The token of the logits last projected, into ``ids`` and ``history``."""
+
+        out = {"token_out": self.ids, "history": self.history, "step": self.step, "position": position}
+        if isinstance(self.lm_head, ops.Int4Matrix):
+            ops.launch_greedy_select_partials(self.proj_ws, **out)
+        else:
+            ops.launch_greedy_select(self.proj_ws, self.config.vocab, self.config.hidden, **out)
+
     def _decode_body(self) -> None:
         assert self._decode_bufs is not None
         self._forward(self.ids, self._decode_bufs)
-        ops.launch_greedy_select(self.proj_ws, self.config.vocab, self.config.hidden, token_out=self.ids,
-                                 history=self.history, step=self.step, position=self.position)
+        self._select(position=self.position)
 
     def _decode_graph(self, steps: int = 1) -> torch.cuda.CUDAGraph:
         """Capture `steps` consecutive one-token steps once (each step reads
@@ -610,7 +618,7 @@ class PackedDecoder:
         workspace = torch.empty(ops.token_logprobs_workspace_bytes(1, c.vocab, top), dtype=torch.uint8, device=self.device)
         self.reset()
         self.prefill(prompt)
-        ops.launch_greedy_select(self.proj_ws, c.vocab, c.hidden, token_out=self.ids, history=self.history, step=self.step)
+        self._select()
         for i in range(max_new_tokens):
             if i and graph is not None:
                 graph.replay()
@@ -651,8 +659,7 @@ class PackedDecoder:
         if events:
             events[0].record()
         self.prefill(prompt)
-        ops.launch_greedy_select(self.proj_ws, self.config.vocab, self.config.hidden, token_out=self.ids,
-                                 history=self.history, step=self.step)
+        self._select()
         if events:
             events[1].record()
         if graph is None:

@@ -424,8 +424,34 @@ def launch_greedy_select(
 ) -> torch.Tensor:
     """Greedy token (lowest index among equal maxima, like ``torch.argmax``) from
     the partials of ``launch_output_projection``, written to ``token_out[0]``;
-    optionally appended to ``history`` at ``step`` and advancing ``position``.
-    The partials of ``launch_int4_projection`` are an int64 tensor, and are known by that."""
+    optionally appended to ``history`` at ``step`` and advancing ``position``."""
+
+    after = _greedy_outputs(workspace, token_out, history, step, position)
+    status = _native.load().nq_greedy_select(workspace.data_ptr(), vocab, hidden, *after)
+    _native.check("nq_greedy_select", status)
+    return token_out
+
+
+def launch_greedy_select_partials(
+    partials: torch.Tensor,
+    *,
+    token_out: torch.Tensor,
+    history: torch.Tensor | None = None,
+    step: torch.Tensor | None = None,
+    position: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``launch_greedy_select`` from the int64 partials of ``launch_int4_projection``."""
+
+    if partials.dtype is not torch.int64 or partials.ndim != 1 or not partials.numel():
+        raise ValueError("greedy select partials must be int64 [count]")
+    after = _greedy_outputs(partials, token_out, history, step, position)
+    status = _native.load().nq_greedy_select_partials(partials.data_ptr(), partials.numel(), *after)
+    _native.check("nq_greedy_select_partials", status)
+    return token_out
+
+
+def _greedy_outputs(workspace, token_out, history, step, position) -> tuple:
+    """Checks of what a greedy selection writes; its arguments in C."""
 
     device = workspace.device
     if token_out.dtype != torch.int64 or token_out.numel() < 1:
@@ -437,17 +463,8 @@ def launch_greedy_select(
     if position is not None:
         _position("greedy select", position, device)
     _check_device("greedy select", device, workspace, token_out, history, step, position)
-    after = (token_out.data_ptr(), _ptr(history), 0 if history is None else history.numel(), _ptr(step), _ptr(position),
-             _stream(device))
-    if workspace.dtype is torch.int64:
-        if workspace.numel() != int4_projection_partials(vocab):
-            raise ValueError("greedy select takes the partials of a projection to the vocabulary")
-        status = _native.load().nq_greedy_select_partials(workspace.data_ptr(), workspace.numel(), *after)
-        _native.check("nq_greedy_select_partials", status)
-        return token_out
-    status = _native.load().nq_greedy_select(workspace.data_ptr(), vocab, hidden, *after)
-    _native.check("nq_greedy_select", status)
-    return token_out
+    return (token_out.data_ptr(), _ptr(history), 0 if history is None else history.numel(), _ptr(step), _ptr(position),
+            _stream(device))
 
 
 # -- 4-bit weights ---------------------------------------------------------------
@@ -527,7 +544,7 @@ def launch_int4_projection(
     """``x @ W.T`` of F32/F16/BF16 ``x`` ``[tokens, in]`` and 4-bit weights, for a few
     tokens (nq_int4_projection): fp32 sums, rounded once to ``out``. For one
     token ``partials`` (int64 ``[int4_projection_partials(out)]``) get what
-    ``launch_greedy_select`` chooses by. Beside ``launch_output_projection``, at a
+    ``launch_greedy_select_partials`` chooses by. Beside ``launch_output_projection``, at a
     quarter of its weight's bytes (src/nanoquant/runtime/cuda_kernels.py:684-712)."""
 
     device = x.device

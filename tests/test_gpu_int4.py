@@ -128,7 +128,7 @@ def test_zeros_of_any_value_and_scales_that_are_zero_or_negative():
     check(ops.launch_int4_projection(x.to(DEV), m.to(DEV)), x, m, 32)
 
 
-@pytest.mark.parametrize("outs,ins,group", [(1, 32, 32), (16, 64, 32), (1000, 256, 64), (50257, 128, 128)])
+@pytest.mark.parametrize("outs,ins,group", [(1, 32, 32), (16, 64, 32), (1000, 256, 64), (50257, 128, 128), (1000, 14336, 64)])
 def test_partials_select_the_first_largest(outs, ins, group):
     m = matrix(outs, ins, group, torch.float16, False, 551)
     if outs > 900:
@@ -141,7 +141,7 @@ def test_partials_select_the_first_largest(outs, ins, group):
     partials = torch.zeros(ops.int4_projection_partials(outs), dtype=torch.int64, device=DEV)
     logits = ops.launch_int4_projection(x.to(DEV), m.to(DEV), partials=partials)
     token = torch.zeros(1, dtype=torch.int64, device=DEV)
-    ops.launch_greedy_select(partials, outs, ins, token_out=token)
+    ops.launch_greedy_select_partials(partials, token_out=token)
     row = logits[0].cpu()
     assert int(token) == int((row == row.max()).nonzero()[0])
     if outs > 900:
@@ -177,3 +177,34 @@ def test_captured_calls_replay_with_other_inputs():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, eager)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_values_at_any_address(dtype):
+    """x, scales, zeros and outputs that begin between their type's vectors."""
+
+    m = matrix(50, 160, 32, dtype, True, 581)
+
+    def moved(t):
+        flat = torch.zeros(t.numel() + 3, dtype=t.dtype, device=DEV)
+        flat[3:] = t.reshape(-1).to(DEV)
+        return flat[3:].view(t.shape)
+
+    x = torch.randn(3, 160, generator=_g(582)).to(dtype)
+    at = ops.Int4Matrix(m.packed.to(DEV), moved(m.scales), moved(m.zeros))
+    out = moved(torch.zeros(3, 50, dtype=dtype))
+    check(ops.launch_int4_projection(moved(x), at, out=out), x, m, 32)
+
+
+def test_work_on_another_stream_with_a_workspace_of_the_callers():
+    m = matrix(300, 10240, 64, torch.float16, False, 591).to(DEV)
+    x = torch.randn(9, 10240, generator=_g(592)).to(DEV)
+    here = ops.launch_int4_projection(x, m)
+    size = ops.int4_projection_workspace_bytes(9, m)
+    assert size > 0
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        there = ops.launch_int4_projection(x, m, workspace=torch.empty(size, dtype=torch.uint8, device=DEV))
+    side.synchronize()
+    assert torch.equal(here, there)

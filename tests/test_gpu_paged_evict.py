@@ -146,6 +146,26 @@ def test_sources_that_sequences_share_stay():
     run_and_check(b, weights, into, page=16, budget=90, first=40, recent=10)
 
 
+def test_outputs_and_workspace_of_the_callers():
+    b, weights, into = evict_batch([9000, 40], kv=2, d=64, page=64, budget=100, first=3, seed=356)
+    cache, batch = b.device()
+    into = torch.tensor(into, dtype=torch.int32, device=DEV)
+    w = weights.to(DEV)
+    args = {"page_table": batch["page_table"], "context_lens": batch["context_lens"], "into": into, "budget": 100, "first": 3}
+    expected = ops.launch_paged_evict(cache, w, **args)
+    size = ops.paged_evict_workspace_bytes(2, cache, batch["page_table"].shape[1], 100)
+    assert size > 0
+    out = ops.Evicted(*(torch.full_like(x, -9) for x in expected))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        got = ops.launch_paged_evict(cache, w, out=out, workspace=torch.empty(size, dtype=torch.uint8, device=DEV), **args)
+    side.synchronize()
+    assert all(x is y for x, y in zip(got, out)) and all(torch.equal(x, y) for x, y in zip(got, expected))
+    with pytest.raises(ValueError, match="outputs"):
+        ops.launch_paged_evict(cache, w, out=out._replace(rows=out.rows[:1]), **args)
+
+
 def test_many_sequences():
     g = _g(360)
     contexts = torch.randint(0, 90, (150,), generator=g).tolist()

@@ -152,6 +152,26 @@ def test_rows_without_a_place():
         assert (out[t] == 0).all() and (lse[t] == -math.inf).all()
 
 
+def test_work_on_another_stream_with_a_workspace_of_the_callers():
+    b = shared_batch([(500, 1), (410, 3), (330, 1)], 320, kv=2, d=128, page=32, seed=165)
+    q = torch.randn(b.tokens, 8, 128, generator=generator(166)).to(DEV)
+    cache, batch = b.device()
+    args = {"shared_rows": 320, "scaling": 0.1, **batch}
+    here = ops.launch_shared_attention(q, cache, **args)
+    size = ops.shared_attention_workspace_bytes(b.tokens, 3, 8, cache, batch["page_table"].shape[1], 320)
+    assert size > 0
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        there = ops.launch_shared_attention(q, cache, workspace=torch.empty(size, dtype=torch.uint8, device=DEV), **args)
+    side.synchronize()
+    assert torch.equal(here, there)
+    with pytest.raises(ValueError, match="lse"):
+        ops.launch_shared_attention(q, cache, lse=torch.empty(b.tokens, 9, device=DEV), **args)
+    with pytest.raises(ValueError, match="shared_rows"):
+        ops.launch_shared_attention(q, cache, **{**args, "shared_rows": 10**6})
+
+
 def test_captured_calls_replay_with_other_lengths():
     """Two graphs with workspaces of their own, and other lengths under one capture."""
 

@@ -30,7 +30,7 @@ def _weigh(kv, *, q=A, dtype=0, tokens=3, q_heads=4, scaling=0.1, lse=A, first=0
     return _native.load().nq_attention_weights(q, dtype, tokens, q_heads, ctypes.byref(kv), scaling, lse, first, weights, out, None)
 
 
-def _evict(kv, *, weights=A, into=A, budget=40, first=0, recent=0, table=A, lens=A, rows=A, workspace=A, size=1 << 40):
+def _evict(kv, *, weights=A, into=A, budget=40, first=0, recent=0, table=2 * A, lens=2 * A, rows=A, workspace=A, size=1 << 40):
     return _native.load().nq_paged_evict(ctypes.byref(kv), weights, into, budget, first, recent, table, lens, rows, workspace, size,
                                          None)
 
@@ -92,6 +92,7 @@ def test_attention_weights(arguments, status):
 
 @pytest.mark.parametrize("arguments,status", [
     ({"weights": None}, -1), ({"into": None}, -1), ({"table": None}, -1), ({"lens": None}, -1), ({"rows": None}, -1),
+    ({"table": A}, -1), ({"lens": A}, -1),  # in place of what the call reads
     ({"budget": 0}, -3), ({"first": -1}, -3), ({"recent": -1}, -3), ({"first": 41}, -3), ({"first": 20, "recent": 21}, -3),
     ({"budget": 1 << 30}, -3),
 ])
