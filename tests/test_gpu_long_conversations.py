@@ -141,3 +141,37 @@ def test_a_conversation_within_a_budget(dtype):
     assert positions == [113, 119, 77]
     step([1, 1, 1], shared)
     step([6, 2, 1], shared)
+
+
+def test_offsets_beyond_32_bits():
+    """The last pages of a cache of 4.6 GB each for K and V give what the same pages
+    give in a small one."""
+
+    kv, d, page, pages, few = 8, 128, 64, 70000, 24
+    g = torch.Generator(device=DEV).manual_seed(431)
+    big, small = ops.paged_cache(pages, kv, page, d, DEV), ops.paged_cache(few, kv, page, d, DEV)
+    for x, y in ((small.k, big.k), (small.v, big.v)):
+        x.view(torch.uint8).copy_(torch.randint(0, 0x7f, x.shape, generator=g, device=DEV, dtype=torch.uint8))
+        y.view(torch.uint8)[-few:] = x.view(torch.uint8)
+    for x, y in ((small.k_scales, big.k_scales), (small.v_scales, big.v_scales)):
+        x.fill_(2.0**-9)
+        y.fill_(2.0**-9)
+    weights = torch.rand(few, kv, page, generator=g, device=DEV)
+    big_weights = torch.zeros(pages, kv, page, device=DEV)
+    big_weights[-few:] = weights
+    table = torch.arange(16, dtype=torch.int32, device=DEV).view(2, 8)
+    table[1, :2] = table[0, :2]
+    into = torch.arange(16, 24, dtype=torch.int32, device=DEV).view(2, 4)
+    batch = {"query_starts": torch.tensor([0, 1, 3], dtype=torch.int32, device=DEV),
+             "context_lens": torch.tensor([500, 400], dtype=torch.int32, device=DEV)}
+    q = torch.randn(3, 32, d, generator=g, device=DEV)
+    results = []
+    for cache, w, ahead in ((small, weights, 0), (big, big_weights, pages - few)):
+        lse = torch.empty(3, 32, device=DEV)
+        out = ops.launch_shared_attention(q, cache, page_table=table + ahead, shared_rows=128, scaling=0.05, lse=lse, **batch)
+        ops.launch_attention_weights(q, cache, lse, w, page_table=table + ahead, scaling=0.05, first=128, **batch)
+        got = ops.launch_paged_evict(cache, w, page_table=table + ahead, context_lens=batch["context_lens"], into=into + ahead,
+                                     budget=300, first=70, recent=30)
+        results.append([out, lse, got.page_table - ahead, got.rows, w[-few:], cache.k.view(torch.uint8)[-few:],
+                        cache.v.view(torch.uint8)[-few:], cache.k_scales[-few:], cache.v_scales[-few:]])
+    assert all(torch.equal(x, y) for x, y in zip(*results))
