@@ -46,6 +46,10 @@ __device__ __forceinline__ float sum_rows(float (&w)[16], int n) {
 template <bool TURNS>
 constexpr int kWavesOf = TURNS ? 8 : 4;
 
+// Single tokens are bound by the wait for the table's entries and then for K and q
+// (32 sequences of up to 4000 rows: 81 MB in 33.4 us; pages of 16 rows are 2 KB of K each). Prompts are bound by the vector
+// unit: 16 exponentials, 16 fused and 16 plain additions a product of 16 rows (1531 tokens
+// after 517: 8e9 products and sums in 53 us, the first rows' workgroups the last to end).
 // TURNS: the waves of a workgroup hold the same cache rows and take the query rows in
 // turn; otherwise each wave has cache rows of its own and takes all query rows.
 template <int D, int QT, bool TURNS>
@@ -180,6 +184,15 @@ __global__ __launch_bounds__(kWavesOf<TURNS>* kWave) void k_attention_weights(co
     }
 }
 
+// Whether the waves of a workgroup take the query rows of one tile in turn (`rows` of
+// a sequence, `waves` tiles of all): where tiles are too few for the chip, or there are so many rows
+// that the last tiles' would keep it waiting. bf16, 32/8 heads of 128, in turn and not:
+// one sequence after 512 rows, 32 tokens (128 rows) 9.0 and 13.6 us, 128 tokens 13 and 33, 1531
+// tokens 53 and 269; four of 512 tokens (512 tiles) 45 and 100; eight after 1000 (1088 tiles), 64 tokens (256 rows) 47
+// and 27, 128 tokens 56 and 43, 512 tokens (2048 rows) 129 and 141; 32 of 64 tokens 95 and 38. Up to 64
+// rows a wave has four products' worth: never.
+bool takes_turns(int64_t rows, int64_t waves) { return rows > 64 && (waves < 768 || rows > 1024); }
+
 template <int D, int QT>
 int launch_as(WeightArgs& a, bool turns, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.p.batch) * a.slots * a.p.kv_heads));
@@ -221,9 +234,11 @@ extern "C" int nq_attention_weights(const void* q, int32_t q_dtype, int64_t toke
     a.q_heads = q_heads;
     a.group = q_heads / kv->kv_heads;
     a.first = static_cast<int32_t>(first);
-    const bool turns = tokens * a.group > 64 * kv->batch;
     const int64_t tiles = (cache_rows + kTile - 1) / kTile - first / kTile, units = kv->batch * kv->kv_heads;
+    const bool turns = takes_turns((tokens * a.group + kv->batch - 1) / kv->batch, units * tiles);
     const int64_t most = turns ? tiles : (tiles + kWavesOf<false> - 1) / kWavesOf<false>;
+    // (32 sequences of one token after up to 4000 rows, 8 heads: 33.7 us with 4096 or 8192 workgroups, 36.3 with
+    // 2048, 39.8 with 1024.)
     a.slots = static_cast<int32_t>(std::max(int64_t{1}, std::min(most, (4096 + units - 1) / units)));
     if (!nq::launchable(units * a.slots, kWavesOf<true> * kWave)) return NQ_ERR_SHAPE;
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -176,6 +176,11 @@ __device__ __forceinline__ void digits_of(const float (&x)[8], uint32_t (&even)[
     unit = finite ? __uint_as_float(static_cast<uint32_t>(k - 22 + 127) << 23) : __builtin_nanf("");
 }
 
+// Large matrices of one token are bound by their bytes (151936 x 4096: 321 MB in 54.9 us, 5.9
+// TB/s, where a copy reaches 5.04): every load takes 256 bytes of a row (64 of each of 16
+// rows, as the products want them, took 70.7 us), LDS turns them. Small ones wait for x, then
+// for the digits and the weights (6912 x 1152: 5.9 us, a launch 1.65). With more tokens than a
+// block has the products' operands come from LDS, 2 KB a chunk and block, and bound it.
 // A workgroup has a slice of the chunks and, share waves to a tile of 16 rows, kWaves / share tiles
 // at a time; the waves of a tile each take a part of a stage's chunks. NB blocks of tokens.
 template <int G, int NB, int ST, int kWaves>
@@ -446,6 +451,18 @@ size_t lds_bytes(int waves, int tokens, int blocks, int groups, int stage) {
            static_cast<size_t>(waves) * wave * sizeof(float);
 }
 
+// How a call is laid out. A workgroup makes the digits of its tokens and slice itself, in
+// LDS, from x (2 to 4 bytes a value from the L2; a launch of its own for them took 4 us).
+//  - One token's digits fit LDS for the whole row (12 KB at 4096 columns). Waves have tiles of
+//    their own from 2048 tiles on, fewer tiles are shared by four waves (4096 columns, one token:
+//    4096 rows 6.5 us shared and 10.2 not, 14336 rows 10.8 and 11.4, 24576 13.6 and 13.7, 32768 16.6 and 15.2).
+//    768 workgroups walk over the tiles of a large matrix (151936 rows 59.4 us; with 512 65.7, 1024
+//    64.6, all at once 64.7, before what LDS has was read ahead: 54.9 since).
+//  - Digits of many tokens that LDS does not hold and few tiles: slices of the row, as many as make 2048 waves,
+//    eight waves of one slice around the same digits, joined in a second launch (11 tokens, 2560 x
+//    10240, groups of 64: 18.3 us; four waves 21.2, 1280 waves 25.3, 2560 waves 28.8).
+//  - Otherwise the row in stages, whose digits are made one after the other.
+// Blocks: more of them read the weights once for more tokens, and hold more registers.
 Int4Plan plan_int4(int64_t tokens, int64_t outs, int64_t ins, int group) {
     constexpr size_t kBudget = 60 * 1024;
     const int groups = kChunk / group, each = 16 / groups / kDigits;

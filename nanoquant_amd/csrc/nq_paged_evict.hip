@@ -143,8 +143,8 @@ struct Writer {
 };
 
 // One workgroup per sequence and kv head. Up to 1024 R rows wait in registers as
-// their keys; more are read again for each level. 24 sequences of up to 6001 rows: see
-// the entry point.
+// their keys; more are read again for each level. Bound by its rounds: table, weights,
+// three levels of counting in LDS (24 sequences of up to 6001 rows, 4 heads: 8.8 us).
 template <int R>
 __global__ __launch_bounds__(kSelectThreads) void k_evict_select(const EvictArgs a) {
     __shared__ uint32_t bins[kBins], counts[2][kSelectWaves], found[2];
@@ -296,14 +296,23 @@ __global__ __launch_bounds__(kSelectThreads) void k_evict_part(const EvictArgs a
 template <int D, int SHIFT>
 constexpr int kMoveThreads = (D << SHIFT) <= 4096 ? 64 : (D << SHIFT) <= 8192 ? 128 : 256;
 
+// Source pages that V's rows of a fresh page come from, first to last, up to which they
+// are read whole, in 16-byte pieces, and their bytes picked from LDS: scattered bytes go
+// to the memory pipe one lane at a time. 131000 rows, pages of 128, cut to a half (2 or 3 pages each) 115 us,
+// 163 gathered; to a quarter 94 and 108; to an eighth (8 or 9) 85 and 86; to a thirty-second 87 and 82. Pages
+// of 16: to a half 121 and 159, to an eighth 84 and 78, to a thirty-second 82 and 47.
+constexpr int kMostSpan = 8;
+
 // One workgroup per sequence, fresh page, kv head and K or V. A thread holds its
 // share of the page's bytes in registers until the page's scale is known: 16-byte
 // pieces of K's rows, words of four rows of V's lines, whose bytes it gathers. A page
 // waits for its rows' numbers, their pages and their bytes one after the other and
-// does little in between, so small pages take one wave: as many of them as possible wait at once.
+// does little in between, so small pages take one wave: as many of them as possible wait
+// at once (24 sequences to 2000 rows, pages of 32 rows of 64: 23.0 us the call, 34.3 with 256 threads each).
 template <int D, int SHIFT, bool IS_V>
 __device__ __forceinline__ void move_page(const EvictArgs& a, int64_t to, const int64_t* source, const float* scales,
-                                          const uint32_t* keep, uint32_t& top, int count) {
+                                          const uint32_t* keep, uint32_t& top, int count, const int* place,
+                                          const int32_t* table, int span, int g, u32x4* block) {
     constexpr int kThreads = kMoveThreads<D, SHIFT>, kPage = 1 << SHIFT, kBytes = D << SHIFT;
     constexpr int kUnits = kBytes / (IS_V ? 4 : 16) / kThreads, kWords = IS_V ? 1 : 4;
     constexpr int kAtOnce = IS_V && kUnits > 16 ? 16 : kUnits;
@@ -314,20 +323,57 @@ __device__ __forceinline__ void move_page(const EvictArgs& a, int64_t to, const 
     const auto row_of_unit = [&](int i) { return IS_V ? 4 * quad : i / (D / 16); };
     uint32_t w[kUnits][kWords];
     if constexpr (IS_V) {
-        const uint8_t* from[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) from[j] = p.v + source[4 * quad + j];
         const uint32_t kept = keep[quad];
+        if (span <= kMostSpan) {
+            // Whole source pages through LDS, the next one on its way while bytes are picked.
+            constexpr int kPieces = kBytes / 16 / kThreads;
+            static_assert(kPieces * 16 * kThreads == kBytes, "a page is whole rounds of 16-byte pieces");
+            u32x4 piece[kPieces];
+            const auto load = [&](int i) {
+                const int32_t id = table[i];
+                const int64_t at = (static_cast<uint32_t>(id) < static_cast<uint32_t>(p.pages) ? static_cast<int64_t>(id) : 0) * p.kv_heads + g;
 #pragma unroll
-        for (int k0 = 0; k0 < kUnits; k0 += kAtOnce) {
-            uint32_t bytes[kAtOnce][4];
+                for (int k = 0; k < kPieces; ++k)
+                    piece[k] = reinterpret_cast<const u32x4*>(p.v + at * kBytes)[threadIdx.x + k * kThreads];
+            };
+            int mine[4];
 #pragma unroll
-            for (int k = 0; k < kAtOnce; ++k)
+            for (int j = 0; j < 4; ++j) mine[j] = place[4 * quad + j];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) bytes[k][j] = from[j][((threadIdx.x + (k0 + k) * kThreads) / (kPage / 4)) * kPage];
+            for (int k = 0; k < kUnits; ++k) w[k][0] = 0;
+            load(0);
+            for (int i = 0; i < span; ++i) {
+                if (i) __syncthreads();  // the page before is read
 #pragma unroll
-            for (int k = 0; k < kAtOnce; ++k)
-                w[k0 + k][0] = ((bytes[k][0] | bytes[k][1] << 8 | bytes[k][2] << 16 | bytes[k][3] << 24) & kept) | (~kept & 0x7f7f7f7fu);
+                for (int k = 0; k < kPieces; ++k) block[threadIdx.x + k * kThreads] = piece[k];
+                __syncthreads();
+                load(min(i + 1, span - 1));
+                const uint8_t* bytes = reinterpret_cast<const uint8_t*>(block) + threadIdx.x / (kPage / 4) * kPage;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (mine[j] >> SHIFT != i) continue;
+#pragma unroll
+                    for (int k = 0; k < kUnits; ++k)
+                        w[k][0] |= static_cast<uint32_t>(bytes[k * (kThreads / (kPage / 4)) * kPage + (mine[j] & (kPage - 1))]) << (8 * j);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kUnits; ++k) w[k][0] = (w[k][0] & kept) | (~kept & 0x7f7f7f7fu);
+        } else {
+            const uint8_t* from[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) from[j] = p.v + source[4 * quad + j];
+#pragma unroll
+            for (int k0 = 0; k0 < kUnits; k0 += kAtOnce) {
+                uint32_t bytes[kAtOnce][4];
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) bytes[k][j] = from[j][((threadIdx.x + (k0 + k) * kThreads) / (kPage / 4)) * kPage];
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k)
+                    w[k0 + k][0] = ((bytes[k][0] | bytes[k][1] << 8 | bytes[k][2] << 16 | bytes[k][3] << 24) & kept) | (~kept & 0x7f7f7f7fu);
+            }
         }
     } else {
         u32x4 v[kUnits];
@@ -397,6 +443,8 @@ __global__ __launch_bounds__((kMoveThreads<D, SHIFT>)) void k_evict_move(const E
     __shared__ int64_t source[kPage];    // each row's offset in K, or in line 0 of V; any page's where there is none
     __shared__ float scales[kPage];      // 0 behind the last row
     __shared__ uint32_t keep[kPage / 4];  // a byte for each row, 0 where its page is none
+    __shared__ int place[kPage];         // each row's place behind the first one's page; negative behind the last row
+    __shared__ u32x4 block[(D << SHIFT) / 16];
     __shared__ uint32_t top;
     const Pages& p = a.p;
     const int g = blockIdx.x % p.kv_heads;
@@ -409,7 +457,9 @@ __global__ __launch_bounds__((kMoveThreads<D, SHIFT>)) void k_evict_move(const E
     // What does not wait for anything is loaded together.
     const int context = p.contexts[b];
     const int32_t id = a.into[static_cast<int64_t>(b) * a.slots + slot];
-    const int row = a.rows[(static_cast<int64_t>(b) * p.kv_heads + g) * a.budget + first + min(static_cast<int>(threadIdx.x), count - 1)];
+    const int32_t* rows = a.rows + (static_cast<int64_t>(b) * p.kv_heads + g) * a.budget + first;
+    const int row = rows[min(static_cast<int>(threadIdx.x), count - 1)];
+    const int lowest = rows[0] >> SHIFT, span = (rows[count - 1] >> SHIFT) - lowest + 1;
     if (min(max(context, 0), p.table_pages << SHIFT) <= a.budget) return;
     if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.pages)) return;
     const int64_t to = static_cast<int64_t>(id) * p.kv_heads + g;
@@ -419,14 +469,16 @@ __global__ __launch_bounds__((kMoveThreads<D, SHIFT>)) void k_evict_move(const E
         const bool on = static_cast<uint32_t>(from) < static_cast<uint32_t>(p.pages);
         const int64_t at = static_cast<int64_t>(on ? from : 0) * p.kv_heads + g;
         const int offset = row & (kPage - 1);
+        place[threadIdx.x] = there ? row - (lowest << SHIFT) : -1;
         source[threadIdx.x] = is_v ? at * (D << SHIFT) + offset : ((at << SHIFT) + offset) * D;
         reinterpret_cast<uint8_t*>(keep)[threadIdx.x] = on ? 0xff : 0;
         scales[threadIdx.x] = !there ? 0.0f : on ? (is_v ? p.v_scales : p.k_scales)[at] : 1.0f;
         if (!is_v && there) a.weights[(to << SHIFT) + threadIdx.x] = on ? a.weights[(at << SHIFT) + offset] : __builtin_nanf("");
     }
     __syncthreads();
-    if (is_v) move_page<D, SHIFT, true>(a, to, source, scales, keep, top, count);
-    else move_page<D, SHIFT, false>(a, to, source, scales, keep, top, count);
+    const int32_t* from = p.table + static_cast<int64_t>(b) * p.table_pages + lowest;
+    if (is_v) move_page<D, SHIFT, true>(a, to, source, scales, keep, top, count, place, from, span, g, block);
+    else move_page<D, SHIFT, false>(a, to, source, scales, keep, top, count, place, from, span, g, block);
 }
 
 template <int D, int SHIFT>
@@ -448,9 +500,12 @@ int launch_move(const EvictArgs& a, hipStream_t stream) {
 
 constexpr int kFewKeys = 8, kManyKeys = 32;
 
-// Parts of a sequence's rows, or 0 where a workgroup takes a sequence and head alone.
+// Parts of a sequence's rows, or 0 where a workgroup takes a sequence and head alone: where its
+// registers hold the keys parts gain nothing (2, 4 and 8 sequences of 20000 rows, 8 heads: 55, 78 and 116 us
+// either way), and where there are workgroups for half of the chip they cost (16: 193 us, 208 in parts). One sequence of
+// 131000 rows takes 33 us in parts, 356 by a workgroup that reads them again and again.
 int64_t parts_of(int64_t units, int64_t rows) {
-    if (rows <= kSelectThreads * kFewKeys || units >= 128) return 0;
+    if (rows <= kSelectThreads * kManyKeys || units >= 128) return 0;
     return (rows + kPart - 1) / kPart;
 }
 

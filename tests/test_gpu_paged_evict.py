@@ -147,7 +147,7 @@ def test_sources_that_sequences_share_stay():
 
 
 def test_outputs_and_workspace_of_the_callers():
-    b, weights, into = evict_batch([9000, 40], kv=2, d=64, page=64, budget=100, first=3, seed=356)
+    b, weights, into = evict_batch([9000, 40], kv=2, d=64, page=64, budget=100, first=3, seed=356, extra_entries=400)
     cache, batch = b.device()
     into = torch.tensor(into, dtype=torch.int32, device=DEV)
     w = weights.to(DEV)
@@ -200,8 +200,10 @@ def test_captured_calls_replay_with_other_lengths_and_weights():
 
 
 @pytest.mark.parametrize("contexts,kv,page,budget,first,recent,kind", [
-    ([20000, 9000, 8193], 2, 64, 5000, 10, 300, "spread"),     # parts of a sequence's rows
-    ([70001], 3, 128, 20000, 4, 64, "spread"),
+    ([20000, 9000, 8193], 2, 64, 5000, 10, 300, "spread"),
+    ([70001], 3, 128, 20000, 4, 64, "spread"),                # parts of a sequence's rows
+    ([33000, 8300, 8192, 24577], 2, 64, 8192, 0, 8192, "spread"),
+    ([40001, 16390], 2, 32, 9000, 5, 0, "few"),
     ([70001], 3, 128, 20000, 4, 64, "equal"),
     ([40000, 100], 1, 16, 39999, 0, 0, "few"),
     ([33000], 128, 64, 1000, 0, 20, "spread"),                 # more rows than registers hold keys

@@ -103,8 +103,9 @@ def test_paged_evict(arguments, status):
 def test_paged_evict_workspace():
     lib = _native.load()
     assert lib.nq_paged_evict_workspace_bytes(1, 2, 64, 100, 500) == 0
+    assert lib.nq_paged_evict_workspace_bytes(1, 2, 64, 512, 500) == 0
     need = lib.nq_paged_evict_workspace_bytes(1, 2, 64, 1000, 500)
-    assert need == 2 * 8 * 3 * 2048 * 4
+    assert need == 2 * 8 * 3 * 2048 * 4  # 64000 rows in parts of 8192
     kv = _kv(page_size=64, table_pages=1000, batch=1)
     assert _evict(kv, budget=500, size=need - 1) == -5
     assert _evict(kv, budget=500, workspace=None) == -1
