@@ -152,3 +152,18 @@ def test_captured_calls_replay_with_other_lengths():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, eager)
+
+
+@pytest.mark.parametrize("q_dtype,d", [(torch.float32, 64), (torch.bfloat16, 128), (torch.float16, 256), (torch.float32, 256)])
+def test_many_rows_of_waves_with_tiles_of_their_own(q_dtype, d):
+    """Under a wide page table tens of tokens are not taken in turn."""
+
+    _say("weights not in turn", q_dtype, d)
+    b = shared_batch([(100, 40), (3, 30)], 0, kv=2, d=d, page=128, seed=261, ahead=1, behind=1, extra_entries=200)
+    q = torch.randn(b.tokens, 8, d, generator=generator(262)).to(q_dtype)
+    lse = olc.attention_lse(q, b.host(), b.table, b.spans, page=128, scaling=d**-0.5).float()
+    start = torch.rand(b.k_bytes.shape[0], 2, 128, generator=generator(263))
+    expected, spread, written = olc.attention_weights(q, b.host(), lse, start, b.table, b.spans, page=128, scaling=d**-0.5, first=7)
+    cache, batch = b.device()
+    got = ops.launch_attention_weights(q.to(DEV), cache, lse.to(DEV), start.to(DEV), scaling=d**-0.5, first=7, **batch)
+    check_weights(got, expected, spread, written, start, q_dtype=q_dtype, d=d, lse=lse.double(), n=160)
