@@ -112,26 +112,34 @@ __global__ __launch_bounds__(kWavesOf<TURNS>* kWave) void k_attention_weights(co
             float up, lse;
             int pos;
         };
-        const auto load = [&](int r0) {
+        // The lane's next row, its token's place and its head in the group: stepped, not divided.
+        constexpr int kStep = TURNS ? 16 * kWaves : 16;
+        const int step_places = kStep / a.group, step_heads = kStep - step_places * a.group;
+        int r0 = from + (TURNS ? 16 * wave : 0);
+        int r = r0 + n, place = r / a.group, sub = r - place * a.group;
+        const auto load = [&] {
             Rows x;
-            const int r = r0 + n;
             const bool on = r < all;
-            const int place = on ? r / a.group : 0, head = on ? g * a.group + r - place * a.group : 0;
             x.pos = on ? row_of(context, place, cache_rows) : -1;
-            const int64_t at = static_cast<int64_t>(begin + place) * a.q_heads + head;
+            const int64_t at = on ? static_cast<int64_t>(begin + place) * a.q_heads + g * a.group + sub : 0;
             x.lse = on ? a.lse[at] : 0.0f;
             x.up = load_query<QT, kQSteps>(a.q, at * D + 16 * grp, on, x.part);
+            r += kStep;
+            place += step_places;
+            sub += step_heads;
+            if (sub >= a.group) {
+                sub -= a.group;
+                ++place;
+            }
             return x;
         };
         if (tile < tiles) {
-            constexpr int kStep = TURNS ? 16 * kWaves : 16;
-            int r0 = from + (TURNS ? 16 * wave : 0);
             Rows x;
-            if (r0 < all) x = load(r0);
+            if (r0 < all) x = load();
             for (; r0 < all; r0 += kStep) {
                 Rows next;
                 if constexpr (kHeld) {
-                    next = load(min(r0 + kStep, all));  // behind the last one: nothing
+                    next = load();  // behind the last one: nothing
                 } else {
                     // K's bytes as the compiler may not know them: it would widen them all ahead of the
                     // loop and take the registers of other waves (32 sequences: 33.6 us, 42.5 so).
@@ -168,7 +176,7 @@ __global__ __launch_bounds__(kWavesOf<TURNS>* kWave) void k_attention_weights(co
                     for (int j = 0; j < kBlock; ++j) w[j] += exp2_hw(fmaf(sc[j >> 2][j & 3], f, -lse));
                 }
                 if constexpr (kHeld) x = next;
-                else if (r0 + kStep < all) x = load(r0 + kStep);
+                else if (r0 + kStep < all) x = load();
             }
         }
         float total = sum_rows(w, n);
