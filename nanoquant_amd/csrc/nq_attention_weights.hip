@@ -3,8 +3,8 @@
 //   W[j, g] (+)= sum over tokens t that see j, q heads h of kv head g
 //                of e^(scaling q[t, h] . K_j - lse[t, h])
 // The attention's log-sum-exps make the weights final at once: one pass over K,
-// no maximum, no second pass. A wave holds 64 cache rows of one kv head and forms
-// S^T = K Q^T as the attention does (nq_paged_attention.h): a lane has 16 rows of
+// no maximum, no second pass. A wave holds 16, 32 or 64 cache rows of one kv head
+// and forms S^T = K Q^T as the attention does (nq_paged_attention.h): a lane has a quarter of them for
 // one query row, whose exponentials it adds up over the query rows, 16 at a time;
 // the 16 lanes of a row are added once, at the end. Each cache row belongs to one
 // wave (or, joined in LDS in wave order, to one workgroup), so there are no
@@ -29,10 +29,15 @@ struct WeightArgs {
     int32_t q_heads, group, first, slots;  // slots: workgroups of a sequence and kv head
 };
 
-// 16 values of each lane summed over the 16 lanes of a row: lane n of a row gets the sum of value n.
-__device__ __forceinline__ float sum_rows(float (&w)[16], int n) {
+// N values of each lane summed over the 16 lanes of a row: lane n of a row gets the sum of value n % N.
+template <int N>
+__device__ __forceinline__ float sum_rows(float (&w)[N], int n) {
 #pragma unroll
-    for (int half = 8; half > 0; half /= 2) {
+    for (int half = 8; half >= N; half /= 2)
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] += __shfl_xor(w[j], half, kWave);
+#pragma unroll
+    for (int half = N / 2; half > 0; half /= 2) {
         const bool upper = n & half;
 #pragma unroll
         for (int j = 0; j < half; ++j) {
@@ -47,18 +52,20 @@ template <bool TURNS>
 constexpr int kWavesOf = TURNS ? 8 : 4;
 
 // Single tokens are bound by the wait for the table's entries and then for K and q
-// (32 sequences of up to 4000 rows: 81 MB in 33.4 us; pages of 16 rows are 2 KB of K each). Prompts are bound by the vector
+// (32 sequences of up to 4000 rows: 81 MB in 26.5 us; pages of 16 rows are 2 KB of K each). Prompts are bound by the vector
 // unit: 16 exponentials, 16 fused and 16 plain additions a product of 16 rows (1531 tokens
 // after 517: 8e9 products and sums in 53 us, the first rows' workgroups the last to end).
 // TURNS: the waves of a workgroup hold the same cache rows and take the query rows in
 // turn; otherwise each wave has cache rows of its own and takes all query rows.
-template <int D, int QT, bool TURNS>
+// ROWS: cache rows of a tile.
+template <int D, int QT, bool TURNS, int ROWS>
 __global__ __launch_bounds__(kWavesOf<TURNS>* kWave) void k_attention_weights(const WeightArgs a) {
     constexpr int kWaves = kWavesOf<TURNS>;
-    constexpr int kChunks = D / 64, kQSteps = 2 * kChunks, QP = Query<QT>::kParts, kBlock = 16;
+    constexpr int kChunks = D / 64, kQSteps = 2 * kChunks, QP = Query<QT>::kParts;
+    constexpr int kBlock = ROWS / 4, kScores = ROWS / 16;  // rows of a lane; products of 16 rows
     // Many query rows: K is widened once, and the next rows of q are on their way, where there are registers for it.
     constexpr bool kHeld = TURNS && QT != NQ_DTYPE_F32 && D <= 128;
-    __shared__ float join[TURNS ? kWaves : 1][kTile];
+    __shared__ float join[TURNS ? kWaves : 1][kWave];
     const Pages& p = a.p;
     const int lane = threadIdx.x & (kWave - 1), n = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -72,37 +79,37 @@ __global__ __launch_bounds__(kWavesOf<TURNS>* kWave) void k_attention_weights(co
     const int all = (end - begin) * a.group;
     const int32_t* table = p.table + static_cast<int64_t>(b) * p.table_pages;
     if (end <= begin || rows <= a.first) return;
-    const int tiles = (rows + kTile - 1) / kTile, per = TURNS ? 1 : kWaves;
-    for (int at = a.first / kTile + slot * per; at < tiles; at += a.slots * per) {
-        const int tile = at + (TURNS ? 0 : wave), base = tile * kTile;
+    const int tiles = (rows + ROWS - 1) / ROWS, per = TURNS ? 1 : kWaves;
+    for (int at = a.first / ROWS + slot * per; at < tiles; at += a.slots * per) {
+        const int tile = at + (TURNS ? 0 : wave), base = tile * ROWS;
         float w[kBlock];
 #pragma unroll
         for (int j = 0; j < kBlock; ++j) w[j] = 0.0f;
-        // Block n / 4 of 16 rows for K, block grp for the scores; blocks behind the last row read the last row's page.
+        // Block n / 4 of kBlock rows for K, block grp for the scores; blocks behind the last row read the last row's page.
         const auto entry = [&](int block) { return table[min(base + kBlock * block, rows - 1) >> p.page_shift]; };
         const int id_k = entry(n >> 2), id = entry(grp);
         const auto base_of = [&](int i) {
             return static_cast<int64_t>(static_cast<uint32_t>(i) < static_cast<uint32_t>(p.pages) ? i : 0) * p.kv_heads + g;
         };
         const float k_scale = p.k_scales[base_of(id)];
-        u32x4 kf[4][kChunks];
+        u32x4 kf[kScores][kChunks];
         const uint8_t* k_at = p.k + (base_of(id_k) * page + ((base + kBlock * (n >> 2)) & (page - 1)) + (n & 3)) * D + 16 * grp;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < kScores; ++t)
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) kf[t][c] = *reinterpret_cast<const u32x4*>(k_at + 4 * t * D + 64 * c);
         // Query rows before this see none of the tile's rows.
         const int64_t blind = static_cast<int64_t>(base) - context;
         const int from = blind > 0 ? static_cast<int>(min(blind * a.group, static_cast<int64_t>(all))) & ~15 : 0;
-        const int row = base + kBlock * grp + n;
-        const bool mine = row >= a.first && row < rows && static_cast<uint32_t>(id) < static_cast<uint32_t>(p.pages);
+        const int row = base + kBlock * grp + (n & (kBlock - 1));
+        const bool mine = n < kBlock && row >= a.first && row < rows && static_cast<uint32_t>(id) < static_cast<uint32_t>(p.pages);
         const int64_t place_of_row = base_of(id) * page + (row & (page - 1));
         float old = 0.0f;
         if (!TURNS || wave == 0) old = a.before[place_of_row];  // a page's row, whatever it is
-        u32x4 wide[kHeld ? 4 : 1][kHeld ? kQSteps : 1];
+        u32x4 wide[kHeld ? kScores : 1][kHeld ? kQSteps : 1];
         if constexpr (kHeld) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int t = 0; t < kScores; ++t)
 #pragma unroll
                 for (int c = 0; c < kQSteps; ++c) wide[t][c] = widen_k<QT>(kf[t][c / 2][2 * (c & 1)], kf[t][c / 2][2 * (c & 1) + 1]);
         }
@@ -142,15 +149,15 @@ __global__ __launch_bounds__(kWavesOf<TURNS>* kWave) void k_attention_weights(co
                     next = load();  // behind the last one: nothing
                 } else {
                     // K's bytes as the compiler may not know them: it would widen them all ahead of the
-                    // loop and take the registers of other waves (32 sequences: 33.6 us, 42.5 so).
+                    // loop and take the registers of other waves (32 sequences, tiles of 64 rows: 33.6 us, 42.5 so).
 #pragma unroll
-                    for (int t = 0; t < 4; ++t)
+                    for (int t = 0; t < kScores; ++t)
 #pragma unroll
                         for (int c = 0; c < kChunks; ++c) asm volatile("" : "+v"(kf[t][c]));
                 }
-                f32x4 sc[4];
+                f32x4 sc[kScores];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
+                for (int t = 0; t < kScores; ++t) {
                     sc[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
                     for (int c = 0; c < kQSteps; ++c) {
@@ -201,21 +208,37 @@ __global__ __launch_bounds__(kWavesOf<TURNS>* kWave) void k_attention_weights(co
 // rows a wave has four products' worth: never.
 bool takes_turns(int64_t rows, int64_t waves) { return rows > 64 && (waves < 768 || rows > 1024); }
 
+// Cache rows of a tile, by a sequence's mean query rows and the number of tiles of 64. A wave's steps wait for one
+// another (table, K, q, products, exponentials, sums), and all but the wait are shorter for fewer rows: with 16, 32 and
+// 64 rows one token after 700 takes 4.1, 5.1 and 8.4 us, eight after 1000 5.3, 6.1 and 8.9, 32 after 1000 (4352 tiles)
+// 12.6, 12.8 and 17.6, 32 of up to 4000 25.3, 26.5 and 33.7, one after 131000 71, 56 and 72. With more query rows
+// reading q for every tile weighs more: eight sequences of 64 tokens, 256 query rows, 42, 28 and 26.
+// In turn, 32 and 64 rows: one sequence after 512, 32 tokens (72 tiles) 5.6 and 9.1, 512 tokens (128 tiles) 19.4 and
+// 23.1, two of 512 (256 tiles) 38 and 24.
+int tile_rows(bool turns, int64_t rows, int64_t tiles) {
+    if (turns) return tiles < 192 ? 32 : 64;
+    if (rows > 64) return 64;
+    return rows <= 16 && tiles < 4096 ? 16 : 32;
+}
+
 template <int D, int QT>
-int launch_as(WeightArgs& a, bool turns, hipStream_t stream) {
+int launch_as(WeightArgs& a, bool turns, int rows, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.p.batch) * a.slots * a.p.kv_heads));
     const dim3 block(static_cast<unsigned>((turns ? kWavesOf<true> : kWavesOf<false>) * kWave));
-    if (turns) hipLaunchKernelGGL((k_attention_weights<D, QT, true>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((k_attention_weights<D, QT, false>), grid, block, 0, stream, a);
+    if (turns && rows == 32) hipLaunchKernelGGL((k_attention_weights<D, QT, true, 32>), grid, block, 0, stream, a);
+    else if (turns) hipLaunchKernelGGL((k_attention_weights<D, QT, true, 64>), grid, block, 0, stream, a);
+    else if (rows == 16) hipLaunchKernelGGL((k_attention_weights<D, QT, false, 16>), grid, block, 0, stream, a);
+    else if (rows == 32) hipLaunchKernelGGL((k_attention_weights<D, QT, false, 32>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((k_attention_weights<D, QT, false, 64>), grid, block, 0, stream, a);
     return nq::launch_status();
 }
 
 template <int D>
-int launch_for(WeightArgs& a, int q_dtype, bool turns, hipStream_t stream) {
+int launch_for(WeightArgs& a, int q_dtype, bool turns, int rows, hipStream_t stream) {
     switch (q_dtype) {
-        case NQ_DTYPE_F32: return launch_as<D, NQ_DTYPE_F32>(a, turns, stream);
-        case NQ_DTYPE_F16: return launch_as<D, NQ_DTYPE_F16>(a, turns, stream);
-        default: return launch_as<D, NQ_DTYPE_BF16>(a, turns, stream);
+        case NQ_DTYPE_F32: return launch_as<D, NQ_DTYPE_F32>(a, turns, rows, stream);
+        case NQ_DTYPE_F16: return launch_as<D, NQ_DTYPE_F16>(a, turns, rows, stream);
+        default: return launch_as<D, NQ_DTYPE_BF16>(a, turns, rows, stream);
     }
 }
 
@@ -242,17 +265,21 @@ extern "C" int nq_attention_weights(const void* q, int32_t q_dtype, int64_t toke
     a.q_heads = q_heads;
     a.group = q_heads / kv->kv_heads;
     a.first = static_cast<int32_t>(first);
-    const int64_t tiles = (cache_rows + kTile - 1) / kTile - first / kTile, units = kv->batch * kv->kv_heads;
-    const bool turns = takes_turns((tokens * a.group + kv->batch - 1) / kv->batch, units * tiles);
+    const int64_t units = kv->batch * kv->kv_heads;
+    int64_t tiles = (cache_rows + kTile - 1) / kTile - first / kTile;
+    const int64_t mean = (tokens * a.group + kv->batch - 1) / kv->batch;
+    const bool turns = takes_turns(mean, units * tiles);
+    const int rows = tile_rows(turns, mean, units * tiles);
+    tiles = (cache_rows + rows - 1) / rows - first / rows;
     const int64_t most = turns ? tiles : (tiles + kWavesOf<false> - 1) / kWavesOf<false>;
-    // (32 sequences of one token after up to 4000 rows, 8 heads: 33.7 us with 4096 or 8192 workgroups, 36.3 with
+    // (32 sequences of one token after up to 4000 rows, 8 heads, tiles of 64 rows: 33.7 us with 4096 or 8192 workgroups, 36.3 with
     // 2048, 39.8 with 1024.)
     a.slots = static_cast<int32_t>(std::max(int64_t{1}, std::min(most, (4096 + units - 1) / units)));
     if (!nq::launchable(units * a.slots, kWavesOf<true> * kWave)) return NQ_ERR_SHAPE;
     hipStream_t st = static_cast<hipStream_t>(stream);
     switch (kv->head_dim) {
-        case 64: return launch_for<64>(a, q_dtype, turns, st);
-        case 128: return launch_for<128>(a, q_dtype, turns, st);
-        default: return launch_for<256>(a, q_dtype, turns, st);
+        case 64: return launch_for<64>(a, q_dtype, turns, rows, st);
+        case 128: return launch_for<128>(a, q_dtype, turns, rows, st);
+        default: return launch_for<256>(a, q_dtype, turns, rows, st);
     }
 }

@@ -167,3 +167,25 @@ def test_many_rows_of_waves_with_tiles_of_their_own(q_dtype, d):
     cache, batch = b.device()
     got = ops.launch_attention_weights(q.to(DEV), cache, lse.to(DEV), start.to(DEV), scaling=d**-0.5, first=7, **batch)
     check_weights(got, expected, spread, written, start, q_dtype=q_dtype, d=d, lse=lse.double(), n=160)
+
+
+@pytest.mark.parametrize("q_dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lengths,page,extra", [
+    ([(150, 2), (70, 1)], 32, 0),         # few query rows under a short table
+    ([(150, 2), (70, 1)], 128, 520),      # and under a wide one
+    ([(150, 9), (70, 10)], 32, 0),        # tens of query rows
+    ([(150, 41), (70, 30)], 128, 30),     # taken in turn, in tiles of 64 rows
+    ([(150, 41), (70, 30)], 16, 0),       # and of 32
+])
+def test_each_size_of_tile(lengths, page, extra, d, q_dtype):
+    _say("weights by tiles", lengths, page, extra, d, q_dtype)
+    b = shared_batch(lengths, 0, kv=2, d=d, page=page, seed=271, ahead=1, behind=1, extra_entries=extra)
+    q = torch.randn(b.tokens, 8, d, generator=generator(272)).to(q_dtype)
+    lse = olc.attention_lse(q, b.host(), b.table, b.spans, page=page, scaling=d**-0.5).float()
+    start = torch.rand(b.k_bytes.shape[0], 2, page, generator=generator(273))
+    cache, batch = b.device()
+    for first in (0, 83):
+        expected, spread, written = olc.attention_weights(q, b.host(), lse, start, b.table, b.spans, page=page, scaling=d**-0.5, first=first)
+        got = ops.launch_attention_weights(q.to(DEV), cache, lse.to(DEV), start.to(DEV), scaling=d**-0.5, first=first, **batch)
+        check_weights(got, expected, spread, written, start, q_dtype=q_dtype, d=d, lse=lse.double(), n=164)
