@@ -201,7 +201,7 @@ __global__ __launch_bounds__(kWavesOf<TURNS>* kWave) void k_attention_weights(co
 
 // Whether the waves of a workgroup take the query rows of one tile in turn (`rows` of
 // a sequence, `waves` tiles of all): where tiles are too few for the chip, or there are so many rows
-// that the last tiles' would keep it waiting. bf16, 32/8 heads of 128, in turn and not:
+// that the last tiles' would keep it waiting. bf16, 32/8 heads of 128, tiles of 64 rows, in turn and not:
 // one sequence after 512 rows, 32 tokens (128 rows) 9.0 and 13.6 us, 128 tokens 13 and 33, 1531
 // tokens 53 and 269; four of 512 tokens (512 tiles) 45 and 100; eight after 1000 (1088 tiles), 64 tokens (256 rows) 47
 // and 27, 128 tokens 56 and 43, 512 tokens (2048 rows) 129 and 141; 32 of 64 tokens 95 and 38. Up to 64
