@@ -473,7 +473,8 @@ Int4Plan plan_int4(int64_t tokens, int64_t outs, int64_t ins, int group) {
     p.blocks = at_once <= 3 ? static_cast<int>(at_once) : 6;
     p.passes = static_cast<int>((blocks + p.blocks - 1) / p.blocks);
     const int held = static_cast<int>(std::min<int64_t>(tokens, int64_t{p.blocks} * each));
-    // Chunks whose digits LDS holds at once.
+    // Chunks whose digits LDS holds at once. (Four more waves of the slices' form bring their own 5.5 to 6.5 KB each on
+    // top: at most 87 KB of a workgroup, of 160.)
     const size_t fixed = lds_bytes(4, held, p.blocks, groups, 0), each_chunk = lds_bytes(4, held, p.blocks, groups, 1) - fixed;
     const int most = static_cast<int>(std::min<int64_t>(chunks, std::max<int64_t>(1, static_cast<int64_t>((kBudget - std::min(fixed, kBudget)) / each_chunk))));
     p.slices = 1;

@@ -88,6 +88,18 @@ def test_every_nibble_is_its_value_at_every_place():
     assert torch.allclose(got, w.T, rtol=3 * 2.0**-24, atol=0)
 
 
+@pytest.mark.parametrize("tokens,ins,outs,group", [(6, 12288, 300, 32), (6, 28672, 37, 32), (30, 14336, 300, 128)])
+def test_slices_whose_workgroups_hold_more_than_64_kb(tokens, ins, outs, group):
+    """Eight waves around digits of many chunks: 71 to 75 KB of LDS."""
+
+    _say("int4 lds", tokens, ins, outs, group)
+    m = matrix(outs, ins, group, torch.float16, True, 511)
+    x = torch.randn(tokens, ins, generator=_g(512))
+    got = ops.launch_int4_projection(x.to(DEV), m.to(DEV))
+    check(got, x, m, group)
+    assert torch.equal(ops.launch_int4_projection(x.to(DEV), m.to(DEV)), got)
+
+
 @pytest.mark.parametrize("size", [1e-38, 1e-30, 2.0**-100, 1.0, 3e37, "ulp"])
 def test_sizes(size):
     """Values near fp32's ends, and largest values just below a power of two."""
