@@ -492,9 +492,10 @@ _INT4_GROUPS = (32, 64, 128)
 
 
 def int4_matrix(weight: torch.Tensor, group: int = 128, scale_dtype: torch.dtype = torch.float16) -> Int4Matrix:
-    """``weight`` ``[out, in]`` rounded to 4 bits: for each group of columns the scale
-    that brings its largest value to 7, or its lowest to -8 where that is the smaller scale.
-    Once, before serving."""
+    """``weight`` ``[out, in]`` rounded to 4 bits: for each group of columns the larger of
+    the scales that bring its largest value to 7 and its lowest to -8. A weight that is not
+    finite, or a group whose scale is beyond ``scale_dtype``, is refused. Once, before serving
+    (the check waits for the device)."""
 
     if weight.ndim != 2 or weight.shape[1] % 32 or group not in _INT4_GROUPS or scale_dtype not in _FLOAT:
         raise ValueError("4-bit weights need [out, in] with in a multiple of 32 and groups of 32, 64 or 128")
@@ -507,9 +508,12 @@ def int4_matrix(weight: torch.Tensor, group: int = 128, scale_dtype: torch.dtype
         scale = torch.maximum(w.amax(-1) / 7, -w.amin(-1) / 8).to(scale_dtype)
         scales[first:first + 8192] = scale
         scale = scale.float()
-        q = torch.where(scale[..., None] > 0, w / scale[..., None], 0.0).round_().clamp_(-8, 7).add_(8).to(torch.uint8)
+        q = torch.where(scale[..., None] > 0, w / scale[..., None], 0.0).round_().clamp_(-8, 7).add_(8).nan_to_num_().to(torch.uint8)
         q = q.view(q.shape[0], -1)[:, :ins]
         packed[first:first + 8192] = q[:, 0::2] | (q[:, 1::2] << 4)
+    # A weight that is NaN or infinite makes its group's scale so.
+    if not bool(torch.isfinite(scales).all()):
+        raise ValueError(f"4-bit weights need finite values whose groups' scales {scale_dtype} holds")
     return Int4Matrix(packed, scales)
 
 
