@@ -641,11 +641,12 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 && NT == 2 ? 1 : 2) void k_p
             const float m_use = m_run[u] == -INFINITY ? 0.0f : m_run[u];
             // The fused subtraction sees what rounding took off the largest score: half a
             // step of it, which is no number to raise 2 to where scores pass 2^30. They
-            // are rounded first there, so that the largest has the weight that it has in fp32.
-            if (__ballot(fabsf(m_use) > 0x1p24f)) {
+            // are rounded first there, so that the largest has the weight that it has in fp32: by query
+            // row, so that one row's scores change no bit of another's result.
+            if (const bool large = fabsf(m_use) > 0x1p24f; __ballot(large)) {
 #pragma unroll
-                for (int j = 0; j < kBlock; ++j) sc[j >> 2][u][j & 3] *= f[u];
-                f[u] = 1.0f;
+                for (int j = 0; j < kBlock; ++j) sc[j >> 2][u][j & 3] *= large ? f[u] : 1.0f;
+                f[u] = large ? 1.0f : f[u];
             }
             float sum = 0.0f;
 #pragma unroll
