@@ -170,8 +170,8 @@ __global__ __launch_bounds__(kWavesOf<TURNS>* kWave) void k_attention_weights(co
                 }
                 const float f = k_scale * a.scale * x.up, lse = x.lse * 1.4426950408889634f;
                 const int seen = x.pos + 1 - (base + kBlock * grp);
-                const bool large = __ballot(fabsf(lse) > kLarge);
-                if (__ballot(seen < kBlock) || large) {
+                const bool large = fabsf(lse) > kLarge;  // of this lane's query row alone
+                if (__ballot(seen < kBlock || large)) {
 #pragma unroll
                     for (int j = 0; j < kBlock; ++j) {
                         float y = fmaf(sc[j >> 2][j & 3], f, -lse);
