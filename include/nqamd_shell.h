@@ -168,7 +168,7 @@ int nq_greedy_select(const void* workspace, int64_t vocab, int64_t hidden, int64
 int nq_greedy_select_partials(const void* partials, int64_t count, int64_t* token_out, int64_t* history,
                               int64_t history_capacity, int32_t* step, int32_t* position, void* stream);
 
-/* Workspace bytes of nq_int4_projection (0: none needed; -1: refused sizes). */
+/* Workspace bytes of nq_int4_projection, whatever the type of x (0: none needed; -1: refused sizes). */
 int64_t nq_int4_projection_workspace_bytes(int64_t tokens, int64_t out_features, int64_t in_features, int32_t group);
 
 /* Partials (8 bytes each) that nq_int4_projection leaves for one token. */
@@ -177,13 +177,14 @@ int64_t nq_int4_projection_partials(int64_t out_features);
 /* Products with 4-bit weights and group scales:
  *   y[t, o] = sum_i scales[o, i / group] * (w[o, i] - zeros[o, i / group]) * x[t, i]
  * x F32/F16/BF16 [tokens, in_features] (1 to 65535 tokens; the form is that of a few: the weights
- * are read once for up to 30 tokens with groups of 128, 12 with 64 and 6 with 32); packed
+ * are read once for up to 30 tokens (24 of fp32) with groups of 128, 12 with 64 and 6 with 32); packed
  * [out_features, in_features / 2], byte j of a row holding column 2 j in its low
  * four bits and 2 j + 1 in its high ones, 16-byte aligned; scales F32/F16/BF16 [out_features,
  * ceil(in_features / group)], zeros uint8 of the same shape (NULL: 8), any value
  * from 0 to 255; y F32/F16/BF16 [tokens, out_features]. group 32, 64 or 128,
- * in_features a multiple of 32. x is read to 2^-23 of its largest value in a group (or of 2^-100), sums
- * within a group are exact, those of groups fp32 in a fixed order. A token that
+ * in_features a multiple of 32. x is read to 2^-31 of its largest value in a group where it is fp32 (or of 2^-96), to 2^-23
+ * where it has 16 bits (or of 2^-100): its values are exact down to 2^-7 (fp32), 2^-12 (fp16) and
+ * 2^-15 (bf16) of that largest one. Sums within a group are exact, those of groups fp32 in a fixed order. A token that
  * holds an infinity or a NaN gives NaN. partials, for one token (NULL: not
  * wanted), get the largest value of each 16 rows for nq_greedy_select_partials.
  * Stands beside nq_output_projection for a weight of a quarter of its bytes

@@ -1,12 +1,19 @@
 // Products of a few tokens with 4-bit weights and group scales:
 //   y[t, o] = sum_i s[o, i / G] (w[o, i] - z[o, i / G]) x[t, i]
 //
-// Exact integer arithmetic inside a group: x is held as three int8 digits of base
-// 256 and one exponent for each token and group (within 2^-23 of the group's
-// largest value), the nibbles are int8 operands as they are, and
+// Exact integer arithmetic inside a group: x is held as int8 digits of base 256 and
+// one exponent for each token and group, the nibbles are int8 operands as they are, and
 // v_mfma_i32_16x16x64_i8 sums them. Per group and row
-//   y += s 2^e 256^d (sum_i w_i x_id - z sum_i x_id), d = 0, 1, 2,
+//   y += s 2^e 256^d (sum_i w_i x_id - z sum_i x_id), d = 0, 1, 2 (and 3 for fp32 x),
 // in fp32, the digits' sums sum_i x_id known beforehand.
+//
+// Digits: a 16-bit x has three, within 2^-23 of its group's largest value, so that bf16 values
+// are exact down to 2^-15 of it and fp16 values down to 2^-12 (what is lost below is less than their own
+// rounding down to 2^-14 and 2^-11); fp32 x has four, within 2^-31, exact down to 2^-7 of it. With three, an
+// fp32 value far below another one of its group whose weights are at the zero point (so that nothing hides the
+// loss) would keep few bits of its own. Four cost one token of a large matrix nothing (151936 x 4096: 55.9
+// us, 56.0 with three), 11 tokens of 2560 x 10240, groups of 64, 19.0 us for 17.2, and 30 of 4096 x 4096, groups of
+// 128, 25.1 for 21.2 (24 tokens at once, not 30).
 //
 // A chunk is 128 columns: lane 16 q + r of a wave holds 16 bytes of row r, columns 32 q
 // to 32 q + 31, whose low nibbles (even columns) are the A operand of one product and
@@ -21,7 +28,7 @@
 
 namespace {
 
-constexpr int kWave = 64, kChunk = 128, kDigits = 3;
+constexpr int kWave = 64, kChunk = 128;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
@@ -47,10 +54,13 @@ struct Int4Args {
     int32_t share, slice, stage;
 };
 
+// Digits of x by its type.
+constexpr int digits_for(int x_dtype) { return x_dtype == NQ_DTYPE_F32 ? 4 : 3; }
+
 // Groups of a chunk, columns of B that one of them has, and tokens of these.
-template <int G>
+template <int G, int DG>
 struct Shape {
-    static constexpr int kGroups = kChunk / G, kColumns = 16 / kGroups, kTokens = kColumns / kDigits;
+    static constexpr int kGroups = kChunk / G, kColumns = 16 / kGroups, kTokens = kColumns / DG;
 };
 
 __device__ __forceinline__ uint64_t order_of(float v, uint32_t row) {
@@ -132,11 +142,13 @@ __device__ __forceinline__ void widen8(const Eight& v, int dtype, float (&x)[8])
     }
 }
 
-// Eight adjacent columns of a token as digits.
-template <int G>
-__device__ __forceinline__ void digits_of(const float (&x)[8], uint32_t (&even)[kDigits], uint32_t (&odd)[kDigits],
-                                          int (&sum)[kDigits], float& unit) {
+// Eight adjacent columns of a token as DG digits.
+template <int G, int DG>
+__device__ __forceinline__ void digits_of(const float (&x)[8], uint32_t (&even)[DG], uint32_t (&odd)[DG], int (&sum)[DG],
+                                          float& unit) {
     constexpr int kGroup = G / 8;  // lanes of a group
+    constexpr int kBits = 8 * DG - 2, kLowest = DG == 4 ? -96 : -100;  // 2^(kBits - kLowest) is a number
+    constexpr uint32_t kBias = 0x80808080u >> (32 - 8 * DG);
     float most = 0.0f;
     bool finite = true;
 #pragma unroll
@@ -150,15 +162,15 @@ __device__ __forceinline__ void digits_of(const float (&x)[8], uint32_t (&even)[
     finite = most < INFINITY;
     // The largest value is below 2^(k + 1), or so near it that a rounding reaches it: 2^(k + 2).
     const uint32_t bits = __float_as_uint(most);
-    const int k = max(static_cast<int>(bits >> 23) - 127 + ((bits & 0x7fffffu) > 0x7e0000u ? 1 : 0), -100);
-    const float up = finite ? __uint_as_float(static_cast<uint32_t>(22 - k + 127) << 23) : 0.0f;
-    // n + 0x808080 has the digits plus 128 each as its bytes: n is at least -2^23 and at
-    // most 2^22 * 1.984375 = 0x7f0000.
+    const int k = max(static_cast<int>(bits >> 23) - 127 + ((bits & 0x7fffffu) > 0x7e0000u ? 1 : 0), kLowest);
+    const float up = finite ? __uint_as_float(static_cast<uint32_t>(kBits - k + 127) << 23) : 0.0f;
+    // n + 0x808080 (or 0x80808080) has the digits plus 128 each as its bytes: n is at most
+    // 2^22 * 1.984375 = 0x7f0000 (2^30 * 1.984375 = 0x7f000000) either way.
     uint32_t u[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) u[j] = static_cast<uint32_t>(finite ? static_cast<int>(rintf(x[j] * up)) : 0) + 0x808080u;
+    for (int j = 0; j < 8; ++j) u[j] = static_cast<uint32_t>(finite ? static_cast<int>(rintf(x[j] * up)) : 0) + kBias;
 #pragma unroll
-    for (int d = 0; d < kDigits; ++d) {
+    for (int d = 0; d < DG; ++d) {
         // Byte d of four values in a word.
         const uint32_t pair = 0x0c0c0400u + 0x0101u * d;
         const auto four = [&](uint32_t a, uint32_t b, uint32_t e, uint32_t f) {
@@ -170,10 +182,10 @@ __device__ __forceinline__ void digits_of(const float (&x)[8], uint32_t (&even)[
                                         __builtin_amdgcn_sdot4(static_cast<int>(odd[d]), 0x01010101, 0, false), false);
     }
 #pragma unroll
-    for (int d = 0; d < kDigits; ++d)
+    for (int d = 0; d < DG; ++d)
 #pragma unroll
         for (int m = 1; m < kGroup; m *= 2) sum[d] += __shfl_xor(sum[d], m, kWave);
-    unit = finite ? __uint_as_float(static_cast<uint32_t>(k - 22 + 127) << 23) : __builtin_nanf("");
+    unit = finite ? __uint_as_float(static_cast<uint32_t>(k - kBits + 127) << 23) : __builtin_nanf("");
 }
 
 // Large matrices of one token are bound by their bytes (151936 x 4096: 321 MB in 54.9 us, 5.9
@@ -183,10 +195,10 @@ __device__ __forceinline__ void digits_of(const float (&x)[8], uint32_t (&even)[
 // block has the products' operands come from LDS, 2 KB a chunk and block, and bound it.
 // A workgroup has a slice of the chunks and, share waves to a tile of 16 rows, kWaves / share tiles
 // at a time; the waves of a tile each take a part of a stage's chunks. NB blocks of tokens.
-template <int G, int NB, int ST, int kWaves>
+template <int G, int NB, int ST, int kWaves, int DG>
 __global__ __launch_bounds__(kWaves* kWave, kWaves == 8 ? 1 : NB <= 3 ? 3 : 2) void k_int4_product(const Int4Args a) {
     constexpr int kThreads = kWaves * kWave;
-    using S = Shape<G>;
+    using S = Shape<G, DG>;
     constexpr int kTogether = NB <= 2 ? 2 : 1;
     constexpr int kMost = kAtOnce * S::kGroups;  // groups whose scales a wave holds in LDS
     extern __shared__ u32x4 lds[];
@@ -194,7 +206,7 @@ __global__ __launch_bounds__(kWaves* kWave, kWaves == 8 ? 1 : NB <= 3 ? 3 : 2) v
     uint8_t* digits = reinterpret_cast<uint8_t*>(lds) + 64;
     const int first = blockIdx.z * NB * S::kTokens, tokens = min(NB * S::kTokens, a.tokens - first);
     const int line = line_bytes(a.stage);
-    Column* columns = reinterpret_cast<Column*>(digits + tokens * kDigits * line);  // [stage][NB][16]
+    Column* columns = reinterpret_cast<Column*>(digits + tokens * DG * line);  // [stage][NB][16]
     float* mine_f = reinterpret_cast<float*>(columns + a.stage * NB * 16);
     const int lane = threadIdx.x & (kWave - 1), c = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -209,7 +221,7 @@ __global__ __launch_bounds__(kWaves* kWave, kWaves == 8 ? 1 : NB <= 3 ? 3 : 2) v
     const int chunk0 = blockIdx.y * a.slice, chunk1 = min(chunk0 + a.slice, a.chunks);
     const int part = wave % a.share;
     const int64_t half = a.ins / 2;
-    const int group = c / S::kColumns, in_group = c % S::kColumns, local = in_group / kDigits, digit = in_group % kDigits;
+    const int group = c / S::kColumns, in_group = c % S::kColumns, local = in_group / DG, digit = in_group % DG;
     const bool mine = q * S::kGroups / 4 == group && local < S::kTokens;
     // Where this lane's operand of a block begins in LDS, and its odd columns' behind; 0: zeros.
     int from_at[NB], odd_at[NB];
@@ -217,7 +229,7 @@ __global__ __launch_bounds__(kWaves* kWave, kWaves == 8 ? 1 : NB <= 3 ? 3 : 2) v
     for (int b = 0; b < NB; ++b) {
         const int token = b * S::kTokens + local;
         const bool on = mine && token < tokens;
-        from_at[b] = on ? 64 + (token * kDigits + digit) * line + 16 * q : 0;
+        from_at[b] = on ? 64 + (token * DG + digit) * line + 16 * q : 0;
         odd_at[b] = on ? 64 : 0;
     }
 
@@ -235,20 +247,20 @@ __global__ __launch_bounds__(kWaves* kWave, kWaves == 8 ? 1 : NB <= 3 ? 3 : 2) v
         const auto round = [&](int i, const Eight& bits) {
             const int t = i & 15, token = tokens == 1 ? 0 : i / (16 * n), at = (i >> 4) - token * n;
             float x[8];
-            uint32_t even[kDigits], odd[kDigits];
-            int sum[kDigits];
+            uint32_t even[DG], odd[DG];
+            int sum[DG];
             float unit;
             widen8(bits, a.x_dtype, x);
-            digits_of<G>(x, even, odd, sum, unit);
+            digits_of<G, DG>(x, even, odd, sum, unit);
             const int block = token / S::kTokens, in_block = token - block * S::kTokens;
             float power = 1.0f;
 #pragma unroll
-            for (int d = 0; d < kDigits; ++d) {
-                uint32_t* to = reinterpret_cast<uint32_t*>(digits + (token * kDigits + d) * line + at * kChunk);
+            for (int d = 0; d < DG; ++d) {
+                uint32_t* to = reinterpret_cast<uint32_t*>(digits + (token * DG + d) * line + at * kChunk);
                 to[t] = even[d];
                 to[16 + t] = odd[d];
                 if (t % (G / 8) == 0)
-                    columns[(at * NB + block) * 16 + t / (G / 8) * S::kColumns + in_block * kDigits + d] =
+                    columns[(at * NB + block) * 16 + t / (G / 8) * S::kColumns + in_block * DG + d] =
                         Column{unit * power, static_cast<float>(sum[d])};
                 power *= 256.0f;
             }
@@ -263,7 +275,7 @@ __global__ __launch_bounds__(kWaves* kWave, kWaves == 8 ? 1 : NB <= 3 ? 3 : 2) v
     };
     // Columns that no token has.
     for (int i = threadIdx.x; i < a.stage * NB * 16; i += kThreads) {
-        const int at = i & 15, t = at % S::kColumns / kDigits;
+        const int at = i & 15, t = at % S::kColumns / DG;
         if (t >= S::kTokens || (i >> 4) % NB * S::kTokens + t >= tokens) columns[i] = Column{0.0f, 0.0f};
     }
 
@@ -404,7 +416,7 @@ __global__ __launch_bounds__(kWaves* kWave, kWaves == 8 ? 1 : NB <= 3 ? 3 : 2) v
                     for (int o = 0; o < kWaves; ++o) {
                         if (o >= a.share) break;
 #pragma unroll
-                        for (int d = kDigits - 1; d >= 0; --d) y += sums[o * kEach + c * kRow + t * kDigits + d];
+                        for (int d = DG - 1; d >= 0; --d) y += sums[o * kEach + c * kRow + t * DG + d];
                     }
                     const bool there = tile < a.tiles && row0 + c < a.outs;
                     if (a.partial) {
@@ -445,15 +457,15 @@ __global__ __launch_bounds__(256) void k_int4_join(const Int4Args a, int slices)
 
 int64_t chunks_of(int64_t ins) { return (ins + kChunk - 1) / kChunk; }
 
-size_t lds_bytes(int waves, int tokens, int blocks, int groups, int stage) {
+size_t lds_bytes(int waves, int tokens, int digits, int blocks, int groups, int stage) {
     const int wave = groups == 1 ? kEachWave<1> : groups == 2 ? kEachWave<2> : kEachWave<4>;
-    return 64 + static_cast<size_t>(tokens) * kDigits * line_bytes(stage) + static_cast<size_t>(stage) * blocks * 16 * sizeof(Column) +
+    return 64 + static_cast<size_t>(tokens) * digits * line_bytes(stage) + static_cast<size_t>(stage) * blocks * 16 * sizeof(Column) +
            static_cast<size_t>(waves) * wave * sizeof(float);
 }
 
 // How a call is laid out. A workgroup makes the digits of its tokens and slice itself, in
 // LDS, from x (2 to 4 bytes a value from the L2; a launch of its own for them took 4 us).
-//  - One token's digits fit LDS for the whole row (12 KB at 4096 columns). Waves have tiles of
+//  - One token's digits fit LDS for the whole row (12 KB at 4096 columns, 16 of fp32). Waves have tiles of
 //    their own from 2048 tiles on, fewer tiles are shared by four waves (4096 columns, one token:
 //    4096 rows 6.5 us shared and 10.2 not, 14336 rows 10.8 and 11.4, 24576 13.6 and 13.7, 32768 16.6 and 15.2).
 //    768 workgroups walk over the tiles of a large matrix (151936 rows 59.4 us; with 512 65.7, 1024
@@ -463,9 +475,9 @@ size_t lds_bytes(int waves, int tokens, int blocks, int groups, int stage) {
 //    10240, groups of 64: 18.3 us; four waves 21.2, 1280 waves 25.3, 2560 waves 28.8).
 //  - Otherwise the row in stages, whose digits are made one after the other.
 // Blocks: more of them read the weights once for more tokens, and hold more registers.
-Int4Plan plan_int4(int64_t tokens, int64_t outs, int64_t ins, int group) {
+Int4Plan plan_int4(int64_t tokens, int64_t outs, int64_t ins, int group, int digits) {
     constexpr size_t kBudget = 60 * 1024;
-    const int groups = kChunk / group, each = 16 / groups / kDigits;
+    const int groups = kChunk / group, each = 16 / groups / digits;
     const int64_t blocks = (tokens + each - 1) / each, chunks = chunks_of(ins), tiles = (outs + 15) / 16;
     Int4Plan p{};
     p.passes = static_cast<int>((blocks + 5) / 6);
@@ -475,7 +487,7 @@ Int4Plan plan_int4(int64_t tokens, int64_t outs, int64_t ins, int group) {
     const int held = static_cast<int>(std::min<int64_t>(tokens, int64_t{p.blocks} * each));
     // Chunks whose digits LDS holds at once. (Four more waves of the slices' form bring their own 5.5 to 6.5 KB each on
     // top: at most 87 KB of a workgroup, of 160.)
-    const size_t fixed = lds_bytes(4, held, p.blocks, groups, 0), each_chunk = lds_bytes(4, held, p.blocks, groups, 1) - fixed;
+    const size_t fixed = lds_bytes(4, held, digits, p.blocks, groups, 0), each_chunk = lds_bytes(4, held, digits, p.blocks, groups, 1) - fixed;
     const int most = static_cast<int>(std::min<int64_t>(chunks, std::max<int64_t>(1, static_cast<int64_t>((kBudget - std::min(fixed, kBudget)) / each_chunk))));
     p.slices = 1;
     p.waves = 4;
@@ -497,39 +509,47 @@ Int4Plan plan_int4(int64_t tokens, int64_t outs, int64_t ins, int group) {
     return p;
 }
 
-template <int G, int NB, int ST, int WV>
+template <int G, int NB, int ST, int DG, int WV>
 int launch_on(const Int4Args& a, const Int4Plan& p, hipStream_t stream) {
-    const int held = std::min(a.tokens, NB * Shape<G>::kTokens);
+    using S = Shape<G, DG>;
+    const int held = std::min(a.tokens, NB * S::kTokens);
     const dim3 grid(static_cast<unsigned>(p.groups), static_cast<unsigned>(p.slices), static_cast<unsigned>(p.passes));
-    hipLaunchKernelGGL((k_int4_product<G, NB, ST, WV>), grid, dim3(WV * kWave), lds_bytes(WV, held, NB, Shape<G>::kGroups, a.stage), stream, a);
+    hipLaunchKernelGGL((k_int4_product<G, NB, ST, WV, DG>), grid, dim3(WV * kWave), lds_bytes(WV, held, DG, NB, S::kGroups, a.stage),
+                       stream, a);
     return nq::launch_status();
 }
 
-template <int G, int NB, int ST>
+template <int G, int NB, int ST, int DG>
 int launch_as(const Int4Args& a, const Int4Plan& p, hipStream_t stream) {
     if constexpr (NB == 6) {
-        if (p.waves == 8) return launch_on<G, NB, ST, 8>(a, p, stream);
+        if (p.waves == 8) return launch_on<G, NB, ST, DG, 8>(a, p, stream);
     }
-    return launch_on<G, NB, ST, 4>(a, p, stream);
+    return launch_on<G, NB, ST, DG, 4>(a, p, stream);
 }
 
-template <int G, int NB>
+template <int G, int NB, int DG>
 int launch_with(const Int4Args& a, const Int4Plan& p, int scale_dtype, hipStream_t stream) {
     switch (scale_dtype) {
-        case NQ_DTYPE_F32: return launch_as<G, NB, NQ_DTYPE_F32>(a, p, stream);
-        case NQ_DTYPE_F16: return launch_as<G, NB, NQ_DTYPE_F16>(a, p, stream);
-        default: return launch_as<G, NB, NQ_DTYPE_BF16>(a, p, stream);
+        case NQ_DTYPE_F32: return launch_as<G, NB, NQ_DTYPE_F32, DG>(a, p, stream);
+        case NQ_DTYPE_F16: return launch_as<G, NB, NQ_DTYPE_F16, DG>(a, p, stream);
+        default: return launch_as<G, NB, NQ_DTYPE_BF16, DG>(a, p, stream);
+    }
+}
+
+template <int G, int DG>
+int launch_blocks(const Int4Args& a, const Int4Plan& p, int scale_dtype, hipStream_t stream) {
+    switch (p.blocks) {
+        case 1: return launch_with<G, 1, DG>(a, p, scale_dtype, stream);
+        case 2: return launch_with<G, 2, DG>(a, p, scale_dtype, stream);
+        case 3: return launch_with<G, 3, DG>(a, p, scale_dtype, stream);
+        default: return launch_with<G, 6, DG>(a, p, scale_dtype, stream);
     }
 }
 
 template <int G>
 int launch_for(const Int4Args& a, const Int4Plan& p, int scale_dtype, hipStream_t stream) {
-    switch (p.blocks) {
-        case 1: return launch_with<G, 1>(a, p, scale_dtype, stream);
-        case 2: return launch_with<G, 2>(a, p, scale_dtype, stream);
-        case 3: return launch_with<G, 3>(a, p, scale_dtype, stream);
-        default: return launch_with<G, 6>(a, p, scale_dtype, stream);
-    }
+    return digits_for(a.x_dtype) == 4 ? launch_blocks<G, 4>(a, p, scale_dtype, stream)
+                                      : launch_blocks<G, 3>(a, p, scale_dtype, stream);
 }
 
 }  // namespace
@@ -538,9 +558,13 @@ extern "C" int64_t nq_int4_projection_workspace_bytes(int64_t tokens, int64_t ou
     if (tokens <= 0 || tokens > 65535 || out_features <= 0 || out_features > 0x7fffffff || in_features <= 0 || in_features % 32 ||
         in_features > (1 << 24) || (group != 32 && group != 64 && group != 128))
         return -1;
-    const Int4Plan p = plan_int4(tokens, out_features, in_features, group);
-    if (!nq::launchable(p.groups * p.slices * p.passes, p.waves * kWave)) return -1;
-    return p.slices == 1 ? 0 : p.slices * tokens * out_features * static_cast<int64_t>(sizeof(float));
+    int64_t most = 0;
+    for (const int digits : {3, 4}) {  // whatever the type of x
+        const Int4Plan p = plan_int4(tokens, out_features, in_features, group, digits);
+        if (!nq::launchable(p.groups * p.slices * p.passes, p.waves * kWave)) return -1;
+        if (p.slices > 1) most = std::max(most, p.slices * tokens * out_features * static_cast<int64_t>(sizeof(float)));
+    }
+    return most;
 }
 
 extern "C" int64_t nq_int4_projection_partials(int64_t out_features) { return out_features <= 0 ? -1 : (out_features + 15) / 16; }
@@ -557,7 +581,7 @@ extern "C" int nq_int4_projection(const void* x, int32_t x_dtype, int64_t tokens
     if (workspace_bytes < need) return NQ_ERR_WORKSPACE;
     if ((reinterpret_cast<uintptr_t>(packed) | reinterpret_cast<uintptr_t>(workspace)) & 15) return NQ_ERR_ALIGNMENT;
     if (reinterpret_cast<uintptr_t>(partials) & 7) return NQ_ERR_ALIGNMENT;
-    const Int4Plan p = plan_int4(tokens, out_features, in_features, group);
+    const Int4Plan p = plan_int4(tokens, out_features, in_features, group, digits_for(x_dtype));
     Int4Args a{};
     a.x = x;
     a.packed = static_cast<const uint8_t*>(packed);

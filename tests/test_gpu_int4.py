@@ -220,3 +220,27 @@ def test_work_on_another_stream_with_a_workspace_of_the_callers():
         there = ops.launch_int4_projection(x, m, workspace=torch.empty(size, dtype=torch.uint8, device=DEV))
     side.synchronize()
     assert torch.equal(here, there)
+
+
+@pytest.mark.parametrize("tokens,ins,outs,group", [(1, 128, 40, 128), (5, 128, 40, 128), (9, 160, 33, 64), (3, 128, 200, 32),
+                                                   (1, 4096, 64, 32), (11, 10240, 48, 64)])
+def test_fp32_values_beside_one_that_meets_no_weight(tokens, ins, outs, group):
+    """A column 10^5 times the others whose weights are all at the zero point: fp32 x is read to 2^-31
+    of it, and nothing of it is in the result. A value's digits add up to 3.02 times it at most (1.502 to 0.498 where the
+    highest is 1), whatever its neighbours are."""
+
+    _say("int4 outlier", tokens, ins, outs, group)
+    m = matrix(outs, ins, group, torch.float32, False, 601)
+    column = 37 + 64 * (ins // 128 // 2)
+    m.packed[:, column // 2] = (m.packed[:, column // 2] & 15) | 0x80
+    x = torch.randn(tokens, ins, generator=_g(602))
+    x[:, column] = 1e5
+    w = olc.int4_dense(m.packed, m.scales, m.zeros, group)
+    assert (w[:, column] == 0).all()
+    got = ops.launch_int4_projection(x.to(DEV), m.to(DEV)).cpu().double()
+    expected, top = x.double() @ w.T, by_group(x.double(), ins, group)
+    adds = 3 + -(-ins // 128) + 3 * (128 // group) * 4
+    sizes = 3.02 * (x.double().abs() @ w.abs().T)  # the column itself has no weight
+    bound = 1.01 * 2.0**-31 * (top @ w.abs().T) + 2.0**-24 * adds * sizes + HALF_STEP[torch.float32] * expected.abs()
+    worst = float(((got - expected).abs() / bound).max())
+    assert worst <= 1, worst
