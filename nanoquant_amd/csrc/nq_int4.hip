@@ -567,7 +567,9 @@ extern "C" int64_t nq_int4_projection_workspace_bytes(int64_t tokens, int64_t ou
     return most;
 }
 
-extern "C" int64_t nq_int4_projection_partials(int64_t out_features) { return out_features <= 0 ? -1 : (out_features + 15) / 16; }
+extern "C" int64_t nq_int4_projection_partials(int64_t out_features) {
+    return out_features <= 0 || out_features > 0x7fffffff ? -1 : (out_features + 15) / 16;
+}
 
 extern "C" int nq_int4_projection(const void* x, int32_t x_dtype, int64_t tokens, const void* packed, const void* scales,
                                   int32_t scale_dtype, const uint8_t* zeros, int64_t out_features, int64_t in_features,

@@ -61,3 +61,9 @@ def test_a_text_scored_by_rows_takes_stages():
     for digits in DIGITS:
         p = plan(256, 151936, 4096, 128, digits)
         assert p.slices == 1 and p.stage < p.slice and p.passes > 1 and p.blocks == 6
+
+
+def test_partials_of_sizes_at_the_limits():
+    count = _native.load().nq_int4_projection_partials
+    assert [count(n) for n in (1, 16, 17, 0x7FFFFFFF)] == [1, 1, 2, 1 << 27]
+    assert [count(n) for n in (0, -1, 0x80000000, (1 << 63) - 1)] == [-1] * 4
