@@ -55,6 +55,140 @@ nq_linear_desc desc_for(int64_t in, int64_t out, int64_t rank, const Buffer& wor
     return d;
 }
 
+// A call's workspace, or an alignment's worth where it needs none.
+Buffer workspace(int64_t bytes) { return Buffer(static_cast<size_t>(bytes > 0 ? bytes : 256)); }
+
+// Ragged batches over the 8-bit paged cache: sizes at their limits and odd ones
+// through every plan, argument errors, and calls up to their launches.
+void serving_calls() {
+    constexpr int64_t kMost32 = 0x7fffffff, kMost64 = INT64_MAX;
+    const int64_t counts[] = {-1, 0, 1, 2, 3, 17, 64, 65, 1000, 65535, 65536, 1 << 20, (1 << 24) - 32, 1 << 24, 0x3fffffff,
+                              kMost32 - 1, kMost32, kMost64};
+    for (const int64_t tokens : counts)
+        for (const int64_t size : counts) {
+            for (const int32_t group : {0, 32, 64, 128})
+                for (const int64_t ins : {int64_t{0}, int64_t{32}, int64_t{1152}, int64_t{10240}, int64_t{1} << 24, kMost64})
+                    expect(nq_int4_projection_workspace_bytes(tokens, size, ins, group) >= -1, "4-bit workspace", 0);
+            expect(nq_int4_projection_partials(size) >= -1, "4-bit partials", 0);
+            for (const int64_t batch : counts)
+                for (const int32_t page : {0, 16, 128}) {
+                    for (const int32_t heads : {0, 4, 65535})
+                        expect(nq_paged_evict_workspace_bytes(batch, heads, page, size, tokens) >= -1, "evict workspace", 0);
+                    for (const int32_t kv_heads : {1, 8})
+                        for (const int32_t head_dim : {64, 96, 128, 256}) {
+                            const int64_t paged = nq_paged_attention_workspace_bytes(tokens, batch, 32, kv_heads, head_dim, page, size);
+                            expect(paged >= -1 && paged <= int64_t{1} << 30, "paged attention workspace", 0);
+                            for (const int64_t shared : {int64_t{-1}, int64_t{0}, int64_t{1000}, kMost64}) {
+                                const int64_t w = nq_shared_attention_workspace_bytes(tokens, batch, 32, kv_heads, head_dim, page, size, shared);
+                                expect(w >= -1 && w <= int64_t{1} << 30, "shared attention workspace", 0);
+                            }
+                        }
+                }
+            for (const int32_t top : {-1, 0, 5, 32, 33})
+                expect(nq_token_logprobs_workspace_bytes(tokens, size, top) >= -1, "logprobs workspace", 0);
+        }
+
+    Buffer cache(1 << 20), scales(1 << 16), lens(1 << 16), table(1 << 16), x(1 << 20), y(1 << 20), into(1 << 16), rows(1 << 20);
+    const auto fp = [](const Buffer& b) { return static_cast<float*>(b.p); };
+    const auto ints = [](const Buffer& b) { return static_cast<int32_t*>(b.p); };
+    const int dtypes[] = {NQ_DTYPE_F32, NQ_DTYPE_F16, NQ_DTYPE_BF16};
+    for (const int32_t head_dim : {64, 128, 256})
+        for (const int32_t page : {16, 32, 64, 128})
+            for (const int64_t batch : {1, 3, 65, 300})
+                for (const int64_t tokens : {1, 40, 700, 5000})
+                    for (const int64_t pages : {3, 200, 9000}) {
+                        nq_paged_kv kv;
+                        std::memset(&kv, 0, sizeof(kv));
+                        kv.k_pages = kv.v_pages = cache.p;
+                        kv.k_scales = kv.v_scales = fp(scales);
+                        kv.num_pages = 1000000;
+                        kv.kv_heads = 4;
+                        kv.head_dim = head_dim;
+                        kv.page_size = page;
+                        kv.page_table = ints(table);
+                        kv.table_pages = pages;
+                        kv.query_starts = kv.context_lens = ints(lens);
+                        kv.batch = batch;
+                        const int type = dtypes[(batch + tokens) % 3];
+                        int st = nq_paged_append(x.p, x.p, x.p, type, tokens, 16, scales.p, scales.p, NQ_DTYPE_F32, 1e-6f, fp(y), fp(y),
+                                                 40000, &kv, y.p, type, nullptr);
+                        expect(launch_refused(st), "paged append", st);
+                        st = nq_paged_append_at(x.p, x.p, x.p, type, tokens, 16, nullptr, nullptr, NQ_DTYPE_F32, 1e-6f, fp(y), fp(y),
+                                                kMost64, &kv, ints(lens), y.p, type, nullptr);
+                        expect(launch_refused(st), "paged append at", st);
+                        int64_t need = nq_paged_attention_workspace_bytes(tokens, batch, 16, 4, head_dim, page, pages);
+                        {
+                            const Buffer ws = workspace(need);
+                            st = nq_paged_attention(x.p, type, tokens, 16, &kv, 0.1f, y.p, type, ws.p, need, nullptr);
+                            expect(launch_refused(st), "paged attention", st);
+                        }
+                        for (const int64_t shared : {int64_t{0}, page * pages / 2, page * pages}) {
+                            need = nq_shared_attention_workspace_bytes(tokens, batch, 16, 4, head_dim, page, pages, shared);
+                            const Buffer ws = workspace(need);
+                            st = nq_shared_attention(x.p, type, tokens, 16, &kv, shared, 0.1f, y.p, type, fp(y), ws.p, need, nullptr);
+                            expect(launch_refused(st), "shared attention", st);
+                            if (need > 0) {
+                                st = nq_shared_attention(x.p, type, tokens, 16, &kv, shared, 0.1f, y.p, type, nullptr, ws.p, need - 1, nullptr);
+                                expect(st == NQ_ERR_WORKSPACE, "shared attention short workspace", st);
+                            }
+                        }
+                        for (const int64_t first : {int64_t{0}, int64_t{33}, page * pages - 1})
+                            expect(launch_refused(nq_attention_weights(x.p, type, tokens, 16, &kv, 0.1f, fp(y), first, fp(y), fp(y), nullptr)),
+                                   "attention weights", 0);
+                        expect(nq_attention_weights(x.p, type, tokens, 16, &kv, 0.1f, fp(y), page * pages, fp(y), fp(y), nullptr) == NQ_OK,
+                               "attention weights of no row", 0);
+                        for (const int64_t budget : {int64_t{1}, int64_t{50}, page * pages, page * pages + 1}) {
+                            need = nq_paged_evict_workspace_bytes(batch, 4, page, pages, budget);
+                            const Buffer ws = workspace(need);
+                            if (need < 0) {  // more pages to move than a launch has workgroups
+                                st = nq_paged_evict(&kv, fp(y), ints(into), budget, 0, 0, ints(rows), ints(x), ints(rows), ws.p, 256, nullptr);
+                                expect(st == NQ_ERR_SHAPE && batch > 64 && budget > 100000, "evict of a size that it refuses", st);
+                                continue;
+                            }
+                            st = nq_paged_evict(&kv, fp(y), ints(into), budget, budget / 3, budget / 4, ints(rows), ints(x), ints(rows), ws.p, need,
+                                                nullptr);
+                            expect(launch_refused(st), "evict", st);
+                            st = nq_paged_evict(&kv, fp(y), ints(into), budget, budget, 1, ints(rows), ints(x), ints(rows), ws.p, need, nullptr);
+                            expect(st == NQ_ERR_SHAPE, "evict more than its budget", st);
+                        }
+                    }
+    expect(nq_paged_append(nullptr, nullptr, nullptr, 0, 1, 1, nullptr, nullptr, 0, 0.0f, nullptr, nullptr, 1, nullptr, nullptr, 0, nullptr) ==
+               NQ_ERR_ARGUMENT, "paged append null", 0);
+    expect(nq_shared_attention(x.p, 0, 1, 1, nullptr, 0, 0.1f, y.p, 0, nullptr, nullptr, 0, nullptr) == NQ_ERR_ARGUMENT, "shared attention null", 0);
+    expect(nq_attention_weights(x.p, 0, 1, 1, nullptr, 0.1f, fp(y), 0, fp(y), fp(y), nullptr) == NQ_ERR_ARGUMENT, "attention weights null", 0);
+    expect(nq_paged_evict(nullptr, nullptr, nullptr, 1, 0, 0, nullptr, nullptr, nullptr, nullptr, 0, nullptr) == NQ_ERR_ARGUMENT, "evict null", 0);
+
+    for (const int32_t group : {32, 64, 128})
+        for (const int64_t tokens : {1, 2, 5, 11, 31, 256, 65535})
+            for (const int64_t outs : {1, 100, 12304, 49268})
+                for (const int64_t ins : {32, 1152, 10240, 30912})
+                    for (const int x_dtype : dtypes) {
+                        const int64_t need = nq_int4_projection_workspace_bytes(tokens, outs, ins, group);
+                        expect(need >= 0, "4-bit workspace", 0);
+                        const Buffer ws(256);  // not touched on the host
+                        int st = nq_int4_projection(x.p, x_dtype, tokens, cache.p, scales.p, dtypes[tokens % 3],
+                                                    static_cast<uint8_t*>(scales.p), outs, ins, group, y.p, NQ_DTYPE_BF16,
+                                                    tokens == 1 ? rows.p : nullptr, ws.p, need, nullptr);
+                        expect(launch_refused(st), "4-bit projection", st);
+                        if (need == 0) continue;
+                        st = nq_int4_projection(x.p, x_dtype, tokens, cache.p, scales.p, NQ_DTYPE_F16, nullptr, outs, ins, group, y.p, NQ_DTYPE_F32,
+                                                nullptr, ws.p, need - 1, nullptr);
+                        expect(st == NQ_ERR_WORKSPACE, "4-bit short workspace", st);
+                    }
+    expect(nq_int4_projection(nullptr, 0, 1, nullptr, nullptr, 0, nullptr, 1, 32, 32, nullptr, 0, nullptr, nullptr, 0, nullptr) == NQ_ERR_ARGUMENT,
+           "4-bit null", 0);
+    int st = nq_greedy_select_partials(rows.p, 9496, static_cast<int64_t*>(y.p), nullptr, 0, nullptr, nullptr, nullptr);
+    expect(launch_refused(st), "greedy select partials", st);
+    for (const int64_t count : {int64_t{1}, int64_t{1531}})
+        for (const int32_t top : {0, 5, 32}) {
+            const int64_t need = nq_token_logprobs_workspace_bytes(count, 151936, top);
+            const Buffer ws = workspace(need);
+            st = nq_token_logprobs(x.p, NQ_DTYPE_F32, count, 151936, 151936, static_cast<int64_t*>(y.p), top, fp(y), fp(y),
+                                   static_cast<int64_t*>(y.p), fp(y), ws.p, need, nullptr);
+            expect(launch_refused(st), "token logprobs", st);
+        }
+}
+
 }  // namespace
 
 int main() {
@@ -64,6 +198,7 @@ int main() {
         return 77;
     }
     expect(nq_abi_version() > 0, "abi version", 0);
+    expect(nq_tiles_header_bytes() > 0, "tiles header", 0);
     for (int s = -20; s <= 1; ++s) expect(nq_status_string(s) != nullptr, "status string", s);
 
     // Argument errors.
@@ -255,6 +390,8 @@ int main() {
         st = nq_read_stream(big.p, 1 << 20, static_cast<uint32_t*>(counts.p), 64, nullptr);
         expect(launch_refused(st), "read stream", st);
     }
+
+    serving_calls();
 
     std::printf("%s: %d failed checks\n", failures ? "FAILED" : "ok", failures);
     return failures ? 1 : 0;
