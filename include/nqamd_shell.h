@@ -348,7 +348,8 @@ int64_t nq_paged_evict_workspace_bytes(int64_t batch, int32_t kv_heads, int32_t 
  * table does not name count as NaN; an entry of into that names no page writes nothing but
  * page_table_out. into's pages stand there once, and in no sequence's part of the page table.
  * Values beyond fp32 become NaN. Outputs lie apart from the arrays that the call reads. kv->query_starts is not read and may be NULL.
- * first + recent <= budget. Keys keep the rotation of their position: the
+ * first + recent <= budget. context_lens counts the rows of tokens that a call has just appended too; page_table_out
+ * has no entry behind the budget's last page for tokens to come. Keys keep the rotation of their position: the
  * tokens appended next have other positions than cache rows (nq_paged_append_at). */
 int nq_paged_evict(const nq_paged_kv* kv, float* weights, const int32_t* into, int64_t budget, int64_t first,
                    int64_t recent, int32_t* page_table_out, int32_t* context_lens_out, int32_t* rows_out,

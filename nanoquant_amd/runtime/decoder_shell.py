@@ -566,7 +566,8 @@ class PackedDecoder:
         the ids before it, the entropy of that distribution and its `top`
         likeliest tokens. One prompt pass, then the output projection row by row
         (the logits that a decode step at that row would see, 0.18 ms each at
-        151936 x 4096; with a 4-bit ``lm_head`` SCORE_ROWS rows at once) and one
+        151936 x 4096; with a 4-bit ``lm_head`` SCORE_ROWS rows at once, the
+        same but for the order of fp32 sums) and one
         ``launch_token_logprobs`` for SCORE_ROWS rows. Leaves the decoder as
         ``prefill(ids)`` does."""
 

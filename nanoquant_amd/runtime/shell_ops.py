@@ -964,7 +964,9 @@ def launch_paged_evict(
     the heaviest by ``weights`` (``launch_attention_weights``). The rows that stay
     move in their order to the free pages ``into`` (int32 ``[batch, ceil(budget /
     page_size) - first // page_size]``), but for the whole pages of the first rows, which stay where
-    they are (nq_paged_evict). The keys keep the positions they were rotated at:
+    they are (nq_paged_evict). ``context_lens`` are the rows that the sequences hold by now, those
+    of the call whose attention was added last among them. The new table has no entries behind the
+    budget: pages for tokens to come go behind them. The keys keep the positions they were rotated at:
     ``launch_paged_append`` takes those of the next tokens as ``rope_starts``. The reference
     keeps every row (src/nanoquant/runtime/transformers_generation.py:262-418)."""
 
