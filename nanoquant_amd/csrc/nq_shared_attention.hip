@@ -116,11 +116,17 @@ int64_t share_bytes(const SharedPlan& plan, int64_t rows, int kv_heads, int head
 // shared rows and up to 700 of their own, 32/8 heads of 128, 34 us; with 128 workgroups 50, 192 38, 384
 // 39, 512 39, 1024 48. Slots of 16 rows read the shared rows twice as often: 36 at their best. Above 64
 // query rows to a sequence its own rows fill the slots, and nothing is gained by sharing.
+// Where the table has room for long histories behind the shared rows, a split for each 96 tiles of them, up to
+// 16, of at least 8 tiles, as plan_attention has: one long conversation among short ones does not keep one
+// workgroup (4096 shared rows, 32 sequences of one token, one with 100000 rows of its own: 115 us, 879 without, 118
+// in nq_paged_attention; 16 sequences, the others 300 rows: 73 us, 117 in splits of at least 4 tiles, 305
+// without). It costs batches of more than 64 short sequences under such a table their empty splits (128 of
+// them: 126 us, 51 without, 227 in nq_paged_attention); 32 take 27 us either way.
 // (32 KB of shared K and V of one head meet 32 query rows at a time: the vector unit widens them and takes
 // the exponentials, about as long as the bytes take.)
 SharedPlan plan_shared(int64_t tokens, int64_t batch, int q_heads, int kv_heads, int head_dim, int page, int64_t cache_rows,
                        int64_t shared_rows) {
-    constexpr int64_t kMostMean = 64, kMostBytes = int64_t{1} << 30, kTarget = 512, kShared = 256;
+    constexpr int64_t kMostMean = 64, kMostBytes = int64_t{1} << 30, kTarget = 512, kShared = 256, kSkew = 96;
     const int64_t rows = tokens * (q_heads / kv_heads), mean = (rows + batch - 1) / batch;
     const int grain = std::max(page, kTile);
     SharedPlan plan{};
@@ -130,15 +136,20 @@ SharedPlan plan_shared(int64_t tokens, int64_t batch, int q_heads, int kv_heads,
         plan.own = AttnPlan{};
         plan.own.shared = true;
         plan.own.waves = 4;
-        plan.own.least = 4;
         plan.own.rows = rows <= 16 ? 16 : 32;
         plan.own.slots = static_cast<int>(rows / plan.own.rows + batch);
         const int64_t slots = (rows + plan.own.rows - 1) / plan.own.rows;
-        const int64_t units = static_cast<int64_t>(plan.own.slots) * kv_heads;
-        plan.own.splits = static_cast<int>(std::max(int64_t{1}, std::min({kTarget / units, (own_tiles + 3) / 4, int64_t{kMostShares}})));
         const int64_t splits = std::max(int64_t{1}, std::min({kShared / (slots * kv_heads), (tiles + 3) / 4, int64_t{kMostShares}}));
         plan.per = static_cast<int>((tiles + splits - 1) / splits);
         plan.splits = static_cast<int>((tiles + plan.per - 1) / plan.per);
+        const int64_t units = static_cast<int64_t>(plan.own.slots) * kv_heads;
+        const int64_t alone = (mean + plan.own.rows - 1) / plan.own.rows * kv_heads;
+        const int64_t skew = std::min({own_tiles / kSkew, int64_t{16}, kTarget / alone});
+        plan.own.least = skew > kTarget / units ? 8 : 4;
+        const int64_t each = kv_heads * plan.own.rows * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+        const int64_t room = (kMostBytes / each - slots * plan.splits) / plan.own.slots;
+        plan.own.splits = static_cast<int>(std::max(int64_t{1}, std::min({std::max(kTarget / units, skew), (own_tiles + 3) / 4,
+                                                                         int64_t{kMostShares}, room})));
         if (share_bytes(plan, rows, kv_heads, head_dim) <= kMostBytes) return plan;
     }
     // Each sequence's slots are full of its own rows, or there is nothing to share.
