@@ -51,9 +51,10 @@ __device__ __forceinline__ float sum_rows(float (&w)[N], int n) {
 template <bool TURNS>
 constexpr int kWavesOf = TURNS ? 8 : 4;
 
-// Single tokens are bound by the wait for the table's entries and then for K and q
-// (32 sequences of up to 4000 rows: 81 MB in 26.5 us; pages of 16 rows are 2 KB of K each). Prompts are bound by the vector
-// unit: 16 exponentials, 16 fused and 16 plain additions a product of 16 rows (1531 tokens
+// Single tokens are bound by the wait for the table's entries and then for K and q (56% of a wave's cycles), and
+// by the vector unit, which works in 66% of the SIMDs' (32 sequences of up to 4000 rows: 81 MB in 26.5 us; pages of 16
+// rows are 2 KB of K each). Prompts: 16 exponentials, 16 fused and 16 plain additions a product of 16 rows take 52% of the
+// SIMDs' cycles, the matrix unit 18%, and two waves to a SIMD wait in 56% of theirs (1531 tokens
 // after 517: 8e9 products and sums in 53 us, the first rows' workgroups the last to end).
 // TURNS: the waves of a workgroup hold the same cache rows and take the query rows in
 // turn; otherwise each wave has cache rows of its own and takes all query rows.
