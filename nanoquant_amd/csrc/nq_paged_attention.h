@@ -605,7 +605,8 @@ __global__ __launch_bounds__(WAVES* kWave, D == 256 && NT == 2 ? 1 : 2) void k_p
 
         const bool masked = base + TILE > low_pos + 1;  // uniform: some row of the wave does not see them all
         if (masked) {
-            // Rows that nobody sees may have any scale: the scores are multiplied here.
+            // Rows that nobody sees may have any scale: the scores are multiplied here, for all query rows of
+            // the wave. (So the last bits of a result hang on the positions of the rows beside it, never on their values.)
 #pragma unroll
             for (int u = 0; u < NT; ++u) {
                 const int seen = pos[u] + 1 - (base + kBlock * grp);
