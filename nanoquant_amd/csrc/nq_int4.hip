@@ -12,8 +12,8 @@
 // rounding down to 2^-14 and 2^-11); fp32 x has four, within 2^-31, exact down to 2^-7 of it. With three, an
 // fp32 value far below another one of its group whose weights are at the zero point (so that nothing hides the
 // loss) would keep few bits of its own. Four cost one token of a large matrix nothing (151936 x 4096: 55.9
-// us, 56.0 with three), 11 tokens of 2560 x 10240, groups of 64, 19.0 us for 17.2, and 30 of 4096 x 4096, groups of
-// 128, 25.1 for 21.2 (24 tokens at once, not 30).
+// us, 56.0 with three), 11 tokens of 2560 x 10240, groups of 64, 17.8 us for 17.2, and with groups of 128 what reading the
+// weights for 4 tokens to a block and 24 at once does, not 5 and 30 (4096 x 4096: 5 tokens 11.7 us for 9.9, 30 24.4 for 21.3).
 //
 // A chunk is 128 columns: lane 16 q + r of a wave holds 16 bytes of row r, columns 32 q
 // to 32 q + 31, whose low nibbles (even columns) are the A operand of one product and
@@ -476,7 +476,10 @@ size_t lds_bytes(int waves, int tokens, int digits, int blocks, int groups, int 
 //  - Otherwise the row in stages, whose digits are made one after the other.
 // Blocks: more of them read the weights once for more tokens, and hold more registers.
 Int4Plan plan_int4(int64_t tokens, int64_t outs, int64_t ins, int group, int digits) {
-    constexpr size_t kBudget = 60 * 1024;
+    // As many chunks as three digits of them fit 60 KB, and two workgroups a compute unit either way (fp32, 11 tokens of
+    // 2560 x 10240, groups of 64: 17.8 us, 19.0 with 60 KB; 16 of 6912 x 4096, groups of 128: 23.4 and 26.0; 6 of 14336
+    // x 4096, groups of 32: 33.7 and 36.8; but 8 of it, groups of 128: 30.5 and 23.2, whose slices do better).
+    const size_t budget = (digits == 4 ? 78 : 60) * 1024;
     const int groups = kChunk / group, each = 16 / groups / digits;
     const int64_t blocks = (tokens + each - 1) / each, chunks = chunks_of(ins), tiles = (outs + 15) / 16;
     Int4Plan p{};
@@ -486,9 +489,9 @@ Int4Plan plan_int4(int64_t tokens, int64_t outs, int64_t ins, int group, int dig
     p.passes = static_cast<int>((blocks + p.blocks - 1) / p.blocks);
     const int held = static_cast<int>(std::min<int64_t>(tokens, int64_t{p.blocks} * each));
     // Chunks whose digits LDS holds at once. (Four more waves of the slices' form bring their own 5.5 to 6.5 KB each on
-    // top: at most 87 KB of a workgroup, of 160.)
+    // top: at most 87 KB of a workgroup, 103 with four digits, of 160.)
     const size_t fixed = lds_bytes(4, held, digits, p.blocks, groups, 0), each_chunk = lds_bytes(4, held, digits, p.blocks, groups, 1) - fixed;
-    const int most = static_cast<int>(std::min<int64_t>(chunks, std::max<int64_t>(1, static_cast<int64_t>((kBudget - std::min(fixed, kBudget)) / each_chunk))));
+    const int most = static_cast<int>(std::min<int64_t>(chunks, std::max<int64_t>(1, static_cast<int64_t>((budget - std::min(fixed, budget)) / each_chunk))));
     p.slices = 1;
     p.waves = 4;
     p.share = tiles * p.passes >= 2048 ? 1 : 4;

@@ -6,7 +6,8 @@ from __future__ import annotations
 
 from typing import NamedTuple
 
-CHUNK, BUDGET, MOST_WAVES, WALKERS, MOST_SLICES = 128, 60 * 1024, 2048, 768, 16
+CHUNK, MOST_WAVES, WALKERS, MOST_SLICES = 128, 2048, 768, 16
+BUDGET = {3: 60 * 1024, 4: 78 * 1024}  # by digits
 AT_ONCE = 4
 
 
@@ -49,7 +50,7 @@ def plan(tokens: int, outs: int, ins: int, group: int, digits: int) -> Plan:
     passes = _up(wanted, blocks)
     held = min(tokens, blocks * each)
     fixed = lds_bytes(4, held, digits, blocks, groups, 0)
-    most = min(chunks, max(1, (BUDGET - min(fixed, BUDGET)) // (lds_bytes(4, held, digits, blocks, groups, 1) - fixed)))
+    most = min(chunks, max(1, (BUDGET[digits] - min(fixed, BUDGET[digits])) // (lds_bytes(4, held, digits, blocks, groups, 1) - fixed)))
     work = tiles * passes
     slices, waves, share = 1, 4, 1 if work >= MOST_WAVES else 4
     if most < chunks and work < MOST_WAVES:

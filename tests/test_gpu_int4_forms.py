@@ -18,10 +18,11 @@ pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="n
 SHAPES = [
     # tokens, in, out, group
     (31, 1024, 16400, 128), (7, 2048, 16400, 32), (4, 2048, 32784, 32), (33, 288, 16948, 128),  # stages, passes, a short last one
-    (1, 9152, 35227, 32), (5, 2336, 33599, 128), (3, 3040, 36113, 32),
+    (1, 10944, 32951, 32), (5, 2592, 33544, 128), (6, 1952, 34248, 64),
     (1, 64, 12304, 32), (1, 64, 32752, 32), (3, 96, 12466, 32), (7, 32, 6240, 32), (14, 64, 13218, 128), (9, 32, 12332, 128),  # shared, walking
-    (1, 9312, 26427, 32), (2, 4448, 25558, 32), (3, 2976, 24856, 32),  # slices, walking
-    (1, 18976, 16450, 32), (7, 25056, 3, 128), (12, 14752, 18, 128), (4, 30912, 20, 32),  # slices in stages
+    (1, 11360, 24715, 64), (2, 5792, 24749, 32), (3, 3840, 24908, 32),  # slices, walking
+    (1, 32160, 11271, 32), (8, 24800, 3, 128), (6, 30784, 18, 64), (5, 31552, 20, 32),  # slices in stages
+    (4, 30688, 27, 32), (4, 36320, 20, 32),  # 87 KB of LDS (bf16), 103 (fp32)
     (1, 32, 32814, 32), (1, 32, 49268, 32), (2, 32, 49224, 32), (3, 32, 49379, 32), (7, 64, 24866, 32),
 ]
 
